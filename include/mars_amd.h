@@ -688,6 +688,147 @@ typedef struct mars_serve_bench {
 } mars_serve_bench;
 int mars_bench_serve(mars_graph* g, mars_ctx* ctx_global, mars_ctx* ctx_episode, mars_serve_bench* bench);
 
+/* ---- reading: attention over a paged cache of the memories' tokens --------------------
+ * No reference counterpart. A query returns which memories matter; a model that answers from
+ * them reads their tokens. A mars_reader holds the geometry (heads, types, pages, rotary
+ * positions) and the scratch of that step; the cache, its tables and all tensors are the
+ * caller's device memory. Per step of a batch of requests: mars_kv_plan once, then per
+ * layer mars_kv_store and mars_kv_attend; mars_kv_release when requests end.
+ * The calls run on `stream` (a hipStream_t; NULL = the null stream), allocate nothing and
+ * return without waiting, so they can be captured into a HIP graph. One reader serves one
+ * stream at a time (calls that overlap share its scratch and race). Lengths, tables and
+ * slots are read on the device: their values are not checked on the host, and kernels keep
+ * every access inside the arrays described to them whatever they hold. */
+#define MARS_DTYPE_F16  0
+#define MARS_DTYPE_BF16 1
+#define MARS_KV_MAX_REQUESTS 4096
+
+typedef struct mars_reader_desc {
+    int32_t q_heads;           /* a multiple of kv_heads, at most 64 per kv head              */
+    int32_t kv_heads;
+    int32_t head_dim;          /* 64, 128 or 256                                              */
+    int32_t dtype;             /* MARS_DTYPE_*: q, k, v, the cache and the output             */
+    int32_t page_size;         /* tokens per page: 16, 32, 64, 128 or 256                     */
+    int32_t rope_dim;          /* leading elements of a head that turn (a multiple of 16; 0: none) */
+    int32_t rope_axes;         /* position axes: 1, or up to 3 (time, height, width)          */
+    int32_t rope_adjacent;     /* pairs that turn: 0 (i, i + rope_dim/2), 1 (2i, 2i + 1)      */
+    int32_t rope_sections[3];  /* frequencies of each axis, in order; their sum is rope_dim / 2 */
+    int32_t pad0;
+    double  rope_theta;        /* frequency i: rope_theta^(-2i / rope_dim) per position       */
+} mars_reader_desc;
+typedef struct mars_reader mars_reader;
+int mars_reader_create(const mars_reader_desc* desc, mars_reader** out);
+int mars_reader_destroy(mars_reader* r);
+
+/* Lays out one step: R requests with cached_lens[r] tokens in the cache add new_lens[r]
+ * tokens each (>= 0; negative counts as 0), rows of the step's tensors in request order.
+ * Request r's row of block_table holds the ceil(cached / page_size) pages it owns; the pages it
+ * needs more are taken from the top of free_pages (free_count[0] of them) and written behind
+ * those. Requests are served in order; one that needs pages is served if it and all before it
+ * fit what is free. One whose tokens exceed its table row (max_pages) or the num_tokens rows
+ * of the step takes none and is not served. Outputs (all device):
+ *   q_start[R + 1]      first row of each request; q_start[R] = total of new_lens
+ *   kv_lens[R]          tokens with this step's (cached + new), 0 if not served
+ *   slots[num_tokens]   page * page_size + offset of each new token; -1 if not served or past the total
+ *   positions[num_tokens]  its index within the request; 0 past the total
+ *   free_count_out[1]   pages left (a later step reads it as its free_count)
+ * Outputs must not overlap inputs (kv_lens is the next step's cached_lens: use two arrays in turn).
+ * R <= MARS_KV_MAX_REQUESTS. */
+typedef struct mars_kv_plan_args {
+    const int32_t* new_lens;
+    const int32_t* cached_lens;
+    int32_t*       block_table;     /* R x max_pages */
+    const int32_t* free_pages;
+    const int32_t* free_count;
+    int32_t*       q_start;
+    int32_t*       kv_lens;
+    int64_t*       slots;
+    int32_t*       positions;
+    int32_t*       free_count_out;
+    int32_t        num_requests;
+    int32_t        max_pages;
+    int32_t        num_tokens;
+    int32_t        free_capacity;   /* entries of free_pages */
+} mars_kv_plan_args;
+int mars_kv_plan(const mars_reader* r, const mars_kv_plan_args* args, void* stream);
+
+/* Gives back the pages of the requests with done[r] != 0: the ceil(kv_lens[r] / page_size) pages
+ * of their table rows are pushed onto free_pages in request order, free_count[0] grows, and
+ * kv_lens[r] becomes 0. Pages beyond free_capacity are dropped. */
+int mars_kv_release(const mars_reader* r, const int32_t* done, int32_t* kv_lens, const int32_t* block_table,
+                    int32_t num_requests, int32_t max_pages, int32_t* free_pages, int32_t* free_count,
+                    int32_t free_capacity, void* stream);
+
+/* The cache of one layer: k_pages is (page, kv_head, token, element), v_pages is (page, kv_head,
+ * element, token): the values of one element lie next to each other over the tokens, as the
+ * product of weights and values reads them. A page's heads are dense; page strides (in
+ * elements, a multiple of 8, 0 = dense) let the layers of a model interleave. times / episodes: a timestamp and
+ * an episode id per slot (num_pages x page_size, NULL where no call uses them), shared by the layers. */
+typedef struct mars_kv_cache {
+    void*    k_pages;
+    void*    v_pages;
+    float*   times;
+    int32_t* episodes;
+    int64_t  k_page_stride;
+    int64_t  v_page_stride;
+    int32_t  num_pages;
+    int32_t  pad0;
+} mars_kv_cache;
+
+/* Turns q and k by their rotary positions (rounded once, angles exact to fp32 for any int32
+ * position) and writes k, v, times and episodes to the tokens' slots. Rows: token t, head h of q
+ * at q + t * q_stride + h * head_dim (elements; strides a multiple of 8); positions[a * num_tokens + t]
+ * on axis a. q_out may be q. k and v NULL: only q is turned; q NULL: only k and v are stored. times /
+ * episodes NULL: left as they are. A slot outside the cache (-1: a token without one) stores
+ * nothing; q is turned all the same. Two tokens of one call must not name one slot.
+ * inverse != 0 turns the other way: the gradient of the rotation with respect to its input. */
+typedef struct mars_kv_store_args {
+    const void*    q;
+    const void*    k;
+    const void*    v;
+    void*          q_out;
+    const int32_t* positions;       /* rope_axes x num_tokens; NULL if rope_dim is 0 */
+    const int64_t* slots;           /* num_tokens; NULL if k and v are */
+    const float*   times;
+    const int32_t* episodes;
+    int64_t        q_stride, k_stride, v_stride, q_out_stride;
+    int32_t        num_tokens;
+    int32_t        inverse;
+} mars_kv_store_args;
+int mars_kv_store(const mars_reader* r, const mars_kv_cache* cache, const mars_kv_store_args* args, void* stream);
+
+/* Attention of every request's new tokens over its cached tokens (theirs included: store first).
+ * Request r's rows are q_start[r] .. q_start[r + 1] - 1, n of them; row i stands at position
+ * p = kv_lens[r] - n + i. Query head h reads kv head h / (q_heads / kv_heads). For key j of the request:
+ *   s = scale * <q, k_j>;  cap > 0: s = cap * tanh(s / cap);
+ *   decay: s -= decay[h] * max(0, q_times[row] - times[j])   (weights decayed by age, as retrieval scores are)
+ * and j is seen if j <= p or j < prefix_lens[r], and, with q_episodes, if the query's or the key's episode
+ * is negative or both are equal. out = sum softmax(s)_j v_j over the keys seen; a row that sees
+ * none is 0 with lse -inf. Keys not seen have no effect, whatever the cache holds there (NaN too).
+ * The sums are fp32; weights are rounded to the cache's type for the product with v.
+ * max_new: an upper bound of the requests' new tokens if the caller knows one (0: unknown); it picks
+ * the kernel, and a wrong one costs speed alone. num_tokens rows of q; rows no request owns are left. */
+typedef struct mars_kv_attend_args {
+    const void*    q;
+    void*          out;
+    float*         lse;             /* num_tokens x q_heads, log of the sum of exp(s); NULL: not wanted */
+    const int32_t* q_start;         /* R + 1 */
+    const int32_t* kv_lens;         /* R */
+    const int32_t* block_table;     /* R x max_pages */
+    const float*   decay;           /* q_heads; NULL: none (else cache times and q_times are needed) */
+    const float*   q_times;         /* num_tokens */
+    const int32_t* q_episodes;      /* num_tokens; NULL: none (else cache episodes are needed) */
+    const int32_t* prefix_lens;     /* R; NULL: none */
+    int64_t        q_stride, out_stride;   /* elements between tokens, a multiple of 8 */
+    float          scale;           /* 0: head_dim^-0.5 */
+    float          cap;             /* 0: none */
+    int32_t        num_requests;
+    int32_t        max_pages;
+    int32_t        num_tokens;
+    int32_t        max_new;
+} mars_kv_attend_args;
+int mars_kv_attend(const mars_reader* r, const mars_kv_cache* cache, const mars_kv_attend_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

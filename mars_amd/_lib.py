@@ -192,6 +192,39 @@ class CorpusParamsC(C.Structure):
     ]
 
 
+class ReaderDescC(C.Structure):
+    _fields_ = [("q_heads", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32), ("dtype", C.c_int32),
+                ("page_size", C.c_int32), ("rope_dim", C.c_int32), ("rope_axes", C.c_int32), ("rope_adjacent", C.c_int32),
+                ("rope_sections", C.c_int32 * 3), ("pad0", C.c_int32), ("rope_theta", C.c_double)]
+
+
+class KvPlanArgsC(C.Structure):
+    _fields_ = [("new_lens", C.c_void_p), ("cached_lens", C.c_void_p), ("block_table", C.c_void_p), ("free_pages", C.c_void_p),
+                ("free_count", C.c_void_p), ("q_start", C.c_void_p), ("kv_lens", C.c_void_p), ("slots", C.c_void_p),
+                ("positions", C.c_void_p), ("free_count_out", C.c_void_p), ("num_requests", C.c_int32),
+                ("max_pages", C.c_int32), ("num_tokens", C.c_int32), ("free_capacity", C.c_int32)]
+
+
+class KvCacheC(C.Structure):
+    _fields_ = [("k_pages", C.c_void_p), ("v_pages", C.c_void_p), ("times", C.c_void_p), ("episodes", C.c_void_p),
+                ("k_page_stride", C.c_int64), ("v_page_stride", C.c_int64), ("num_pages", C.c_int32), ("pad0", C.c_int32)]
+
+
+class KvStoreArgsC(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("q_out", C.c_void_p), ("positions", C.c_void_p),
+                ("slots", C.c_void_p), ("times", C.c_void_p), ("episodes", C.c_void_p), ("q_stride", C.c_int64),
+                ("k_stride", C.c_int64), ("v_stride", C.c_int64), ("q_out_stride", C.c_int64), ("num_tokens", C.c_int32),
+                ("inverse", C.c_int32)]
+
+
+class KvAttendArgsC(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("out", C.c_void_p), ("lse", C.c_void_p), ("q_start", C.c_void_p), ("kv_lens", C.c_void_p),
+                ("block_table", C.c_void_p), ("decay", C.c_void_p), ("q_times", C.c_void_p), ("q_episodes", C.c_void_p),
+                ("prefix_lens", C.c_void_p), ("q_stride", C.c_int64), ("out_stride", C.c_int64), ("scale", C.c_float),
+                ("cap", C.c_float), ("num_requests", C.c_int32), ("max_pages", C.c_int32), ("num_tokens", C.c_int32),
+                ("max_new", C.c_int32)]
+
+
 VP = C.c_void_p
 I32 = C.c_int32
 I64 = C.c_int64
@@ -283,6 +316,12 @@ SIGNATURES = {
                                    C.POINTER(TiledStatsC)]),
     "mars_host_alloc": (C.c_int, [C.c_size_t, C.POINTER(VP)]),
     "mars_host_free": (C.c_int, [VP]),
+    "mars_reader_create": (C.c_int, [C.POINTER(ReaderDescC), C.POINTER(VP)]),
+    "mars_reader_destroy": (C.c_int, [VP]),
+    "mars_kv_plan": (C.c_int, [VP, C.POINTER(KvPlanArgsC), VP]),
+    "mars_kv_release": (C.c_int, [VP, VP, VP, VP, I32, I32, VP, VP, I32, VP]),
+    "mars_kv_store": (C.c_int, [VP, C.POINTER(KvCacheC), C.POINTER(KvStoreArgsC), VP]),
+    "mars_kv_attend": (C.c_int, [VP, C.POINTER(KvCacheC), C.POINTER(KvAttendArgsC), VP]),
     # mars_corpus.h
     "mars_corpus_default": (None, [C.POINTER(CorpusParamsC), I64, I32, C.c_uint64]),
     "mars_corpus_generate": (C.c_int, [C.POINTER(CorpusParamsC), VP, VP, VP, VP, I32]),

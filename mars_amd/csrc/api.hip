@@ -91,6 +91,8 @@ bool episode_scoped_active(const Graph& g, const mars_retrieval_config& c) {
 
 }  // namespace
 
+int require_device(int* dev) { return ensure_device(dev); }
+
 int set_error(int code, const char* fmt, ...) {
     va_list ap;
     va_start(ap, fmt);

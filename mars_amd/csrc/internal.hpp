@@ -28,6 +28,9 @@ namespace mars {
 // ---- error reporting ---------------------------------------------------------
 int set_error(int code, const char* fmt, ...);
 
+// The current device, which has to be a gfx950 (MARS_ERR_NODEVICE, MARS_ERR_HIP otherwise).
+int require_device(int* dev);
+
 // Takes the device address of mars_query_batch_static's scratch array on `dev` (the
 // current device) once; mars_init and mars_graph_create call it.
 int noalloc_prepare(int dev);

@@ -1,0 +1,170 @@
+"""What the reading path refuses, before any device work: geometries, shapes, types, strides and missing arrays."""
+from __future__ import annotations
+
+import ctypes as C
+
+import numpy as np
+import pytest
+
+from mars_amd import _lib
+from mars_amd._lib import MarsError, check, lib
+from mars_amd.reader import PagedCache, Reader
+
+INVALID, CAPACITY, UNSUPPORTED, NODEVICE = -1, -4, -5, -6
+
+
+class Fake:
+    """An array that is only described: `shape`, `stride`, `dtype` and an aligned address that nothing reads."""
+
+    def __init__(self, *shape, dtype="float16", strides=None, ptr=1 << 20):
+        self.shape, self.dtype, self._ptr = shape, dtype, ptr
+        self._s = strides or tuple(int(np.prod(shape[i + 1:])) for i in range(len(shape)))
+
+    def data_ptr(self):
+        return self._ptr
+
+    def stride(self, i):
+        return self._s[i]
+
+
+@pytest.mark.parametrize("bad,code", [
+    (dict(q_heads=5, kv_heads=2), INVALID), (dict(q_heads=0, kv_heads=0), INVALID), (dict(q_heads=2, kv_heads=4), INVALID),
+    (dict(q_heads=65, kv_heads=1), UNSUPPORTED), (dict(head_dim=96), UNSUPPORTED), (dict(page_size=8), UNSUPPORTED),
+    (dict(page_size=48), UNSUPPORTED), (dict(page_size=512), UNSUPPORTED), (dict(rope_dim=66), INVALID), (dict(rope_dim=24), INVALID),
+    (dict(rope_dim=64, rope_sections=(30,)), INVALID), (dict(rope_dim=64, rope_sections=(40, -8)), INVALID),
+    (dict(rope_dim=64, rope_theta=1.0), INVALID), (dict(rope_dim=64, rope_theta=float("inf")), INVALID),
+])
+def test_reader_geometries(bad, code):
+    with pytest.raises(MarsError) as e:
+        Reader(**{**dict(q_heads=4, kv_heads=2, head_dim=64), **bad})
+    assert e.value.code == code
+
+
+def test_reader_types():
+    with pytest.raises(ValueError):
+        Reader(dtype="float32")
+    with pytest.raises(ValueError):
+        Reader(rope_dim=64, rope_sections=(8, 8, 8, 8))
+    desc = _lib.ReaderDescC(4, 2, 64, 7, 16)
+    out = C.c_void_p()
+    assert lib.mars_reader_create(C.byref(desc), C.byref(out)) == UNSUPPORTED and not out
+    assert lib.mars_reader_create(None, C.byref(out)) == INVALID
+    assert lib.mars_reader_destroy(None) == 0
+
+
+def test_caches():
+    ok = dict(k=Fake(9, 2, 16, 64), v=Fake(9, 2, 64, 16))
+    PagedCache(ok["k"], ok["v"])
+    PagedCache(Fake(9, 2, 16, 64, strides=(4096, 1024, 64, 1)), Fake(9, 2, 64, 16, strides=(4096, 1024, 16, 1)))
+    for k, v in ((Fake(9, 2, 16, 64), Fake(9, 2, 16, 64)), (Fake(9, 2, 64), ok["v"]), (ok["k"], Fake(9, 2, 64, 16, dtype="bfloat16")),
+                 (Fake(9, 2, 16, 64, dtype="float32"), Fake(9, 2, 64, 16, dtype="float32")),
+                 (Fake(9, 2, 16, 64, strides=(2048, 64, 128, 1)), ok["v"]), (ok["k"], Fake(8, 2, 64, 16))):
+        with pytest.raises(ValueError):
+            PagedCache(k, v)
+    for t, e in ((Fake(9 * 16 - 1, dtype="float32"), None), (Fake(9, 16, dtype="float16"), None), (None, Fake(9, 16, dtype="float32"))):
+        with pytest.raises(ValueError):
+            PagedCache(ok["k"], ok["v"], t, e)
+
+
+def a_reader(**kw):
+    """A Reader without a device behind it: every call below is refused before its handle is used."""
+    r = Reader.__new__(Reader)
+    r.q_heads, r.kv_heads, r.head_dim, r.dtype, r.page_size, r.rope_dim, r.rope_axes = 4, 2, 64, "float16", 16, 64, 1
+    r.handle = C.c_void_p()
+    for k, v in kw.items():
+        setattr(r, k, v)
+    return r
+
+
+CACHE = (Fake(9, 2, 16, 64), Fake(9, 2, 64, 16))
+
+
+def i32(*shape):
+    return Fake(*shape, dtype="int32")
+
+
+@pytest.mark.parametrize("change", [
+    dict(q=Fake(7, 4, 32)), dict(q=Fake(7, 3, 64)), dict(q=Fake(7, 4, 64, dtype="bfloat16")), dict(q=Fake(7, 4, 64, strides=(256, 1, 4))),
+    dict(out=Fake(6, 4, 64)), dict(q_start=i32(3)), dict(q_start=Fake(4, dtype="int64")), dict(kv_lens=Fake(3, dtype="float32")),
+    dict(table=i32(2, 5)), dict(table=i32(3)), dict(lse=Fake(7, 4)), dict(decay=Fake(3, dtype="float32")), dict(q_times=Fake(6, dtype="float32")),
+    dict(q_eps=i32(8)), dict(prefix=i32(2)), dict(cache=PagedCache(Fake(9, 4, 16, 64), Fake(9, 4, 64, 16))),
+    dict(cache=PagedCache(Fake(9, 2, 32, 64), Fake(9, 2, 64, 32))), dict(table=Fake(3, 5, dtype="int32", strides=(1, 3))),
+])
+def test_attend_shapes(change):
+    a = dict(cache=PagedCache(*CACHE), q=Fake(7, 4, 64), out=Fake(7, 4, 64), q_start=i32(4), kv_lens=i32(3), table=i32(3, 5), lse=None, decay=None,
+             q_times=None, q_eps=None, prefix=None)
+    a.update(change)
+    with pytest.raises(ValueError):
+        a_reader().attend(a["cache"], a["q"], a["out"], a["q_start"], a["kv_lens"], a["table"], lse=a["lse"], decay=a["decay"],
+                          q_times=a["q_times"], q_episodes=a["q_eps"], prefix_lens=a["prefix"])
+
+
+@pytest.mark.parametrize("change", [
+    dict(q=None, k=None, v=None), dict(v=None), dict(slots=None), dict(slots=i32(7)), dict(positions=None), dict(positions=i32(2, 7)),
+    dict(positions=Fake(7, dtype="float32")), dict(k=Fake(7, 4, 64)), dict(k=Fake(6, 2, 64)), dict(times=Fake(6, dtype="float32")),
+    dict(episodes=Fake(7, dtype="float32")), dict(cache=None), dict(q_out=Fake(7, 4, 32)),
+])
+def test_store_shapes(change):
+    a = dict(cache=PagedCache(*CACHE), q=Fake(7, 4, 64), k=Fake(7, 2, 64), v=Fake(7, 2, 64), positions=i32(7), slots=Fake(7, dtype="int64"),
+             q_out=None, times=None, episodes=None)
+    a.update(change)
+    with pytest.raises(ValueError):
+        a_reader().store(a.pop("cache"), a.pop("q"), a.pop("k"), a.pop("v"), a.pop("positions"), a.pop("slots"), **a)
+
+
+@pytest.mark.parametrize("change", [dict(cached=i32(4)), dict(table=i32(2, 5)), dict(count=i32(2)), dict(q_start=i32(3)), dict(slots=i32(7)),
+                                    dict(positions=i32(8)), dict(left=i32(0))])
+def test_plan_shapes(change):
+    a = dict(cached=i32(3), table=i32(3, 5), count=i32(1), q_start=i32(4), slots=Fake(7, dtype="int64"), positions=i32(7), left=i32(1))
+    a.update(change)
+    with pytest.raises(ValueError):
+        a_reader().plan(i32(3), a["cached"], a["table"], i32(20), a["count"], q_start=a["q_start"], kv_lens=i32(3), slots=a["slots"],
+                        positions=a["positions"], free_count_out=a["left"])
+
+
+def test_null_arguments():
+    """The C entries report a missing handle or argument block, and touch nothing."""
+    for name, args in (("mars_kv_plan", (None, None, None)), ("mars_kv_store", (None, None, None, None)),
+                       ("mars_kv_attend", (None, None, None, None)), ("mars_kv_release", (None, None, None, None, 1, 1, None, None, 1, None))):
+        with pytest.raises(MarsError) as e:
+            check(getattr(lib, name)(*args), name)
+        assert e.value.code == INVALID
+
+
+@pytest.mark.gpu
+def test_c_refusals():
+    """Arguments that only the C entries can check, on a live reader; nothing is launched."""
+    import mars_amd
+    mars_amd.init(0)
+    r = Reader(4, 2, 64, "float16", 16, rope_dim=64)
+    p = 1 << 20
+
+    def cache(**kw):
+        return _lib.KvCacheC(**{**dict(k_pages=p, v_pages=p, num_pages=9), **kw})
+
+    good = dict(q=p, out=p, q_start=p, kv_lens=p, block_table=p, q_stride=256, out_stride=256, num_requests=3, max_pages=5, num_tokens=7)
+
+    def attend(c=None, **kw):
+        a = _lib.KvAttendArgsC(**{**good, **kw})
+        return lib.mars_kv_attend(r.handle, C.byref(c or cache()), C.byref(a), None)
+
+    for kw, code in ((dict(q=None), INVALID), (dict(num_requests=0), INVALID), (dict(num_requests=4097), CAPACITY), (dict(max_pages=0), INVALID),
+                     (dict(max_pages=2 ** 28), CAPACITY), (dict(num_tokens=-1), INVALID), (dict(num_tokens=2 ** 30), CAPACITY), (dict(q_stride=248), INVALID),
+                     (dict(q_stride=260), INVALID), (dict(q=p + 2), INVALID), (dict(out_stride=12), INVALID), (dict(cap=-1.0), INVALID),
+                     (dict(cap=float("nan")), INVALID), (dict(scale=float("inf")), INVALID), (dict(decay=p), INVALID), (dict(q_episodes=p), INVALID),
+                     (dict(max_new=-1), INVALID)):
+        assert attend(**kw) == code, kw
+    for c in (cache(k_pages=None), cache(num_pages=0), cache(k_page_stride=8), cache(v_page_stride=4097), cache(k_pages=p + 8), cache(times=p + 4)):
+        assert attend(c) == INVALID
+    assert attend(num_tokens=0) == 0                     # nothing to do
+    store = dict(q=p, k=p, v=p, q_out=p, positions=p, slots=p, q_stride=256, k_stride=128, v_stride=128, q_out_stride=256, num_tokens=7)
+    for kw in (dict(q=None, k=None, v=None), dict(v=None), dict(q_out=None), dict(slots=None), dict(positions=None), dict(k_stride=120), dict(v_stride=130),
+               dict(q_out_stride=512), dict(times=p), dict(episodes=p), dict(num_tokens=-1), dict(k=p + 2)):
+        a = _lib.KvStoreArgsC(**{**store, **kw})
+        assert lib.mars_kv_store(r.handle, C.byref(cache()), C.byref(a), None) == INVALID, kw
+    plan = dict(new_lens=p, cached_lens=p, block_table=p, free_pages=p, free_count=p, q_start=p, kv_lens=p, slots=p, positions=p,
+                free_count_out=p + 64, num_requests=3, max_pages=5, num_tokens=7, free_capacity=9)
+    for kw, code in ((dict(new_lens=None), INVALID), (dict(slots=None), INVALID), (dict(free_count_out=p), INVALID), (dict(num_requests=0), INVALID),
+                     (dict(num_requests=4097), CAPACITY), (dict(max_pages=0), INVALID), (dict(free_capacity=-1), INVALID), (dict(num_tokens=-1), INVALID)):
+        a = _lib.KvPlanArgsC(**{**plan, **kw})
+        assert lib.mars_kv_plan(r.handle, C.byref(a), None) == code, kw
