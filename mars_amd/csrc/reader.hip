@@ -302,11 +302,12 @@ int mars_reader_create(const mars_reader_desc* d, mars_reader** out) try {
             MARS_HIP(hipMemcpy(r->freq, f.data(), size_t(half) * sizeof(uint64_t), hipMemcpyHostToDevice));
             MARS_HIP(hipMemcpy(r->axis, axis.data(), size_t(half) * sizeof(int32_t), hipMemcpyHostToDevice));
         }
-        const size_t slots = size_t(2) * kFewItems;
-        MARS_TRY(dmalloc(&r->part_o, slots * kFewRows * size_t(d->head_dim)));
-        MARS_TRY(dmalloc(&r->part_ml, slots * kFewRows));
-        MARS_TRY(dmalloc(&r->arrived, slots));
-        MARS_HIP(hipMemset(r->arrived, 0, slots * sizeof(uint32_t)));
+        constexpr size_t few = size_t(2) << kFewItemsLog2, many = size_t(2) << kManyItemsLog2;
+        constexpr size_t rows = std::max(few * kFewRows, many * kManyRows);
+        MARS_TRY(dmalloc(&r->part_o, rows * size_t(d->head_dim)));
+        MARS_TRY(dmalloc(&r->part_ml, rows));
+        MARS_TRY(dmalloc(&r->arrived, std::max(few, many)));
+        MARS_HIP(hipMemset(r->arrived, 0, std::max(few, many) * sizeof(uint32_t)));
         MARS_HIP(hipDeviceSynchronize());
         return MARS_OK;
     }();
@@ -423,7 +424,8 @@ int mars_kv_attend(const mars_reader* r, const mars_kv_cache* c, const mars_kv_a
     a.q_stride = s->q_stride; a.out_stride = s->out_stride;
     a.k_stride = c->k_page_stride ? c->k_page_stride : dense;
     a.v_stride = c->v_page_stride ? c->v_page_stride : dense;
-    a.scale_log2 = float(s->cap > 0.0f ? 2.0 * kLog2e * scale / double(s->cap) : kLog2e * scale);
+    a.q_flip = scale < 0.0 ? 0x80008000u : 0u;
+    a.scale_log2 = float(std::fabs(s->cap > 0.0f ? 2.0 * kLog2e * scale / double(s->cap) : kLog2e * scale));
     a.cap_log2 = float(kLog2e * double(s->cap));
     a.requests = s->num_requests; a.max_pages = s->max_pages; a.tokens = s->num_tokens; a.num_pages = c->num_pages;
     a.q_heads = d.q_heads; a.kv_heads = d.kv_heads; a.group = d.q_heads / d.kv_heads;

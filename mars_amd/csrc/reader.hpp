@@ -26,8 +26,11 @@ constexpr int32_t kMaxRequests = MARS_KV_MAX_REQUESTS;
 
 // Keys' work items of a launch: about this many chunks over the cache's length. Partial slots:
 // twice as many (a request longer than a chunk of C keys has at most 2 L / C chunks).
-constexpr int32_t kFewItems = 1024;
+constexpr int32_t kFewItemsLog2 = 10;
 constexpr int32_t kFewRows = 16;
+constexpr int32_t kFewMost = 16;             // rows of a request that k_attend_few serves best
+constexpr int32_t kManyItemsLog2 = 9;
+constexpr int32_t kManyRows = 128;
 constexpr int32_t kMaxSplits = 256;
 
 struct AttendArgs {
@@ -49,15 +52,15 @@ struct AttendArgs {
     float2* part_ml;
     uint32_t* arrived;
     int64_t q_stride, out_stride, k_stride, v_stride;
-    float scale_log2;      // scale * log2(e); with a cap: 2 * log2(e) * scale / cap
+    uint32_t q_flip;       // sign bits of a pair of q's elements if the scale is negative
+    float scale_log2;      // |scale| * log2(e); with a cap: 2 * log2(e) * scale / cap
     float cap_log2;        // cap * log2(e); 0: no cap
     int32_t requests, max_pages, tokens, num_pages;
     int32_t q_heads, kv_heads, group;
     int32_t page_shift;
     int32_t rows_lo, rows_hi;   // this launch serves requests with rows_lo < rows <= rows_hi (rows = tokens * group)
-    int32_t items;              // wanted number of key chunks
 };
 
-int launch_attend(const mars_reader& r, AttendArgs a, int32_t max_new, hipStream_t s);
+int launch_attend(const mars_reader& r, const AttendArgs& a, int32_t max_new, hipStream_t s);
 
 }  // namespace mars
