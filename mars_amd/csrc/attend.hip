@@ -212,38 +212,90 @@ __device__ Item find_item(const AttendArgs& a, uint32_t b, int bm, int min_chunk
     return sh.item;
 }
 
+// Partials pass between workgroups of one launch, on any XCD: as relaxed atomics of agent scope, which go through to
+// where every XCD sees them, the writers' completed before they count themselves in. (Plain stores and a fence at agent
+// scope write back and drop a whole L2 per workgroup: 64 single tokens over 4,096 keys took 497 us so.)
+__device__ inline void put_part(float* p, f32x4 v) {
+    const u32x4 b = __builtin_bit_cast(u32x4, v);
+    __hip_atomic_store(reinterpret_cast<uint64_t*>(p), uint64_t(b[1]) << 32 | b[0], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __hip_atomic_store(reinterpret_cast<uint64_t*>(p) + 1, uint64_t(b[3]) << 32 | b[2], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ inline void put_part(float2* p, float2 v) {
+    __hip_atomic_store(reinterpret_cast<uint64_t*>(p), uint64_t(__float_as_uint(v.y)) << 32 | __float_as_uint(v.x), __ATOMIC_RELAXED,
+                       __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ inline uint64_t get_part(const void* p) {
+    return __hip_atomic_load(static_cast<const uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ inline f32x4 get_part4(const float* p) {
+    const uint64_t lo = get_part(p), hi = get_part(p + 2);
+    return __builtin_bit_cast(f32x4, u32x4{uint32_t(lo), uint32_t(lo >> 32), uint32_t(hi), uint32_t(hi >> 32)});
+}
+__device__ inline float2 get_part2(const float2* p) {
+    const uint64_t v = get_part(p);
+    return make_float2(__uint_as_float(uint32_t(v)), __uint_as_float(uint32_t(v >> 32)));
+}
+
 // Called by every thread of a workgroup that wrote one split's partial: the tile's last workgroup to arrive joins the
-// splits, in their order.
+// splits. Each sum is taken in the order of the splits by one thread, or, where there are few rows, by up to 8
+// threads whose parts are then added in their order: the same bits whoever arrives last.
+template <int BM>
+struct JoinLds {
+    int last;
+    float lpart[8][BM];
+    __attribute__((aligned(16))) float part[8][128 * 4];     // 256 / ways units each
+};
 template <typename T, int D, int BM>
-__device__ void join_splits(const AttendArgs& a, const Item& it, int row0, int n, int& last) {
+__device__ void join_splits(const AttendArgs& a, const Item& it, int row0, int n, JoinLds<BM>& lds) {
     const int tid = int(threadIdx.x);
-    __threadfence();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(kWaitVm0);                    // this wave's stores have reached every XCD's view
     __syncthreads();
-    if (tid == 0) last = atomicAdd(&a.arrived[it.part], 1u) == uint32_t(it.splits - 1);
+    if (tid == 0) lds.last = __hip_atomic_fetch_add(&a.arrived[it.part], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == uint32_t(it.splits - 1);
     __syncthreads();
-    if (!last) return;
-    __threadfence();
-    if (tid == 0) a.arrived[it.part] = 0;
-    const int valid = min(BM, n * a.group - it.tile * BM);
-    for (int e = tid; e < valid * (D / 4); e += 256) {
-        const int rr = e / (D / 4), d4 = e % (D / 4);
-        float top = -kInf;
-        for (int s = 0; s < it.splits; ++s) top = fmaxf(top, a.part_ml[int64_t(it.part + s) * BM + rr].x);
+    if (!lds.last) return;
+    if (tid == 0) __hip_atomic_store(&a.arrived[it.part], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const int valid = min(BM, n * a.group - it.tile * BM), units = valid * (D / 4);
+    int ways = 1;                                            // threads per unit of 4 elements
+    while (ways < 8 && units * ways * 2 <= 256 && ways < it.splits) ways *= 2;
+    const float2* const ml = a.part_ml + int64_t(it.part) * BM;
+    const float* const po = a.part_o + int64_t(it.part) * BM * D;
+    for (int e0 = 0; e0 < units; e0 += 256 / ways) {
+        const int w = tid / (256 / ways), e = e0 + tid % (256 / ways), rr = e / (D / 4), d4 = e % (D / 4);
         f32x4 sum = {0, 0, 0, 0};
-        float lsum = 0.0f;
-        for (int s = 0; s < it.splits; ++s) {
-            const float2 p = a.part_ml[int64_t(it.part + s) * BM + rr];
-            const float w = p.x == -kInf ? 0.0f : __builtin_amdgcn_exp2f(p.x - top);
-            lsum += w * p.y;
-            sum += w * *reinterpret_cast<const f32x4*>(a.part_o + (int64_t(it.part + s) * BM + rr) * D + d4 * 4);
+        float lsum = 0.0f, top = -kInf;
+        if (e < units) {
+#pragma unroll 4
+            for (int s = 0; s < it.splits; ++s) top = fmaxf(top, get_part2(ml + s * BM + rr).x);
+#pragma unroll 4
+            for (int s = w; s < it.splits; s += ways) {
+                const float2 p = get_part2(ml + s * BM + rr);
+                const float f = p.x == -kInf ? 0.0f : __builtin_amdgcn_exp2f(p.x - top);
+                lsum += f * p.y;
+                sum += f * get_part4(po + (int64_t(s) * BM + rr) * D + d4 * 4);
+            }
         }
-        const int mm = it.tile * BM + rr, ii = mm / a.group, hh = it.head * a.group + mm - ii * a.group;
-        const float inv = 1.0f / lsum;
-        T* const op = static_cast<T*>(a.out) + (int64_t(row0) + ii) * a.out_stride + int64_t(hh) * D + d4 * 4;
+        if (ways > 1) {                                      // units fit one round then
+            float* const mine = &lds.part[w][0];
+            *reinterpret_cast<f32x4*>(mine + (tid % (256 / ways)) * 4) = sum;
+            if (d4 == 0 && e < units) lds.lpart[w][rr] = lsum;
+            __syncthreads();
+            if (w == 0 && e < units) {
+                lsum = 0.0f;
+                for (int v = 0; v < ways; ++v) lsum += lds.lpart[v][rr];
+                for (int v = 1; v < ways; ++v) sum += *reinterpret_cast<const f32x4*>(&lds.part[v][tid * 4]);
+            }
+        }
+        if (w == 0 && e < units) {
+            const int mm = it.tile * BM + rr, ii = mm / a.group, hh = it.head * a.group + mm - ii * a.group;
+            const float inv = 1.0f / lsum;
+            typename Vec<T>::v4 o;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) op[j] = top == -kInf ? T(0.0f) : T(sum[j] * inv);
-        if (a.lse && d4 == 0)
-            a.lse[(int64_t(row0) + ii) * a.q_heads + hh] = top == -kInf ? -kInf : (top + __builtin_amdgcn_logf(lsum)) * kLn2;
+            for (int j = 0; j < 4; ++j) o[j] = top == -kInf ? T(0.0f) : T(sum[j] * inv);
+            *reinterpret_cast<typename Vec<T>::v4*>(static_cast<T*>(a.out) + (int64_t(row0) + ii) * a.out_stride + int64_t(hh) * D + d4 * 4) = o;
+            if (a.lse && d4 == 0)
+                a.lse[(int64_t(row0) + ii) * a.q_heads + hh] = top == -kInf ? -kInf : (top + __builtin_amdgcn_logf(lsum)) * kLn2;
+        }
     }
 }
 
@@ -274,48 +326,48 @@ __device__ void add_not_finite(const AttendArgs& a, const Item& it, int row0, in
             T* const o = static_cast<T*>(a.out) + row * a.out_stride + int64_t(hq) * D + d;
             *o = T(float(*o) + sum);
         } else {
-            a.part_o[(int64_t(it.part + it.split) * BM + rr) * D + d] += sum;
+            float* const o = a.part_o + (int64_t(it.part + it.split) * BM + rr) * D + d;
+            const float was = __hip_atomic_load(o, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            __hip_atomic_store(o, was + sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
     }
 }
 
 // ---- few rows: 16 at a time, keys straight from the cache to registers -----------------
-// Bound by the cache's bytes. 4 waves take the 32-key steps of the chunk in turn; a wave reads
-// its step's K and V rows into registers (16 bytes a lane) one step ahead, so that 12 waves of
-// a CU keep some 100 KB of loads in flight, and the waves' sums are joined at the end.
-template <typename T, int D>
-__global__ __launch_bounds__(256) void k_attend_few(AttendArgs a) {
+// Bound by the cache's bytes. 4 waves take the steps of the chunk in turn (64 keys; 32 for heads of 256), and a wave
+// keeps its next step's K and V on the way to registers (16 bytes a lane; whole 128-byte lines, from K rows over the
+// elements and from V rows over the step's keys) while it computes this one: 8 waves of a CU have up to 256 KB in
+// flight. The waves' sums are joined at the end.
+template <typename T, int D, bool EXTRA>
+__global__ __launch_bounds__(256, D > 128 ? 1 : 2) void k_attend_few(AttendArgs a) {
     using V = typename Vec<T>::v8;
-    constexpr int KC = D / 32, VB = D / 16;
-    __shared__ SchedLds sched;
-    __shared__ float ml[4][16][2];
-    __shared__ __attribute__((aligned(16))) float ob[2][16][D + 4];
-    __shared__ int arrived_last, any_dirty;
+    constexpr int KC = D / 32, VB = D / 16, NH = D > 128 ? 1 : 2, STEP = 32 * NH;      // NH: halves of 32 keys in a step
+    __shared__ union {
+        SchedLds sched;
+        struct { float ml[4][16][2]; __attribute__((aligned(16))) float ob[2][16][D + 4]; } wave;
+        JoinLds<kFewRows> join;
+    } lds;
+    __shared__ int any_dirty;
     if (threadIdx.x == 0) any_dirty = 0;
-    const Item it = find_item(a, blockIdx.x, kFewRows, 256, kFewItemsLog2, sched);
+    const Item it = find_item(a, blockIdx.x, kFewRows, 256, kFewItemsLog2, lds.sched);
     if (!it.found) return;
     const int tid = int(threadIdx.x), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 15, h = lane >> 4;
-    const int r = it.request, P1 = (1 << a.page_shift) - 1;
+    const int r = __builtin_amdgcn_readfirstlane(it.request), head = __builtin_amdgcn_readfirstlane(it.head);
+    const int P1 = (1 << a.page_shift) - 1;
     const int row0 = max(a.q_start[r], 0), n = min(a.q_start[r + 1], a.tokens) - row0;
     const int keys = int(min(int64_t(max(a.kv_lens[r], 0)), int64_t(a.max_pages) << a.page_shift));
     const int m = it.tile * kFewRows + col;                 // this lane's row: token i, head of the group
     const bool row_ok = m < n * a.group;
-    const int i = row_ok ? m / a.group : 0, hq = it.head * a.group + (row_ok ? m - i * a.group : 0);
+    const int i = row_ok ? m / a.group : 0, hq = head * a.group + (row_ok ? m - i * a.group : 0);
     const int64_t row = int64_t(row0) + i;
     const int prefix = a.prefix ? min(max(a.prefix[r], 0), keys) : 0;
     const int limit = row_ok ? min(max(keys - n + i + 1, prefix), keys) : 0;   // keys [0, limit) may be seen
-    const float dec = a.decay ? a.decay[hq] * 1.4426950408889634f : 0.0f;
-    const float tq = a.decay ? a.q_times[row] : 0.0f;
-    const int eq = a.q_eps ? a.q_eps[row] : -1;
+    const float dec = EXTRA && a.decay ? a.decay[hq] * 1.4426950408889634f : 0.0f;
+    const float tq = EXTRA && a.decay ? a.q_times[row] : 0.0f;
+    const int eq = EXTRA && a.q_eps ? a.q_eps[row] : -1;
 
-    V q[KC];
-    const T* const qp = static_cast<const T*>(a.q) + row * a.q_stride + int64_t(hq) * D + h * 8;
-#pragma unroll
-    for (int c = 0; c < KC; ++c) q[c] = load_q<V>(qp + c * 32, a.q_flip);
-
-    int lo = limit, hi = limit;                             // over the wave's rows
-    if (!row_ok) lo = INT32_MAX;
+    int lo = row_ok ? limit : INT32_MAX, hi = limit;        // over the rows
 #pragma unroll
     for (int o = 1; o < 16; o <<= 1) {
         lo = min(lo, __shfl_xor(lo, o));
@@ -323,84 +375,114 @@ __global__ __launch_bounds__(256) void k_attend_few(AttendArgs a) {
     }
     lo = __builtin_amdgcn_readfirstlane(lo);
     hi = __builtin_amdgcn_readfirstlane(hi);
-    const int k0 = it.split * it.chunk, k1 = min(k0 + it.chunk, hi);
-    const int steps = k1 > k0 ? (k1 - k0 + 31) >> 5 : 0;
+    const int k0 = __builtin_amdgcn_readfirstlane(it.split * it.chunk), k1 = min(k0 + __builtin_amdgcn_readfirstlane(it.chunk), hi);
+    const int steps = k1 > k0 ? (k1 - k0 + STEP - 1) / STEP : 0;
 
-    const int32_t* const table = a.table + int64_t(r) * a.max_pages;
+    const TablePtr table = table_row(a, r);
     const int last_page = keys > 0 ? (keys - 1) >> a.page_shift : 0;
-    const int ki = 8 * (col >> 2) + (col & 3);              // key of A row `col`, first block (the second: + 4)
-    const T* const kp = static_cast<const T*>(a.k_pages) + (int64_t(it.head) << a.page_shift) * D + h * 8;
-    const T* const vp = static_cast<const T*>(a.v_pages) + (int64_t(it.head) << a.page_shift) * D + (int64_t(col) << a.page_shift);
-    auto page_at = [&](int key) {
-        const int id = table[min(key >> a.page_shift, last_page)];
-        return uint32_t(id) < uint32_t(a.num_pages) ? id : 0;
+    // K: A row `col` of block b holds key 8 (col / 4) + 4 b + col % 4 of 32, so that registers 4 b + j of S hold key 8 h + 4 b + j
+    const int kg = col >> 3, kin = 8 * ((col >> 2) & 1) + (col & 3);             // group of 16 keys, key within it (b = 0)
+    const T* const kp = static_cast<const T*>(a.k_pages) + ((int64_t(head) << a.page_shift) + kin) * D + h * 8;
+    const T* const vp = static_cast<const T*>(a.v_pages) + ((int64_t(head) * D + col) << a.page_shift) + (h & 1) * 8;
+    int pages[2 * NH], v_pages[2 * NH];                     // of the step on the way: K's, and (loaded later) V's
+    auto find_pages = [&](int s) {
+#pragma unroll
+        for (int u = 0; u < 2 * NH; ++u) pages[u] = page_of(a, table, k0 + s * STEP + u * 16, last_page);
     };
-    V kf[2][KC], vf[VB];
-    f32x4 tk[2];
-    i32x4 ek[2];
+    V kf[NH][2][KC], vf[NH][VB];
+    f32x4 tk[NH][2];
+    i32x4 ek[NH][2];
     auto load_k = [&](int s) {
-        const int key = k0 + s * 32 + ki;
-        const T* const p = kp + page_at(key) * a.k_stride + int64_t(key & P1) * D;
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
+        for (int b2 = 0; b2 < NH; ++b2) {
+            const int kt = k0 + s * STEP + b2 * 32;
+            const int64_t o0 = pages[2 * b2] * a.k_stride + int64_t(kt & P1) * D, o1 = pages[2 * b2 + 1] * a.k_stride + int64_t((kt + 16) & P1) * D;
+            const T* const p = kp + (kg ? o1 : o0);
 #pragma unroll
-            for (int c = 0; c < KC; ++c) kf[b][c] = load16<V>(p + b * 4 * D + c * 32);
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int c = 0; c < KC; ++c) kf[b2][b][c] = load16<V>(p + b * 4 * D + c * 32);
+        }
     };
     auto load_v = [&](int s) {
-        const int key = k0 + s * 32 + h * 8, pg = page_at(key);
-        const T* const p = vp + pg * a.v_stride + (key & P1);
 #pragma unroll
-        for (int d = 0; d < VB; ++d) vf[d] = load16<V>(p + (int64_t(d) * 16 << a.page_shift));
-        const int64_t slot = (int64_t(pg) << a.page_shift) + (key & P1);
-        if (a.k_times) { tk[0] = *reinterpret_cast<const f32x4*>(a.k_times + slot); tk[1] = *reinterpret_cast<const f32x4*>(a.k_times + slot + 4); }
-        if (a.k_eps) { ek[0] = *reinterpret_cast<const i32x4*>(a.k_eps + slot); ek[1] = *reinterpret_cast<const i32x4*>(a.k_eps + slot + 4); }
+        for (int b2 = 0; b2 < NH; ++b2) {
+            const int kt = k0 + s * STEP + b2 * 32, a0 = kt & P1, a1 = (kt + 16) & P1;
+            const T* const p = vp + (h & 2 ? v_pages[2 * b2 + 1] * a.v_stride + a1 : v_pages[2 * b2] * a.v_stride + a0);
+#pragma unroll
+            for (int d = 0; d < VB; ++d) vf[b2][d] = load16<V>(p + (int64_t(d) * 16 << a.page_shift));
+            const int64_t slot = (int64_t(h & 2 ? v_pages[2 * b2 + 1] : v_pages[2 * b2]) << a.page_shift) + (h & 2 ? a1 : a0) + (h & 1) * 8;
+            if (EXTRA && a.k_times) { tk[b2][0] = *reinterpret_cast<const f32x4*>(a.k_times + slot); tk[b2][1] = *reinterpret_cast<const f32x4*>(a.k_times + slot + 4); }
+            if (EXTRA && a.k_eps) { ek[b2][0] = *reinterpret_cast<const i32x4*>(a.k_eps + slot); ek[b2][1] = *reinterpret_cast<const i32x4*>(a.k_eps + slot + 4); }
+        }
     };
 
+    if (wave < steps) find_pages(wave);
+    V q[KC];
+    const T* const qp = static_cast<const T*>(a.q) + row * a.q_stride + int64_t(hq) * D + h * 8;
+#pragma unroll
+    for (int c = 0; c < KC; ++c) q[c] = load_q<V>(qp + c * 32, a.q_flip);
     f32x4 o[VB];
 #pragma unroll
     for (int d = 0; d < VB; ++d) o[d] = f32x4{0, 0, 0, 0};
     float mref = 0.0f, mtop = -kInf, l = 0.0f;              // mtop: -inf until the row has seen a key, then mref + kSlack
     bool dirty = false;                                     // a value that is not finite was left out
 
-    if (wave < steps) { load_k(wave); load_v(wave); }
+    auto keep_pages = [&] {
+#pragma unroll
+        for (int u = 0; u < 2 * NH; ++u) v_pages[u] = pages[u];
+    };
+    if (wave < steps) {
+        load_k(wave);
+        keep_pages();
+        load_v(wave);
+        find_pages(wave + 4);
+    }
     for (int s = wave; s < steps; s += 4) {
-        const int kb = k0 + s * 32 + h * 8;                 // this lane's 8 keys
-        f32x4 acc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+        const int ks = k0 + s * STEP;
+        f32x4 acc[NH][2];
 #pragma unroll
-        for (int c = 0; c < KC; ++c) {
-            acc[0] = Vec<T>::mma(kf[0][c], q[c], acc[0]);
-            acc[1] = Vec<T>::mma(kf[1][c], q[c], acc[1]);
+        for (int b2 = 0; b2 < NH; ++b2)
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                acc[b2][b] = f32x4{0, 0, 0, 0};
+#pragma unroll
+                for (int c = 0; c < KC; ++c) acc[b2][b] = Vec<T>::mma(kf[b2][b][c], q[c], acc[b2][b]);
+            }
+        const bool more = s + 4 < steps;
+        if (more) {
+            load_k(s + 4);
+            keep_pages();
+            find_pages(s + 8);
         }
-        if (s + 4 < steps) load_k(s + 4);
-        float x[8];
+        // x[8 b2 + j]: this lane's key ks + 32 b2 + 8 h + j
+        float x[8 * NH];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = acc[j >> 2][j & 3] * a.scale_log2;
-        if (a.cap_log2 != 0.0f) {
+        for (int j = 0; j < 8 * NH; ++j) x[j] = acc[j >> 3][(j >> 2) & 1][j & 3] * a.scale_log2;
+        if (EXTRA && a.cap_log2 != 0.0f) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
+            for (int j = 0; j < 8 * NH; ++j)
                 x[j] = a.cap_log2 * (1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x[j])));
         }
-        if (a.k_times) {
+        if (EXTRA && a.k_times) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] -= dec * fmaxf(0.0f, tq - tk[j >> 2][j & 3]);
+            for (int j = 0; j < 8 * NH; ++j) x[j] -= dec * fmaxf(0.0f, tq - tk[j >> 3][(j >> 2) & 1][j & 3]);
         }
-        uint32_t seen = 0xFFu;
-        const bool whole = k0 + s * 32 + 32 <= lo && !a.k_eps;
+        const bool whole = ks + STEP <= lo && !(EXTRA && a.k_eps);
         if (!whole) {
-            seen = kb >= limit ? 0u : (kb + 8 <= limit ? 0xFFu : (1u << (limit - kb)) - 1u);
-            if (a.k_eps) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const int e = ek[j >> 2][j & 3];
-                    if (!(e < 0 || eq < 0 || e == eq)) seen &= ~(1u << j);
+            for (int j = 0; j < 8 * NH; ++j) {
+                bool in = ks + 32 * (j >> 3) + 8 * h + (j & 7) < limit;
+                if (EXTRA && a.k_eps) {
+                    const int e = ek[j >> 3][(j >> 2) & 1][j & 3];
+                    in = in && (e < 0 || eq < 0 || e == eq);
                 }
+                x[j] = in ? x[j] : -kInf;
             }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = (seen >> j) & 1u ? x[j] : -kInf;
         }
         float top = x[0];
 #pragma unroll
-        for (int j = 1; j < 8; ++j) top = fmaxf(top, x[j]);
+        for (int j = 1; j < 8 * NH; ++j) top = fmaxf(top, x[j]);
         if (__any(top > mtop)) {
             top = fmaxf(top, __shfl_xor(top, 16));
             top = fmaxf(top, __shfl_xor(top, 32));
@@ -415,40 +497,48 @@ __global__ __launch_bounds__(256) void k_attend_few(AttendArgs a) {
                 for (int d = 0; d < VB; ++d) o[d] *= f;
             }
         }
-        V p;
+        V p[NH];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
+        for (int j = 0; j < 8 * NH; ++j) {
             const float w = __builtin_amdgcn_exp2f(x[j] - mref);
             l += w;
-            p[j] = T(w);
+            p[j >> 3][j & 7] = T(w);
         }
-        if (whole) {
-#pragma unroll
-            for (int d = 0; d < VB; ++d) o[d] = Vec<T>::mma(vf[d], p, o[d]);
-        } else {
+        if (!whole) {
             // some row does not see some key: see add_not_finite. Slots past the request's keys hold anything.
             uint32_t odd = 0;
 #pragma unroll
-            for (int d = 0; d < VB; ++d) {
-                u32x4 b = __builtin_bit_cast(u32x4, vf[d]);
-                if (kb + 8 > keys) {
+            for (int b2 = 0; b2 < NH; ++b2) {
+                const int kb = ks + 32 * b2 + 8 * h;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) b[j] &= kb + 2 * j >= keys ? 0u : kb + 2 * j + 1 >= keys ? 0xFFFFu : ~0u;
+                for (int d = 0; d < VB; ++d) {
+                    u32x4 b = __builtin_bit_cast(u32x4, vf[b2][d]);
+                    if (kb + 8 > keys) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) b[j] &= kb + 2 * j >= keys ? 0u : kb + 2 * j + 1 >= keys ? 0xFFFFu : ~0u;
+                    }
+                    const uint32_t full = exponents_full<T>(b);
+                    odd |= full;
+                    if (__any(full != 0)) b = finite_part<T>(b);
+                    vf[b2][d] = __builtin_bit_cast(V, b);
                 }
-                const uint32_t full = exponents_full<T>(b);
-                odd |= full;
-                if (__any(full != 0)) b = finite_part<T>(b);
-                o[d] = Vec<T>::mma(__builtin_bit_cast(V, b), p, o[d]);
             }
             if (__any(odd != 0)) dirty = true;
         }
-        if (s + 4 < steps) load_v(s + 4);
+#pragma unroll
+        for (int b2 = 0; b2 < NH; ++b2)
+#pragma unroll
+            for (int d = 0; d < VB; ++d) o[d] = Vec<T>::mma(vf[b2][d], p[b2], o[d]);
+        if (more) load_v(s + 4);
     }
 
     // join the waves: references first, then sums and O, in wave order
+    auto& ml = lds.wave.ml;
+    auto& ob = lds.wave.ob;
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
     float mw = mtop == -kInf ? -kInf : mref;
+    __syncthreads();                                        // the item has been read
     if (h == 0) ml[wave][col][0] = mw;
     if (dirty && lane == 0) any_dirty = 1;
     __syncthreads();
@@ -484,16 +574,19 @@ __global__ __launch_bounds__(256) void k_attend_few(AttendArgs a) {
             const float inv = mall == -kInf ? 0.0f : 1.0f / lall;
             T* const op = static_cast<T*>(a.out) + row * a.out_stride + int64_t(hq) * D + h * 4;
 #pragma unroll
-            for (int d = 0; d < VB; ++d)
+            for (int d = 0; d < VB; ++d) {
+                typename Vec<T>::v4 w;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) op[d * 16 + j] = mall == -kInf ? T(0.0f) : T(o[d][j] * inv);
+                for (int j = 0; j < 4; ++j) w[j] = mall == -kInf ? T(0.0f) : T(o[d][j] * inv);
+                *reinterpret_cast<typename Vec<T>::v4*>(op + d * 16) = w;
+            }
             if (a.lse && h == 0) a.lse[row * a.q_heads + hq] = mall == -kInf ? -kInf : (mall + __builtin_amdgcn_logf(lall)) * kLn2;
         }
         if (row_ok && joined) {
             float* const po = a.part_o + (int64_t(it.part + it.split) * kFewRows + col) * D + h * 4;
 #pragma unroll
-            for (int d = 0; d < VB; ++d) *reinterpret_cast<f32x4*>(po + d * 16) = o[d];
-            if (h == 0) a.part_ml[int64_t(it.part + it.split) * kFewRows + col] = make_float2(mall, lall);
+            for (int d = 0; d < VB; ++d) put_part(po + d * 16, o[d]);
+            if (h == 0) put_part(a.part_ml + int64_t(it.part + it.split) * kFewRows + col, make_float2(mall, lall));
         }
     }
     if (any_dirty) {
@@ -501,7 +594,8 @@ __global__ __launch_bounds__(256) void k_attend_few(AttendArgs a) {
         add_not_finite<T, D, kFewRows>(a, it, row0, n, keys, prefix, k0, min(k0 + it.chunk, keys));
     }
     if (!joined) return;
-    join_splits<T, D, kFewRows>(a, it, row0, n, arrived_last);
+    __syncthreads();
+    join_splits<T, D, kFewRows>(a, it, row0, n, lds.join);
 }
 
 // ---- many rows: 128 at a time, keys staged through LDS ----------------------------------
@@ -525,7 +619,7 @@ template <typename T, int D, bool EXTRA>
 __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void k_attend_many(AttendArgs a) {
     using V = typename Vec<T>::v8;
     constexpr int KS = D / 16, DB = D / 32, RC = D / 8;      // k-steps of S, blocks of O, 16-byte pieces of a key's row
-    __shared__ __attribute__((aligned(16))) union { ManyLds<D> tiles; SchedLds sched; int last; } lds;
+    __shared__ __attribute__((aligned(16))) union { ManyLds<D> tiles; SchedLds sched; JoinLds<kManyRows> join; } lds;
     ManyLds<D>& sh = lds.tiles;
     const Item it = find_item(a, blockIdx.x, kManyRows, 256, kManyItemsLog2, lds.sched);
     if (!it.found) return;
@@ -775,26 +869,26 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void k_attend_many(AttendArgs
         for (int d = 0; d < DB; ++d)
 #pragma unroll
             for (int g = 0; g < 4; ++g)
-                *reinterpret_cast<f32x4*>(po + d * 32 + g * 8) = f32x4{o[d][g * 4], o[d][g * 4 + 1], o[d][g * 4 + 2], o[d][g * 4 + 3]};
-        if (h == 0) a.part_ml[at] = make_float2(empty ? -kInf : mref, l);
+                put_part(po + d * 32 + g * 8, f32x4{o[d][g * 4], o[d][g * 4 + 1], o[d][g * 4 + 2], o[d][g * 4 + 3]});
+        if (h == 0) put_part(a.part_ml + at, make_float2(empty ? -kInf : mref, l));
     }
     __syncthreads();                                         // the LDS of the tiles is free, the rows are written
-    if (tid == 0) lds.last = 0;
+    if (tid == 0) lds.join.last = 0;
     __syncthreads();
-    if (dirty) lds.last = 1;
+    if (dirty) lds.join.last = 1;
     __syncthreads();
-    if (lds.last) add_not_finite<T, D, kManyRows>(a, it, row0, n, keys, prefix, k0, min(k0 + it.chunk, keys));
+    if (lds.join.last) add_not_finite<T, D, kManyRows>(a, it, row0, n, keys, prefix, k0, min(k0 + it.chunk, keys));
     if (it.splits == 1) return;
     __syncthreads();
-    join_splits<T, D, kManyRows>(a, it, row0, n, lds.last);
+    join_splits<T, D, kManyRows>(a, it, row0, n, lds.join);
 }
 
-template <typename T, int D>
+template <typename T, int D, bool EXTRA>
 int launch_few(AttendArgs a, hipStream_t s) {
     const int64_t tiles = int64_t(a.tokens) * a.group / kFewRows + std::min(a.requests, a.tokens);
     const int64_t grid = (1 << kFewItemsLog2) + tiles * a.kv_heads;
     MARS_CHECK(grid <= INT32_MAX, MARS_ERR_CAPACITY, "%lld tiles of rows", (long long)grid);
-    MARS_LAUNCH((k_attend_few<T, D>), dim3(unsigned(grid)), dim3(256), 0, s, a);
+    MARS_LAUNCH((k_attend_few<T, D, EXTRA>), dim3(unsigned(grid)), dim3(256), 0, s, a);
     return MARS_OK;
 }
 
@@ -814,16 +908,17 @@ int launch_dim(AttendArgs a, int32_t max_new, hipStream_t s) {
     // a request that breaks the bound is served by the other kernel.
     const int64_t most = std::min<int64_t>(max_new > 0 ? max_new : a.tokens, a.tokens) * a.group;
     const bool few_only = most <= kFewMost, many_only = !few_only && a.requests == 1;
+    const bool extra = a.cap_log2 != 0.0f || a.k_times || a.k_eps;
     if (!many_only) {
         AttendArgs f = a;
         f.rows_lo = 0;
         f.rows_hi = few_only ? INT32_MAX : kFewMost;
-        MARS_TRY((launch_few<T, D>(f, s)));
+        if (extra) MARS_TRY((launch_few<T, D, true>(f, s)));
+        else MARS_TRY((launch_few<T, D, false>(f, s)));
     }
     if (!few_only) {
         a.rows_lo = many_only ? 0 : kFewMost;
         a.rows_hi = INT32_MAX;
-        const bool extra = a.cap_log2 != 0.0f || a.k_times || a.k_eps;
         if (extra) MARS_TRY((launch_many<T, D, true>(a, s)));
         else MARS_TRY((launch_many<T, D, false>(a, s)));
     }
