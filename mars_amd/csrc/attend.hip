@@ -115,18 +115,37 @@ __device__ inline int page_of(const AttendArgs& a, TablePtr table, int key, int 
     return uint32_t(id) < uint32_t(a.num_pages) ? id : 0;
 }
 
-// One unit of a launch's work: a tile of rows of a request under one kv head, over a range of its keys.
-struct Item {
-    int32_t request, tile, head, split, splits, chunk;
-    int32_t part;              // first partial slot of the tile's splits
-    int32_t tiles;             // of the request
-    bool found;
+// A piece of a launch's work: a tile of rows of a request under one kv head, over the keys [k0, k1). Where several pieces
+// share the tile (splits > 1), each writes a partial: piece 0 to slot0, piece i > 0 to slot1 + (i - 1) * slot_step.
+struct Part {
+    int32_t request, tile, head;
+    int32_t row0, n, keys;     // the request's first row, its new tokens, its keys
+    int32_t k0, k1;
+    int32_t chunk;             // keys of a piece (k_attend_many)
+    int32_t splits, slot, slot0, slot1, slot_step;
+    __device__ int slot_of(int i) const { return i == 0 ? slot0 : slot1 + (i - 1) * slot_step; }
 };
 
 struct SchedLds {
+    int64_t sum[3][4];
     uint64_t wsum[4];
-    Item item;
+    Part part;
+    bool found;
 };
+
+__device__ inline int64_t uniform(int64_t v) {
+    return int64_t(uint64_t(uint32_t(__builtin_amdgcn_readfirstlane(int(uint64_t(v) >> 32)))) << 32 | uint32_t(__builtin_amdgcn_readfirstlane(int(v))));
+}
+
+// The same part in scalar registers (all threads read one copy).
+__device__ inline Part uniform_part(const Part& p) {
+    Part q;
+    const int32_t* const from = reinterpret_cast<const int32_t*>(&p);
+    int32_t* const to = reinterpret_cast<int32_t*>(&q);
+#pragma unroll
+    for (int i = 0; i < int(sizeof(Part) / 4); ++i) to[i] = __builtin_amdgcn_readfirstlane(from[i]);
+    return q;
+}
 
 __device__ inline int64_t wave_sum(int64_t v) {
 #pragma unroll
@@ -134,46 +153,67 @@ __device__ inline int64_t wave_sum(int64_t v) {
     return v;
 }
 
-// Rows of request r that this launch serves, in tiles of `bm`, and its keys.
-__device__ inline void request_of(const AttendArgs& a, int r, int bm, int* tiles, int* keys) {
-    *tiles = 0;
-    *keys = 0;
-    if (r >= a.requests) return;
-    const int n = max(0, min(a.q_start[r + 1], a.tokens) - max(a.q_start[r], 0));
-    const int rows = n * a.group;
-    if (rows <= a.rows_lo || rows > a.rows_hi) return;
-    *tiles = (rows + bm - 1) / bm;
-    *keys = int(min(int64_t(max(a.kv_lens[r], 0)), int64_t(a.max_pages) << a.page_shift));
+// Request r, its rows in tiles of `bm`, and its keys; no tiles if the other of the two kernels serves it: requests of up
+// to a.few_rows rows are k_attend_few's.
+struct Request { int row0, n, tiles, keys; };
+template <bool FEW>
+__device__ inline Request request_of(const AttendArgs& a, int r) {
+    constexpr int bm = FEW ? kFewRows : kManyRows;
+    Request q{0, 0, 0, 0};
+    if (r >= a.requests) return q;
+    const int start = a.q_start[r], end = a.q_start[r + 1], len = a.kv_lens[r];
+    q.row0 = max(start, 0);
+    q.n = max(0, min(end, a.tokens) - q.row0);
+    const int rows = q.n * a.group;
+    if ((rows <= a.few_rows) != FEW) return q;
+    q.tiles = (rows + bm - 1) / bm;
+    q.keys = int(min(int64_t(max(len, 0)), int64_t(a.max_pages) << a.page_shift));
+    return q;
 }
 
-// Workgroup b's item, from the lengths alone: every workgroup of 256 threads sums the launch's work (key steps of 32
-// over all tiles), cuts the keys into chunks of work / 2^items_log2, and finds the request that its number falls to. The
-// launch has enough workgroups for every item (fewer than 2^31); the last ones may find none.
-__device__ Item find_item(const AttendArgs& a, uint32_t b, int bm, int min_chunk, int items_log2, SchedLds& sh) {
+// Workgroup b's item of k_attend_many, from the lengths alone: every workgroup of 256 threads sums the launch's tiles
+// and work (key steps of 32 over all tiles), cuts the keys into chunks, and finds the request that its number falls to.
+// Where there are fewer tiles than three quarters of the workgroups that the CUs hold, chunks of a 2^9-th of all the
+// tiles' keys (2 x 511 tokens over 2,500 keys, 256 tiles: 77 us, 104 us whole); with more tiles, no chunk has to be
+// smaller than a CU's share of the work (768 tiles of causal rows up to 4,001 keys: 112 us whole, 144 us cut once).
+// A tile has at most 2 L / C chunks where it has two, and C is at least sum(L) / 2^9 by either rule: 2^10 partial slots.
+// The launch has enough workgroups for every item (fewer than 2^31); the last ones may find none. JOIN: the items are
+// the blocks of kJoinRows rows of the tiles in several pieces instead, the block's number in Part::slot.
+template <bool JOIN>
+__device__ bool find_item(const AttendArgs& a, uint32_t b, SchedLds& sh) {
     const int tid = int(threadIdx.x), lane = tid & 63, wave = tid >> 6;
-    int tiles0 = 0, keys0 = 0;
-    int64_t work = 0;
-    for (int r0 = 0; r0 < a.requests; r0 += 256) {
-        int tiles, keys;
-        request_of(a, r0 + tid, bm, &tiles, &keys);
-        if (r0 == 0) { tiles0 = tiles; keys0 = keys; }
-        work += int64_t(tiles) * ((keys + 31) >> 5);
-    }
-    work = wave_sum(work);
-    if (lane == 0) sh.wsum[wave] = uint64_t(work);
-    if (tid == 0) sh.item.found = false;
+    const Request first = request_of<false>(a, tid);
+    // the rows of a tile see L - n / 2 keys on average (not less than half of the L keys)
+    int64_t full = 0, mean = 0, tiles_sum = 0;
+    auto add = [&](const Request& q) {
+        full += int64_t(q.tiles) * ((q.keys + 31) >> 5);
+        mean += int64_t(q.tiles) * ((max(q.keys - q.n / 2, q.keys / 2) + 31) >> 5);
+        tiles_sum += q.tiles;
+    };
+    add(first);
+    for (int r0 = 256; r0 < a.requests; r0 += 256) add(request_of<false>(a, r0 + tid));
+    full = wave_sum(full);
+    mean = wave_sum(mean);
+    tiles_sum = wave_sum(tiles_sum);
+    if (lane == 0) { sh.sum[0][wave] = full; sh.sum[1][wave] = mean; sh.sum[2][wave] = tiles_sum; }
+    if (tid == 0) sh.found = false;
     __syncthreads();
-    work = int64_t(sh.wsum[0] + sh.wsum[1] + sh.wsum[2] + sh.wsum[3]) * a.kv_heads;
-    const int64_t per = (work * 32 + (int64_t(1) << items_log2) - 1) >> items_log2;
-    const uint32_t chunk0 = (uint32_t(min(max(per, int64_t(min_chunk)), int64_t(INT32_MAX) - 255)) + 255) & ~255u;
+    int64_t sums[3];
+#pragma unroll
+    for (int x = 0; x < 3; ++x) sums[x] = (sh.sum[x][0] + sh.sum[x][1] + sh.sum[x][2] + sh.sum[x][3]) * a.kv_heads;
+    if (sums[2] == 0) return false;
+    constexpr int64_t slots = 1 << kManyItemsLog2;
+    const int64_t per = sums[2] < slots * 3 / 4 ? (sums[0] * 32 + slots - 1) / slots : (sums[1] * 64 + slots - 1) / slots;
+    const uint32_t chunk0 = (uint32_t(min(max(per, int64_t(kMinChunk)), int64_t(INT32_MAX) - 255)) + 255) & ~255u;
     uint32_t items_before = 0, parts_before = 0;
     for (int r0 = 0; r0 < a.requests; r0 += 256) {
-        int tiles = tiles0, keys = keys0;
-        if (r0) request_of(a, r0 + tid, bm, &tiles, &keys);
+        const Request q = r0 ? request_of<false>(a, r0 + tid) : first;
+        const int tiles = q.tiles, keys = q.keys;
         // no more than kMaxSplits chunks a request
         const uint32_t chunk = max(chunk0, (uint32_t(keys) + kMaxSplits * 256 - 1) / (kMaxSplits * 256) * 256);
         const uint32_t splits = max(1u, (uint32_t(keys) + chunk - 1) / chunk);
-        const uint32_t items = uint32_t(tiles) * uint32_t(a.kv_heads) * splits, parts = splits > 1 ? items : 0;
+        const uint32_t heads = uint32_t(tiles) * uint32_t(a.kv_heads), parts = splits > 1 ? heads * splits : 0;
+        const uint32_t each = JOIN ? (splits > 1 ? kManyRows / kJoinRows : 0) : splits, items = heads * each;
         uint32_t xi = items, xp = parts;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
@@ -193,32 +233,38 @@ __device__ Item find_item(const AttendArgs& a, uint32_t b, int bm, int min_chunk
         }
         const uint32_t mine = bi + xi - items;
         if (b >= mine && b - mine < items) {
-            const uint32_t local = b - mine, tile_head = local / splits, tile = tile_head / uint32_t(a.kv_heads);
-            Item it;
-            it.request = r0 + tid;
-            it.split = int32_t(local - tile_head * splits);
-            it.tile = int32_t(tile);
-            it.head = int32_t(tile_head - tile * uint32_t(a.kv_heads));
-            it.splits = int32_t(splits);
-            it.chunk = int32_t(min(chunk, uint32_t(INT32_MAX / 2)));
-            it.part = int32_t(bp + xp - parts + tile_head * splits);
-            it.tiles = tiles;
-            it.found = true;
-            sh.item = it;
+            const uint32_t local = b - mine, tile_head = local / each, tile = tile_head / uint32_t(a.kv_heads);
+            const int32_t split = int32_t(local - tile_head * each), c = int32_t(min(chunk, uint32_t(INT32_MAX / 2)));
+            Part& pt = sh.part;
+            pt.request = r0 + tid;
+            pt.tile = int32_t(uint32_t(tiles) - 1 - tile);   // later rows see more keys: first
+            pt.head = int32_t(tile_head - tile * uint32_t(a.kv_heads));
+            pt.row0 = q.row0;
+            pt.n = q.n;
+            pt.keys = keys;
+            pt.chunk = c;
+            pt.k0 = split * c;
+            pt.k1 = min(keys, pt.k0 + c);
+            pt.splits = int32_t(splits);
+            pt.slot0 = int32_t(bp + xp - parts + tile_head * splits);
+            pt.slot1 = pt.slot0 + 1;
+            pt.slot_step = 1;
+            pt.slot = JOIN ? split : pt.slot0 + split;
+            sh.found = true;
         }
         if (b < items_before) break;
     }
     __syncthreads();
-    return sh.item;
+    return sh.found;
 }
 
 // Partials pass between workgroups of one launch, on any XCD: as relaxed atomics of agent scope, which go through to
 // where every XCD sees them, the writers' completed before they count themselves in. (Plain stores and a fence at agent
 // scope write back and drop a whole L2 per workgroup: 64 single tokens over 4,096 keys took 497 us so.)
-__device__ inline void put_part(float* p, f32x4 v) {
-    const u32x4 b = __builtin_bit_cast(u32x4, v);
-    __hip_atomic_store(reinterpret_cast<uint64_t*>(p), uint64_t(b[1]) << 32 | b[0], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    __hip_atomic_store(reinterpret_cast<uint64_t*>(p) + 1, uint64_t(b[3]) << 32 | b[2], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+// A wave's stores of such a kind are fast where they fill whole lines, so rows of O are laid out in LDS first.
+__device__ inline void put_part(float* p, float2 v) {
+    __hip_atomic_store(reinterpret_cast<uint64_t*>(p), uint64_t(__float_as_uint(v.y)) << 32 | __float_as_uint(v.x), __ATOMIC_RELAXED,
+                       __HIP_MEMORY_SCOPE_AGENT);
 }
 __device__ inline void put_part(float2* p, float2 v) {
     __hip_atomic_store(reinterpret_cast<uint64_t*>(p), uint64_t(__float_as_uint(v.y)) << 32 | __float_as_uint(v.x), __ATOMIC_RELAXED,
@@ -236,81 +282,169 @@ __device__ inline float2 get_part2(const float2* p) {
     return make_float2(__uint_as_float(uint32_t(v)), __uint_as_float(uint32_t(v >> 32)));
 }
 
-// Called by every thread of a workgroup that wrote one split's partial: the tile's last workgroup to arrive joins the
-// splits. Each sum is taken in the order of the splits by one thread, or, where there are few rows, by up to 8
-// threads whose parts are then added in their order: the same bits whoever arrives last.
-template <int BM>
+// This wave's stores have reached where every XCD sees them. (A workgroup barrier alone does not wait for that: plain
+// accesses of one CU meet in its L1, which these pass by.)
+__device__ inline void stores_done() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(kWaitVm0);
+    asm volatile("" ::: "memory");
+}
+
+// Joins the pieces of a tile of k_attend_few: the rows' references and weights first (in LDS, 16 threads a row), then 4
+// elements a thread, the partials of 16 pieces on the way together.
+// Each sum is taken in the order of the pieces by one thread, or by up to 4 threads whose parts are then added in
+// their order: the same bits whoever does it.
 struct JoinLds {
     int last;
-    float lpart[8][BM];
-    __attribute__((aligned(16))) float part[8][128 * 4];     // 256 / ways units each
+    float scale[kFewRows], lse[kFewRows];
+    float2 w[kMaxSplits][kFewRows];                         // (max, sum) of a piece, then its weight
+    __attribute__((aligned(16))) float part[4][128 * 4];
 };
-template <typename T, int D, int BM>
-__device__ void join_splits(const AttendArgs& a, const Item& it, int row0, int n, JoinLds<BM>& lds) {
-    const int tid = int(threadIdx.x);
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt(kWaitVm0);                    // this wave's stores have reached every XCD's view
+template <typename T, int D>
+__device__ void join_rows(const AttendArgs& a, const Part& it, JoinLds& lds) {
+    const int tid = int(threadIdx.x), splits = it.splits;
+    const int rows = min(kFewRows, it.n * a.group - it.tile * kFewRows), units = rows * (D / 4);
+    for (int x = tid; x < splits * kFewRows; x += 256)
+        if (x % kFewRows < rows) lds.w[x / kFewRows][x % kFewRows] = get_part2(a.part_ml + int64_t(it.slot_of(x / kFewRows)) * kFewRows + x % kFewRows);
     __syncthreads();
-    if (tid == 0) lds.last = __hip_atomic_fetch_add(&a.arrived[it.part], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == uint32_t(it.splits - 1);
-    __syncthreads();
-    if (!lds.last) return;
-    if (tid == 0) __hip_atomic_store(&a.arrived[it.part], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    const int valid = min(BM, n * a.group - it.tile * BM), units = valid * (D / 4);
-    int ways = 1;                                            // threads per unit of 4 elements
-    while (ways < 8 && units * ways * 2 <= 256 && ways < it.splits) ways *= 2;
-    const float2* const ml = a.part_ml + int64_t(it.part) * BM;
-    const float* const po = a.part_o + int64_t(it.part) * BM * D;
-    for (int e0 = 0; e0 < units; e0 += 256 / ways) {
-        const int w = tid / (256 / ways), e = e0 + tid % (256 / ways), rr = e / (D / 4), d4 = e % (D / 4);
-        f32x4 sum = {0, 0, 0, 0};
-        float lsum = 0.0f, top = -kInf;
-        if (e < units) {
-#pragma unroll 4
-            for (int s = 0; s < it.splits; ++s) top = fmaxf(top, get_part2(ml + s * BM + rr).x);
-#pragma unroll 4
-            for (int s = w; s < it.splits; s += ways) {
-                const float2 p = get_part2(ml + s * BM + rr);
-                const float f = p.x == -kInf ? 0.0f : __builtin_amdgcn_exp2f(p.x - top);
-                lsum += f * p.y;
-                sum += f * get_part4(po + (int64_t(s) * BM + rr) * D + d4 * 4);
-            }
-        }
-        if (ways > 1) {                                      // units fit one round then
-            float* const mine = &lds.part[w][0];
-            *reinterpret_cast<f32x4*>(mine + (tid % (256 / ways)) * 4) = sum;
-            if (d4 == 0 && e < units) lds.lpart[w][rr] = lsum;
-            __syncthreads();
-            if (w == 0 && e < units) {
-                lsum = 0.0f;
-                for (int v = 0; v < ways; ++v) lsum += lds.lpart[v][rr];
-                for (int v = 1; v < ways; ++v) sum += *reinterpret_cast<const f32x4*>(&lds.part[v][tid * 4]);
-            }
-        }
-        if (w == 0 && e < units) {
-            const int mm = it.tile * BM + rr, ii = mm / a.group, hh = it.head * a.group + mm - ii * a.group;
-            const float inv = 1.0f / lsum;
-            typename Vec<T>::v4 o;
+    {
+        const int rr = tid >> 4, s0 = tid & 15;
+        float top = -kInf, sum = 0.0f;
+        if (rr < rows)
+            for (int s = s0; s < splits; s += 16) top = fmaxf(top, lds.w[s][rr].x);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) o[j] = top == -kInf ? T(0.0f) : T(sum[j] * inv);
-            *reinterpret_cast<typename Vec<T>::v4*>(static_cast<T*>(a.out) + (int64_t(row0) + ii) * a.out_stride + int64_t(hh) * D + d4 * 4) = o;
-            if (a.lse && d4 == 0)
-                a.lse[(int64_t(row0) + ii) * a.q_heads + hh] = top == -kInf ? -kInf : (top + __builtin_amdgcn_logf(lsum)) * kLn2;
+        for (int o = 1; o < 16; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
+        if (rr < rows)
+            for (int s = s0; s < splits; s += 16) {
+                const float2 p = lds.w[s][rr];
+                const float f = p.x == -kInf ? 0.0f : __builtin_amdgcn_exp2f(p.x - top);
+                sum += f * p.y;
+                lds.w[s][rr].x = f;
+            }
+#pragma unroll
+        for (int o = 1; o < 16; o <<= 1) sum += __shfl_xor(sum, o);
+        if (rr < rows && s0 == 0) {
+            lds.scale[rr] = top == -kInf ? -kInf : 1.0f / sum;       // -inf: the row sees no key
+            lds.lse[rr] = top == -kInf ? -kInf : (top + __builtin_amdgcn_logf(sum)) * kLn2;
         }
     }
+    __syncthreads();
+    int ways = 1;                                            // threads per unit of 4 elements
+    while (ways < 4 && units * ways * 2 <= 256 && ways < splits) ways *= 2;
+    const int per = 256 / ways, w = tid / per;
+    constexpr int U = 16;
+    for (int base = 0; base < units; base += per) {
+        const int e = base + tid % per, rr = e / (D / 4), d4 = e % (D / 4);
+        f32x4 sum = {0, 0, 0, 0};
+        if (e < units) {
+            const float* const po = a.part_o + rr * D + d4 * 4;
+            for (int s = w; s < splits; s += U * ways) {
+                f32x4 o[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if (s + u * ways < splits) o[u] = get_part4(po + int64_t(it.slot_of(s + u * ways)) * kFewRows * D);
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if (s + u * ways < splits) sum += lds.w[s + u * ways][rr].x * o[u];
+            }
+        }
+        if (ways > 1) {                                      // then every thread has one unit or none
+            *reinterpret_cast<f32x4*>(&lds.part[w][(tid % per) * 4]) = sum;
+            __syncthreads();
+            for (int v = 1; v < ways && w == 0; ++v) sum += *reinterpret_cast<const f32x4*>(&lds.part[v][tid * 4]);
+        }
+        if (e >= units || w) continue;
+        const int mm = it.tile * kFewRows + rr, ii = mm / a.group, hh = it.head * a.group + mm - ii * a.group;
+        const float scale = lds.scale[rr];
+        typename Vec<T>::v4 o;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[j] = scale == -kInf ? T(0.0f) : T(sum[j] * scale);
+        *reinterpret_cast<typename Vec<T>::v4*>(static_cast<T*>(a.out) + (int64_t(it.row0) + ii) * a.out_stride + int64_t(hh) * D + d4 * 4) = o;
+        if (a.lse && d4 == 0) a.lse[(int64_t(it.row0) + ii) * a.q_heads + hh] = lds.lse[rr];
+    }
+}
+
+// Called by every thread of a workgroup that wrote one piece's partial: the tile's last workgroup to arrive joins them.
+template <typename T, int D>
+__device__ void join_last(const AttendArgs& a, const Part& it, JoinLds& lds) {
+    stores_done();
+    __syncthreads();
+    if (threadIdx.x == 0)
+        lds.last = __hip_atomic_fetch_add(&a.arrived[it.slot0], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == uint32_t(it.splits - 1);
+    __syncthreads();
+    if (!lds.last) return;
+    if (threadIdx.x == 0) __hip_atomic_store(&a.arrived[it.slot0], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    join_rows<T, D>(a, it, lds);
+}
+
+// The steps of `STEP` keys that some row of the workgroup can see by its episode, of a window of kWindow steps: the
+// others are neither read nor computed. A key is read if its episode is negative, some row's is, or it lies between the
+// least and the greatest of the rows' (exact where the rows ask within one episode, as single tokens do, and where
+// episodes follow each other). Entry: the step within the window, kMixed added where rows and keys have to be compared
+// one by one.
+constexpr int kWindow = 512, kMixed = 1 << 15;
+struct StepLds {
+    uint16_t flag[kWindow], list[kWindow];
+    int count;
+    int eq_min[4], eq_max[4];                                // of the waves' rows
+};
+template <int STEP>
+__device__ int list_steps(const AttendArgs& a, int request, int last_page, int k0, int k1, int w0, int steps, int eq_min, int eq_max, StepLds& lds) {
+    const int lane = int(threadIdx.x) & 63, wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6);
+    const int n = min(kWindow, steps - w0);
+    __syncthreads();                                         // the list before is done with
+    constexpr int U = 8;                                     // steps whose loads are on the way together
+    for (int t0 = wave; t0 < n; t0 += 4 * U) {
+        int64_t page[U];
+        int e[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int key = min(k0 + (w0 + t0 + 4 * u) * STEP + lane, k1 - 1);
+            const int id = a.table[int64_t(request) * a.max_pages + min(key >> a.page_shift, last_page)];
+            page[u] = uint32_t(id) < uint32_t(a.num_pages) ? id : 0;
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int key = min(k0 + (w0 + t0 + 4 * u) * STEP + lane, k1 - 1);
+            e[u] = a.k_eps[(page[u] << a.page_shift) + (key & ((1 << a.page_shift) - 1))];
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int t = t0 + 4 * u;
+            const bool in = lane < STEP && k0 + (w0 + t) * STEP + lane < k1;
+            const bool any = __any(in && (eq_min < 0 || e[u] < 0 || (e[u] >= eq_min && e[u] <= eq_max)));
+            const bool alike = eq_max < 0 || __all(!in || e[u] < 0) || (eq_min == eq_max && __all(!in || e[u] == eq_min));
+            if (lane == 0 && t < n) lds.flag[t] = any ? uint16_t(t + (alike ? 0 : kMixed)) : uint16_t(0xFFFF);
+        }
+    }
+    __syncthreads();
+    if (wave == 0) {
+        int count = 0;
+        for (int t0 = 0; t0 < n; t0 += 64) {
+            const uint16_t f = t0 + lane < n ? lds.flag[t0 + lane] : uint16_t(0xFFFF);
+            const uint64_t on = __ballot(f != 0xFFFF);
+            if (f != 0xFFFF) lds.list[count + __popcll(on & ((1ull << lane) - 1))] = f;
+            count += __popcll(on);
+        }
+        if (lane == 0) lds.count = count;
+    }
+    __syncthreads();
+    return __builtin_amdgcn_readfirstlane(lds.count);
 }
 
 // Infinities and NaN among the values. A weight of 0 times one of them is NaN, so where some row of a step does not see
 // some key, the products take them as 0, and the workgroup, once its rows are written, adds them to the rows that do see
 // them here: every (row, element) looks through the keys [k0, k1). (Rare, and slow.)
 template <typename T, int D, int BM>
-__device__ void add_not_finite(const AttendArgs& a, const Item& it, int row0, int n, int keys, int prefix, int k0, int k1) {
+__device__ void add_not_finite(const AttendArgs& a, const Part& it, int prefix) {
+    const int row0 = it.row0, n = it.n, keys = it.keys;
     const int valid = min(BM, n * a.group - it.tile * BM);
     for (int e = int(threadIdx.x); e < valid * D; e += 256) {
         const int rr = e / D, d = e % D, m = it.tile * BM + rr, i = m / a.group, hq = it.head * a.group + m - i * a.group;
         const int64_t row = int64_t(row0) + i;
-        const int end = min(k1, min(max(keys - n + i + 1, prefix), keys));
+        const int end = min(it.k1, min(max(keys - n + i + 1, prefix), keys));
         float sum = 0.0f;
-        for (int k = k0; k < end; ++k) {
+        for (int k = it.k0; k < end; ++k) {
             const int id = a.table[int64_t(it.request) * a.max_pages + (k >> a.page_shift)];
             const int64_t page = uint32_t(id) < uint32_t(a.num_pages) ? id : 0;
             const int off = k & ((1 << a.page_shift) - 1);
@@ -326,37 +460,45 @@ __device__ void add_not_finite(const AttendArgs& a, const Item& it, int row0, in
             T* const o = static_cast<T*>(a.out) + row * a.out_stride + int64_t(hq) * D + d;
             *o = T(float(*o) + sum);
         } else {
-            float* const o = a.part_o + (int64_t(it.part + it.split) * BM + rr) * D + d;
-            const float was = __hip_atomic_load(o, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            __hip_atomic_store(o, was + sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            float* const o = (BM == kFewRows ? a.part_o : a.many_o) + (int64_t(it.slot) * BM + rr) * D + d;
+            if (BM == kFewRows) {
+                const float was = __hip_atomic_load(o, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                __hip_atomic_store(o, was + sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            } else {
+                *o += sum;
+            }
         }
     }
 }
 
 // ---- few rows: 16 at a time, keys straight from the cache to registers -----------------
-// Bound by the cache's bytes. 4 waves take the steps of the chunk in turn (64 keys; 32 for heads of 256), and a wave
-// keeps its next step's K and V on the way to registers (16 bytes a lane; whole 128-byte lines, from K rows over the
+// Bound by the cache's bytes. A piece's steps (64 keys; 32 for heads of 256) go to 4 waves in turn, and a wave keeps
+// its next step's K and V on the way to registers (16 bytes a lane; whole 128-byte lines, from K rows over the
 // elements and from V rows over the step's keys) while it computes this one: 8 waves of a CU have up to 256 KB in
 // flight. The waves' sums are joined at the end.
-template <typename T, int D, bool EXTRA>
-__global__ __launch_bounds__(256, D > 128 ? 1 : 2) void k_attend_few(AttendArgs a) {
-    using V = typename Vec<T>::v8;
-    constexpr int KC = D / 32, VB = D / 16, NH = D > 128 ? 1 : 2, STEP = 32 * NH;      // NH: halves of 32 keys in a step
-    __shared__ union {
-        SchedLds sched;
+template <int D>
+struct FewLds {
+    union {
         struct { float ml[4][16][2]; __attribute__((aligned(16))) float ob[2][16][D + 4]; } wave;
-        JoinLds<kFewRows> join;
-    } lds;
-    __shared__ int any_dirty;
-    if (threadIdx.x == 0) any_dirty = 0;
-    const Item it = find_item(a, blockIdx.x, kFewRows, 256, kFewItemsLog2, lds.sched);
-    if (!it.found) return;
-    const int tid = int(threadIdx.x), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+        JoinLds join;
+        StepLds steps;
+    };
+    int any_dirty;
+};
+// Keys of a step: what the registers of two waves a SIMD hold, K and V and what the extra terms need.
+template <int D, bool EXTRA>
+constexpr int few_step() { return D > 128 || (D == 128 && EXTRA) ? 32 : 64; }
+
+template <typename T, int D, bool EXTRA, int STEP>
+__device__ void few_part(const AttendArgs& a, const Part& it, FewLds<D>& lds) {
+    using V = typename Vec<T>::v8;
+    constexpr int KC = D / 32, VB = D / 16, NH = STEP / 32;      // NH: halves of 32 keys in a step
+    int tid = int(threadIdx.x);
+    asm volatile("" : "+v"(tid));                          // nothing of a piece is kept in registers for the next
+    const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 15, h = lane >> 4;
-    const int r = __builtin_amdgcn_readfirstlane(it.request), head = __builtin_amdgcn_readfirstlane(it.head);
-    const int P1 = (1 << a.page_shift) - 1;
-    const int row0 = max(a.q_start[r], 0), n = min(a.q_start[r + 1], a.tokens) - row0;
-    const int keys = int(min(int64_t(max(a.kv_lens[r], 0)), int64_t(a.max_pages) << a.page_shift));
+    const int r = it.request, head = it.head, row0 = it.row0, n = it.n, keys = it.keys, P1 = (1 << a.page_shift) - 1;
+    if (tid == 0) lds.any_dirty = 0;                        // read after barriers
     const int m = it.tile * kFewRows + col;                 // this lane's row: token i, head of the group
     const bool row_ok = m < n * a.group;
     const int i = row_ok ? m / a.group : 0, hq = head * a.group + (row_ok ? m - i * a.group : 0);
@@ -375,7 +517,16 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void k_attend_few(AttendArgs 
     }
     lo = __builtin_amdgcn_readfirstlane(lo);
     hi = __builtin_amdgcn_readfirstlane(hi);
-    const int k0 = __builtin_amdgcn_readfirstlane(it.split * it.chunk), k1 = min(k0 + __builtin_amdgcn_readfirstlane(it.chunk), hi);
+    const bool listed = EXTRA && a.k_eps;
+    int eq_min = row_ok ? eq : INT32_MAX, eq_max = row_ok ? eq : INT32_MIN;
+    if (listed) {
+#pragma unroll
+        for (int o = 1; o < 16; o <<= 1) {
+            eq_min = min(eq_min, __shfl_xor(eq_min, o));
+            eq_max = max(eq_max, __shfl_xor(eq_max, o));
+        }
+    }
+    const int k0 = it.k0, k1 = min(it.k1, hi);
     const int steps = k1 > k0 ? (k1 - k0 + STEP - 1) / STEP : 0;
 
     const TablePtr table = table_row(a, r);
@@ -417,7 +568,6 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void k_attend_few(AttendArgs 
         }
     };
 
-    if (wave < steps) find_pages(wave);
     V q[KC];
     const T* const qp = static_cast<const T*>(a.q) + row * a.q_stride + int64_t(hq) * D + h * 8;
 #pragma unroll
@@ -432,14 +582,19 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void k_attend_few(AttendArgs 
 #pragma unroll
         for (int u = 0; u < 2 * NH; ++u) v_pages[u] = pages[u];
     };
-    if (wave < steps) {
-        load_k(wave);
+    for (int w0 = 0; w0 < steps; w0 += kWindow) {
+    const int count = listed ? list_steps<STEP>(a, r, last_page, k0, k1, w0, steps, eq_min, eq_max, lds.steps) : steps;
+    auto step_at = [&](int x) { return listed ? w0 + (__builtin_amdgcn_readfirstlane(int(lds.steps.list[x])) & (kWindow - 1)) : x; };
+    if (wave < count) {
+        find_pages(step_at(wave));
+        load_k(step_at(wave));
         keep_pages();
-        load_v(wave);
-        find_pages(wave + 4);
+        load_v(step_at(wave));
+        if (wave + 4 < count) find_pages(step_at(wave + 4));
     }
-    for (int s = wave; s < steps; s += 4) {
-        const int ks = k0 + s * STEP;
+    for (int x0 = wave; x0 < count; x0 += 4) {
+        const int ks = k0 + step_at(x0) * STEP;
+        const bool mixed = listed && (__builtin_amdgcn_readfirstlane(int(lds.steps.list[x0])) & kMixed);
         f32x4 acc[NH][2];
 #pragma unroll
         for (int b2 = 0; b2 < NH; ++b2)
@@ -449,11 +604,12 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void k_attend_few(AttendArgs 
 #pragma unroll
                 for (int c = 0; c < KC; ++c) acc[b2][b] = Vec<T>::mma(kf[b2][b][c], q[c], acc[b2][b]);
             }
-        const bool more = s + 4 < steps;
+        const bool more = x0 + 4 < count;
+        const int next = more ? step_at(x0 + 4) : 0;
         if (more) {
-            load_k(s + 4);
+            load_k(next);
             keep_pages();
-            find_pages(s + 8);
+            if (x0 + 8 < count) find_pages(step_at(x0 + 8));
         }
         // x[8 b2 + j]: this lane's key ks + 32 b2 + 8 h + j
         float x[8 * NH];
@@ -468,12 +624,12 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void k_attend_few(AttendArgs 
 #pragma unroll
             for (int j = 0; j < 8 * NH; ++j) x[j] -= dec * fmaxf(0.0f, tq - tk[j >> 3][(j >> 2) & 1][j & 3]);
         }
-        const bool whole = ks + STEP <= lo && !(EXTRA && a.k_eps);
+        const bool whole = ks + STEP <= lo && !mixed;
         if (!whole) {
 #pragma unroll
             for (int j = 0; j < 8 * NH; ++j) {
                 bool in = ks + 32 * (j >> 3) + 8 * h + (j & 7) < limit;
-                if (EXTRA && a.k_eps) {
+                if (mixed) {
                     const int e = ek[j >> 3][(j >> 2) & 1][j & 3];
                     in = in && (e < 0 || eq < 0 || e == eq);
                 }
@@ -529,7 +685,9 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void k_attend_few(AttendArgs 
         for (int b2 = 0; b2 < NH; ++b2)
 #pragma unroll
             for (int d = 0; d < VB; ++d) o[d] = Vec<T>::mma(vf[b2][d], p[b2], o[d]);
-        if (more) load_v(s + 4);
+        if (more) load_v(next);
+    }
+    if (!listed) break;
     }
 
     // join the waves: references first, then sums and O, in wave order
@@ -538,9 +696,9 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void k_attend_few(AttendArgs 
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
     float mw = mtop == -kInf ? -kInf : mref;
-    __syncthreads();                                        // the item has been read
+    __syncthreads();                                        // the list of steps is done with
     if (h == 0) ml[wave][col][0] = mw;
-    if (dirty && lane == 0) any_dirty = 1;
+    if (dirty && lane == 0) lds.any_dirty = 1;
     __syncthreads();
     float mall = ml[0][col][0];
 #pragma unroll
@@ -582,20 +740,170 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void k_attend_few(AttendArgs 
             }
             if (a.lse && h == 0) a.lse[row * a.q_heads + hq] = mall == -kInf ? -kInf : (mall + __builtin_amdgcn_logf(lall)) * kLn2;
         }
-        if (row_ok && joined) {
-            float* const po = a.part_o + (int64_t(it.part + it.split) * kFewRows + col) * D + h * 4;
+        if (joined) {
 #pragma unroll
-            for (int d = 0; d < VB; ++d) put_part(po + d * 16, o[d]);
-            if (h == 0) put_part(a.part_ml + int64_t(it.part + it.split) * kFewRows + col, make_float2(mall, lall));
+            for (int d = 0; d < VB; ++d) *reinterpret_cast<f32x4*>(&ob[0][col][d * 16 + h * 4]) = o[d];
+            if (row_ok && h == 0) put_part(a.part_ml + int64_t(it.slot) * kFewRows + col, make_float2(mall, lall));
         }
     }
-    if (any_dirty) {
+    if (joined) {
         __syncthreads();
-        add_not_finite<T, D, kFewRows>(a, it, row0, n, keys, prefix, k0, min(k0 + it.chunk, keys));
+        const int valid = min(kFewRows, n * a.group - it.tile * kFewRows);
+        float* const po = a.part_o + int64_t(it.slot) * kFewRows * D;
+        for (int e = tid; e < valid * (D / 2); e += 256)
+            put_part(po + e * 2, *reinterpret_cast<const float2*>(&ob[0][e / (D / 2)][e % (D / 2) * 2]));
+    }
+    if (lds.any_dirty) {
+        stores_done();                                      // of the partials
+        __syncthreads();
+        add_not_finite<T, D, kFewRows>(a, it, prefix);
     }
     if (!joined) return;
     __syncthreads();
-    join_splits<T, D, kFewRows>(a, it, row0, n, lds.join);
+    join_last<T, D>(a, it, lds.join);
+}
+
+// The launch's work is one line of steps, request after request, tile after tile, kv head after kv head, and workgroup w
+// of G takes the w-th of G equal lengths of it: the bytes of the cache are dealt out evenly whatever the requests'
+// lengths, in one round. An end of a length that falls within kFewCut steps of a tile's first or last one moves there
+// (short requests are not cut), so a workgroup has at most two pieces that others share: its first and its last.
+constexpr int kFewCut = 4;
+struct SpanLds {
+    int64_t start[257];        // of 256 requests: steps of the launch before each
+    int32_t row0[256], n[256], keys[256];
+    int64_t wsum[4];
+    int32_t wmost[4];
+    int32_t at, most;          // most: steps of the longest tile so far
+};
+__device__ inline int steps_of(int keys, int step) { return max(1, (keys + step - 1) / step); }
+__device__ inline int units_of(const AttendArgs& a, int n) { return (n * a.group + kFewRows - 1) / kFewRows * a.kv_heads; }
+
+// Requests r0 .. r0 + 255 into the LDS; returns the launch's steps up to their end (base: before them).
+__device__ int64_t load_span(const AttendArgs& a, int r0, int64_t base, int step, SpanLds& lds) {
+    const int tid = int(threadIdx.x), lane = tid & 63, wave = tid >> 6;
+    const Request q = request_of<true>(a, r0 + tid);
+    const int64_t work = int64_t(q.tiles) * a.kv_heads * steps_of(q.keys, step);
+    int64_t x = work;
+    int most = steps_of(q.keys, step);
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) most = max(most, __shfl_xor(most, o));
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int64_t y = __shfl_up((long long)x, unsigned(o));
+        if (lane >= o) x += y;
+    }
+    __syncthreads();                                        // the requests before are done with
+    if (lane == 63) { lds.wsum[wave] = x; lds.wmost[wave] = most; }
+    __syncthreads();
+    int64_t sum = base, mine = base;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        if (w < wave) mine += lds.wsum[w];
+        sum += lds.wsum[w];
+    }
+    lds.start[tid] = mine + x - work;
+    lds.row0[tid] = q.row0;
+    lds.n[tid] = q.tiles ? q.n : 0;
+    lds.keys[tid] = q.keys;
+    if (tid == 0) {
+        lds.start[256] = sum;
+        lds.most = max(r0 ? lds.most : 0, max(max(lds.wmost[0], lds.wmost[1]), max(lds.wmost[2], lds.wmost[3])));
+    }
+    __syncthreads();
+    return uniform(sum);
+}
+
+template <int D>
+struct FewShared {
+    FewLds<D> part;
+    SpanLds span;
+};
+template <typename T, int D, bool EXTRA, int STEP>
+__device__ void few_rows(const AttendArgs& a, int block, int blocks, FewShared<D>& shared) {
+    FewLds<D>& lds = shared.part;
+    SpanLds& sp = shared.span;
+    const int tid = int(threadIdx.x);
+    const int64_t w = block;
+    int r0 = 0;
+    int64_t end = load_span(a, 0, 0, STEP, sp), total = end;
+    for (int r = 256; r < a.requests; r += 256) total = load_span(a, r, total, STEP, sp);
+    const int most = __builtin_amdgcn_readfirstlane(sp.most);
+    if (a.requests > 256) end = load_span(a, 0, 0, STEP, sp);            // back to the first
+    // no tile in more than kMaxSplits pieces
+    const int64_t span = max((total + blocks - 1) / blocks, int64_t((most + kMaxSplits - 2) / (kMaxSplits - 1))), x0 = w * span, x1 = min(x0 + span, total);
+    if (x0 >= total) return;                                // no steps at all, or none for this workgroup
+    while (x0 >= end) {
+        r0 += 256;
+        end = load_span(a, r0, end, STEP, sp);
+    }
+    if (x0 >= sp.start[tid] && x0 < sp.start[tid + 1]) sp.at = tid;
+    __syncthreads();
+    int k = __builtin_amdgcn_readfirstlane(sp.at), steps = steps_of(__builtin_amdgcn_readfirstlane(sp.keys[k]), STEP);
+    // the first tile and step: ends near a tile's own move to it
+    int unit, s0;
+    {
+        const int64_t local = x0 - uniform(sp.start[k]);
+        unit = __builtin_amdgcn_readfirstlane(int(local / steps));
+        s0 = __builtin_amdgcn_readfirstlane(int(local - int64_t(unit) * steps));
+        if (s0 < min(kFewCut, (steps + 1) / 2)) s0 = 0;
+        else if (steps - s0 < kFewCut) { s0 = 0; ++unit; }
+    }
+    bool first = true;
+    for (;;) {
+        while (unit >= units_of(a, __builtin_amdgcn_readfirstlane(sp.n[k]))) {      // on to the next request that has rows
+            unit = 0;
+            if (r0 + ++k >= a.requests) return;
+            if (k < 256) continue;
+            r0 += 256;
+            end = load_span(a, r0, end, STEP, sp);
+            k = 0;
+        }
+        Part it;
+        it.request = r0 + k;
+        it.row0 = __builtin_amdgcn_readfirstlane(sp.row0[k]);
+        it.n = __builtin_amdgcn_readfirstlane(sp.n[k]);
+        it.keys = __builtin_amdgcn_readfirstlane(sp.keys[k]);
+        steps = steps_of(it.keys, STEP);
+        const int64_t u0 = uniform(sp.start[k]) + int64_t(unit) * steps, left = x1 - u0;       // the tile's first step; ours of it
+        const int low = min(kFewCut, (steps + 1) / 2);
+        if (left < low) return;
+        const int s1 = left >= steps || steps - left < kFewCut ? steps : int(left);
+        it.tile = unit / a.kv_heads;
+        it.head = unit - it.tile * a.kv_heads;
+        it.k0 = s0 * STEP;
+        it.k1 = min(s1 * STEP, it.keys);
+        it.splits = 1;
+        it.chunk = 0;
+        it.slot = it.slot0 = it.slot1 = it.slot_step = 0;
+        if (s0 > 0 || s1 < steps) {
+            // the cuts of this tile: ends c span with low <= c span - u0 <= steps - kFewCut. The piece before the first is
+            // the last of workgroup c - 1, the one after cut c the first of workgroup c.
+            const int64_t c0 = (u0 + low + span - 1) / span, c1 = (u0 + steps - kFewCut) / span;
+            it.splits = int(c1 - c0) + 2;
+            it.slot0 = int(2 * (c0 - 1) + 1);
+            it.slot1 = int(2 * c0);
+            it.slot_step = 2;
+            it.slot = s0 > 0 ? int(2 * w) : it.slot0;
+        }
+        if (!first) __syncthreads();                        // the LDS of the piece before is done with
+        first = false;
+        few_part<T, D, EXTRA, STEP>(a, uniform_part(it), lds);
+        if (left <= steps) return;
+        s0 = 0;
+        ++unit;
+    }
+}
+
+// How many keys the rows of a tile of k_attend_many see at most: limits grow with the token, so its last row's.
+__device__ inline int tile_end(const AttendArgs& a, const Part& it) {
+    const int last = min((it.tile * kManyRows + kManyRows - 1) / a.group, it.n - 1);
+    const int prefix = a.prefix ? min(max(a.prefix[it.request], 0), it.keys) : 0;
+    return min(max(it.keys - it.n + last + 1, prefix), it.keys);
+}
+// Sets the tile's pieces to those that its rows see keys of; false if piece `piece` is none of them.
+__device__ inline bool own_pieces(const AttendArgs& a, Part* it, int piece) {
+    it->splits = min(it->splits, max(1, (tile_end(a, *it) + it->chunk - 1) / it->chunk));
+    return piece < it->splits;
 }
 
 // ---- many rows: 128 at a time, keys staged through LDS ----------------------------------
@@ -615,21 +923,26 @@ struct ManyLds {
     int32_t eps[2][kManyKeys];
 };
 
+template <int D>
+struct ManyShared {
+    union { ManyLds<D> tiles; SchedLds sched; int any_dirty; };
+    StepLds list;
+};
 template <typename T, int D, bool EXTRA>
-__global__ __launch_bounds__(256, D > 128 ? 1 : 2) void k_attend_many(AttendArgs a) {
+__device__ void many_rows(const AttendArgs& a, int block, ManyShared<D>& lds) {
     using V = typename Vec<T>::v8;
     constexpr int KS = D / 16, DB = D / 32, RC = D / 8;      // k-steps of S, blocks of O, 16-byte pieces of a key's row
-    __shared__ __attribute__((aligned(16))) union { ManyLds<D> tiles; SchedLds sched; JoinLds<kManyRows> join; } lds;
+    StepLds& list = lds.list;
     ManyLds<D>& sh = lds.tiles;
-    const Item it = find_item(a, blockIdx.x, kManyRows, 256, kManyItemsLog2, lds.sched);
-    if (!it.found) return;
+    if (!find_item<false>(a, block, lds.sched)) return;
+    Part it = uniform_part(lds.sched.part);
+    if (!own_pieces(a, &it, it.slot - it.slot0)) return;
     __syncthreads();                                         // the item is read before its LDS is used again
     const int tid = int(threadIdx.x), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 31, h = lane >> 5;
-    const int r = __builtin_amdgcn_readfirstlane(it.request), head = __builtin_amdgcn_readfirstlane(it.head);
+    const int r = it.request, head = it.head;
     const int P1 = (1 << a.page_shift) - 1;
-    const int row0 = max(a.q_start[r], 0), n = min(a.q_start[r + 1], a.tokens) - row0;
-    const int keys = int(min(int64_t(max(a.kv_lens[r], 0)), int64_t(a.max_pages) << a.page_shift));
+    const int row0 = it.row0, n = it.n, keys = it.keys;
     const int m = it.tile * kManyRows + wave * 32 + col;     // this lane's row: token i, head of the group
     const bool row_ok = m < n * a.group;
     const int i = row_ok ? m / a.group : 0, hq = head * a.group + (row_ok ? m - i * a.group : 0);
@@ -657,12 +970,24 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void k_attend_many(AttendArgs
     }
     lo = __builtin_amdgcn_readfirstlane(lo);
     hi = __builtin_amdgcn_readfirstlane(hi);
-    // the workgroup's last row sees the most keys: limits grow with the token
-    const int last_i = min((it.tile * kManyRows + kManyRows - 1) / a.group, n - 1);
-    const int end = min(max(keys - n + last_i + 1, prefix), keys);
+    const int end = tile_end(a, it);
     const int first_limit = min(max(keys - n + it.tile * kManyRows / a.group + 1, prefix), keys);
-    const int k0 = it.split * it.chunk, k1 = min(k0 + it.chunk, end);
+    const int k0 = it.k0, k1 = min(it.k1, end);
     const int steps = __builtin_amdgcn_readfirstlane(k1 > k0 ? (k1 - k0 + kManyKeys - 1) / kManyKeys : 0);
+
+    const bool listed = EXTRA && a.k_eps;
+    int eq_min = row_ok ? eq : INT32_MAX, eq_max = row_ok ? eq : INT32_MIN;
+    if (listed) {
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            eq_min = min(eq_min, __shfl_xor(eq_min, o));
+            eq_max = max(eq_max, __shfl_xor(eq_max, o));
+        }
+        if (lane == 0) { list.eq_min[wave] = eq_min; list.eq_max[wave] = eq_max; }
+        __syncthreads();
+        eq_min = min(min(list.eq_min[0], list.eq_min[1]), min(list.eq_min[2], list.eq_min[3]));
+        eq_max = max(max(list.eq_max[0], list.eq_max[1]), max(list.eq_max[2], list.eq_max[3]));
+    }
 
     const TablePtr table = table_row(a, r);
     const int last_page = keys > 0 ? (keys - 1) >> a.page_shift : 0;
@@ -724,21 +1049,25 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void k_attend_many(AttendArgs
     const uint32_t koff = uint32_t(ki * RC + (h ^ kswz(ki))) * 16, voff = uint32_t(col * 8 + (h ^ vswz(col))) * 16;
     const char* const kl = reinterpret_cast<const char*>(&sh.k[0][0]);
     const char* const vl = reinterpret_cast<const char*>(&sh.v[0][0]);
-    if (steps > 0) {
-        find_pages(0);
-        stage(0, 0);
-        find_pages(1);
+    for (int w0 = 0; w0 < steps; w0 += kWindow) {
+    const int count = listed ? list_steps<kManyKeys>(a, r, last_page, k0, k1, w0, steps, eq_min, eq_max, list) : steps;
+    auto step_at = [&](int x) { return listed ? w0 + (__builtin_amdgcn_readfirstlane(int(list.list[x])) & (kWindow - 1)) : x; };
+    if (count > 0) {
+        find_pages(step_at(0));
+        stage(step_at(0), 0);
+        if (count > 1) find_pages(step_at(1));
     }
-    for (int s = 0; s < steps; ++s) {
-        const int buf = s & 1;
+    for (int x0 = 0; x0 < count; ++x0) {
+        const int buf = x0 & 1;
         tile_barrier();                                      // the tile is in LDS; nobody reads the other buffer any more
-        if (s + 1 < steps) {
-            stage(s + 1, buf ^ 1);
-            find_pages(s + 2);
+        const int kt = k0 + step_at(x0) * kManyKeys;
+        const bool mixed = listed && (__builtin_amdgcn_readfirstlane(int(list.list[x0])) & kMixed);
+        if (x0 + 1 < count) {
+            stage(step_at(x0 + 1), buf ^ 1);
+            if (x0 + 2 < count) find_pages(step_at(x0 + 2));
         }
         const uint32_t kb = buf * uint32_t(sizeof(sh.k[0])) + koff, vb = buf * uint32_t(sizeof(sh.v[0])) + voff;
-        const int kt = k0 + s * kManyKeys;
-        if (kt + kManyKeys > first_limit || (EXTRA && a.k_eps)) {
+        if (kt + kManyKeys > first_limit || mixed) {
             // some row of the workgroup does not see some key: each thread looks over its pieces of V (see add_not_finite;
             // slots past the request's keys hold anything and become 0)
 #pragma unroll
@@ -768,8 +1097,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void k_attend_many(AttendArgs
 #pragma unroll
             for (int c = 0; c < KS; ++c) x[b] = Vec<T>::mma32(load16<V>(kl + (kb ^ (c * 32)) + b * 32 * RC * 16), q[c], x[b]);
         }
-        bool whole = kt + kManyKeys <= lo;
-        uint32_t seen = ~0u;                                 // bit 16 b + j
+        const bool whole = kt + kManyKeys <= lo && !mixed;
         if constexpr (EXTRA) {
 #pragma unroll
             for (int b = 0; b < 2; ++b)
@@ -789,25 +1117,29 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void k_attend_many(AttendArgs
                     for (int j = 0; j < 16; ++j)
                         x[b][j] -= dec * fmaxf(0.0f, tq - sh.times[buf][b * 32 + (j >> 3) * 16 + h * 8 + (j & 7)]);
             }
-            if (a.k_eps) {
-                whole = false;
-#pragma unroll
-                for (int b = 0; b < 2; ++b)
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        const int e = sh.eps[buf][b * 32 + (j >> 3) * 16 + h * 8 + (j & 7)];
-                        if (!(e < 0 || eq < 0 || e == eq)) seen &= ~(1u << (16 * b + j));
-                    }
-            }
         }
         if (!whole) {
+            // bit j: this lane's row sees key kt + j
+            uint64_t seen = limit - kt >= 64 ? ~0ull : limit > kt ? (1ull << (limit - kt)) - 1 : 0ull;
+            if (EXTRA && mixed) {
+                // by the tile's few different episodes, each with the keys that have it
+                const int e = sh.eps[buf][lane];
+                uint64_t rest = keys - kt >= 64 ? ~0ull : (1ull << (keys - kt)) - 1, by_episode = 0;
+                while (rest) {
+                    const int v = __builtin_amdgcn_readlane(e, __builtin_ctzll(rest));
+                    const uint64_t with = __ballot(e == v);
+                    by_episode |= v < 0 || eq < 0 || eq == v ? with : 0ull;
+                    rest &= ~with;
+                }
+                seen &= by_episode;
+            }
+            seen >>= 8 * h;                                  // bit 32 b + 16 (j / 8) + j % 8: register j of block b
 #pragma unroll
             for (int b = 0; b < 2; ++b)
 #pragma unroll
                 for (int j = 0; j < 16; ++j) {
-                    const bool in = kt + b * 32 + (j >> 3) * 16 + h * 8 + (j & 7) < limit && ((seen >> (16 * b + j)) & 1u);
-                    if (!in) seen &= ~(1u << (16 * b + j));
-                    x[b][j] = in ? x[b][j] : -kInf;
+                    const uint32_t in = uint32_t(__builtin_amdgcn_sbfe(int(seen >> (32 * b)), (j >> 3) * 16 + (j & 7), 1));
+                    x[b][j] = __uint_as_float((__float_as_uint(x[b][j]) & in) | (__float_as_uint(-kInf) & ~in));
                 }
         }
         const float c = EXTRA ? 1.0f : a.scale_log2;         // not negative: a negative scale turns q's sign
@@ -844,6 +1176,8 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void k_attend_many(AttendArgs
 #pragma unroll
             for (int d = 0; d < DB; ++d) o[d] = Vec<T>::mma32(load16<V>(vl + (vb ^ (t * 32)) + d * 32 * 8 * 16), p[t], o[d]);
     }
+    if (!listed) break;
+    }
 
     l += __shfl_xor(l, 32);
     const bool empty = mtop == -kInf;
@@ -863,74 +1197,120 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void k_attend_many(AttendArgs
         if (a.lse && h == 0) a.lse[row * a.q_heads + hq] = empty ? -kInf : (mref + __builtin_amdgcn_logf(l)) * kLn2;
     }
     if (it.splits > 1 && row_ok) {
-        const int64_t at = int64_t(it.part + it.split) * kManyRows + wave * 32 + col;
-        float* const po = a.part_o + at * D + h * 4;
+        const int64_t at = int64_t(it.slot) * kManyRows + wave * 32 + col;
+        float* const po = a.many_o + at * D + h * 4;
 #pragma unroll
         for (int d = 0; d < DB; ++d)
 #pragma unroll
             for (int g = 0; g < 4; ++g)
-                put_part(po + d * 32 + g * 8, f32x4{o[d][g * 4], o[d][g * 4 + 1], o[d][g * 4 + 2], o[d][g * 4 + 3]});
-        if (h == 0) put_part(a.part_ml + at, make_float2(empty ? -kInf : mref, l));
+                *reinterpret_cast<f32x4*>(po + d * 32 + g * 8) = f32x4{o[d][g * 4], o[d][g * 4 + 1], o[d][g * 4 + 2], o[d][g * 4 + 3]};
+        if (h == 0) a.many_ml[at] = make_float2(empty ? -kInf : mref, l);
     }
     __syncthreads();                                         // the LDS of the tiles is free, the rows are written
-    if (tid == 0) lds.join.last = 0;
+    if (tid == 0) lds.any_dirty = 0;
     __syncthreads();
-    if (dirty) lds.join.last = 1;
+    if (dirty) lds.any_dirty = 1;
     __syncthreads();
-    if (lds.join.last) add_not_finite<T, D, kManyRows>(a, it, row0, n, keys, prefix, k0, min(k0 + it.chunk, keys));
-    if (it.splits == 1) return;
-    __syncthreads();
-    join_splits<T, D, kManyRows>(a, it, row0, n, lds.join);
+    if (lds.any_dirty) add_not_finite<T, D, kManyRows>(a, it, prefix);
 }
 
-template <typename T, int D, bool EXTRA>
-int launch_few(AttendArgs a, hipStream_t s) {
-    const int64_t tiles = int64_t(a.tokens) * a.group / kFewRows + std::min(a.requests, a.tokens);
-    const int64_t grid = (1 << kFewItemsLog2) + tiles * a.kv_heads;
-    MARS_CHECK(grid <= INT32_MAX, MARS_ERR_CAPACITY, "%lld tiles of rows", (long long)grid);
-    MARS_LAUNCH((k_attend_few<T, D, EXTRA>), dim3(unsigned(grid)), dim3(256), 0, s, a);
-    return MARS_OK;
-}
-
-template <typename T, int D, bool EXTRA>
-int launch_many(AttendArgs a, hipStream_t s) {
-    const int64_t tiles = int64_t(a.tokens) * a.group / kManyRows + std::min(a.requests, a.tokens);
-    const int64_t grid = (1 << kManyItemsLog2) + tiles * a.kv_heads;
-    MARS_CHECK(grid <= INT32_MAX, MARS_ERR_CAPACITY, "%lld tiles of rows", (long long)grid);
-    MARS_LAUNCH((k_attend_many<T, D, EXTRA>), dim3(unsigned(grid)), dim3(256), 0, s, a);
-    return MARS_OK;
-}
-
+// Joins the pieces that k_attend_many left: their partials come to megabytes, too much for the one workgroup that arrives
+// last (2 requests of 64 tokens over 8,000 keys: 114 us so). A thread takes 4 elements of a row and has the references and
+// partials of 8 pieces on the way together; the sums are taken in the order of the pieces.
 template <typename T, int D>
+__global__ __launch_bounds__(256) void k_attend_join(AttendArgs a) {
+    __shared__ SchedLds sched;
+    for (int block = int(blockIdx.x);; block += int(gridDim.x)) {
+    if (!find_item<true>(a, block, sched)) return;
+    Part it = uniform_part(sched.part);
+    __syncthreads();                                         // the item is read before the next is looked for
+    const int r0 = it.slot * kJoinRows, rows = min(kJoinRows, it.n * a.group - it.tile * kManyRows - r0);
+    if (!own_pieces(a, &it, 0) || it.splits == 1) continue;
+    const float2* const ml = a.many_ml + int64_t(it.slot0) * kManyRows + r0;
+    const float* const po = a.many_o + (int64_t(it.slot0) * kManyRows + r0) * D;
+    for (int e = int(threadIdx.x); e < rows * (D / 4); e += 256) {
+        const int rr = e / (D / 4), d4 = e % (D / 4);
+        constexpr int U = 8;
+        float top = -kInf, l = 0.0f;
+        f32x4 sum = {0, 0, 0, 0};
+        for (int s = 0; s < it.splits; s += U) {
+            float2 p[U];
+            f32x4 o[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int64_t at = int64_t(min(s + u, it.splits - 1)) * kManyRows + rr;
+                p[u] = ml[at];
+                o[u] = *reinterpret_cast<const f32x4*>(po + at * D + d4 * 4);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (s + u >= it.splits || p[u].x == -kInf) continue;
+                const float next = fmaxf(top, p[u].x), was = top == -kInf ? 0.0f : __builtin_amdgcn_exp2f(top - next);
+                const float f = __builtin_amdgcn_exp2f(p[u].x - next);
+                l = top == -kInf ? f * p[u].y : l * was + f * p[u].y;
+                sum = top == -kInf ? f * o[u] : sum * was + f * o[u];
+                top = next;
+            }
+        }
+        const int mm = it.tile * kManyRows + r0 + rr, ii = mm / a.group, hh = it.head * a.group + mm - ii * a.group;
+        const float inv = 1.0f / l;
+        typename Vec<T>::v4 w;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = top == -kInf ? T(0.0f) : T(sum[j] * inv);
+        *reinterpret_cast<typename Vec<T>::v4*>(static_cast<T*>(a.out) + (int64_t(it.row0) + ii) * a.out_stride + int64_t(hh) * D + d4 * 4) = w;
+        if (a.lse && d4 == 0)
+            a.lse[(int64_t(it.row0) + ii) * a.q_heads + hh] = top == -kInf ? -kInf : (top + __builtin_amdgcn_logf(l)) * kLn2;
+    }    }
+}
+
+// ---- the kernels ------------------------------------------------------------------------
+template <typename T, int D, bool EXTRA>
+__global__ __launch_bounds__(256, D > 128 ? 1 : 2) void k_attend_few(AttendArgs a) {
+    __shared__ __attribute__((aligned(16))) FewShared<D> lds;
+    few_rows<T, D, EXTRA, few_step<D, EXTRA>()>(a, int(blockIdx.x), int(gridDim.x), lds);
+}
+
+template <typename T, int D, bool EXTRA>
+__global__ __launch_bounds__(256, D > 128 ? 1 : 2) void k_attend_many(AttendArgs a) {
+    __shared__ __attribute__((aligned(16))) ManyShared<D> lds;
+    many_rows<T, D, EXTRA>(a, int(blockIdx.x), lds);
+}
+
+template <typename T, int D, bool EXTRA>
 int launch_dim(AttendArgs a, int32_t max_new, hipStream_t s) {
-    // Requests of at most kFewMost rows (new tokens x query heads per kv head) go to k_attend_few, the others to
-    // k_attend_many, in a launch of their own each. A bound on the new tokens that rules one of them out saves its launch;
-    // a request that breaks the bound is served by the other kernel.
+    // Requests of at most kFewMost rows (new tokens x query heads per kv head) are k_attend_few's, the others
+    // k_attend_many's. Where a bound on the new tokens rules one of them out, the other serves every request, also one that
+    // breaks the bound.
+    const int64_t rows = int64_t(a.tokens) * a.group, keys = int64_t(a.max_pages) << a.page_shift;
     const int64_t most = std::min<int64_t>(max_new > 0 ? max_new : a.tokens, a.tokens) * a.group;
     const bool few_only = most <= kFewMost, many_only = !few_only && a.requests == 1;
-    const bool extra = a.cap_log2 != 0.0f || a.k_times || a.k_eps;
-    if (!many_only) {
-        AttendArgs f = a;
-        f.rows_lo = 0;
-        f.rows_hi = few_only ? INT32_MAX : kFewMost;
-        if (extra) MARS_TRY((launch_few<T, D, true>(f, s)));
-        else MARS_TRY((launch_few<T, D, false>(f, s)));
-    }
-    if (!few_only) {
-        a.rows_lo = many_only ? 0 : kFewMost;
-        a.rows_hi = INT32_MAX;
-        if (extra) MARS_TRY((launch_many<T, D, true>(a, s)));
-        else MARS_TRY((launch_many<T, D, false>(a, s)));
+    a.few_rows = few_only ? INT32_MAX : many_only ? -1 : kFewMost;
+    // few: one workgroup for each that the CUs hold at a time, fewer where there are not so many steps
+    const int64_t few_tiles = few_only ? rows / kFewRows + std::min(a.requests, a.tokens) : std::min(a.requests, a.tokens);
+    constexpr int step = few_step<D, EXTRA>();
+    const int64_t few = std::min<int64_t>(few_tiles * a.kv_heads * ((keys + step - 1) / step), few_groups(D));
+    if (!many_only) MARS_LAUNCH((k_attend_few<T, D, EXTRA>), dim3(unsigned(few)), dim3(256), 0, s, a);
+    if (few_only) return MARS_OK;
+    // many: no more than chunks of kMinChunk or more of the tiles' keys, or 2^kManyItemsLog2 chunks and one for each tile
+    const int64_t tiles = rows / kManyRows + std::min<int64_t>(a.requests, rows / (kFewMost + 1));
+    const int64_t many = std::min(tiles * a.kv_heads * ((keys + kMinChunk - 1) / kMinChunk), (int64_t(1) << kManyItemsLog2) + tiles * a.kv_heads);
+    MARS_CHECK(many <= INT32_MAX, MARS_ERR_CAPACITY, "%lld tiles of rows", (long long)tiles);
+    MARS_LAUNCH((k_attend_many<T, D, EXTRA>), dim3(unsigned(many)), dim3(256), 0, s, a);
+    // no tile is in pieces where a row of the table is one chunk
+    if (keys > kMinChunk) {
+        const int64_t blocks = std::min<int64_t>(tiles * a.kv_heads * (kManyRows / kJoinRows), 1024);
+        MARS_LAUNCH((k_attend_join<T, D>), dim3(unsigned(blocks)), dim3(256), 0, s, a);
     }
     return MARS_OK;
 }
 
 template <typename T>
 int launch_typed(const mars_reader& r, const AttendArgs& a, int32_t max_new, hipStream_t s) {
+    const bool extra = a.cap_log2 != 0.0f || a.k_times || a.k_eps;
     switch (r.d.head_dim) {
-        case 64: return launch_dim<T, 64>(a, max_new, s);
-        case 128: return launch_dim<T, 128>(a, max_new, s);
-        default: return launch_dim<T, 256>(a, max_new, s);
+        case 64: return extra ? launch_dim<T, 64, true>(a, max_new, s) : launch_dim<T, 64, false>(a, max_new, s);
+        case 128: return extra ? launch_dim<T, 128, true>(a, max_new, s) : launch_dim<T, 128, false>(a, max_new, s);
+        default: return extra ? launch_dim<T, 256, true>(a, max_new, s) : launch_dim<T, 256, false>(a, max_new, s);
     }
 }
 

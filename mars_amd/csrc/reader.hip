@@ -302,12 +302,12 @@ int mars_reader_create(const mars_reader_desc* d, mars_reader** out) try {
             MARS_HIP(hipMemcpy(r->freq, f.data(), size_t(half) * sizeof(uint64_t), hipMemcpyHostToDevice));
             MARS_HIP(hipMemcpy(r->axis, axis.data(), size_t(half) * sizeof(int32_t), hipMemcpyHostToDevice));
         }
-        constexpr size_t few = size_t(2) << kFewItemsLog2, many = size_t(2) << kManyItemsLog2;
-        constexpr size_t rows = std::max(few * kFewRows, many * kManyRows);
+        r->few_slots = size_t(2) * few_groups(d->head_dim);
+        const size_t rows = r->few_slots * kFewRows + (size_t(2) << kManyItemsLog2) * kManyRows;
         MARS_TRY(dmalloc(&r->part_o, rows * size_t(d->head_dim)));
         MARS_TRY(dmalloc(&r->part_ml, rows));
-        MARS_TRY(dmalloc(&r->arrived, std::max(few, many)));
-        MARS_HIP(hipMemset(r->arrived, 0, std::max(few, many) * sizeof(uint32_t)));
+        MARS_TRY(dmalloc(&r->arrived, r->few_slots));
+        MARS_HIP(hipMemset(r->arrived, 0, r->few_slots * sizeof(uint32_t)));
         MARS_HIP(hipDeviceSynchronize());
         return MARS_OK;
     }();
@@ -421,6 +421,8 @@ int mars_kv_attend(const mars_reader* r, const mars_kv_cache* c, const mars_kv_a
     a.q_start = s->q_start; a.kv_lens = s->kv_lens; a.table = s->block_table;
     a.decay = s->decay; a.q_times = s->q_times; a.q_eps = s->q_episodes; a.prefix = s->prefix_lens;
     a.part_o = r->part_o; a.part_ml = r->part_ml; a.arrived = r->arrived;
+    a.many_o = r->part_o + r->few_slots * kFewRows * size_t(d.head_dim);
+    a.many_ml = r->part_ml + r->few_slots * kFewRows;
     a.q_stride = s->q_stride; a.out_stride = s->out_stride;
     a.k_stride = c->k_page_stride ? c->k_page_stride : dense;
     a.v_stride = c->v_page_stride ? c->v_page_stride : dense;

@@ -13,8 +13,9 @@ struct mars_reader {
     // Rotary frequencies in 2^-64 turns per position (theta^(-2i/dim) / 2 pi) and the axis of each: rope_dim / 2 entries.
     uint64_t* freq = nullptr;
     int32_t* axis = nullptr;
-    // Split attention: partial outputs, their (max, sum) and one arrival counter per joined tile.
-    // The counters are 0 between calls (the last arriver resets its own).
+    // Split attention: partial outputs and their (max, sum), those of k_attend_few (few_slots x 16 rows) before those of
+    // k_attend_many, and an arrival counter per tile of k_attend_few, 0 between calls (the last arriver resets its own).
+    size_t few_slots = 0;
     float* part_o = nullptr;
     float2* part_ml = nullptr;
     uint32_t* arrived = nullptr;
@@ -24,13 +25,15 @@ namespace mars {
 
 constexpr int32_t kMaxRequests = MARS_KV_MAX_REQUESTS;
 
-// Keys' work items of a launch: about this many chunks over the cache's length. Partial slots:
-// twice as many (a request longer than a chunk of C keys has at most 2 L / C chunks).
-constexpr int32_t kFewItemsLog2 = 10;
+// Workgroups of a k_attend_few launch: as many as 256 CUs hold at a time by their registers. Two partial slots each.
+constexpr int32_t few_groups(int32_t head_dim) { return head_dim == 64 ? 768 : head_dim == 128 ? 512 : 256; }
+// k_attend_many cuts the keys of all its tiles into at most about 2^9 chunks; partial slots for twice as many.
 constexpr int32_t kFewRows = 16;
 constexpr int32_t kFewMost = 16;             // rows of a request that k_attend_few serves best
 constexpr int32_t kManyItemsLog2 = 9;
 constexpr int32_t kManyRows = 128;
+constexpr int32_t kJoinRows = 32;            // of a tile's rows, joined by a workgroup
+constexpr int32_t kMinChunk = 256;           // keys of a work item, unless the request has fewer (a multiple of 256)
 constexpr int32_t kMaxSplits = 256;
 
 struct AttendArgs {
@@ -50,6 +53,8 @@ struct AttendArgs {
     const int32_t* prefix;
     float* part_o;
     float2* part_ml;
+    float* many_o;
+    float2* many_ml;
     uint32_t* arrived;
     int64_t q_stride, out_stride, k_stride, v_stride;
     uint32_t q_flip;       // sign bits of a pair of q's elements if the scale is negative
@@ -58,7 +63,7 @@ struct AttendArgs {
     int32_t requests, max_pages, tokens, num_pages;
     int32_t q_heads, kv_heads, group;
     int32_t page_shift;
-    int32_t rows_lo, rows_hi;   // this launch serves requests with rows_lo < rows <= rows_hi (rows = tokens * group)
+    int32_t few_rows;           // requests of up to so many rows are k_attend_few's
 };
 
 int launch_attend(const mars_reader& r, const AttendArgs& a, int32_t max_new, hipStream_t s);
