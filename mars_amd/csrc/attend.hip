@@ -130,7 +130,6 @@ struct SchedLds {
     int64_t sum[3][4];
     uint64_t wsum[4];
     Part part;
-    bool found;
 };
 
 __device__ inline int64_t uniform(int64_t v) {
@@ -180,40 +179,54 @@ __device__ inline Request request_of(const AttendArgs& a, int r) {
 // The launch has enough workgroups for every item (fewer than 2^31); the last ones may find none. JOIN: the items are
 // the blocks of kJoinRows rows of the tiles in several pieces instead, the block's number in Part::slot.
 template <bool JOIN>
-__device__ bool find_item(const AttendArgs& a, uint32_t b, SchedLds& sh) {
-    const int tid = int(threadIdx.x), lane = tid & 63, wave = tid >> 6;
-    const Request first = request_of<false>(a, tid);
-    // the rows of a tile see L - n / 2 keys on average (not less than half of the L keys)
-    int64_t full = 0, mean = 0, tiles_sum = 0;
-    auto add = [&](const Request& q) {
-        full += int64_t(q.tiles) * ((q.keys + 31) >> 5);
-        mean += int64_t(q.tiles) * ((max(q.keys - q.n / 2, q.keys / 2) + 31) >> 5);
-        tiles_sum += q.tiles;
-    };
-    add(first);
-    for (int r0 = 256; r0 < a.requests; r0 += 256) add(request_of<false>(a, r0 + tid));
-    full = wave_sum(full);
-    mean = wave_sum(mean);
-    tiles_sum = wave_sum(tiles_sum);
-    if (lane == 0) { sh.sum[0][wave] = full; sh.sum[1][wave] = mean; sh.sum[2][wave] = tiles_sum; }
-    if (tid == 0) sh.found = false;
-    __syncthreads();
-    int64_t sums[3];
+struct ManySched {
+    const AttendArgs& a;
+    SchedLds& sh;
+    Request q;                 // this thread's, of the 256 that are looked at: r0 on
+    int r0;
+    uint32_t chunk0, chunk, splits, each, items, mine, part;
+    uint32_t before, end, parts_end;   // items before these 256 and up to their end; partial slots up to there
+
+    // false: no request is k_attend_many's. All threads call it, and find(), together.
+    __device__ ManySched(const AttendArgs& args, SchedLds& lds) : a(args), sh(lds) {}
+    __device__ bool start() {
+        const int tid = int(threadIdx.x), lane = tid & 63, wave = tid >> 6;
+        q = request_of<false>(a, tid);
+        // the rows of a tile see L - n / 2 keys on average (not less than half of the L keys)
+        int64_t full = 0, mean = 0, tiles = 0;
+        auto add = [&](const Request& x) {
+            full += int64_t(x.tiles) * ((x.keys + 31) >> 5);
+            mean += int64_t(x.tiles) * ((max(x.keys - x.n / 2, x.keys / 2) + 31) >> 5);
+            tiles += x.tiles;
+        };
+        add(q);
+        for (int r = 256; r < a.requests; r += 256) add(request_of<false>(a, r + tid));
+        full = wave_sum(full);
+        mean = wave_sum(mean);
+        tiles = wave_sum(tiles);
+        if (lane == 0) { sh.sum[0][wave] = full; sh.sum[1][wave] = mean; sh.sum[2][wave] = tiles; }
+        __syncthreads();
+        int64_t sums[3];
 #pragma unroll
-    for (int x = 0; x < 3; ++x) sums[x] = (sh.sum[x][0] + sh.sum[x][1] + sh.sum[x][2] + sh.sum[x][3]) * a.kv_heads;
-    if (sums[2] == 0) return false;
-    constexpr int64_t slots = 1 << kManyItemsLog2;
-    const int64_t per = sums[2] < slots * 3 / 4 ? (sums[0] * 32 + slots - 1) / slots : (sums[1] * 64 + slots - 1) / slots;
-    const uint32_t chunk0 = (uint32_t(min(max(per, int64_t(kMinChunk)), int64_t(INT32_MAX) - 255)) + 255) & ~255u;
-    uint32_t items_before = 0, parts_before = 0;
-    for (int r0 = 0; r0 < a.requests; r0 += 256) {
-        const Request q = r0 ? request_of<false>(a, r0 + tid) : first;
-        const int tiles = q.tiles, keys = q.keys;
+        for (int x = 0; x < 3; ++x) sums[x] = (sh.sum[x][0] + sh.sum[x][1] + sh.sum[x][2] + sh.sum[x][3]) * a.kv_heads;
+        if (sums[2] == 0) return false;
+        constexpr int64_t slots = 1 << kManyItemsLog2;
+        const int64_t per = sums[2] < slots * 3 / 4 ? (sums[0] * 32 + slots - 1) / slots : (sums[1] * 64 + slots - 1) / slots;
+        chunk0 = (uint32_t(min(max(per, int64_t(kMinChunk)), int64_t(INT32_MAX) - 255)) + 255) & ~255u;
+        r0 = 0;
+        end = parts_end = 0;
+        scan();
+        return true;
+    }
+    // The items of requests r0 .. r0 + 255, whose lengths are in q.
+    __device__ void scan() {
+        const int lane = int(threadIdx.x) & 63, wave = int(threadIdx.x) >> 6;
         // no more than kMaxSplits chunks a request
-        const uint32_t chunk = max(chunk0, (uint32_t(keys) + kMaxSplits * 256 - 1) / (kMaxSplits * 256) * 256);
-        const uint32_t splits = max(1u, (uint32_t(keys) + chunk - 1) / chunk);
-        const uint32_t heads = uint32_t(tiles) * uint32_t(a.kv_heads), parts = splits > 1 ? heads * splits : 0;
-        const uint32_t each = JOIN ? (splits > 1 ? kManyRows / kJoinRows : 0) : splits, items = heads * each;
+        chunk = max(chunk0, (uint32_t(q.keys) + kMaxSplits * 256 - 1) / (kMaxSplits * 256) * 256);
+        splits = max(1u, (uint32_t(q.keys) + chunk - 1) / chunk);
+        const uint32_t heads = uint32_t(q.tiles) * uint32_t(a.kv_heads), parts = splits > 1 ? heads * splits : 0;
+        each = JOIN ? (splits > 1 ? kManyRows / kJoinRows : 0) : splits;
+        items = heads * each;
         uint32_t xi = items, xp = parts;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
@@ -223,40 +236,50 @@ __device__ bool find_item(const AttendArgs& a, uint32_t b, SchedLds& sh) {
         __syncthreads();
         if (lane == 63) sh.wsum[wave] = (uint64_t(xi) << 32) | xp;
         __syncthreads();
-        uint32_t bi = items_before, bp = parts_before;
+        before = end;
+        mine = end + xi - items;
+        part = parts_end + xp - parts;
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
             const uint64_t s = sh.wsum[w];
-            if (w < wave) { bi += uint32_t(s >> 32); bp += uint32_t(s); }
-            items_before += uint32_t(s >> 32);
-            parts_before += uint32_t(s);
+            if (w < wave) { mine += uint32_t(s >> 32); part += uint32_t(s); }
+            end += uint32_t(s >> 32);
+            parts_end += uint32_t(s);
         }
-        const uint32_t mine = bi + xi - items;
+    }
+    // Item b into *out, for calls with rising b; false: there are not so many.
+    __device__ bool find(uint32_t b, Part* out) {
+        while (b >= end) {
+            r0 += 256;
+            if (r0 >= a.requests) return false;
+            q = request_of<false>(a, r0 + int(threadIdx.x));
+            scan();
+        }
+        __syncthreads();                                     // the item before has been read
         if (b >= mine && b - mine < items) {
             const uint32_t local = b - mine, tile_head = local / each, tile = tile_head / uint32_t(a.kv_heads);
             const int32_t split = int32_t(local - tile_head * each), c = int32_t(min(chunk, uint32_t(INT32_MAX / 2)));
             Part& pt = sh.part;
-            pt.request = r0 + tid;
-            pt.tile = int32_t(uint32_t(tiles) - 1 - tile);   // later rows see more keys: first
+            pt.request = r0 + int(threadIdx.x);
+            pt.tile = int32_t(uint32_t(q.tiles) - 1 - tile); // later rows see more keys: first
             pt.head = int32_t(tile_head - tile * uint32_t(a.kv_heads));
             pt.row0 = q.row0;
             pt.n = q.n;
-            pt.keys = keys;
+            pt.keys = q.keys;
             pt.chunk = c;
             pt.k0 = split * c;
-            pt.k1 = min(keys, pt.k0 + c);
+            pt.k1 = min(q.keys, pt.k0 + c);
             pt.splits = int32_t(splits);
-            pt.slot0 = int32_t(bp + xp - parts + tile_head * splits);
+            pt.slot0 = int32_t(part + tile_head * splits);
             pt.slot1 = pt.slot0 + 1;
             pt.slot_step = 1;
             pt.slot = JOIN ? split : pt.slot0 + split;
-            sh.found = true;
         }
-        if (b < items_before) break;
+        __syncthreads();
+        *out = uniform_part(sh.part);
+        return true;
     }
-    __syncthreads();
-    return sh.found;
-}
+};
 
 // Partials pass between workgroups of one launch, on any XCD: as relaxed atomics of agent scope, which go through to
 // where every XCD sees them, the writers' completed before they count themselves in. (Plain stores and a fence at agent
@@ -934,8 +957,11 @@ __device__ void many_rows(const AttendArgs& a, int block, ManyShared<D>& lds) {
     constexpr int KS = D / 16, DB = D / 32, RC = D / 8;      // k-steps of S, blocks of O, 16-byte pieces of a key's row
     StepLds& list = lds.list;
     ManyLds<D>& sh = lds.tiles;
-    if (!find_item<false>(a, block, lds.sched)) return;
-    Part it = uniform_part(lds.sched.part);
+    Part it;
+    {
+        ManySched<false> sched(a, lds.sched);
+        if (!sched.start() || !sched.find(uint32_t(block), &it)) return;
+    }
     if (!own_pieces(a, &it, it.slot - it.slot0)) return;
     __syncthreads();                                         // the item is read before its LDS is used again
     const int tid = int(threadIdx.x), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -1219,11 +1245,11 @@ __device__ void many_rows(const AttendArgs& a, int block, ManyShared<D>& lds) {
 // partials of 8 pieces on the way together; the sums are taken in the order of the pieces.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void k_attend_join(AttendArgs a) {
-    __shared__ SchedLds sched;
-    for (int block = int(blockIdx.x);; block += int(gridDim.x)) {
-    if (!find_item<true>(a, block, sched)) return;
-    Part it = uniform_part(sched.part);
-    __syncthreads();                                         // the item is read before the next is looked for
+    __shared__ SchedLds lds;
+    ManySched<true> sched(a, lds);
+    if (!sched.start()) return;
+    Part it;
+    for (uint32_t block = blockIdx.x; sched.find(block, &it); block += gridDim.x) {
     const int r0 = it.slot * kJoinRows, rows = min(kJoinRows, it.n * a.group - it.tile * kManyRows - r0);
     if (!own_pieces(a, &it, 0) || it.splits == 1) continue;
     const float2* const ml = a.many_ml + int64_t(it.slot0) * kManyRows + r0;

@@ -32,7 +32,7 @@ constexpr int32_t kFewRows = 16;
 constexpr int32_t kFewMost = 16;             // rows of a request that k_attend_few serves best
 constexpr int32_t kManyItemsLog2 = 9;
 constexpr int32_t kManyRows = 128;
-constexpr int32_t kJoinRows = 32;            // of a tile's rows, joined by a workgroup
+constexpr int32_t kJoinRows = 16;            // of a tile's rows, joined by a workgroup
 constexpr int32_t kMinChunk = 256;           // keys of a work item, unless the request has fewer (a multiple of 256)
 constexpr int32_t kMaxSplits = 256;
 
