@@ -22,7 +22,7 @@ namespace {
 // it to the table, so no workgroup waits for another's writes. Launch and latency bound: two
 // block scans and a dozen dependent LDS reads.
 constexpr int kPlanThreads = 512;
-constexpr int kPlanTokens = 4096;                        // rows of the step per workgroup
+constexpr int kPlanTokens = 1024;                        // rows of the step per workgroup
 constexpr int kPlanPer = kMaxRequests / kPlanThreads;    // requests per thread, consecutive
 
 // Exclusive prefix of v over the block's threads; *total = the block's sum.
@@ -110,13 +110,13 @@ __global__ __launch_bounds__(kPlanThreads) void k_kv_plan(mars_kv_plan_args a, i
     if (blockIdx.x == 0)
         for (int r = tid; r <= R; r += kPlanThreads) a.q_start[r] = start[r];
 
-    // the pages handed out: the requests dealt over the workgroups' waves
-    const int wave = int(blockIdx.x) * (kPlanThreads / 64) + (tid >> 6), waves = int(gridDim.x) * (kPlanThreads / 64);
-    for (int r = wave; r < R; r += waves) {
+    // the pages handed out: the requests dealt over the workgroups' threads, 8 to each
+    const int eighth = (int(blockIdx.x) * kPlanThreads + tid) >> 3, eighths = int(gridDim.x) * kPlanThreads >> 3;
+    for (int r = eighth; r < R; r += eighths) {
         if (fresh[r] < 0) continue;
         const int64_t len = int64_t(cached[r]) + (start[r + 1] - start[r]);
         const int have = int((int64_t(cached[r]) + page - 1) >> page_shift), pages = int((len + page - 1) >> page_shift);
-        for (int j = have + (tid & 63); j < pages; j += 64)
+        for (int j = have + (tid & 7); j < pages; j += 8)
             a.block_table[int64_t(r) * a.max_pages + j] = a.free_pages[free - 1 - (fresh[r] + j - have)];
     }
     // slots and positions of this workgroup's rows
@@ -193,7 +193,8 @@ __device__ inline void turn(int32_t pos, uint64_t f, float* sn, float* cs) {
     sincospif(float(int32_t(uint32_t(phase >> 32))) * 0x1p-31f, sn, cs);
 }
 
-// One workgroup: one token. Threads over (head, pair); values one by one.
+// Few tokens: a workgroup to each, a pair of values a thread and turn. Latency bound.
+constexpr int32_t kStoreFew = 256;
 template <typename T>
 __global__ __launch_bounds__(256) void k_kv_store(StoreArgs a) {
     const int t = int(blockIdx.x), half = a.rope_dim / 2, D = a.head_dim;
@@ -229,6 +230,140 @@ __global__ __launch_bounds__(256) void k_kv_store(StoreArgs a) {
         static_cast<T*>(a.v_pages)[page * a.v_stride + int64_t(e) * P + off] = v[t * a.s.v_stride + e];
     if (threadIdx.x == 0 && a.times && a.s.times) a.times[slot] = a.s.times[t];
     if (threadIdx.x == 0 && a.eps && a.s.episodes) a.eps[slot] = a.s.episodes[t];
+}
+
+// Many tokens: a workgroup takes kTile of them under one kv head: its k and v, and the group's q heads. The angles of the
+// tokens are computed once a workgroup (LDS), q and k move in pieces of 16 bytes, and v, whose pages hold the tokens of an
+// element side by side, goes through LDS: where 8 consecutive tokens fill 8 consecutive slots from a multiple of 8 on
+// they are written as 16 bytes, and the lanes of a wave fill whole rows of a page; other tokens value by value.
+// Bound by the bytes in and out: 4,099 tokens of 32/8 heads of 128, 101 MB, SSS.
+template <int D>
+constexpr int store_tile() { return D == 256 ? 32 : 64; }
+
+template <typename T, int D>
+__global__ __launch_bounds__(256) void k_kv_store_tile(StoreArgs a) {
+    typedef T v8 __attribute__((ext_vector_type(8)));
+    constexpr int kTile = store_tile<D>(), VS = D + 2;
+    __shared__ __attribute__((aligned(16))) float2 turns[kTile][D / 2];          // cos, sin
+    __shared__ __attribute__((aligned(16))) T vt[kTile][VS];
+    __shared__ int64_t slot_of[kTile];
+    __shared__ uint8_t lead[kTile];                          // first of 8 written together
+    __shared__ uint8_t groups[kTile / 8], singles[kTile];
+    __shared__ int counts[2];
+    const int t0 = int(blockIdx.x) * kTile, head = int(blockIdx.y), tid = int(threadIdx.x);
+    const int nt = min(kTile, a.s.num_tokens - t0), half = a.rope_dim / 2, P = 1 << a.page_shift;
+    const T* const q = static_cast<const T*>(a.s.q);
+    const T* const k = static_cast<const T*>(a.s.k);
+    const T* const v = static_cast<const T*>(a.s.v);
+    const int group = q ? a.q_heads / a.kv_heads : 0;
+
+    if (tid < kTile) {
+        const int64_t s = k && tid < nt ? a.s.slots[t0 + tid] : -1;
+        slot_of[tid] = s >= 0 && s < a.slots ? s : -1;
+    }
+    if (v) {
+        for (int e = tid; e < nt * (D / 8); e += 256) {
+            const int i = e / (D / 8), c = e % (D / 8);
+            const v8 x = *reinterpret_cast<const v8*>(v + (t0 + i) * a.s.v_stride + head * D + c * 8);
+            typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+            const u4 w = __builtin_bit_cast(u4, x);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) reinterpret_cast<uint32_t*>(&vt[i][c * 8])[j] = w[j];
+        }
+    }
+    for (int e = tid; e < nt * half; e += 256) {
+        const int i = e / half, f = e % half;
+        float sn, cs;
+        turn(a.s.positions[int64_t(a.axis[f]) * a.s.num_tokens + t0 + i], a.freq[f], &sn, &cs);
+        turns[i][f] = make_float2(cs, a.s.inverse ? -sn : sn);
+    }
+    __syncthreads();
+    if (k && tid < kTile) {
+        const int64_t s = slot_of[tid];
+        bool first = s >= 0 && s % 8 == 0 && tid + 8 <= nt;
+        for (int j = 1; j < 8 && first; ++j) first = slot_of[tid + j] == s + j;
+        lead[tid] = first;
+    }
+    __syncthreads();
+    if (k && tid < 64) {                                     // one wave: the groups, and the tokens of none
+        const bool in = tid < kTile && slot_of[tid] >= 0;
+        const int at = in ? int(slot_of[tid] % 8) : 0;
+        const bool first = tid < kTile && lead[tid], alone = in && !(tid >= at && lead[tid - at]);
+        const uint64_t gs = __ballot(first), ss = __ballot(alone), below = (1ull << tid) - 1;
+        if (first) groups[__popcll(gs & below)] = uint8_t(tid);
+        if (alone) singles[__popcll(ss & below)] = uint8_t(tid);
+        if (tid == 0) { counts[0] = __popcll(gs); counts[1] = __popcll(ss); }
+        if (head == 0 && in) {
+            if (a.times && a.s.times) a.times[slot_of[tid]] = a.s.times[t0 + tid];
+            if (a.eps && a.s.episodes) a.eps[slot_of[tid]] = a.s.episodes[t0 + tid];
+        }
+    }
+
+    // q and k: a thread takes two pieces of 8 elements of a head, the partners of each other where they turn (both are read
+    // before either is written: q_out may be q)
+    const int heads = group + (k ? 1 : 0), turning = half / 8;
+    for (int e = tid; e < nt * heads * (D / 16); e += 256) {
+        const int c = e % (D / 16), ih = e / (D / 16), i = ih / heads, hh = ih % heads;
+        const bool is_q = hh < group;
+        if (!is_q && slot_of[i] < 0) continue;
+        const T* const x = is_q ? q + (t0 + i) * a.s.q_stride + (head * group + hh) * D : k + (t0 + i) * a.s.k_stride + head * D;
+        T* const to = is_q ? static_cast<T*>(a.s.q_out) + (t0 + i) * a.s.q_out_stride + (head * group + hh) * D
+                           : static_cast<T*>(a.k_pages) + (slot_of[i] >> a.page_shift) * a.k_stride + (int64_t(head) * P + (slot_of[i] & (P - 1))) * D;
+        const bool turns_c = c < turning;
+        const int p0 = turns_c && !a.adjacent ? c * 8 : c * 16, p1 = turns_c && !a.adjacent ? half + c * 8 : c * 16 + 8;
+        const v8 y = *reinterpret_cast<const v8*>(x + p0), z = *reinterpret_cast<const v8*>(x + p1);
+        v8 u = y, w = z;
+        if (turns_c && !a.adjacent) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float2 f = turns[i][c * 8 + j];
+                const float yy = float(y[j]), zz = float(z[j]);
+                u[j] = T(yy * f.x - zz * f.y);
+                w[j] = T(yy * f.y + zz * f.x);
+            }
+        } else if (turns_c) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float2 f = turns[i][c * 8 + j];        // pair j of the 16 elements
+                const float yy = float(j < 4 ? y[2 * j] : z[2 * j - 8]), zz = float(j < 4 ? y[2 * j + 1] : z[2 * j - 7]);
+                const T lo = T(yy * f.x - zz * f.y), hi = T(yy * f.y + zz * f.x);
+                if (j < 4) { u[2 * j] = lo; u[2 * j + 1] = hi; }
+                else { w[2 * j - 8] = lo; w[2 * j - 7] = hi; }
+            }
+        }
+        *reinterpret_cast<v8*>(to + p0) = u;
+        *reinterpret_cast<v8*>(to + p1) = w;
+    }
+    if (!v) return;
+    __syncthreads();
+    T* const vp = static_cast<T*>(a.v_pages) + int64_t(head) * D * P;
+    const int ng = counts[0], ns = counts[1];
+    for (int e = tid; e < ng * D; e += 256) {
+        const int d = e / ng, i = groups[e % ng];
+        v8 x;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = vt[i + j][d];
+        *reinterpret_cast<v8*>(vp + (slot_of[i] >> a.page_shift) * a.v_stride + (int64_t(d) << a.page_shift) + (slot_of[i] & (P - 1))) = x;
+    }
+    for (int e = tid; e < ns * D; e += 256) {
+        const int d = e / ns, i = singles[e % ns];
+        vp[(slot_of[i] >> a.page_shift) * a.v_stride + (int64_t(d) << a.page_shift) + (slot_of[i] & (P - 1))] = vt[i][d];
+    }
+}
+
+template <typename T, int D>
+int launch_store_tile(const StoreArgs& a, hipStream_t s) {
+    const unsigned tiles = unsigned((a.s.num_tokens + store_tile<D>() - 1) / store_tile<D>());
+    MARS_LAUNCH((k_kv_store_tile<T, D>), dim3(tiles, unsigned(a.kv_heads)), dim3(256), 0, s, a);
+    return MARS_OK;
+}
+template <typename T>
+int launch_store(const StoreArgs& a, hipStream_t s) {
+    if (a.s.num_tokens <= kStoreFew) {
+        MARS_LAUNCH((k_kv_store<T>), dim3(unsigned(a.s.num_tokens)), dim3(256), 0, s, a);
+        return MARS_OK;
+    }
+    return a.head_dim == 64 ? launch_store_tile<T, 64>(a, s) : a.head_dim == 128 ? launch_store_tile<T, 128>(a, s) : launch_store_tile<T, 256>(a, s);
 }
 
 int check_cache(const mars_reader& r, const mars_kv_cache& c) {
@@ -389,9 +524,7 @@ int mars_kv_store(const mars_reader* r, const mars_kv_cache* c, const mars_kv_st
     a.page_shift = r->page_shift;
     MARS_TRY(use_device(r->device));
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    if (d.dtype == MARS_DTYPE_F16) MARS_LAUNCH((k_kv_store<_Float16>), dim3(unsigned(s->num_tokens)), dim3(256), 0, st, a);
-    else MARS_LAUNCH((k_kv_store<__bf16>), dim3(unsigned(s->num_tokens)), dim3(256), 0, st, a);
-    return MARS_OK;
+    return d.dtype == MARS_DTYPE_F16 ? launch_store<_Float16>(a, st) : launch_store<__bf16>(a, st);
 }
 
 int mars_kv_attend(const mars_reader* r, const mars_kv_cache* c, const mars_kv_attend_args* s, void* stream) {

@@ -72,27 +72,38 @@ class DeviceArray:
     def stride(self, i: int) -> int:
         return self._strides[i]
 
+    def is_contiguous(self) -> bool:
+        return True
+
+
+def _dense(x) -> bool:
+    try:
+        return x.is_contiguous()
+    except AttributeError:
+        n = 1
+        for i in range(len(x.shape) - 1, -1, -1):
+            if x.shape[i] != 1 and x.stride(i) != n:
+                return False
+            n *= x.shape[i]
+        return True
+
 
 def _arg(x, name: str, dtype: str, shape=None) -> Optional[int]:
     """The address of a dense array of the given type and shape (None: any length)."""
     if x is None:
         return None
-    if _dtype(x) != dtype:
+    if _NAMES.get(x.dtype) != dtype and _dtype(x) != dtype:
         raise ValueError(f"{name}: {_dtype(x)}, expected {dtype}")
-    have = x.shape
-    if shape is not None and tuple(have) != shape:
-        raise ValueError(f"{name}: shape {tuple(have)}, expected {shape}")
-    n = 1
-    for i in range(len(have) - 1, -1, -1):
-        if have[i] != 1 and x.stride(i) != n:
-            raise ValueError(f"{name}: not dense")
-        n *= have[i]
+    if shape is not None and x.shape != shape:
+        raise ValueError(f"{name}: shape {tuple(x.shape)}, expected {shape}")
+    if not _dense(x):
+        raise ValueError(f"{name}: not dense")
     return x.data_ptr()
 
 
 def _rows(x, name: str, dtype: str, tokens: Optional[int], heads: int, dim: int):
     """Address and token stride of a (tokens, heads, dim) array with dense heads."""
-    if _dtype(x) != dtype:
+    if _NAMES.get(x.dtype) != dtype and _dtype(x) != dtype:
         raise ValueError(f"{name}: {_dtype(x)}, expected {dtype}")
     s = x.shape
     if len(s) != 3 or s[1] != heads or s[2] != dim or (tokens is not None and s[0] != tokens):
@@ -120,6 +131,7 @@ class PagedCache:
         self.k_pages, self.v_pages, self.times, self.episodes = k_pages, v_pages, times, episodes
         self.num_pages, self.kv_heads, self.page_size, self.head_dim = n, h, p, d
         self.dtype = _dtype(k_pages)
+        self.geometry = (h, p, d, self.dtype)
         strides = [x.stride(0) if n > 1 else 0 for x in (k_pages, v_pages)]
         for name, x, want in (("times", times, "float32"), ("episodes", episodes, "int32")):
             if x is not None and int(np.prod(tuple(x.shape), dtype=np.int64)) != n * p:
@@ -144,6 +156,7 @@ class Reader:
         self.q_heads, self.kv_heads = int(q_heads), int(q_heads if kv_heads is None else kv_heads)
         self.head_dim, self.dtype, self.page_size = int(head_dim), dtype, int(page_size)
         self.rope_dim, self.rope_axes = int(rope_dim), len(sections)
+        self.geometry = (self.kv_heads, self.page_size, self.head_dim, self.dtype)
         desc = _lib.ReaderDescC(self.q_heads, self.kv_heads, self.head_dim, _DTYPES[dtype], self.page_size, self.rope_dim,
                                 self.rope_axes, int(bool(rope_adjacent)),
                                 (C.c_int32 * 3)(*(list(sections) + [0] * (3 - len(sections)))), 0, float(rope_theta))
@@ -162,7 +175,7 @@ class Reader:
             pass
 
     def _cache(self, cache: PagedCache):
-        if (cache.kv_heads, cache.page_size, cache.head_dim, cache.dtype) != (self.kv_heads, self.page_size, self.head_dim, self.dtype):
+        if cache.geometry != self.geometry:
             raise ValueError(f"cache of {cache.kv_heads} heads of {cache.head_dim}, pages of {cache.page_size}, {cache.dtype}; the reader has "
                              f"{self.kv_heads}, {self.head_dim}, {self.page_size}, {self.dtype}")
         return cache.ref
@@ -170,10 +183,10 @@ class Reader:
     def plan(self, new_lens, cached_lens, block_table, free_pages, free_count, *, q_start, kv_lens, slots, positions,
              free_count_out, stream: int = 0) -> None:
         """Block table rows extended, and q_start, kv_lens, slots, positions of a step (mars_kv_plan)."""
-        r, t = int(new_lens.shape[0]), int(slots.shape[0])
+        r, t = new_lens.shape[0], slots.shape[0]
         if len(block_table.shape) != 2:
             raise ValueError(f"block_table: shape {tuple(block_table.shape)}, expected (requests, pages)")
-        width = int(block_table.shape[1])
+        width = block_table.shape[1]
         a = _lib.KvPlanArgsC(
             _arg(new_lens, "new_lens", "int32", (r,)), _arg(cached_lens, "cached_lens", "int32", (r,)),
             _arg(block_table, "block_table", "int32", (r, width)), _arg(free_pages, "free_pages", "int32"),
@@ -225,17 +238,19 @@ class Reader:
                cap: float = 0.0, decay=None, q_times=None, q_episodes=None, prefix_lens=None, max_new: int = 0,
                stream: int = 0) -> None:
         """Attention of each request's rows of q over its cached tokens, into out (mars_kv_attend)."""
-        t, r = int(q.shape[0]), int(kv_lens.shape[0])
+        t, r = q.shape[0], kv_lens.shape[0]
         ref = self._cache(cache)
         qp, qs = _rows(q, "q", self.dtype, None, self.q_heads, self.head_dim)
         op, os_ = _rows(out, "out", self.dtype, t, self.q_heads, self.head_dim)
         if len(block_table.shape) != 2:
             raise ValueError(f"block_table: shape {tuple(block_table.shape)}, expected (requests, pages)")
-        width = int(block_table.shape[1])
+        width = block_table.shape[1]
         a = _lib.KvAttendArgsC(
             qp, op, _arg(lse, "lse", "float32", (t, self.q_heads)), _arg(q_start, "q_start", "int32", (r + 1,)),
             _arg(kv_lens, "kv_lens", "int32", (r,)), _arg(block_table, "block_table", "int32", (r, width)),
             _arg(decay, "decay", "float32", (self.q_heads,)), _arg(q_times, "q_times", "float32", (t,)),
             _arg(q_episodes, "q_episodes", "int32", (t,)), _arg(prefix_lens, "prefix_lens", "int32", (r,)),
             qs, os_, scale, cap, r, width, t, max_new)
-        check(lib.mars_kv_attend(self.handle, ref, C.byref(a), stream), "mars_kv_attend")
+        rc = lib.mars_kv_attend(self.handle, ref, C.byref(a), stream)
+        if rc:
+            check(rc, "mars_kv_attend")

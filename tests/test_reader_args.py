@@ -70,6 +70,7 @@ def a_reader(**kw):
     """A Reader without a device behind it: every call below is refused before its handle is used."""
     r = Reader.__new__(Reader)
     r.q_heads, r.kv_heads, r.head_dim, r.dtype, r.page_size, r.rope_dim, r.rope_axes = 4, 2, 64, "float16", 16, 64, 1
+    r.geometry = (2, 16, 64, "float16")
     r.handle = C.c_void_p()
     for k, v in kw.items():
         setattr(r, k, v)
