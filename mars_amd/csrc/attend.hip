@@ -510,7 +510,7 @@ struct FewLds {
 };
 // Keys of a step: what the registers of two waves a SIMD hold, K and V and what the extra terms need.
 template <int D, bool EXTRA>
-constexpr int few_step() { return D > 128 || (D == 128 && EXTRA) ? 32 : 64; }
+constexpr int few_step() { return D > 128 || EXTRA ? 32 : 64; }
 
 template <typename T, int D, bool EXTRA, int STEP>
 __device__ void few_part(const AttendArgs& a, const Part& it, FewLds<D>& lds) {
@@ -790,7 +790,7 @@ __device__ void few_part(const AttendArgs& a, const Part& it, FewLds<D>& lds) {
 // of G takes the w-th of G equal lengths of it: the bytes of the cache are dealt out evenly whatever the requests'
 // lengths, in one round. An end of a length that falls within kFewCut steps of a tile's first or last one moves there
 // (short requests are not cut), so a workgroup has at most two pieces that others share: its first and its last.
-constexpr int kFewCut = 4;
+constexpr int kFewCut = 4, kFewSpan = 1;
 struct SpanLds {
     int64_t start[257];        // of 256 requests: steps of the launch before each
     int32_t row0[256], n[256], keys[256];
@@ -853,7 +853,7 @@ __device__ void few_rows(const AttendArgs& a, int block, int blocks, FewShared<D
     const int most = __builtin_amdgcn_readfirstlane(sp.most);
     if (a.requests > 256) end = load_span(a, 0, 0, STEP, sp);            // back to the first
     // no tile in more than kMaxSplits pieces
-    const int64_t span = max((total + blocks - 1) / blocks, int64_t((most + kMaxSplits - 2) / (kMaxSplits - 1))), x0 = w * span, x1 = min(x0 + span, total);
+    const int64_t span = max(max((total + blocks - 1) / blocks, int64_t(kFewSpan)), int64_t((most + kMaxSplits - 2) / (kMaxSplits - 1))), x0 = w * span, x1 = min(x0 + span, total);
     if (x0 >= total) return;                                // no steps at all, or none for this workgroup
     while (x0 >= end) {
         r0 += 256;
@@ -1291,7 +1291,7 @@ __global__ __launch_bounds__(256) void k_attend_join(AttendArgs a) {
 
 // ---- the kernels ------------------------------------------------------------------------
 template <typename T, int D, bool EXTRA>
-__global__ __launch_bounds__(256, D > 128 ? 1 : 2) void k_attend_few(AttendArgs a) {
+__global__ __launch_bounds__(256, D > 128 ? 1 : D == 128 ? 2 : 3) void k_attend_few(AttendArgs a) {
     __shared__ __attribute__((aligned(16))) FewShared<D> lds;
     few_rows<T, D, EXTRA, few_step<D, EXTRA>()>(a, int(blockIdx.x), int(gridDim.x), lds);
 }
