@@ -405,7 +405,7 @@ __device__ void join_last(const AttendArgs& a, const Part& it, JoinLds& lds) {
 // least and the greatest of the rows' (exact where the rows ask within one episode, as single tokens do, and where
 // episodes follow each other). Entry: the step within the window, kMixed added where rows and keys have to be compared
 // one by one.
-constexpr int kWindow = 512, kMixed = 1 << 15;
+constexpr int kWindow = 128, kMixed = 1 << 15;
 struct StepLds {
     uint16_t flag[kWindow], list[kWindow];
     int count;

@@ -534,7 +534,7 @@ int mars_kv_attend(const mars_reader* r, const mars_kv_cache* c, const mars_kv_a
     MARS_CHECK(s->num_requests <= kMaxRequests, MARS_ERR_CAPACITY, "%d requests (at most %d)", s->num_requests, kMaxRequests);
     MARS_TRY(check_cache(*r, *c));
     const mars_reader_desc& d = r->d;
-    MARS_CHECK(int64_t(s->max_pages) * d.page_size <= INT32_MAX, MARS_ERR_CAPACITY, "%d pages of %d tokens a row", s->max_pages, d.page_size);
+    MARS_CHECK(int64_t(s->max_pages) * d.page_size <= (1 << 30), MARS_ERR_CAPACITY, "%d pages of %d tokens a row", s->max_pages, d.page_size);
     MARS_CHECK(int64_t(s->num_tokens) * d.q_heads <= INT32_MAX, MARS_ERR_CAPACITY, "%d tokens of %d heads", s->num_tokens, d.q_heads);
     MARS_TRY(check_rows("q", s->q, s->q_stride, int64_t(d.q_heads) * d.head_dim));
     MARS_TRY(check_rows("out", s->out, s->out_stride, int64_t(d.q_heads) * d.head_dim));

@@ -379,6 +379,40 @@ def test_attend_many_requests():
         check_attend(Reader(2, 1, 64, "float16", 16), "float16", q, k, v, q_start, lens, table, max_new=(0, 2))
 
 
+@pytest.mark.parametrize("n,requests", [(1, 300), (20, 96), (40, 300)])
+def test_attend_shared_pages_and_long_lists(n, requests):
+    """Requests that share the pages of one long context, each within an episode of its own: lists of steps longer than a
+    window, more requests than a workgroup looks at together, tiles enough that no keys are split."""
+    rng = np.random.default_rng(n)
+    L, hq, hkv, D, page, dtype = (8_300 if n == 20 else 700), 4, 4, 64, 16, "float16"
+    one, k, v = make_cache(rng, [L], hkv, D, dtype, page)
+    table = np.repeat(one, requests, 0)
+    k_eps = np.full(k.shape[0] * page, -9, np.int32)
+    j = np.arange(L)
+    k_eps[table[0][j // page] * page + j % page] = np.where(j < 30, -1, j // 50)
+    q_eps = np.repeat(rng.integers(-1, L // 50, requests), n).astype(np.int32)
+    q_eps[0] = L // 50 - 1
+    q = ref.to_bits(rng.standard_normal((n * requests, hq, D)), dtype)
+    check_attend(Reader(hq, hkv, D, dtype, page), dtype, q, k, v, np.arange(requests + 1) * n, [L] * requests, table, max_new=(0, n),
+                 q_eps=q_eps, k_eps=k_eps)
+
+
+@pytest.mark.parametrize("requests,spread", [(3, 0), (40, 400), (200, 37), (600, 300)])
+def test_attend_spans(requests, spread):
+    """Lengths dealt out to workgroups: pieces that begin and end inside requests, at their edges, and requests too short to cut."""
+    rng = np.random.default_rng(requests)
+    hq, hkv, D, page, dtype = 2, 1, 64, 16, "bfloat16"
+    L = 2_600
+    one, k, v = make_cache(rng, [L], hkv, D, dtype, page)
+    lens = [int(x) for x in np.clip(rng.integers(0, spread + 1, requests) * rng.integers(0, 12, requests) + (L if requests == 3 else 0), 0, L)]
+    table = np.repeat(one, requests, 0)
+    q = ref.to_bits(rng.standard_normal((requests, hq, D)), dtype)
+    check_attend(Reader(hq, hkv, D, dtype, page), dtype, q, k, v, np.arange(requests + 1), lens, table, max_new=(1,),
+                 decay=np.full(hq, 0.01, np.float32), q_times=np.full(requests, 600, np.float32),
+                 k_times=rng.uniform(0, 600, k.shape[0] * page).astype(np.float32))
+    check_attend(Reader(hq, hkv, D, dtype, page), dtype, q, k, v, np.arange(requests + 1), lens, table, max_new=(0, 1))
+
+
 @pytest.mark.parametrize("n", [1, 40])
 def test_attend_rows_that_see_nothing(n):
     """Requests that were not served (kv_lens 0), episodes without a token, ages that leave no weight: rows of zeros, lse -inf."""
