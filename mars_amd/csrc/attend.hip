@@ -56,6 +56,20 @@ __device__ inline void lds_barrier() {
     asm volatile("" ::: "memory");
 }
 
+// A pointer the wave holds in SGPRs (the same in every lane), for loads of the form scalar base plus 32-bit offset: the
+// compiler does not see what it is made of, or it would add the lane's offset to a part of it ahead of the loop and form
+// 64-bit addresses in vector registers.
+__device__ inline const char* uniform_ptr(const char* p) {
+    uint64_t u = reinterpret_cast<uint64_t>(p);
+    u = uint64_t(uint32_t(__builtin_amdgcn_readfirstlane(int(u >> 32)))) << 32 | uint32_t(__builtin_amdgcn_readfirstlane(int(u)));
+    asm volatile("" : "+s"(u));
+    return reinterpret_cast<const char*>(u);
+}
+__device__ inline uint32_t here(uint32_t v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
+
 // 16 (or 4) bytes per lane from global memory straight into LDS: lane l's go to lds + 16 l (4 l) bytes.
 __device__ inline void dma16(const void* g, void* lds) { __builtin_amdgcn_global_load_lds(g, (__attribute__((address_space(3))) void*)lds, 16, 0, 0); }
 __device__ inline void dma4(const void* g, void* lds) { __builtin_amdgcn_global_load_lds(g, (__attribute__((address_space(3))) void*)lds, 4, 0, 0); }
@@ -1024,8 +1038,12 @@ __device__ void many_rows(const AttendArgs& a, int block, ManyShared<D>& lds) {
     constexpr int KR = 256 / RC;                             // rows of K per load of the workgroup
     const int krow = tid / RC, kpiece = (tid % RC) ^ kswz(krow), vrow = tid >> 3, vkey = ((tid & 7) ^ vswz(vrow)) * 8;
     static_assert(KR % 16 == 0 || D == 256, "a thread's pieces keep their place in the row");
-    const char* const kp = static_cast<const char*>(a.k_pages) + ((int64_t(head) << a.page_shift) * D + krow % 16 * D) * 2;
-    const char* const vp = static_cast<const char*>(a.v_pages) + ((int64_t(head) << a.page_shift) * D + (int64_t(vrow) << a.page_shift)) * 2;
+    // a thread's place in a row of pieces is the same for every load: addresses are a scalar base and a constant offset
+    const char* const kp = static_cast<const char*>(a.k_pages) + (int64_t(head) << a.page_shift) * D * 2;
+    const char* const vp = static_cast<const char*>(a.v_pages) + (int64_t(head) << a.page_shift) * D * 2;
+    const uint32_t k_at = uint32_t(krow % 16 * D * 2 + kpiece * 16);
+    const uint32_t k_at2 = D == 256 ? uint32_t((krow + 8) * D * 2 + ((tid % RC) ^ kswz(krow + 8)) * 16) : k_at;     // odd loads
+    const uint32_t v_at = uint32_t((vrow << a.page_shift) + vkey) * 2;
     int pages[4];                                            // of the next tile's 4 groups of 16 keys
     auto find_pages = [&](int s) {
 #pragma unroll
@@ -1037,18 +1055,21 @@ __device__ void many_rows(const AttendArgs& a, int block, ManyShared<D>& lds) {
         for (int j = 0; j < RC / 4; ++j) {
             const int u = KR == 32 ? 2 * j + (wave >> 1) : (j * KR) >> 4;      // the wave's rows lie in this group of 16 keys
             const int pg = KR == 32 ? (wave >> 1 ? pages[2 * j + 1] : pages[2 * j]) : pages[(j * KR) >> 4];
-            const char* const base = kp + (pg * a.k_stride + int64_t((kt + u * 16) & P1) * D) * 2;
-            const int piece = D == 256 ? (tid % RC) ^ kswz(krow + j * KR) : kpiece;
-            const int off = (D == 256 ? (j * KR) % 16 * D * 2 : 0) + piece * 16;
-            dma16(base + off, &sh.k[buf][j * 256 + wave * 64]);
+            const char* const base = uniform_ptr(kp + (pg * a.k_stride + int64_t((kt + u * 16) & P1) * D) * 2);
+            dma16(base + here(D == 256 && j % 2 ? k_at2 : k_at), &sh.k[buf][j * 256 + wave * 64]);
         }
-        const int g = vkey >> 4;
-        const int64_t b0 = pages[0] * a.v_stride + ((kt) & P1), b1 = pages[1] * a.v_stride + ((kt + 16) & P1);
-        const int64_t b2 = pages[2] * a.v_stride + ((kt + 32) & P1), b3 = pages[3] * a.v_stride + ((kt + 48) & P1);
-        const char* const p = vp + ((g & 2 ? (g & 1 ? b3 : b2) : (g & 1 ? b1 : b0)) + (vkey & 15)) * 2;
+        if (a.page_shift >= 6) {                             // the tile lies in one page
 #pragma unroll
-        for (int j = 0; j < RC / 4; ++j)
-            dma16(p + (int64_t(j) * 64 << a.page_shift), &sh.v[buf][j * 256 + wave * 64]);
+            for (int j = 0; j < RC / 4; ++j)
+                dma16(uniform_ptr(vp + (pages[0] * a.v_stride + (kt & P1)) * 2 + (int64_t(j) * 64 << a.page_shift)) + here(v_at), &sh.v[buf][j * 256 + wave * 64]);
+        } else {
+            const int g = vkey >> 4;
+            const int64_t b0 = pages[0] * a.v_stride + (kt & P1), b1 = pages[1] * a.v_stride + ((kt + 16) & P1);
+            const int64_t b2 = pages[2] * a.v_stride + ((kt + 32) & P1), b3 = pages[3] * a.v_stride + ((kt + 48) & P1);
+            const char* const p = vp + ((g & 2 ? (g & 1 ? b3 : b2) : (g & 1 ? b1 : b0)) + (vkey & 15)) * 2 + (int64_t(vrow) << a.page_shift) * 2;
+#pragma unroll
+            for (int j = 0; j < RC / 4; ++j) dma16(p + (int64_t(j) * 64 << a.page_shift), &sh.v[buf][j * 256 + wave * 64]);
+        }
         if constexpr (EXTRA) {
             if (wave == 0) {
                 const int e = lane >> 4;
