@@ -646,3 +646,23 @@ def test_another_stream_and_a_graph():
             step()
             check(*io)
     assert hip.hipGraphExecDestroy(exe) == 0 and hip.hipGraphDestroy(graph) == 0 and hip.hipStreamDestroy(stream) == 0
+
+
+def test_read_memories_example():
+    """examples/read_memories.py: every step of its session against the restatement, over the cache as it stands at the end."""
+    import importlib.util
+
+    from conftest import ROOT
+    spec = importlib.util.spec_from_file_location("read_memories", ROOT / "examples" / "read_memories.py")
+    ex = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(ex)
+    s, free = ex.main(say=lambda *_: None)
+    assert free == ex.POOL and len(s.steps) == 6
+    k, v = s.cache.k_pages.numpy().astype(np.float64), s.cache.v_pages.numpy().astype(np.float64)
+    kt, ke = s.cache.times.numpy(), s.cache.episodes.numpy()
+    for t in s.steps:                                    # slots are written once, so the end's cache holds every step's
+        want, _, tol, _ = ref.attend(t["q"].astype(np.float64), k, v, t["start"], t["lens"], t["table"], "float16", cap=30.0,
+                                     decay=s.decay.numpy().astype(np.float64), q_times=t["times"], k_times=kt, q_eps=t["episodes"], k_eps=ke)
+        assert np.all(np.abs(t["out"].astype(np.float64) - want) <= tol)
+    first, last = s.steps[0], s.steps[-1]
+    assert (last["lens"] == np.array(first["new_lens"]) + [5 + i for i in range(3)] + 4).all()
