@@ -804,8 +804,10 @@ int mars_kv_store(const mars_reader* r, const mars_kv_cache* cache, const mars_k
  *   decay: s -= decay[h] * max(0, q_times[row] - times[j])   (weights decayed by age, as retrieval scores are)
  * and j is seen if j <= p or j < prefix_lens[r], and, with q_episodes, if the query's or the key's episode
  * is negative or both are equal. out = sum softmax(s)_j v_j over the keys seen; a row that sees
- * none is 0 with lse -inf. Keys not seen have no effect, whatever the cache holds there (NaN too).
- * The sums are fp32; weights are rounded to the cache's type for the product with v.
+ * none is 0 with lse -inf. Keys not seen have no effect, whatever the cache holds there (NaN too);
+ * an infinity or NaN that a row sees makes that element of the row one of them.
+ * The sums are fp32. For the product with v the weights of requests of many rows are rounded to the
+ * cache's type; those of few rows keep a second value of that type for what the first leaves.
  * max_new: an upper bound of the requests' new tokens if the caller knows one (0: unknown); it picks
  * the kernel, and a wrong one costs speed alone. num_tokens rows of q; rows no request owns are left. */
 typedef struct mars_kv_attend_args {

@@ -690,38 +690,40 @@ __device__ void few_part(const AttendArgs& a, const Part& it, FewLds<D>& lds) {
                 for (int d = 0; d < VB; ++d) o[d] *= f;
             }
         }
-        V p[NH];
+        // the weights as a 16-bit value and a 16-bit rest: the second product is free here, and the output's error is that of
+        // its own rounding alone (with one product sqrt(2) of that, as in k_attend_many)
+        V p[NH], rest[NH];
 #pragma unroll
         for (int j = 0; j < 8 * NH; ++j) {
             const float w = __builtin_amdgcn_exp2f(x[j] - mref);
             l += w;
             p[j >> 3][j & 7] = T(w);
+            rest[j >> 3][j & 7] = T(w - float(p[j >> 3][j & 7]));
         }
-        if (!whole) {
-            // some row does not see some key: see add_not_finite. Slots past the request's keys hold anything.
-            uint32_t odd = 0;
+        // infinities and NaN: see add_not_finite (in every step: a rest may be 0 or negative). Slots past the request's keys
+        // hold anything.
+        uint32_t odd = 0;
 #pragma unroll
-            for (int b2 = 0; b2 < NH; ++b2) {
-                const int kb = ks + 32 * b2 + 8 * h;
+        for (int b2 = 0; b2 < NH; ++b2) {
+            const int kb = ks + 32 * b2 + 8 * h;
 #pragma unroll
-                for (int d = 0; d < VB; ++d) {
-                    u32x4 b = __builtin_bit_cast(u32x4, vf[b2][d]);
-                    if (kb + 8 > keys) {
+            for (int d = 0; d < VB; ++d) {
+                u32x4 b = __builtin_bit_cast(u32x4, vf[b2][d]);
+                if (!whole && kb + 8 > keys) {
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) b[j] &= kb + 2 * j >= keys ? 0u : kb + 2 * j + 1 >= keys ? 0xFFFFu : ~0u;
-                    }
-                    const uint32_t full = exponents_full<T>(b);
-                    odd |= full;
-                    if (__any(full != 0)) b = finite_part<T>(b);
-                    vf[b2][d] = __builtin_bit_cast(V, b);
+                    for (int j = 0; j < 4; ++j) b[j] &= kb + 2 * j >= keys ? 0u : kb + 2 * j + 1 >= keys ? 0xFFFFu : ~0u;
                 }
+                const uint32_t full = exponents_full<T>(b);
+                odd |= full;
+                if (__any(full != 0)) b = finite_part<T>(b);
+                vf[b2][d] = __builtin_bit_cast(V, b);
             }
-            if (__any(odd != 0)) dirty = true;
         }
+        if (__any(odd != 0)) dirty = true;
 #pragma unroll
         for (int b2 = 0; b2 < NH; ++b2)
 #pragma unroll
-            for (int d = 0; d < VB; ++d) o[d] = Vec<T>::mma(vf[b2][d], p[b2], o[d]);
+            for (int d = 0; d < VB; ++d) o[d] = Vec<T>::mma(vf[b2][d], rest[b2], Vec<T>::mma(vf[b2][d], p[b2], o[d]));
         if (more) load_v(next);
     }
     if (!listed) break;
@@ -804,7 +806,7 @@ __device__ void few_part(const AttendArgs& a, const Part& it, FewLds<D>& lds) {
 // of G takes the w-th of G equal lengths of it: the bytes of the cache are dealt out evenly whatever the requests'
 // lengths, in one round. An end of a length that falls within kFewCut steps of a tile's first or last one moves there
 // (short requests are not cut), so a workgroup has at most two pieces that others share: its first and its last.
-constexpr int kFewCut = 4, kFewSpan = 1;
+constexpr int kFewCut = 4;
 struct SpanLds {
     int64_t start[257];        // of 256 requests: steps of the launch before each
     int32_t row0[256], n[256], keys[256];
@@ -867,7 +869,7 @@ __device__ void few_rows(const AttendArgs& a, int block, int blocks, FewShared<D
     const int most = __builtin_amdgcn_readfirstlane(sp.most);
     if (a.requests > 256) end = load_span(a, 0, 0, STEP, sp);            // back to the first
     // no tile in more than kMaxSplits pieces
-    const int64_t span = max(max((total + blocks - 1) / blocks, int64_t(kFewSpan)), int64_t((most + kMaxSplits - 2) / (kMaxSplits - 1))), x0 = w * span, x1 = min(x0 + span, total);
+    const int64_t span = max((total + blocks - 1) / blocks, int64_t((most + kMaxSplits - 2) / (kMaxSplits - 1))), x0 = w * span, x1 = min(x0 + span, total);
     if (x0 >= total) return;                                // no steps at all, or none for this workgroup
     while (x0 >= end) {
         r0 += 256;
@@ -1307,7 +1309,8 @@ __global__ __launch_bounds__(256) void k_attend_join(AttendArgs a) {
         *reinterpret_cast<typename Vec<T>::v4*>(static_cast<T*>(a.out) + (int64_t(it.row0) + ii) * a.out_stride + int64_t(hh) * D + d4 * 4) = w;
         if (a.lse && d4 == 0)
             a.lse[(int64_t(it.row0) + ii) * a.q_heads + hh] = top == -kInf ? -kInf : (top + __builtin_amdgcn_logf(l)) * kLn2;
-    }    }
+    }
+    }
 }
 
 // ---- the kernels ------------------------------------------------------------------------

@@ -457,6 +457,20 @@ def test_attend_not_finite_values(n, dtype):
     check_attend(Reader(hq, hkv, D, dtype, page), dtype, q, k, v, [0, n], [L], table, max_new=(0, n), q_eps=q_eps, k_eps=k_eps)
 
 
+@pytest.mark.parametrize("D,page", [(64, 16), (128, 64), (256, 32)])
+@pytest.mark.parametrize("n", [1, 40])
+def test_attend_not_finite_values_that_all_rows_see(n, D, page):
+    """Infinities and NaN in the middle of what every row sees, keys split and not."""
+    rng = np.random.default_rng(n + D)
+    for L in (400 + n, 3_000):
+        table, k, v = make_cache(rng, [L], 2, D, "float16", page)
+        vb = v.view(np.uint16)
+        for j, g, d, x in ((70, 0, 5, 0x7C00), (71, 0, 6, 0xFC00), (200, 1, 7, 0x7E00), (201, 1, 9, 0x7C00), (300, 1, 9, 0xFC00), (330, 0, 5, 0x7C00)):
+            vb[table[0][j // page], g, d, j % page] = x
+        q = ref.to_bits(rng.standard_normal((n, 4, D)), "float16")
+        check_attend(Reader(4, 2, D, "float16", page), "float16", q, k, v, [0, n], [L], table, max_new=(0, n))
+
+
 def test_attend_scores_of_any_size():
     """Scores far from zero: rows whose largest score is very low, very high, and rising by more than the weights' range."""
     rng = np.random.default_rng(6)
