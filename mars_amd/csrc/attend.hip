@@ -78,14 +78,14 @@ template <typename T> struct Vec;
 template <> struct Vec<_Float16> {
     using v8 = f16x8;
     using v4 = f16x4;
-    static constexpr uint32_t exp_mask = 0x7C00u, one = 0x3C00u;
+    static constexpr uint32_t exp_mask = 0x7C00u;
     __device__ static f32x4 mma(v8 a, v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
     __device__ static f32x16 mma32(v8 a, v8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 };
 template <> struct Vec<__bf16> {
     using v8 = bf16x8;
     using v4 = bf16x4;
-    static constexpr uint32_t exp_mask = 0x7F80u, one = 0x3F80u;
+    static constexpr uint32_t exp_mask = 0x7F80u;
     __device__ static f32x4 mma(v8 a, v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
     __device__ static f32x16 mma32(v8 a, v8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 };
@@ -954,6 +954,15 @@ __device__ inline bool own_pieces(const AttendArgs& a, Part* it, int piece) {
 // are in the softmax.
 constexpr int kManyKeys = 64;
 
+// Heads of 256 have one wave a SIMD, which nothing covers while it waits for LDS: LDS reads and products stay in the order
+// written, and only vector and scalar arithmetic passes (2 x 2,048 tokens over as many cached ones 221 us, 240 us in the
+// compiler's order, with cap and decay 280 and 320 us). With two or three waves a SIMD the compiler's order, and its fewer
+// registers, are as fast or faster (heads of 64 with every term 92 us, 101 us in this order).
+template <int D>
+__device__ inline void reads_first() {
+    if constexpr (D > 128) __builtin_amdgcn_sched_barrier(0x406);
+}
+
 template <int D>
 struct ManyLds {
     u32x4 k[2][kManyKeys * D / 8];
@@ -1139,12 +1148,29 @@ __device__ void many_rows(const AttendArgs& a, int block, ManyShared<D>& lds) {
         }
         if (kt >= hi) continue;                              // the wave's rows end before
         f32x16 x[2];
+        // fragments come from LDS ahead of the products that take them, see reads_first
+        V kf[2][4], vf[2][DB];
+        auto read_k = [&](int g) {
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
+            for (int u = 0; u < 4; ++u) kf[g & 1][u] = load16<V>(kl + (kb ^ ((2 * g + (u >> 1)) * 32)) + (u & 1) * 32 * RC * 16);
+        };
+        auto read_v = [&](int t) {
+#pragma unroll
+            for (int d = 0; d < DB; ++d) vf[t & 1][d] = load16<V>(vl + (vb ^ (t * 32)) + d * 32 * 8 * 16);
+        };
+        read_k(0);
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
 #pragma unroll
             for (int j = 0; j < 16; ++j) x[b][j] = 0.0f;
 #pragma unroll
-            for (int c = 0; c < KS; ++c) x[b] = Vec<T>::mma32(load16<V>(kl + (kb ^ (c * 32)) + b * 32 * RC * 16), q[c], x[b]);
+        for (int g = 0; g < KS / 2; ++g) {
+            if (g + 1 < KS / 2) read_k(g + 1);
+            else read_v(0);
+            reads_first<D>();
+#pragma unroll
+            for (int u = 0; u < 4; ++u) x[u & 1] = Vec<T>::mma32(kf[g & 1][u], q[2 * g + (u >> 1)], x[u & 1]);
+            reads_first<D>();
         }
         const bool whole = kt + kManyKeys <= lo && !mixed;
         if constexpr (EXTRA) {
@@ -1221,9 +1247,13 @@ __device__ void many_rows(const AttendArgs& a, int block, ManyShared<D>& lds) {
                 p[2 * b + (j >> 3)][j & 7] = T(w);
             }
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
+        for (int t = 0; t < 4; ++t) {
+            if (t < 3) read_v(t + 1);
+            reads_first<D>();
 #pragma unroll
-            for (int d = 0; d < DB; ++d) o[d] = Vec<T>::mma32(load16<V>(vl + (vb ^ (t * 32)) + d * 32 * 8 * 16), p[t], o[d]);
+            for (int d = 0; d < DB; ++d) o[d] = Vec<T>::mma32(vf[t & 1][d], p[t], o[d]);
+            reads_first<D>();
+        }
     }
     if (!listed) break;
     }
