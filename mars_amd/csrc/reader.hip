@@ -194,7 +194,7 @@ __device__ inline void turn(int32_t pos, uint64_t f, float* sn, float* cs) {
 }
 
 // Few tokens: a workgroup to each, a pair of values a thread and turn. Latency bound.
-constexpr int32_t kStoreFew = 256;
+constexpr int32_t kStoreFew = 1024;       // see k_kv_store_tile
 template <typename T>
 __global__ __launch_bounds__(256) void k_kv_store(StoreArgs a) {
     const int t = int(blockIdx.x), half = a.rope_dim / 2, D = a.head_dim;
@@ -236,7 +236,9 @@ __global__ __launch_bounds__(256) void k_kv_store(StoreArgs a) {
 // tokens are computed once a workgroup (LDS), q and k move in pieces of 16 bytes, and v, whose pages hold the tokens of an
 // element side by side, goes through LDS: where 8 consecutive tokens fill 8 consecutive slots from a multiple of 8 on
 // they are written as 16 bytes, and the lanes of a wave fill whole rows of a page; other tokens value by value.
-// Bound by the bytes in and out: 4,099 tokens of 32/8 heads of 128, 101 MB, SSS.
+// Bound by the bytes in and out: 4,099 tokens of 32/8 heads of 128, 101 MB, 27 us with all of it in the caches, 37 us from
+// and to memory. Up to kStoreFew tokens (of 32/8 heads of 128) k_kv_store has the shorter call: 1,024 tokens 15.4 us there,
+// 18.5 us here; 2,048 tokens 22.0 us there, 19.7 us here. (12/12 heads of 64: 12 us on both sides, 4,099 tokens 19.8 and 14.4.)
 template <int D>
 constexpr int store_tile() { return D == 256 ? 32 : 64; }
 
