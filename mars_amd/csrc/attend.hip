@@ -522,14 +522,12 @@ struct FewLds {
     };
     int any_dirty;
 };
-// Keys of a step: what the registers of two waves a SIMD hold, K and V and what the extra terms need.
-template <int D, bool EXTRA>
-constexpr int few_step() { return D > 128 || EXTRA ? 32 : 64; }
+constexpr int kFewStep = 32;
 
-template <typename T, int D, bool EXTRA, int STEP>
+template <typename T, int D, bool EXTRA>
 __device__ void few_part(const AttendArgs& a, const Part& it, FewLds<D>& lds) {
     using V = typename Vec<T>::v8;
-    constexpr int KC = D / 32, VB = D / 16, NH = STEP / 32;      // NH: halves of 32 keys in a step
+    constexpr int KC = D / 32, VB = D / 16;
     int tid = int(threadIdx.x);
     asm volatile("" : "+v"(tid));                          // nothing of a piece is kept in registers for the next
     const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -564,45 +562,39 @@ __device__ void few_part(const AttendArgs& a, const Part& it, FewLds<D>& lds) {
         }
     }
     const int k0 = it.k0, k1 = min(it.k1, hi);
-    const int steps = k1 > k0 ? (k1 - k0 + STEP - 1) / STEP : 0;
+    const int steps = k1 > k0 ? (k1 - k0 + kFewStep - 1) / kFewStep : 0;
 
     const TablePtr table = table_row(a, r);
     const int last_page = keys > 0 ? (keys - 1) >> a.page_shift : 0;
-    // K: A row `col` of block b holds key 8 (col / 4) + 4 b + col % 4 of 32, so that registers 4 b + j of S hold key 8 h + 4 b + j
+    // K: A row `col` of block b holds key 8 (col / 4) + 4 b + col % 4 of a step's 32, so that registers 4 b + j of S hold key 8 h + 4 b + j
     const int kg = col >> 3, kin = 8 * ((col >> 2) & 1) + (col & 3);             // group of 16 keys, key within it (b = 0)
     const T* const kp = static_cast<const T*>(a.k_pages) + ((int64_t(head) << a.page_shift) + kin) * D + h * 8;
     const T* const vp = static_cast<const T*>(a.v_pages) + ((int64_t(head) * D + col) << a.page_shift) + (h & 1) * 8;
-    int pages[2 * NH], v_pages[2 * NH];                     // of the step on the way: K's, and (loaded later) V's
+    int pages[2], v_pages[2];                               // of the step on the way: K's, and (loaded later) V's
     auto find_pages = [&](int s) {
 #pragma unroll
-        for (int u = 0; u < 2 * NH; ++u) pages[u] = page_of(a, table, k0 + s * STEP + u * 16, last_page);
+        for (int u = 0; u < 2; ++u) pages[u] = page_of(a, table, k0 + s * kFewStep + u * 16, last_page);
     };
-    V kf[NH][2][KC], vf[NH][VB];
-    f32x4 tk[NH][2];
-    i32x4 ek[NH][2];
+    V kf[2][KC], vf[VB];
+    f32x4 tk[2];
+    i32x4 ek[2];
     auto load_k = [&](int s) {
+        const int kt = k0 + s * kFewStep;
+        const int64_t o0 = pages[0] * a.k_stride + int64_t(kt & P1) * D, o1 = pages[1] * a.k_stride + int64_t((kt + 16) & P1) * D;
+        const T* const p = kp + (kg ? o1 : o0);
 #pragma unroll
-        for (int b2 = 0; b2 < NH; ++b2) {
-            const int kt = k0 + s * STEP + b2 * 32;
-            const int64_t o0 = pages[2 * b2] * a.k_stride + int64_t(kt & P1) * D, o1 = pages[2 * b2 + 1] * a.k_stride + int64_t((kt + 16) & P1) * D;
-            const T* const p = kp + (kg ? o1 : o0);
+        for (int b = 0; b < 2; ++b)
 #pragma unroll
-            for (int b = 0; b < 2; ++b)
-#pragma unroll
-                for (int c = 0; c < KC; ++c) kf[b2][b][c] = load16<V>(p + b * 4 * D + c * 32);
-        }
+            for (int c = 0; c < KC; ++c) kf[b][c] = load16<V>(p + b * 4 * D + c * 32);
     };
     auto load_v = [&](int s) {
+        const int kt = k0 + s * kFewStep, a0 = kt & P1, a1 = (kt + 16) & P1;
+        const T* const p = vp + (h & 2 ? v_pages[1] * a.v_stride + a1 : v_pages[0] * a.v_stride + a0);
 #pragma unroll
-        for (int b2 = 0; b2 < NH; ++b2) {
-            const int kt = k0 + s * STEP + b2 * 32, a0 = kt & P1, a1 = (kt + 16) & P1;
-            const T* const p = vp + (h & 2 ? v_pages[2 * b2 + 1] * a.v_stride + a1 : v_pages[2 * b2] * a.v_stride + a0);
-#pragma unroll
-            for (int d = 0; d < VB; ++d) vf[b2][d] = load16<V>(p + (int64_t(d) * 16 << a.page_shift));
-            const int64_t slot = (int64_t(h & 2 ? v_pages[2 * b2 + 1] : v_pages[2 * b2]) << a.page_shift) + (h & 2 ? a1 : a0) + (h & 1) * 8;
-            if (EXTRA && a.k_times) { tk[b2][0] = *reinterpret_cast<const f32x4*>(a.k_times + slot); tk[b2][1] = *reinterpret_cast<const f32x4*>(a.k_times + slot + 4); }
-            if (EXTRA && a.k_eps) { ek[b2][0] = *reinterpret_cast<const i32x4*>(a.k_eps + slot); ek[b2][1] = *reinterpret_cast<const i32x4*>(a.k_eps + slot + 4); }
-        }
+        for (int d = 0; d < VB; ++d) vf[d] = load16<V>(p + (int64_t(d) * 16 << a.page_shift));
+        const int64_t slot = (int64_t(h & 2 ? v_pages[1] : v_pages[0]) << a.page_shift) + (h & 2 ? a1 : a0) + (h & 1) * 8;
+        if (EXTRA && a.k_times) { tk[0] = *reinterpret_cast<const f32x4*>(a.k_times + slot); tk[1] = *reinterpret_cast<const f32x4*>(a.k_times + slot + 4); }
+        if (EXTRA && a.k_eps) { ek[0] = *reinterpret_cast<const i32x4*>(a.k_eps + slot); ek[1] = *reinterpret_cast<const i32x4*>(a.k_eps + slot + 4); }
     };
 
     V q[KC];
@@ -617,10 +609,10 @@ __device__ void few_part(const AttendArgs& a, const Part& it, FewLds<D>& lds) {
 
     auto keep_pages = [&] {
 #pragma unroll
-        for (int u = 0; u < 2 * NH; ++u) v_pages[u] = pages[u];
+        for (int u = 0; u < 2; ++u) v_pages[u] = pages[u];
     };
     for (int w0 = 0; w0 < steps; w0 += kWindow) {
-    const int count = listed ? list_steps<STEP>(a, r, last_page, k0, k1, w0, steps, eq_min, eq_max, lds.steps) : steps;
+    const int count = listed ? list_steps<kFewStep>(a, r, last_page, k0, k1, w0, steps, eq_min, eq_max, lds.steps) : steps;
     auto step_at = [&](int x) { return listed ? w0 + (__builtin_amdgcn_readfirstlane(int(lds.steps.list[x])) & (kWindow - 1)) : x; };
     if (wave < count) {
         find_pages(step_at(wave));
@@ -630,17 +622,15 @@ __device__ void few_part(const AttendArgs& a, const Part& it, FewLds<D>& lds) {
         if (wave + 4 < count) find_pages(step_at(wave + 4));
     }
     for (int x0 = wave; x0 < count; x0 += 4) {
-        const int ks = k0 + step_at(x0) * STEP;
+        const int ks = k0 + step_at(x0) * kFewStep;
         const bool mixed = listed && (__builtin_amdgcn_readfirstlane(int(lds.steps.list[x0])) & kMixed);
-        f32x4 acc[NH][2];
+        f32x4 acc[2];
 #pragma unroll
-        for (int b2 = 0; b2 < NH; ++b2)
+        for (int b = 0; b < 2; ++b) {
+            acc[b] = f32x4{0, 0, 0, 0};
 #pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                acc[b2][b] = f32x4{0, 0, 0, 0};
-#pragma unroll
-                for (int c = 0; c < KC; ++c) acc[b2][b] = Vec<T>::mma(kf[b2][b][c], q[c], acc[b2][b]);
-            }
+            for (int c = 0; c < KC; ++c) acc[b] = Vec<T>::mma(kf[b][c], q[c], acc[b]);
+        }
         const bool more = x0 + 4 < count;
         const int next = more ? step_at(x0 + 4) : 0;
         if (more) {
@@ -648,26 +638,26 @@ __device__ void few_part(const AttendArgs& a, const Part& it, FewLds<D>& lds) {
             keep_pages();
             if (x0 + 8 < count) find_pages(step_at(x0 + 8));
         }
-        // x[8 b2 + j]: this lane's key ks + 32 b2 + 8 h + j
-        float x[8 * NH];
+        // x[j]: this lane's key ks + 8 h + j
+        float x[8];
 #pragma unroll
-        for (int j = 0; j < 8 * NH; ++j) x[j] = acc[j >> 3][(j >> 2) & 1][j & 3] * a.scale_log2;
+        for (int j = 0; j < 8; ++j) x[j] = acc[j >> 2][j & 3] * a.scale_log2;
         if (EXTRA && a.cap_log2 != 0.0f) {
 #pragma unroll
-            for (int j = 0; j < 8 * NH; ++j)
+            for (int j = 0; j < 8; ++j)
                 x[j] = a.cap_log2 * (1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x[j])));
         }
         if (EXTRA && a.k_times) {
 #pragma unroll
-            for (int j = 0; j < 8 * NH; ++j) x[j] -= dec * fmaxf(0.0f, tq - tk[j >> 3][(j >> 2) & 1][j & 3]);
+            for (int j = 0; j < 8; ++j) x[j] -= dec * fmaxf(0.0f, tq - tk[j >> 2][j & 3]);
         }
-        const bool whole = ks + STEP <= lo && !mixed;
+        const bool whole = ks + kFewStep <= lo && !mixed;
         if (!whole) {
 #pragma unroll
-            for (int j = 0; j < 8 * NH; ++j) {
-                bool in = ks + 32 * (j >> 3) + 8 * h + (j & 7) < limit;
+            for (int j = 0; j < 8; ++j) {
+                bool in = ks + 8 * h + j < limit;
                 if (mixed) {
-                    const int e = ek[j >> 3][(j >> 2) & 1][j & 3];
+                    const int e = ek[j >> 2][j & 3];
                     in = in && (e < 0 || eq < 0 || e == eq);
                 }
                 x[j] = in ? x[j] : -kInf;
@@ -675,7 +665,7 @@ __device__ void few_part(const AttendArgs& a, const Part& it, FewLds<D>& lds) {
         }
         float top = x[0];
 #pragma unroll
-        for (int j = 1; j < 8 * NH; ++j) top = fmaxf(top, x[j]);
+        for (int j = 1; j < 8; ++j) top = fmaxf(top, x[j]);
         if (__any(top > mtop)) {
             top = fmaxf(top, __shfl_xor(top, 16));
             top = fmaxf(top, __shfl_xor(top, 32));
@@ -692,38 +682,33 @@ __device__ void few_part(const AttendArgs& a, const Part& it, FewLds<D>& lds) {
         }
         // the weights as a 16-bit value and a 16-bit rest: the second product is free here, and the output's error is that of
         // its own rounding alone (with one product sqrt(2) of that, as in k_attend_many)
-        V p[NH], rest[NH];
+        V p, rest;
 #pragma unroll
-        for (int j = 0; j < 8 * NH; ++j) {
+        for (int j = 0; j < 8; ++j) {
             const float w = __builtin_amdgcn_exp2f(x[j] - mref);
             l += w;
-            p[j >> 3][j & 7] = T(w);
-            rest[j >> 3][j & 7] = T(w - float(p[j >> 3][j & 7]));
+            p[j] = T(w);
+            rest[j] = T(w - float(p[j]));
         }
         // infinities and NaN: see add_not_finite (in every step: a rest may be 0 or negative). Slots past the request's keys
         // hold anything.
         uint32_t odd = 0;
+        const int kb = ks + 8 * h;
 #pragma unroll
-        for (int b2 = 0; b2 < NH; ++b2) {
-            const int kb = ks + 32 * b2 + 8 * h;
+        for (int d = 0; d < VB; ++d) {
+            u32x4 b = __builtin_bit_cast(u32x4, vf[d]);
+            if (!whole && kb + 8 > keys) {
 #pragma unroll
-            for (int d = 0; d < VB; ++d) {
-                u32x4 b = __builtin_bit_cast(u32x4, vf[b2][d]);
-                if (!whole && kb + 8 > keys) {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) b[j] &= kb + 2 * j >= keys ? 0u : kb + 2 * j + 1 >= keys ? 0xFFFFu : ~0u;
-                }
-                const uint32_t full = exponents_full<T>(b);
-                odd |= full;
-                if (__any(full != 0)) b = finite_part<T>(b);
-                vf[b2][d] = __builtin_bit_cast(V, b);
+                for (int j = 0; j < 4; ++j) b[j] &= kb + 2 * j >= keys ? 0u : kb + 2 * j + 1 >= keys ? 0xFFFFu : ~0u;
             }
+            const uint32_t full = exponents_full<T>(b);
+            odd |= full;
+            if (__any(full != 0)) b = finite_part<T>(b);
+            vf[d] = __builtin_bit_cast(V, b);
         }
         if (__any(odd != 0)) dirty = true;
 #pragma unroll
-        for (int b2 = 0; b2 < NH; ++b2)
-#pragma unroll
-            for (int d = 0; d < VB; ++d) o[d] = Vec<T>::mma(vf[b2][d], rest[b2], Vec<T>::mma(vf[b2][d], p[b2], o[d]));
+        for (int d = 0; d < VB; ++d) o[d] = Vec<T>::mma(vf[d], rest, Vec<T>::mma(vf[d], p, o[d]));
         if (more) load_v(next);
     }
     if (!listed) break;
@@ -806,7 +791,7 @@ __device__ void few_part(const AttendArgs& a, const Part& it, FewLds<D>& lds) {
 // of G takes the w-th of G equal lengths of it: the bytes of the cache are dealt out evenly whatever the requests'
 // lengths, in one round. An end of a length that falls within kFewCut steps of a tile's first or last one moves there
 // (short requests are not cut), so a workgroup has at most two pieces that others share: its first and its last.
-constexpr int kFewCut = 4;
+constexpr int kFewCut = 8;
 struct SpanLds {
     int64_t start[257];        // of 256 requests: steps of the launch before each
     int32_t row0[256], n[256], keys[256];
@@ -814,16 +799,16 @@ struct SpanLds {
     int32_t wmost[4];
     int32_t at, most;          // most: steps of the longest tile so far
 };
-__device__ inline int steps_of(int keys, int step) { return max(1, (keys + step - 1) / step); }
+__device__ inline int steps_of(int keys) { return max(1, (keys + kFewStep - 1) / kFewStep); }
 __device__ inline int units_of(const AttendArgs& a, int n) { return (n * a.group + kFewRows - 1) / kFewRows * a.kv_heads; }
 
 // Requests r0 .. r0 + 255 into the LDS; returns the launch's steps up to their end (base: before them).
-__device__ int64_t load_span(const AttendArgs& a, int r0, int64_t base, int step, SpanLds& lds) {
+__device__ int64_t load_span(const AttendArgs& a, int r0, int64_t base, SpanLds& lds) {
     const int tid = int(threadIdx.x), lane = tid & 63, wave = tid >> 6;
     const Request q = request_of<true>(a, r0 + tid);
-    const int64_t work = int64_t(q.tiles) * a.kv_heads * steps_of(q.keys, step);
+    const int64_t work = int64_t(q.tiles) * a.kv_heads * steps_of(q.keys);
     int64_t x = work;
-    int most = steps_of(q.keys, step);
+    int most = steps_of(q.keys);
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) most = max(most, __shfl_xor(most, o));
 #pragma unroll
@@ -857,27 +842,27 @@ struct FewShared {
     FewLds<D> part;
     SpanLds span;
 };
-template <typename T, int D, bool EXTRA, int STEP>
+template <typename T, int D, bool EXTRA>
 __device__ void few_rows(const AttendArgs& a, int block, int blocks, FewShared<D>& shared) {
     FewLds<D>& lds = shared.part;
     SpanLds& sp = shared.span;
     const int tid = int(threadIdx.x);
     const int64_t w = block;
     int r0 = 0;
-    int64_t end = load_span(a, 0, 0, STEP, sp), total = end;
-    for (int r = 256; r < a.requests; r += 256) total = load_span(a, r, total, STEP, sp);
+    int64_t end = load_span(a, 0, 0, sp), total = end;
+    for (int r = 256; r < a.requests; r += 256) total = load_span(a, r, total, sp);
     const int most = __builtin_amdgcn_readfirstlane(sp.most);
-    if (a.requests > 256) end = load_span(a, 0, 0, STEP, sp);            // back to the first
+    if (a.requests > 256) end = load_span(a, 0, 0, sp);            // back to the first
     // no tile in more than kMaxSplits pieces
     const int64_t span = max((total + blocks - 1) / blocks, int64_t((most + kMaxSplits - 2) / (kMaxSplits - 1))), x0 = w * span, x1 = min(x0 + span, total);
     if (x0 >= total) return;                                // no steps at all, or none for this workgroup
     while (x0 >= end) {
         r0 += 256;
-        end = load_span(a, r0, end, STEP, sp);
+        end = load_span(a, r0, end, sp);
     }
     if (x0 >= sp.start[tid] && x0 < sp.start[tid + 1]) sp.at = tid;
     __syncthreads();
-    int k = __builtin_amdgcn_readfirstlane(sp.at), steps = steps_of(__builtin_amdgcn_readfirstlane(sp.keys[k]), STEP);
+    int k = __builtin_amdgcn_readfirstlane(sp.at), steps = steps_of(__builtin_amdgcn_readfirstlane(sp.keys[k]));
     // the first tile and step: ends near a tile's own move to it
     int unit, s0;
     {
@@ -894,7 +879,7 @@ __device__ void few_rows(const AttendArgs& a, int block, int blocks, FewShared<D
             if (r0 + ++k >= a.requests) return;
             if (k < 256) continue;
             r0 += 256;
-            end = load_span(a, r0, end, STEP, sp);
+            end = load_span(a, r0, end, sp);
             k = 0;
         }
         Part it;
@@ -902,15 +887,15 @@ __device__ void few_rows(const AttendArgs& a, int block, int blocks, FewShared<D
         it.row0 = __builtin_amdgcn_readfirstlane(sp.row0[k]);
         it.n = __builtin_amdgcn_readfirstlane(sp.n[k]);
         it.keys = __builtin_amdgcn_readfirstlane(sp.keys[k]);
-        steps = steps_of(it.keys, STEP);
+        steps = steps_of(it.keys);
         const int64_t u0 = uniform(sp.start[k]) + int64_t(unit) * steps, left = x1 - u0;       // the tile's first step; ours of it
         const int low = min(kFewCut, (steps + 1) / 2);
         if (left < low) return;
         const int s1 = left >= steps || steps - left < kFewCut ? steps : int(left);
         it.tile = unit / a.kv_heads;
         it.head = unit - it.tile * a.kv_heads;
-        it.k0 = s0 * STEP;
-        it.k1 = min(s1 * STEP, it.keys);
+        it.k0 = s0 * kFewStep;
+        it.k1 = min(s1 * kFewStep, it.keys);
         it.splits = 1;
         it.chunk = 0;
         it.slot = it.slot0 = it.slot1 = it.slot_step = 0;
@@ -926,7 +911,7 @@ __device__ void few_rows(const AttendArgs& a, int block, int blocks, FewShared<D
         }
         if (!first) __syncthreads();                        // the LDS of the piece before is done with
         first = false;
-        few_part<T, D, EXTRA, STEP>(a, uniform_part(it), lds);
+        few_part<T, D, EXTRA>(a, uniform_part(it), lds);
         if (left <= steps) return;
         s0 = 0;
         ++unit;
@@ -1347,7 +1332,7 @@ __global__ __launch_bounds__(256) void k_attend_join(AttendArgs a) {
 template <typename T, int D, bool EXTRA>
 __global__ __launch_bounds__(256, D > 128 ? 1 : D == 128 ? 2 : 3) void k_attend_few(AttendArgs a) {
     __shared__ __attribute__((aligned(16))) FewShared<D> lds;
-    few_rows<T, D, EXTRA, few_step<D, EXTRA>()>(a, int(blockIdx.x), int(gridDim.x), lds);
+    few_rows<T, D, EXTRA>(a, int(blockIdx.x), int(gridDim.x), lds);
 }
 
 template <typename T, int D, bool EXTRA>
@@ -1367,8 +1352,7 @@ int launch_dim(AttendArgs a, int32_t max_new, hipStream_t s) {
     a.few_rows = few_only ? INT32_MAX : many_only ? -1 : kFewMost;
     // few: one workgroup for each that the CUs hold at a time, fewer where there are not so many steps
     const int64_t few_tiles = few_only ? rows / kFewRows + std::min(a.requests, a.tokens) : std::min(a.requests, a.tokens);
-    constexpr int step = few_step<D, EXTRA>();
-    const int64_t few = std::min<int64_t>(few_tiles * a.kv_heads * ((keys + step - 1) / step), few_groups(D));
+    const int64_t few = std::min<int64_t>(few_tiles * a.kv_heads * ((keys + kFewStep - 1) / kFewStep), few_groups(D));
     if (!many_only) MARS_LAUNCH((k_attend_few<T, D, EXTRA>), dim3(unsigned(few)), dim3(256), 0, s, a);
     if (few_only) return MARS_OK;
     // many: no more than chunks of kMinChunk or more of the tiles' keys, or 2^kManyItemsLog2 chunks and one for each tile
