@@ -14,7 +14,9 @@
 //  Softmax in base 2 (log2 e is folded into the scale), one pass: each row has a reference
 //  m and sums exp2(s - m), fp32. m moves only when a score exceeds it by more than 8 (in a
 //  wave of rows together): exp2 stays below 2^8, exact in 16-bit range, and the usual step
-//  needs no lane exchange and no rescaling of O.
+//  needs no lane exchange and no rescaling of O. The weights are rounded to 16 bits for the
+//  second product (the matrix cores take no more at that rate); their sum is that of the
+//  unrounded ones, fp32 as every other sum.
 // ============================================================================
 #include "reader.hpp"
 
@@ -187,8 +189,9 @@ __device__ inline Request request_of(const AttendArgs& a, int r) {
 // Workgroup b's item of k_attend_many, from the lengths alone: every workgroup of 256 threads sums the launch's tiles
 // and work (key steps of 32 over all tiles), cuts the keys into chunks, and finds the request that its number falls to.
 // Where there are fewer tiles than three quarters of the workgroups that the CUs hold, chunks of a 2^9-th of all the
-// tiles' keys (2 x 511 tokens over 2,500 keys, 256 tiles: 77 us, 104 us whole); with more tiles, no chunk has to be
-// smaller than a CU's share of the work (768 tiles of causal rows up to 4,001 keys: 112 us whole, 144 us cut once).
+// tiles' keys (2 x 511 tokens over 2,500 keys, 256 tiles: 77 us, 104 us whole; in 2^8 or 2^10 chunks 79 and 95 us, and
+// 511 tokens over 20,511 keys 208 us, 275 and 238); with more tiles, no chunk has to be smaller than a CU's share of the
+// work (768 tiles of causal rows up to 4,001 keys: 112 us whole, 144 us cut once).
 // A tile has at most 2 L / C chunks where it has two, and C is at least sum(L) / 2^9 by either rule: 2^10 partial slots.
 // The launch has enough workgroups for every item (fewer than 2^31); the last ones may find none. JOIN: the items are
 // the blocks of kJoinRows rows of the tiles in several pieces instead, the block's number in Part::slot.
@@ -509,10 +512,11 @@ __device__ void add_not_finite(const AttendArgs& a, const Part& it, int prefix) 
 }
 
 // ---- few rows: 16 at a time, keys straight from the cache to registers -----------------
-// Bound by the cache's bytes. A piece's steps (64 keys; 32 for heads of 256) go to 4 waves in turn, and a wave keeps
-// its next step's K and V on the way to registers (16 bytes a lane; whole 128-byte lines, from K rows over the
-// elements and from V rows over the step's keys) while it computes this one: 8 waves of a CU have up to 256 KB in
-// flight. The waves' sums are joined at the end.
+// Bound by the cache's bytes. A piece's steps go to 4 waves in turn, and a wave keeps its next step's K and V on the way to
+// registers (16 bytes a lane: K rows over the elements, V rows over the step's keys) while it computes this one: 8 waves of
+// a CU have 128 KB in flight for heads of 128. The waves' sums are joined at the end. bf16, 32/8 heads of 128:
+// 64 single tokens over 780 to 7,800 keys (1.15 GB) 215 us, 5.4 TB/s; one over 131,072 (0.54 GB) 110 us.
+// Steps of 64 keys spill: 228 and 119 us (first case with cap and decay: 288 and 225 us).
 template <int D>
 struct FewLds {
     union {
@@ -680,8 +684,8 @@ __device__ void few_part(const AttendArgs& a, const Part& it, FewLds<D>& lds) {
                 for (int d = 0; d < VB; ++d) o[d] *= f;
             }
         }
-        // the weights as a 16-bit value and a 16-bit rest: the second product is free here, and the output's error is that of
-        // its own rounding alone (with one product sqrt(2) of that, as in k_attend_many)
+        // the weights as a 16-bit value and a 16-bit rest: the second product costs little where the cache's bytes bound the
+        // kernel, and the output's error is that of its own rounding alone (with one product 1.4 times that, as in k_attend_many)
         V p, rest;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -791,6 +795,8 @@ __device__ void few_part(const AttendArgs& a, const Part& it, FewLds<D>& lds) {
 // of G takes the w-th of G equal lengths of it: the bytes of the cache are dealt out evenly whatever the requests'
 // lengths, in one round. An end of a length that falls within kFewCut steps of a tile's first or last one moves there
 // (short requests are not cut), so a workgroup has at most two pieces that others share: its first and its last.
+// Cuts 2, 4, 8 steps from an end: 24 x 5 tokens over up to 3,000 keys 23.3, 22.3, 20.4 us, 4 x 4 over 3,000 29.7, 24.7,
+// 25.1 us (with 12 steps of twice the length it was slower again).
 constexpr int kFewCut = 8;
 struct SpanLds {
     int64_t start[257];        // of 256 requests: steps of the launch before each
@@ -931,12 +937,14 @@ __device__ inline bool own_pieces(const AttendArgs& a, Part* it, int piece) {
 }
 
 // ---- many rows: 128 at a time, keys staged through LDS ----------------------------------
-// Bound by the matrix cores and the softmax's vector work together (32 exp2 per lane and tile of
-// 64 keys take as long as the 32 MFMAs). 4 waves of 32 rows each share tiles of 64 keys: K (keys, elements) and
-// V (elements, keys) come by global_load_lds_dwordx4 into two buffers, one tile ahead. 16-byte pieces
-// of a row are XORed with the row number so that the 16 lanes of a fragment read hit
-// the 16 bank groups. The other workgroup of the CU fills the matrix cores while this one's waves
-// are in the softmax.
+// Bound by the matrix cores and the softmax's vector work together, and by the clock, which falls under that load: heads
+// of 128 without extra terms keep the matrix cores busy 48% of the cycles and the vector units 45%, heads of 64 43% and 70%.
+// 4 waves of 32 rows each share tiles of 64 keys: K (keys, elements) and V (elements, keys) come straight into two LDS
+// buffers, one tile ahead. 16-byte pieces of a row are XORed with the row number so that the 16 lanes of a fragment read hit
+// the 16 bank groups (no conflicts counted). The other workgroup of the CU fills the matrix cores while this one's waves are
+// in the softmax. 2 x 4,096 tokens over 8,196 keys, bf16, 32/8 heads of 128: 802 us, 1,030 TFLOP/s (a library product of
+// 8,192 cubed reaches 1,168). With cap and decay a score takes three transcendental instructions instead of one: 2 x 4,001
+// tokens of 12 heads of 64 within their episodes, vector units busy 69%, matrix cores 11%.
 constexpr int kManyKeys = 64;
 
 // Heads of 256 have one wave a SIMD, which nothing covers while it waits for LDS: LDS reads and products stay in the order
@@ -1344,7 +1352,8 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void k_attend_many(AttendArgs
 template <typename T, int D, bool EXTRA>
 int launch_dim(AttendArgs a, int32_t max_new, hipStream_t s) {
     // Requests of at most kFewMost rows (new tokens x query heads per kv head) are k_attend_few's, the others
-    // k_attend_many's. Where a bound on the new tokens rules one of them out, the other serves every request, also one that
+    // k_attend_many's: 64 requests over 3,000 keys of 16 rows 149 us by the one and 152 by the other, of 20 rows (which few
+    // reads the keys twice for) 226 and 154 us, 4 such requests 28.6 and 27.5, 33.6 and 28.0. Where a bound on the new tokens rules one of them out, the other serves every request, also one that
     // breaks the bound.
     const int64_t rows = int64_t(a.tokens) * a.group, keys = int64_t(a.max_pages) << a.page_shift;
     const int64_t most = std::min<int64_t>(max_new > 0 ? max_new : a.tokens, a.tokens) * a.group;
