@@ -942,7 +942,7 @@ __device__ inline bool own_pieces(const AttendArgs& a, Part* it, int piece) {
 // 4 waves of 32 rows each share tiles of 64 keys: K (keys, elements) and V (elements, keys) come straight into two LDS
 // buffers, one tile ahead. 16-byte pieces of a row are XORed with the row number so that the 16 lanes of a fragment read hit
 // the 16 bank groups (no conflicts counted). The other workgroup of the CU fills the matrix cores while this one's waves are
-// in the softmax. 2 x 4,096 tokens over 8,196 keys, bf16, 32/8 heads of 128: 802 us, 1,030 TFLOP/s (a library product of
+// in the softmax. 2 x 4,096 tokens over 8,196 keys, bf16, 32/8 heads of 128: 802 to 827 us on two boxes, about 1,000 TFLOP/s (a product of
 // 8,192 cubed reaches 1,168). With cap and decay a score takes three transcendental instructions instead of one: 2 x 4,001
 // tokens of 12 heads of 64 within their episodes, vector units busy 69%, matrix cores 11%.
 constexpr int kManyKeys = 64;
@@ -1288,7 +1288,9 @@ __device__ void many_rows(const AttendArgs& a, int block, ManyShared<D>& lds) {
 
 // Joins the pieces that k_attend_many left: their partials come to megabytes, too much for the one workgroup that arrives
 // last (2 requests of 64 tokens over 8,000 keys: 114 us so). A thread takes 4 elements of a row and has the references and
-// partials of 8 pieces on the way together; the sums are taken in the order of the pieces.
+// partials of 8 pieces on the way together; the sums are taken in the order of the pieces. Bound by those bytes and, before
+// them, by finding the work: 512 pieces of 128 rows of 128 elements, 34 MB just written, 12.9 us; no pieces at all 5.3 us.
+// (Twice the workgroups: 15.6 and 8.8 us.)
 template <typename T, int D>
 __global__ __launch_bounds__(256) void k_attend_join(AttendArgs a) {
     __shared__ SchedLds lds;
@@ -1310,13 +1312,15 @@ __global__ __launch_bounds__(256) void k_attend_join(AttendArgs a) {
             f32x4 o[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const int64_t at = int64_t(min(s + u, it.splits - 1)) * kManyRows + rr;
+                if (s + u >= it.splits) break;
+                const int64_t at = int64_t(s + u) * kManyRows + rr;
                 p[u] = ml[at];
                 o[u] = *reinterpret_cast<const f32x4*>(po + at * D + d4 * 4);
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                if (s + u >= it.splits || p[u].x == -kInf) continue;
+                if (s + u >= it.splits) break;
+                if (p[u].x == -kInf) continue;
                 const float next = fmaxf(top, p[u].x), was = top == -kInf ? 0.0f : __builtin_amdgcn_exp2f(top - next);
                 const float f = __builtin_amdgcn_exp2f(p[u].x - next);
                 l = top == -kInf ? f * p[u].y : l * was + f * p[u].y;
