@@ -616,106 +616,106 @@ __device__ void few_part(const AttendArgs& a, const Part& it, FewLds<D>& lds) {
         for (int u = 0; u < 2; ++u) v_pages[u] = pages[u];
     };
     for (int w0 = 0; w0 < steps; w0 += kWindow) {
-    const int count = listed ? list_steps<kFewStep>(a, r, last_page, k0, k1, w0, steps, eq_min, eq_max, lds.steps) : steps;
-    auto step_at = [&](int x) { return listed ? w0 + (__builtin_amdgcn_readfirstlane(int(lds.steps.list[x])) & (kWindow - 1)) : x; };
-    if (wave < count) {
-        find_pages(step_at(wave));
-        load_k(step_at(wave));
-        keep_pages();
-        load_v(step_at(wave));
-        if (wave + 4 < count) find_pages(step_at(wave + 4));
-    }
-    for (int x0 = wave; x0 < count; x0 += 4) {
-        const int ks = k0 + step_at(x0) * kFewStep;
-        const bool mixed = listed && (__builtin_amdgcn_readfirstlane(int(lds.steps.list[x0])) & kMixed);
-        f32x4 acc[2];
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {
-            acc[b] = f32x4{0, 0, 0, 0};
-#pragma unroll
-            for (int c = 0; c < KC; ++c) acc[b] = Vec<T>::mma(kf[b][c], q[c], acc[b]);
-        }
-        const bool more = x0 + 4 < count;
-        const int next = more ? step_at(x0 + 4) : 0;
-        if (more) {
-            load_k(next);
+        const int count = listed ? list_steps<kFewStep>(a, r, last_page, k0, k1, w0, steps, eq_min, eq_max, lds.steps) : steps;
+        auto step_at = [&](int x) { return listed ? w0 + (__builtin_amdgcn_readfirstlane(int(lds.steps.list[x])) & (kWindow - 1)) : x; };
+        if (wave < count) {
+            find_pages(step_at(wave));
+            load_k(step_at(wave));
             keep_pages();
-            if (x0 + 8 < count) find_pages(step_at(x0 + 8));
+            load_v(step_at(wave));
+            if (wave + 4 < count) find_pages(step_at(wave + 4));
         }
-        // x[j]: this lane's key ks + 8 h + j
-        float x[8];
+        for (int x0 = wave; x0 < count; x0 += 4) {
+            const int ks = k0 + step_at(x0) * kFewStep;
+            const bool mixed = listed && (__builtin_amdgcn_readfirstlane(int(lds.steps.list[x0])) & kMixed);
+            f32x4 acc[2];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = acc[j >> 2][j & 3] * a.scale_log2;
-        if (EXTRA && a.cap_log2 != 0.0f) {
+            for (int b = 0; b < 2; ++b) {
+                acc[b] = f32x4{0, 0, 0, 0};
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                x[j] = a.cap_log2 * (1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x[j])));
-        }
-        if (EXTRA && a.k_times) {
+                for (int c = 0; c < KC; ++c) acc[b] = Vec<T>::mma(kf[b][c], q[c], acc[b]);
+            }
+            const bool more = x0 + 4 < count;
+            const int next = more ? step_at(x0 + 4) : 0;
+            if (more) {
+                load_k(next);
+                keep_pages();
+                if (x0 + 8 < count) find_pages(step_at(x0 + 8));
+            }
+            // x[j]: this lane's key ks + 8 h + j
+            float x[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] -= dec * fmaxf(0.0f, tq - tk[j >> 2][j & 3]);
-        }
-        const bool whole = ks + kFewStep <= lo && !mixed;
-        if (!whole) {
+            for (int j = 0; j < 8; ++j) x[j] = acc[j >> 2][j & 3] * a.scale_log2;
+            if (EXTRA && a.cap_log2 != 0.0f) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    x[j] = a.cap_log2 * (1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x[j])));
+            }
+            if (EXTRA && a.k_times) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[j] -= dec * fmaxf(0.0f, tq - tk[j >> 2][j & 3]);
+            }
+            const bool whole = ks + kFewStep <= lo && !mixed;
+            if (!whole) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    bool in = ks + 8 * h + j < limit;
+                    if (mixed) {
+                        const int e = ek[j >> 2][j & 3];
+                        in = in && (e < 0 || eq < 0 || e == eq);
+                    }
+                    x[j] = in ? x[j] : -kInf;
+                }
+            }
+            float top = x[0];
+#pragma unroll
+            for (int j = 1; j < 8; ++j) top = fmaxf(top, x[j]);
+            if (__any(top > mtop)) {
+                top = fmaxf(top, __shfl_xor(top, 16));
+                top = fmaxf(top, __shfl_xor(top, 32));
+                const bool none = mtop == -kInf;
+                const float mnew = none ? top : fmaxf(mref, top);
+                if (mnew > -kInf) {                          // not NaN either: the row's sum is then NaN
+                    const float f = none ? 0.0f : __builtin_amdgcn_exp2f(mref - mnew);
+                    mref = mnew;
+                    mtop = mnew + kSlack;
+                    l *= f;
+#pragma unroll
+                    for (int d = 0; d < VB; ++d) o[d] *= f;
+                }
+            }
+            // the weights as a 16-bit value and a 16-bit rest: the second product costs little where the cache's bytes bound the
+            // kernel, and the output's error is that of its own rounding alone (with one product 1.4 times that, as in k_attend_many)
+            V p, rest;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                bool in = ks + 8 * h + j < limit;
-                if (mixed) {
-                    const int e = ek[j >> 2][j & 3];
-                    in = in && (e < 0 || eq < 0 || e == eq);
+                const float w = __builtin_amdgcn_exp2f(x[j] - mref);
+                l += w;
+                p[j] = T(w);
+                rest[j] = T(w - float(p[j]));
+            }
+            // infinities and NaN: see add_not_finite (in every step: a rest may be 0 or negative). Slots past the request's keys
+            // hold anything.
+            uint32_t odd = 0;
+            const int kb = ks + 8 * h;
+#pragma unroll
+            for (int d = 0; d < VB; ++d) {
+                u32x4 b = __builtin_bit_cast(u32x4, vf[d]);
+                if (!whole && kb + 8 > keys) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) b[j] &= kb + 2 * j >= keys ? 0u : kb + 2 * j + 1 >= keys ? 0xFFFFu : ~0u;
                 }
-                x[j] = in ? x[j] : -kInf;
+                const uint32_t full = exponents_full<T>(b);
+                odd |= full;
+                if (__any(full != 0)) b = finite_part<T>(b);
+                vf[d] = __builtin_bit_cast(V, b);
             }
+            if (__any(odd != 0)) dirty = true;
+#pragma unroll
+            for (int d = 0; d < VB; ++d) o[d] = Vec<T>::mma(vf[d], rest, Vec<T>::mma(vf[d], p, o[d]));
+            if (more) load_v(next);
         }
-        float top = x[0];
-#pragma unroll
-        for (int j = 1; j < 8; ++j) top = fmaxf(top, x[j]);
-        if (__any(top > mtop)) {
-            top = fmaxf(top, __shfl_xor(top, 16));
-            top = fmaxf(top, __shfl_xor(top, 32));
-            const bool none = mtop == -kInf;
-            const float mnew = none ? top : fmaxf(mref, top);
-            if (mnew != -kInf) {
-                const float f = none ? 0.0f : __builtin_amdgcn_exp2f(mref - mnew);
-                mref = mnew;
-                mtop = mnew + kSlack;
-                l *= f;
-#pragma unroll
-                for (int d = 0; d < VB; ++d) o[d] *= f;
-            }
-        }
-        // the weights as a 16-bit value and a 16-bit rest: the second product costs little where the cache's bytes bound the
-        // kernel, and the output's error is that of its own rounding alone (with one product 1.4 times that, as in k_attend_many)
-        V p, rest;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float w = __builtin_amdgcn_exp2f(x[j] - mref);
-            l += w;
-            p[j] = T(w);
-            rest[j] = T(w - float(p[j]));
-        }
-        // infinities and NaN: see add_not_finite (in every step: a rest may be 0 or negative). Slots past the request's keys
-        // hold anything.
-        uint32_t odd = 0;
-        const int kb = ks + 8 * h;
-#pragma unroll
-        for (int d = 0; d < VB; ++d) {
-            u32x4 b = __builtin_bit_cast(u32x4, vf[d]);
-            if (!whole && kb + 8 > keys) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) b[j] &= kb + 2 * j >= keys ? 0u : kb + 2 * j + 1 >= keys ? 0xFFFFu : ~0u;
-            }
-            const uint32_t full = exponents_full<T>(b);
-            odd |= full;
-            if (__any(full != 0)) b = finite_part<T>(b);
-            vf[d] = __builtin_bit_cast(V, b);
-        }
-        if (__any(odd != 0)) dirty = true;
-#pragma unroll
-        for (int d = 0; d < VB; ++d) o[d] = Vec<T>::mma(vf[d], rest, Vec<T>::mma(vf[d], p, o[d]));
-        if (more) load_v(next);
-    }
-    if (!listed) break;
+        if (!listed) break;
     }
 
     // join the waves: references first, then sums and O, in wave order
@@ -723,7 +723,7 @@ __device__ void few_part(const AttendArgs& a, const Part& it, FewLds<D>& lds) {
     auto& ob = lds.wave.ob;
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
-    float mw = mtop == -kInf ? -kInf : mref;
+    float mw = mtop == -kInf && l == 0.0f ? -kInf : mref;   // -inf: the row sees no key; with NaN scores alone its sum is NaN
     __syncthreads();                                        // the list of steps is done with
     if (h == 0) ml[wave][col][0] = mw;
     if (dirty && lane == 0) lds.any_dirty = 1;
@@ -1101,158 +1101,158 @@ __device__ void many_rows(const AttendArgs& a, int block, ManyShared<D>& lds) {
     const char* const kl = reinterpret_cast<const char*>(&sh.k[0][0]);
     const char* const vl = reinterpret_cast<const char*>(&sh.v[0][0]);
     for (int w0 = 0; w0 < steps; w0 += kWindow) {
-    const int count = listed ? list_steps<kManyKeys>(a, r, last_page, k0, k1, w0, steps, eq_min, eq_max, list) : steps;
-    auto step_at = [&](int x) { return listed ? w0 + (__builtin_amdgcn_readfirstlane(int(list.list[x])) & (kWindow - 1)) : x; };
-    if (count > 0) {
-        find_pages(step_at(0));
-        stage(step_at(0), 0);
-        if (count > 1) find_pages(step_at(1));
-    }
-    for (int x0 = 0; x0 < count; ++x0) {
-        const int buf = x0 & 1;
-        tile_barrier();                                      // the tile is in LDS; nobody reads the other buffer any more
-        const int kt = k0 + step_at(x0) * kManyKeys;
-        const bool mixed = listed && (__builtin_amdgcn_readfirstlane(int(list.list[x0])) & kMixed);
-        if (x0 + 1 < count) {
-            stage(step_at(x0 + 1), buf ^ 1);
-            if (x0 + 2 < count) find_pages(step_at(x0 + 2));
+        const int count = listed ? list_steps<kManyKeys>(a, r, last_page, k0, k1, w0, steps, eq_min, eq_max, list) : steps;
+        auto step_at = [&](int x) { return listed ? w0 + (__builtin_amdgcn_readfirstlane(int(list.list[x])) & (kWindow - 1)) : x; };
+        if (count > 0) {
+            find_pages(step_at(0));
+            stage(step_at(0), 0);
+            if (count > 1) find_pages(step_at(1));
         }
-        const uint32_t kb = buf * uint32_t(sizeof(sh.k[0])) + koff, vb = buf * uint32_t(sizeof(sh.v[0])) + voff;
-        if (kt + kManyKeys > first_limit || mixed) {
-            // some row of the workgroup does not see some key: each thread looks over its pieces of V (see add_not_finite;
-            // slots past the request's keys hold anything and become 0)
-#pragma unroll
-            for (int j = 0; j < RC / 4; ++j) {
-                u32x4 b = sh.v[buf][j * 256 + tid];
-                const bool past = kt + vkey + 8 > keys;
-                if (past) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int key = kt + vkey + 2 * e;
-                        b[e] &= key >= keys ? 0u : key + 1 >= keys ? 0xFFFFu : ~0u;
-                    }
-                }
-                const bool full = exponents_full<T>(b) != 0;
-                if (full) b = finite_part<T>(b);
-                if (past || full) sh.v[buf][j * 256 + tid] = b;
-                dirty |= full;
+        for (int x0 = 0; x0 < count; ++x0) {
+            const int buf = x0 & 1;
+            tile_barrier();                                      // the tile is in LDS; nobody reads the other buffer any more
+            const int kt = k0 + step_at(x0) * kManyKeys;
+            const bool mixed = listed && (__builtin_amdgcn_readfirstlane(int(list.list[x0])) & kMixed);
+            if (x0 + 1 < count) {
+                stage(step_at(x0 + 1), buf ^ 1);
+                if (x0 + 2 < count) find_pages(step_at(x0 + 2));
             }
-            lds_barrier();
-        }
-        if (kt >= hi) continue;                              // the wave's rows end before
-        f32x16 x[2];
-        // fragments come from LDS ahead of the products that take them, see reads_first
-        V kf[2][4], vf[2][DB];
-        auto read_k = [&](int g) {
+            const uint32_t kb = buf * uint32_t(sizeof(sh.k[0])) + koff, vb = buf * uint32_t(sizeof(sh.v[0])) + voff;
+            if (kt + kManyKeys > first_limit || mixed) {
+                // some row of the workgroup does not see some key: each thread looks over its pieces of V (see add_not_finite;
+                // slots past the request's keys hold anything and become 0)
 #pragma unroll
-            for (int u = 0; u < 4; ++u) kf[g & 1][u] = load16<V>(kl + (kb ^ ((2 * g + (u >> 1)) * 32)) + (u & 1) * 32 * RC * 16);
-        };
-        auto read_v = [&](int t) {
+                for (int j = 0; j < RC / 4; ++j) {
+                    u32x4 b = sh.v[buf][j * 256 + tid];
+                    const bool past = kt + vkey + 8 > keys;
+                    if (past) {
 #pragma unroll
-            for (int d = 0; d < DB; ++d) vf[t & 1][d] = load16<V>(vl + (vb ^ (t * 32)) + d * 32 * 8 * 16);
-        };
-        read_k(0);
+                        for (int e = 0; e < 4; ++e) {
+                            const int key = kt + vkey + 2 * e;
+                            b[e] &= key >= keys ? 0u : key + 1 >= keys ? 0xFFFFu : ~0u;
+                        }
+                    }
+                    const bool full = exponents_full<T>(b) != 0;
+                    if (full) b = finite_part<T>(b);
+                    if (past || full) sh.v[buf][j * 256 + tid] = b;
+                    dirty |= full;
+                }
+                lds_barrier();
+            }
+            if (kt >= hi) continue;                              // the wave's rows end before
+            f32x16 x[2];
+            // fragments come from LDS ahead of the products that take them, see reads_first
+            V kf[2][4], vf[2][DB];
+            auto read_k = [&](int g) {
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
+                for (int u = 0; u < 4; ++u) kf[g & 1][u] = load16<V>(kl + (kb ^ ((2 * g + (u >> 1)) * 32)) + (u & 1) * 32 * RC * 16);
+            };
+            auto read_v = [&](int t) {
 #pragma unroll
-            for (int j = 0; j < 16; ++j) x[b][j] = 0.0f;
-#pragma unroll
-        for (int g = 0; g < KS / 2; ++g) {
-            if (g + 1 < KS / 2) read_k(g + 1);
-            else read_v(0);
-            reads_first<D>();
-#pragma unroll
-            for (int u = 0; u < 4; ++u) x[u & 1] = Vec<T>::mma32(kf[g & 1][u], q[2 * g + (u >> 1)], x[u & 1]);
-            reads_first<D>();
-        }
-        const bool whole = kt + kManyKeys <= lo && !mixed;
-        if constexpr (EXTRA) {
+                for (int d = 0; d < DB; ++d) vf[t & 1][d] = load16<V>(vl + (vb ^ (t * 32)) + d * 32 * 8 * 16);
+            };
+            read_k(0);
 #pragma unroll
             for (int b = 0; b < 2; ++b)
 #pragma unroll
-                for (int j = 0; j < 16; ++j) x[b][j] *= a.scale_log2;
-            if (a.cap_log2 != 0.0f) {
+                for (int j = 0; j < 16; ++j) x[b][j] = 0.0f;
+#pragma unroll
+            for (int g = 0; g < KS / 2; ++g) {
+                if (g + 1 < KS / 2) read_k(g + 1);
+                else read_v(0);
+                reads_first<D>();
+#pragma unroll
+                for (int u = 0; u < 4; ++u) x[u & 1] = Vec<T>::mma32(kf[g & 1][u], q[2 * g + (u >> 1)], x[u & 1]);
+                reads_first<D>();
+            }
+            const bool whole = kt + kManyKeys <= lo && !mixed;
+            if constexpr (EXTRA) {
 #pragma unroll
                 for (int b = 0; b < 2; ++b)
 #pragma unroll
-                    for (int j = 0; j < 16; ++j)
-                        x[b][j] = a.cap_log2 * (1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x[b][j])));
-            }
-            if (a.k_times) {
+                    for (int j = 0; j < 16; ++j) x[b][j] *= a.scale_log2;
+                if (a.cap_log2 != 0.0f) {
 #pragma unroll
-                for (int b = 0; b < 2; ++b)
+                    for (int b = 0; b < 2; ++b)
 #pragma unroll
-                    for (int j = 0; j < 16; ++j)
-                        x[b][j] -= dec * fmaxf(0.0f, tq - sh.times[buf][b * 32 + (j >> 3) * 16 + h * 8 + (j & 7)]);
-            }
-        }
-        if (!whole) {
-            // bit j: this lane's row sees key kt + j
-            uint64_t seen = limit - kt >= 64 ? ~0ull : limit > kt ? (1ull << (limit - kt)) - 1 : 0ull;
-            if (EXTRA && mixed) {
-                // by the tile's few different episodes, each with the keys that have it
-                const int e = sh.eps[buf][lane];
-                uint64_t rest = keys - kt >= 64 ? ~0ull : (1ull << (keys - kt)) - 1, by_episode = 0;
-                while (rest) {
-                    const int v = __builtin_amdgcn_readlane(e, __builtin_ctzll(rest));
-                    const uint64_t with = __ballot(e == v);
-                    by_episode |= v < 0 || eq < 0 || eq == v ? with : 0ull;
-                    rest &= ~with;
+                        for (int j = 0; j < 16; ++j)
+                            x[b][j] = a.cap_log2 * (1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x[b][j])));
                 }
-                seen &= by_episode;
+                if (a.k_times) {
+#pragma unroll
+                    for (int b = 0; b < 2; ++b)
+#pragma unroll
+                        for (int j = 0; j < 16; ++j)
+                            x[b][j] -= dec * fmaxf(0.0f, tq - sh.times[buf][b * 32 + (j >> 3) * 16 + h * 8 + (j & 7)]);
+                }
             }
-            seen >>= 8 * h;                                  // bit 32 b + 16 (j / 8) + j % 8: register j of block b
+            if (!whole) {
+                // bit j: this lane's row sees key kt + j
+                uint64_t seen = limit - kt >= 64 ? ~0ull : limit > kt ? (1ull << (limit - kt)) - 1 : 0ull;
+                if (EXTRA && mixed) {
+                    // by the tile's few different episodes, each with the keys that have it
+                    const int e = sh.eps[buf][lane];
+                    uint64_t rest = keys - kt >= 64 ? ~0ull : (1ull << (keys - kt)) - 1, by_episode = 0;
+                    while (rest) {
+                        const int v = __builtin_amdgcn_readlane(e, __builtin_ctzll(rest));
+                        const uint64_t with = __ballot(e == v);
+                        by_episode |= v < 0 || eq < 0 || eq == v ? with : 0ull;
+                        rest &= ~with;
+                    }
+                    seen &= by_episode;
+                }
+                seen >>= 8 * h;                                  // bit 32 b + 16 (j / 8) + j % 8: register j of block b
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        const uint32_t in = uint32_t(__builtin_amdgcn_sbfe(int(seen >> (32 * b)), (j >> 3) * 16 + (j & 7), 1));
+                        x[b][j] = __uint_as_float((__float_as_uint(x[b][j]) & in) | (__float_as_uint(-kInf) & ~in));
+                    }
+            }
+            const float c = EXTRA ? 1.0f : a.scale_log2;         // not negative: a negative scale turns q's sign
+            float top = x[0][0];
+#pragma unroll
+            for (int j = 1; j < 16; ++j) top = fmaxf(top, x[0][j]);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) top = fmaxf(top, x[1][j]);
+            top *= c;
+            if (__any(top > mtop)) {
+                top = fmaxf(top, __shfl_xor(top, 32));
+                const bool none = mtop == -kInf;
+                const float mnew = none ? top : fmaxf(mref, top);
+                if (mnew > -kInf) {                          // not NaN either: the row's sum is then NaN
+                    const float f = none ? 0.0f : __builtin_amdgcn_exp2f(mref - mnew);
+                    mref = mnew;
+                    mtop = mnew + kSlack;
+                    l *= f;
+#pragma unroll
+                    for (int d = 0; d < DB; ++d) o[d] *= f;
+                }
+            }
+            V p[4];
 #pragma unroll
             for (int b = 0; b < 2; ++b)
 #pragma unroll
                 for (int j = 0; j < 16; ++j) {
-                    const uint32_t in = uint32_t(__builtin_amdgcn_sbfe(int(seen >> (32 * b)), (j >> 3) * 16 + (j & 7), 1));
-                    x[b][j] = __uint_as_float((__float_as_uint(x[b][j]) & in) | (__float_as_uint(-kInf) & ~in));
+                    const float w = __builtin_amdgcn_exp2f(fmaf(x[b][j], c, -mref));
+                    l += w;
+                    p[2 * b + (j >> 3)][j & 7] = T(w);
                 }
-        }
-        const float c = EXTRA ? 1.0f : a.scale_log2;         // not negative: a negative scale turns q's sign
-        float top = x[0][0];
 #pragma unroll
-        for (int j = 1; j < 16; ++j) top = fmaxf(top, x[0][j]);
+            for (int t = 0; t < 4; ++t) {
+                if (t < 3) read_v(t + 1);
+                reads_first<D>();
 #pragma unroll
-        for (int j = 0; j < 16; ++j) top = fmaxf(top, x[1][j]);
-        top *= c;
-        if (__any(top > mtop)) {
-            top = fmaxf(top, __shfl_xor(top, 32));
-            const bool none = mtop == -kInf;
-            const float mnew = none ? top : fmaxf(mref, top);
-            if (mnew != -kInf) {
-                const float f = none ? 0.0f : __builtin_amdgcn_exp2f(mref - mnew);
-                mref = mnew;
-                mtop = mnew + kSlack;
-                l *= f;
-#pragma unroll
-                for (int d = 0; d < DB; ++d) o[d] *= f;
+                for (int d = 0; d < DB; ++d) o[d] = Vec<T>::mma32(vf[t & 1][d], p[t], o[d]);
+                reads_first<D>();
             }
         }
-        V p[4];
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                const float w = __builtin_amdgcn_exp2f(fmaf(x[b][j], c, -mref));
-                l += w;
-                p[2 * b + (j >> 3)][j & 7] = T(w);
-            }
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            if (t < 3) read_v(t + 1);
-            reads_first<D>();
-#pragma unroll
-            for (int d = 0; d < DB; ++d) o[d] = Vec<T>::mma32(vf[t & 1][d], p[t], o[d]);
-            reads_first<D>();
-        }
-    }
-    if (!listed) break;
+        if (!listed) break;
     }
 
     l += __shfl_xor(l, 32);
-    const bool empty = mtop == -kInf;
+    const bool empty = mtop == -kInf && l == 0.0f;           // with NaN scores alone the sum is NaN
     // o[d][j] is element 32 d + 8 (j / 4) + 4 h + j % 4 of row `col`
     if (it.splits == 1 && row_ok) {
         const float inv = empty ? 0.0f : 1.0f / l;
@@ -1298,45 +1298,45 @@ __global__ __launch_bounds__(256) void k_attend_join(AttendArgs a) {
     if (!sched.start()) return;
     Part it;
     for (uint32_t block = blockIdx.x; sched.find(block, &it); block += gridDim.x) {
-    const int r0 = it.slot * kJoinRows, rows = min(kJoinRows, it.n * a.group - it.tile * kManyRows - r0);
-    if (!own_pieces(a, &it, 0) || it.splits == 1) continue;
-    const float2* const ml = a.many_ml + int64_t(it.slot0) * kManyRows + r0;
-    const float* const po = a.many_o + (int64_t(it.slot0) * kManyRows + r0) * D;
-    for (int e = int(threadIdx.x); e < rows * (D / 4); e += 256) {
-        const int rr = e / (D / 4), d4 = e % (D / 4);
-        constexpr int U = 8;
-        float top = -kInf, l = 0.0f;
-        f32x4 sum = {0, 0, 0, 0};
-        for (int s = 0; s < it.splits; s += U) {
-            float2 p[U];
-            f32x4 o[U];
+        const int r0 = it.slot * kJoinRows, rows = min(kJoinRows, it.n * a.group - it.tile * kManyRows - r0);
+        if (!own_pieces(a, &it, 0) || it.splits == 1) continue;
+        const float2* const ml = a.many_ml + int64_t(it.slot0) * kManyRows + r0;
+        const float* const po = a.many_o + (int64_t(it.slot0) * kManyRows + r0) * D;
+        for (int e = int(threadIdx.x); e < rows * (D / 4); e += 256) {
+            const int rr = e / (D / 4), d4 = e % (D / 4);
+            constexpr int U = 8;
+            float top = -kInf, l = 0.0f;
+            f32x4 sum = {0, 0, 0, 0};
+            for (int s = 0; s < it.splits; s += U) {
+                float2 p[U];
+                f32x4 o[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                if (s + u >= it.splits) break;
-                const int64_t at = int64_t(s + u) * kManyRows + rr;
-                p[u] = ml[at];
-                o[u] = *reinterpret_cast<const f32x4*>(po + at * D + d4 * 4);
-            }
+                for (int u = 0; u < U; ++u) {
+                    if (s + u >= it.splits) break;
+                    const int64_t at = int64_t(s + u) * kManyRows + rr;
+                    p[u] = ml[at];
+                    o[u] = *reinterpret_cast<const f32x4*>(po + at * D + d4 * 4);
+                }
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                if (s + u >= it.splits) break;
-                if (p[u].x == -kInf) continue;
-                const float next = fmaxf(top, p[u].x), was = top == -kInf ? 0.0f : __builtin_amdgcn_exp2f(top - next);
-                const float f = __builtin_amdgcn_exp2f(p[u].x - next);
-                l = top == -kInf ? f * p[u].y : l * was + f * p[u].y;
-                sum = top == -kInf ? f * o[u] : sum * was + f * o[u];
-                top = next;
+                for (int u = 0; u < U; ++u) {
+                    if (s + u >= it.splits) break;
+                    if (p[u].x == -kInf) continue;
+                    const float next = fmaxf(top, p[u].x), was = top == -kInf ? 0.0f : __builtin_amdgcn_exp2f(top - next);
+                    const float f = __builtin_amdgcn_exp2f(p[u].x - next);
+                    l = top == -kInf ? f * p[u].y : l * was + f * p[u].y;
+                    sum = top == -kInf ? f * o[u] : sum * was + f * o[u];
+                    top = next;
+                }
             }
+            const int mm = it.tile * kManyRows + r0 + rr, ii = mm / a.group, hh = it.head * a.group + mm - ii * a.group;
+            const float inv = 1.0f / l;
+            typename Vec<T>::v4 w;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = top == -kInf ? T(0.0f) : T(sum[j] * inv);
+            *reinterpret_cast<typename Vec<T>::v4*>(static_cast<T*>(a.out) + (int64_t(it.row0) + ii) * a.out_stride + int64_t(hh) * D + d4 * 4) = w;
+            if (a.lse && d4 == 0)
+                a.lse[(int64_t(it.row0) + ii) * a.q_heads + hh] = top == -kInf ? -kInf : (top + __builtin_amdgcn_logf(l)) * kLn2;
         }
-        const int mm = it.tile * kManyRows + r0 + rr, ii = mm / a.group, hh = it.head * a.group + mm - ii * a.group;
-        const float inv = 1.0f / l;
-        typename Vec<T>::v4 w;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) w[j] = top == -kInf ? T(0.0f) : T(sum[j] * inv);
-        *reinterpret_cast<typename Vec<T>::v4*>(static_cast<T*>(a.out) + (int64_t(it.row0) + ii) * a.out_stride + int64_t(hh) * D + d4 * 4) = w;
-        if (a.lse && d4 == 0)
-            a.lse[(int64_t(it.row0) + ii) * a.q_heads + hh] = top == -kInf ? -kInf : (top + __builtin_amdgcn_logf(l)) * kLn2;
-    }
     }
 }
 

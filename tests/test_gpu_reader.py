@@ -471,6 +471,23 @@ def test_attend_not_finite_values_that_all_rows_see(n, D, page):
         check_attend(Reader(4, 2, D, "float16", page), "float16", q, k, v, [0, n], [L], table, max_new=(0, n))
 
 
+@pytest.mark.parametrize("D,page", [(64, 16), (128, 64), (256, 32)])
+@pytest.mark.parametrize("n", [1, 40])
+def test_attend_scores_that_are_not_numbers(n, D, page):
+    """A row of q that holds NaN, and NaN in the only key that a row sees: the row is NaN, the others are not."""
+    rng = np.random.default_rng(7 * n + D)
+    for L in (n, 400 + n, 3_000):
+        table, k, v = make_cache(rng, [L], 2, D, "float16", page)
+        q = rng.standard_normal((n, 4, D))
+        q[n // 2, 1, 3] = np.nan
+        q = ref.to_bits(q, "float16")
+        check_attend(Reader(4, 2, D, "float16", page), "float16", q, k, v, [0, n], [L], table, max_new=(0, n))
+    table, k, v = make_cache(rng, [n], 2, D, "float16", page)
+    k.view(np.uint16)[table[0][0], 1, 0, 5] = 0x7E00
+    check_attend(Reader(4, 2, D, "float16", page), "float16", ref.to_bits(rng.standard_normal((n, 4, D)), "float16"), k, v, [0, n], [n], table,
+                 max_new=(0, n))
+
+
 def test_attend_scores_of_any_size():
     """Scores far from zero: rows whose largest score is very low, very high, and rising by more than the weights' range."""
     rng = np.random.default_rng(6)
