@@ -263,21 +263,51 @@ __global__ __launch_bounds__(256) void k_kv_store_tile(StoreArgs a) {
         const int64_t s = k && tid < nt ? a.s.slots[t0 + tid] : -1;
         slot_of[tid] = s >= 0 && s < a.slots ? s : -1;
     }
+    // everything the workgroup reads is on the way before the angles are computed: its v, and of q and k the first pieces
+    constexpr int VU = kTile * (D / 8) / 256;
+    v8 vr[VU];
     if (v) {
-        for (int e = tid; e < nt * (D / 8); e += 256) {
-            const int i = e / (D / 8), c = e % (D / 8);
-            const v8 x = *reinterpret_cast<const v8*>(v + (t0 + i) * a.s.v_stride + head * D + c * 8);
-            typedef uint32_t u4 __attribute__((ext_vector_type(4)));
-            const u4 w = __builtin_bit_cast(u4, x);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) reinterpret_cast<uint32_t*>(&vt[i][c * 8])[j] = w[j];
+        for (int u = 0; u < VU; ++u) {
+            const int e = tid + u * 256, i = e / (D / 8), c = e % (D / 8);
+            if (i < nt) vr[u] = *reinterpret_cast<const v8*>(v + (t0 + i) * a.s.v_stride + head * D + c * 8);
         }
     }
+    // q and k: a thread takes two pieces of 8 elements of a head, the partners of each other where they turn (both are read
+    // before either is written: q_out may be q), and four such pairs on the way together
+    constexpr int U = 4;
+    const int heads = group + (k ? 1 : 0), turning = half / 8, pairs = nt * heads * (D / 16);
+    v8 y[U], z[U];
+    auto first_of = [&](int c) { return c < turning && !a.adjacent ? c * 8 : c * 16; };
+    auto second_of = [&](int c) { return c < turning && !a.adjacent ? half + c * 8 : c * 16 + 8; };
+    auto read_pairs = [&](int e0) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int e = e0 + u * 256, c = e % (D / 16), ih = e / (D / 16), i = ih / heads, hh = ih % heads;
+            if (e >= pairs) break;
+            const T* const x = hh < group ? q + (t0 + i) * a.s.q_stride + (head * group + hh) * D : k + (t0 + i) * a.s.k_stride + head * D;
+            y[u] = *reinterpret_cast<const v8*>(x + first_of(c));
+            z[u] = *reinterpret_cast<const v8*>(x + second_of(c));
+        }
+    };
+    read_pairs(tid);
     for (int e = tid; e < nt * half; e += 256) {
         const int i = e / half, f = e % half;
         float sn, cs;
         turn(a.s.positions[int64_t(a.axis[f]) * a.s.num_tokens + t0 + i], a.freq[f], &sn, &cs);
         turns[i][f] = make_float2(cs, a.s.inverse ? -sn : sn);
+    }
+    if (v) {
+#pragma unroll
+        for (int u = 0; u < VU; ++u) {
+            const int e = tid + u * 256, i = e / (D / 8), c = e % (D / 8);
+            typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+            const u4 w = __builtin_bit_cast(u4, vr[u]);
+            if (i < nt) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) reinterpret_cast<uint32_t*>(&vt[i][c * 8])[j] = w[j];
+            }
+        }
     }
     __syncthreads();
     if (k && tid < kTile) {
@@ -301,40 +331,38 @@ __global__ __launch_bounds__(256) void k_kv_store_tile(StoreArgs a) {
         }
     }
 
-    // q and k: a thread takes two pieces of 8 elements of a head, the partners of each other where they turn (both are read
-    // before either is written: q_out may be q)
-    const int heads = group + (k ? 1 : 0), turning = half / 8;
-    for (int e = tid; e < nt * heads * (D / 16); e += 256) {
-        const int c = e % (D / 16), ih = e / (D / 16), i = ih / heads, hh = ih % heads;
-        const bool is_q = hh < group;
-        if (!is_q && slot_of[i] < 0) continue;
-        const T* const x = is_q ? q + (t0 + i) * a.s.q_stride + (head * group + hh) * D : k + (t0 + i) * a.s.k_stride + head * D;
-        T* const to = is_q ? static_cast<T*>(a.s.q_out) + (t0 + i) * a.s.q_out_stride + (head * group + hh) * D
-                           : static_cast<T*>(a.k_pages) + (slot_of[i] >> a.page_shift) * a.k_stride + (int64_t(head) * P + (slot_of[i] & (P - 1))) * D;
-        const bool turns_c = c < turning;
-        const int p0 = turns_c && !a.adjacent ? c * 8 : c * 16, p1 = turns_c && !a.adjacent ? half + c * 8 : c * 16 + 8;
-        const v8 y = *reinterpret_cast<const v8*>(x + p0), z = *reinterpret_cast<const v8*>(x + p1);
-        v8 u = y, w = z;
-        if (turns_c && !a.adjacent) {
+    for (int e0 = tid; e0 < pairs; e0 += U * 256) {
+        if (e0 != tid) read_pairs(e0);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float2 f = turns[i][c * 8 + j];
-                const float yy = float(y[j]), zz = float(z[j]);
-                u[j] = T(yy * f.x - zz * f.y);
-                w[j] = T(yy * f.y + zz * f.x);
-            }
-        } else if (turns_c) {
+        for (int n = 0; n < U; ++n) {
+            const int e = e0 + n * 256, c = e % (D / 16), ih = e / (D / 16), i = ih / heads, hh = ih % heads;
+            if (e >= pairs) break;
+            const bool is_q = hh < group;
+            if (!is_q && slot_of[i] < 0) continue;
+            T* const to = is_q ? static_cast<T*>(a.s.q_out) + (t0 + i) * a.s.q_out_stride + (head * group + hh) * D
+                               : static_cast<T*>(a.k_pages) + (slot_of[i] >> a.page_shift) * a.k_stride + (int64_t(head) * P + (slot_of[i] & (P - 1))) * D;
+            v8 u = y[n], w = z[n];
+            if (c < turning && !a.adjacent) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float2 f = turns[i][c * 8 + j];        // pair j of the 16 elements
-                const float yy = float(j < 4 ? y[2 * j] : z[2 * j - 8]), zz = float(j < 4 ? y[2 * j + 1] : z[2 * j - 7]);
-                const T lo = T(yy * f.x - zz * f.y), hi = T(yy * f.y + zz * f.x);
-                if (j < 4) { u[2 * j] = lo; u[2 * j + 1] = hi; }
-                else { w[2 * j - 8] = lo; w[2 * j - 7] = hi; }
+                for (int j = 0; j < 8; ++j) {
+                    const float2 f = turns[i][c * 8 + j];
+                    const float yy = float(y[n][j]), zz = float(z[n][j]);
+                    u[j] = T(yy * f.x - zz * f.y);
+                    w[j] = T(yy * f.y + zz * f.x);
+                }
+            } else if (c < turning) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float2 f = turns[i][c * 8 + j];    // pair j of the 16 elements
+                    const float yy = float(j < 4 ? y[n][2 * j] : z[n][2 * j - 8]), zz = float(j < 4 ? y[n][2 * j + 1] : z[n][2 * j - 7]);
+                    const T lo = T(yy * f.x - zz * f.y), hi = T(yy * f.y + zz * f.x);
+                    if (j < 4) { u[2 * j] = lo; u[2 * j + 1] = hi; }
+                    else { w[2 * j - 8] = lo; w[2 * j - 7] = hi; }
+                }
             }
+            *reinterpret_cast<v8*>(to + first_of(c)) = u;
+            *reinterpret_cast<v8*>(to + second_of(c)) = w;
         }
-        *reinterpret_cast<v8*>(to + p0) = u;
-        *reinterpret_cast<v8*>(to + p1) = w;
     }
     if (!v) return;
     __syncthreads();
@@ -355,7 +383,7 @@ __global__ __launch_bounds__(256) void k_kv_store_tile(StoreArgs a) {
 
 template <typename T, int D>
 int launch_store_tile(const StoreArgs& a, hipStream_t s) {
-    const unsigned tiles = unsigned((a.s.num_tokens + store_tile<D>() - 1) / store_tile<D>());
+    const unsigned tiles = unsigned((int64_t(a.s.num_tokens) + store_tile<D>() - 1) / store_tile<D>());
     MARS_LAUNCH((k_kv_store_tile<T, D>), dim3(tiles, unsigned(a.kv_heads)), dim3(256), 0, s, a);
     return MARS_OK;
 }
@@ -475,7 +503,7 @@ int mars_kv_plan(const mars_reader* r, const mars_kv_plan_args* a, void* stream)
     MARS_CHECK(a->num_requests <= kMaxRequests, MARS_ERR_CAPACITY, "%d requests (at most %d)", a->num_requests, kMaxRequests);
     MARS_CHECK(a->free_count_out != a->free_count, MARS_ERR_INVALID, "free_count_out is free_count");
     MARS_TRY(use_device(r->device));
-    const int blocks = std::max(1, (a->num_tokens + kPlanTokens - 1) / kPlanTokens);
+    const int64_t blocks = std::max<int64_t>(1, (int64_t(a->num_tokens) + kPlanTokens - 1) / kPlanTokens);
     MARS_LAUNCH(k_kv_plan, dim3(unsigned(blocks)), dim3(kPlanThreads), 0, static_cast<hipStream_t>(stream), *a, r->page_shift);
     return MARS_OK;
 }
