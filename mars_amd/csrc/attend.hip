@@ -37,15 +37,17 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 constexpr float kInf = __builtin_inff();
 constexpr float kLn2 = 0.69314718055994530942f;
-// s_waitcnt immediate (gfx9 encoding: vmcnt[3:0] and [15:14], expcnt[6:4], lgkmcnt[11:8]): all loads, or all LDS accesses, done
+// s_waitcnt immediate (gfx9 encoding: vmcnt[3:0] and [15:14], expcnt[6:4], lgkmcnt[11:8]): all loads, all LDS accesses, or both, done
 constexpr int kWaitVm0 = (7 << 4) | (15 << 8);
+constexpr int kWaitVm0Lgkm0 = 7 << 4;
 constexpr int kWaitLgkm0 = 15 | (3 << 14) | (7 << 4);
 constexpr float kSlack = 8.0f;       // how far a score may exceed the row's reference
 
-// Every load of this wave is done (LDS ones too), and every other wave got here.
+// Every load of this wave is done, those into LDS and the reads of LDS too (a product that takes one may come later: the
+// buffer it was read from is refilled after this), and every other wave got here.
 __device__ inline void tile_barrier() {
     asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt(kWaitVm0);
+    __builtin_amdgcn_s_waitcnt(kWaitVm0Lgkm0);
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
 }
