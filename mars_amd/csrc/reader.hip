@@ -502,6 +502,10 @@ int mars_kv_plan(const mars_reader* r, const mars_kv_plan_args* a, void* stream)
                "%d requests, %d pages a row, %d tokens, %d free entries", a->num_requests, a->max_pages, a->num_tokens, a->free_capacity);
     MARS_CHECK(a->num_requests <= kMaxRequests, MARS_ERR_CAPACITY, "%d requests (at most %d)", a->num_requests, kMaxRequests);
     MARS_CHECK(a->free_count_out != a->free_count, MARS_ERR_INVALID, "free_count_out is free_count");
+    // every workgroup reads the lengths for itself, while the first writes its outputs
+    for (const int32_t* const out : {a->kv_lens, a->q_start})
+        MARS_CHECK(out != a->cached_lens && out != a->new_lens, MARS_ERR_INVALID, "%s is %s",
+                   out == a->kv_lens ? "kv_lens" : "q_start", out == a->cached_lens ? "cached_lens" : "new_lens");
     MARS_TRY(use_device(r->device));
     const int64_t blocks = std::max<int64_t>(1, (int64_t(a->num_tokens) + kPlanTokens - 1) / kPlanTokens);
     MARS_LAUNCH(k_kv_plan, dim3(unsigned(blocks)), dim3(kPlanThreads), 0, static_cast<hipStream_t>(stream), *a, r->page_shift);

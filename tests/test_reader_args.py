@@ -169,3 +169,18 @@ def test_c_refusals():
                      (dict(num_requests=4097), CAPACITY), (dict(max_pages=0), INVALID), (dict(free_capacity=-1), INVALID), (dict(num_tokens=-1), INVALID)):
         a = _lib.KvPlanArgsC(**{**plan, **kw})
         assert lib.mars_kv_plan(r.handle, C.byref(a), None) == code, kw
+
+
+@pytest.mark.gpu
+def test_plan_refuses_lengths_in_place():
+    """kv_lens and q_start are written while other workgroups still read the lengths; nothing is launched."""
+    import mars_amd
+    mars_amd.init(0)
+    r = Reader(4, 2, 64, "float16", 16)
+    at = [(1 << 20) + 256 * i for i in range(10)]
+    names = ("new_lens", "cached_lens", "block_table", "free_pages", "free_count", "q_start", "kv_lens", "slots", "positions", "free_count_out")
+    plan = dict(zip(names, at), num_requests=3, max_pages=5, num_tokens=7, free_capacity=9)
+    for out in ("kv_lens", "q_start"):
+        for lens in ("cached_lens", "new_lens"):
+            a = _lib.KvPlanArgsC(**{**plan, out: plan[lens]})
+            assert lib.mars_kv_plan(r.handle, C.byref(a), None) == INVALID, (out, lens)
