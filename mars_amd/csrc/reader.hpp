@@ -34,7 +34,10 @@ constexpr int32_t kFewMost = 16;             // rows of a request that k_attend_
 constexpr int32_t kManyItemsLog2 = 9;
 constexpr int32_t kManyRows = 128;
 constexpr int32_t kJoinRows = 16;            // of a tile's rows, joined by a workgroup
-constexpr int32_t kMinChunk = 256;           // keys of a work item, unless the request has fewer (a multiple of 256; 512 took the same times within 2%)
+// Keys of a work item, unless the request has fewer; items are multiples of 256. At least 512: two requests of 56 tokens over
+// 1,067 keys (32/8 heads of 64) 27.5 us (22.2), one of 112 tokens over 577 keys among 12 single ones (2/2 of 64) 28.6 us (25.0).
+// At least 128, in multiples of 128: two chunks of 511 tokens among 22 single ones (32/8 of 128) 147 us (122).
+constexpr int32_t kMinChunk = 256;
 constexpr int32_t kMaxSplits = 256;          // pieces of a tile, as many as a join keeps references of in LDS
 
 struct AttendArgs {
