@@ -55,17 +55,18 @@ class Session:
         tokens = len(q)
         q, k, v = up(q), up(k), up(v)
         start, slots, pos = DeviceArray((self.requests + 1,), "int32"), DeviceArray((tokens,), "int64"), DeviceArray((tokens,), "int32")
+        lens = DeviceArray((self.requests,), "int32")
         times, episodes = up(times.astype(np.float32)), up(episodes.astype(np.int32))
         self.reader.plan(up(np.asarray(new_lens, np.int32)), self.lens[0], self.table, self.free, self.left[0], q_start=start,
-                         kv_lens=self.lens[1], slots=slots, positions=pos, free_count_out=self.left[1])
+                         kv_lens=lens, slots=slots, positions=pos, free_count_out=self.left[1], next_lens=self.lens[1])
         self.reader.store(self.cache, q, k, v, up(places.astype(np.int32)), slots, times=times, episodes=episodes)
         out = DeviceArray((tokens, HEADS, DIM), "float16")
-        self.reader.attend(self.cache, q, out, start, self.lens[1], self.table, cap=30.0, decay=self.decay, q_times=times,
+        self.reader.attend(self.cache, q, out, start, lens, self.table, cap=30.0, decay=self.decay, q_times=times,
                            q_episodes=episodes, max_new=int(max(new_lens)))
         self.lens.reverse()
         self.left.reverse()
         y = out.numpy()                                     # waits: every input above may go now
-        self.steps.append(dict(new_lens=list(new_lens), q=q.numpy(), out=y, start=start.numpy(), lens=self.lens[0].numpy(),
+        self.steps.append(dict(new_lens=list(new_lens), q=q.numpy(), out=y, start=start.numpy(), lens=lens.numpy(),
                                table=self.table.numpy(), times=times.numpy(), episodes=episodes.numpy()))
         return y.reshape(tokens, -1).astype(np.float32)
 

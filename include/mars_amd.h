@@ -728,12 +728,14 @@ int mars_reader_destroy(mars_reader* r);
  * fit what is free. One whose tokens exceed its table row (max_pages) or the num_tokens rows
  * of the step takes none and is not served. Outputs (all device):
  *   q_start[R + 1]      first row of each request; q_start[R] = total of new_lens
- *   kv_lens[R]          tokens with this step's (cached + new), 0 if not served
+ *   kv_lens[R]          tokens with this step's (cached + new), 0 if not served: what mars_kv_attend reads
+ *   next_lens[R]        tokens in the cache after the step: cached + new, or cached if not served (its pages
+ *                       stay its own). The next step's cached_lens, and the lengths that mars_kv_release takes
  *   slots[num_tokens]   page * page_size + offset of each new token; -1 if not served or past the total
  *   positions[num_tokens]  its index within the request; 0 past the total
  *   free_count_out[1]   pages left (a later step reads it as its free_count)
- * Outputs must not overlap inputs (kv_lens is the next step's cached_lens: use two arrays in turn).
- * R <= MARS_KV_MAX_REQUESTS. */
+ * Outputs must not overlap inputs or each other (two arrays in turn hold cached_lens and next_lens). The new
+ * tokens of a request that was not served are given again in a later step. R <= MARS_KV_MAX_REQUESTS. */
 typedef struct mars_kv_plan_args {
     const int32_t* new_lens;
     const int32_t* cached_lens;
@@ -749,12 +751,14 @@ typedef struct mars_kv_plan_args {
     int32_t        max_pages;
     int32_t        num_tokens;
     int32_t        free_capacity;   /* entries of free_pages */
+    int32_t*       next_lens;       /* NULL: not wanted; kv_lens says the same where every request is served */
 } mars_kv_plan_args;
 int mars_kv_plan(const mars_reader* r, const mars_kv_plan_args* args, void* stream);
 
 /* Gives back the pages of the requests with done[r] != 0: the ceil(kv_lens[r] / page_size) pages
  * of their table rows are pushed onto free_pages in request order, free_count[0] grows, and
- * kv_lens[r] becomes 0. Pages beyond free_capacity are dropped. */
+ * kv_lens[r] becomes 0. kv_lens: the tokens in the cache (mars_kv_plan's next_lens). Pages beyond
+ * free_capacity are dropped. */
 int mars_kv_release(const mars_reader* r, const int32_t* done, int32_t* kv_lens, const int32_t* block_table,
                     int32_t num_requests, int32_t max_pages, int32_t* free_pages, int32_t* free_count,
                     int32_t free_capacity, void* stream);

@@ -202,7 +202,7 @@ class KvPlanArgsC(C.Structure):
     _fields_ = [("new_lens", C.c_void_p), ("cached_lens", C.c_void_p), ("block_table", C.c_void_p), ("free_pages", C.c_void_p),
                 ("free_count", C.c_void_p), ("q_start", C.c_void_p), ("kv_lens", C.c_void_p), ("slots", C.c_void_p),
                 ("positions", C.c_void_p), ("free_count_out", C.c_void_p), ("num_requests", C.c_int32),
-                ("max_pages", C.c_int32), ("num_tokens", C.c_int32), ("free_capacity", C.c_int32)]
+                ("max_pages", C.c_int32), ("num_tokens", C.c_int32), ("free_capacity", C.c_int32), ("next_lens", C.c_void_p)]
 
 
 class KvCacheC(C.Structure):

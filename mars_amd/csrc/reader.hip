@@ -92,7 +92,10 @@ __global__ __launch_bounds__(kPlanThreads) void k_kv_plan(mars_kv_plan_args a, i
         cached[r] = n_old[i];
         taken += need[i];
         if (served && need[i] > 0) used = taken;
-        if (blockIdx.x == 0) a.kv_lens[r] = served ? n_old[i] + n_new[i] : 0;
+        if (blockIdx.x == 0) {
+            a.kv_lens[r] = served ? n_old[i] + n_new[i] : 0;
+            if (a.next_lens) a.next_lens[r] = n_old[i] + (served ? n_new[i] : 0);
+        }
     }
     if (blockIdx.x == 0) {
         // the last served request that took pages has the largest running count: a maximum, as the prefix grows
@@ -503,9 +506,10 @@ int mars_kv_plan(const mars_reader* r, const mars_kv_plan_args* a, void* stream)
     MARS_CHECK(a->num_requests <= kMaxRequests, MARS_ERR_CAPACITY, "%d requests (at most %d)", a->num_requests, kMaxRequests);
     MARS_CHECK(a->free_count_out != a->free_count, MARS_ERR_INVALID, "free_count_out is free_count");
     // every workgroup reads the lengths for itself, while the first writes its outputs
-    for (const int32_t* const out : {a->kv_lens, a->q_start})
-        MARS_CHECK(out != a->cached_lens && out != a->new_lens, MARS_ERR_INVALID, "%s is %s",
-                   out == a->kv_lens ? "kv_lens" : "q_start", out == a->cached_lens ? "cached_lens" : "new_lens");
+    for (const int32_t* const out : {a->kv_lens, a->q_start, a->next_lens})
+        MARS_CHECK(!out || (out != a->cached_lens && out != a->new_lens), MARS_ERR_INVALID, "%s is %s",
+                   out == a->kv_lens ? "kv_lens" : out == a->q_start ? "q_start" : "next_lens", out == a->cached_lens ? "cached_lens" : "new_lens");
+    MARS_CHECK(!a->next_lens || (a->next_lens != a->kv_lens && a->next_lens != a->q_start), MARS_ERR_INVALID, "next_lens is another output");
     MARS_TRY(use_device(r->device));
     const int64_t blocks = std::max<int64_t>(1, (int64_t(a->num_tokens) + kPlanTokens - 1) / kPlanTokens);
     MARS_LAUNCH(k_kv_plan, dim3(unsigned(blocks)), dim3(kPlanThreads), 0, static_cast<hipStream_t>(stream), *a, r->page_shift);

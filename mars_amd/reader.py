@@ -6,7 +6,7 @@
     r.plan(new_lens, cached_lens, block_table, free_pages, free_count, q_start=..., ...)   # once a step
     r.store(cache, q, k, v, positions, slots, q_out=q, times=..., episodes=...)            # once a layer
     r.attend(cache, q, out, q_start, kv_lens, block_table, decay=..., q_times=..., ...)
-    r.release(done, kv_lens, block_table, free_pages, free_count)                          # ended requests
+    r.release(done, next_lens, block_table, free_pages, free_count)                        # ended requests
 
 The calls mirror mars_kv_* of include/mars_amd.h, which defines their results. They run on
 `stream` (the integer of a hipStream_t; 0 is the null stream) and return without waiting.
@@ -181,8 +181,9 @@ class Reader:
         return cache.ref
 
     def plan(self, new_lens, cached_lens, block_table, free_pages, free_count, *, q_start, kv_lens, slots, positions,
-             free_count_out, stream: int = 0) -> None:
-        """Block table rows extended, and q_start, kv_lens, slots, positions of a step (mars_kv_plan)."""
+             free_count_out, next_lens=None, stream: int = 0) -> None:
+        """Block table rows extended, and q_start, kv_lens, slots, positions of a step (mars_kv_plan). next_lens: the tokens
+        in the cache after it, the next step's cached_lens (kv_lens is 0 for a request that pages did not suffice for)."""
         r, t = new_lens.shape[0], slots.shape[0]
         if len(block_table.shape) != 2:
             raise ValueError(f"block_table: shape {tuple(block_table.shape)}, expected (requests, pages)")
@@ -193,11 +194,11 @@ class Reader:
             _arg(free_count, "free_count", "int32", (1,)), _arg(q_start, "q_start", "int32", (r + 1,)),
             _arg(kv_lens, "kv_lens", "int32", (r,)), _arg(slots, "slots", "int64", (t,)),
             _arg(positions, "positions", "int32", (t,)), _arg(free_count_out, "free_count_out", "int32", (1,)),
-            r, width, t, int(free_pages.shape[0]))
+            r, width, t, int(free_pages.shape[0]), _arg(next_lens, "next_lens", "int32", (r,)))
         check(lib.mars_kv_plan(self.handle, C.byref(a), stream), "mars_kv_plan")
 
     def release(self, done, kv_lens, block_table, free_pages, free_count, stream: int = 0) -> None:
-        """The pages of requests with done != 0 pushed onto free_pages; their kv_lens become 0 (mars_kv_release)."""
+        """The pages of requests with done != 0 pushed onto free_pages; their kv_lens (plan's next_lens) become 0 (mars_kv_release)."""
         r = int(done.shape[0])
         width = int(block_table.shape[1])
         check(lib.mars_kv_release(self.handle, _arg(done, "done", "int32", (r,)), _arg(kv_lens, "kv_lens", "int32", (r,)),

@@ -106,6 +106,59 @@ def test_release_and_plan_again():
     np.testing.assert_array_equal(small.numpy(), want[:6])
 
 
+@pytest.mark.parametrize("seed", [0, 1, 2])
+def test_plan_again_after_a_shortage(seed):
+    """Step after step from a pool that runs out: a request that was not served keeps its tokens, positions and pages, goes on
+    where it stood once others have ended, and every page is back exactly once at the end."""
+    rng = np.random.default_rng(seed)
+    R, page, width, pool = 6, 16, 6, 14
+    r = Reader(page_size=page)
+    table, free = dev(np.full((R, width), -1, np.int32)), dev(rng.permutation(pool).astype(np.int32))
+    lens = [dev(np.zeros(R, np.int32)) for _ in range(2)]
+    left = [dev(np.array([pool], np.int32)) for _ in range(2)]
+    have, short, again = np.zeros(R, np.int64), np.zeros(R, bool), 0
+    where = [{} for _ in range(R)]                       # slot of each of a request's tokens
+    for step in range(40):
+        new = rng.integers(0, 20, R).astype(np.int32)
+        T = int(new.sum())
+        q_start, kv, slots, pos = (DeviceArray((n,), d) for n, d in ((R + 1, "int32"), (R, "int32"), (T, "int64"), (T, "int32")))
+        r.plan(dev(new), lens[0], table, free, left[0], q_start=q_start, kv_lens=kv, slots=slots, positions=pos, free_count_out=left[1],
+               next_lens=lens[1])
+        want = ref.plan(new, have.astype(np.int32), table.numpy(), free.numpy(), int(left[0].numpy()[0]), T, page)
+        kv, slots, pos, start = kv.numpy(), slots.numpy(), pos.numpy(), q_start.numpy()
+        np.testing.assert_array_equal(kv, want[2])
+        served = (kv == have + new)
+        np.testing.assert_array_equal(kv[~served], 0)
+        for i in range(R):
+            rows = slice(start[i], start[i + 1])
+            np.testing.assert_array_equal(pos[rows], have[i] + np.arange(new[i]))
+            if served[i]:
+                where[i].update(zip(pos[rows].tolist(), slots[rows].tolist()))
+                again += bool(short[i] and have[i] and new[i])
+            else:
+                assert np.all(slots[rows] == -1)
+        short = ~served
+        have = np.where(served, have + new, have)
+        np.testing.assert_array_equal(lens[1].numpy(), have)
+        now = table.numpy()
+        held = [now[i, :-(-int(have[i]) // page)].tolist() for i in range(R)]
+        pages = sum(held, [])
+        assert len(set(pages)) == len(pages) == pool - int(left[1].numpy()[0]) and all(0 <= x < pool for x in pages)
+        for i in range(R):                               # every token lies where its table row says, those of earlier steps too
+            assert where[i] == {p: held[i][p // page] * page + p % page for p in range(int(have[i]))}
+        lens.reverse()
+        left.reverse()
+        done = rng.random(R) < (0.25 if step < 39 else 2)
+        r.release(dev(done.astype(np.int32)), lens[0], table, free, left[0])
+        have[done] = 0
+        for i in np.nonzero(done)[0]:
+            where[i] = {}
+        np.testing.assert_array_equal(lens[0].numpy(), have)
+    assert again > 0                                     # the case that this is about did occur
+    np.testing.assert_array_equal(left[0].numpy(), [pool])
+    np.testing.assert_array_equal(np.sort(free.numpy()), np.arange(pool))
+
+
 # ---- store --------------------------------------------------------------------------
 def run_store(tokens, hq, hkv, D, dtype, page, rope, sections, adjacent=False, packed=True, interleaved=False, in_place=False, inverse=False,
               seed=0, slots=None, pages=None, big=False):

@@ -184,3 +184,22 @@ def test_plan_refuses_lengths_in_place():
         for lens in ("cached_lens", "new_lens"):
             a = _lib.KvPlanArgsC(**{**plan, out: plan[lens]})
             assert lib.mars_kv_plan(r.handle, C.byref(a), None) == INVALID, (out, lens)
+
+
+@pytest.mark.gpu
+def test_plan_refuses_next_lens_in_place():
+    """next_lens is written while other workgroups still read the lengths, and beside kv_lens and q_start."""
+    import mars_amd
+    from mars_amd.reader import DeviceArray
+    mars_amd.init(0)
+    r = Reader(4, 2, 64, "float16", 16)
+    names = ("new_lens", "cached_lens", "block_table", "free_pages", "free_count", "q_start", "kv_lens", "slots", "positions", "free_count_out",
+             "next_lens")
+    arrays = {n: DeviceArray.from_numpy(np.zeros(64, np.int64)) for n in names}
+    plan = dict({n: x.data_ptr() for n, x in arrays.items()}, num_requests=3, max_pages=5, num_tokens=7, free_capacity=9)
+    for other in ("cached_lens", "new_lens", "kv_lens", "q_start"):
+        a = _lib.KvPlanArgsC(**{**plan, "next_lens": plan[other]})
+        assert lib.mars_kv_plan(r.handle, C.byref(a), None) == INVALID, other
+    for more in (plan, dict(plan, next_lens=None)):      # three requests without tokens
+        assert lib.mars_kv_plan(r.handle, C.byref(_lib.KvPlanArgsC(**more)), None) == 0
+    assert not any(arrays[n].numpy().any() for n in ("q_start", "kv_lens", "next_lens", "free_count_out"))
