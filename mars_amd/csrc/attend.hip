@@ -16,7 +16,8 @@
 //  wave of rows together): exp2 stays below 2^8, exact in 16-bit range, and the usual step
 //  needs no lane exchange and no rescaling of O. The weights are rounded to 16 bits for the
 //  second product (the matrix cores take no more at that rate); their sum is that of the
-//  unrounded ones, fp32 as every other sum.
+//  unrounded ones, fp32 as every other sum. A lane adds a step's weights up before it adds them to
+//  the row's sum: one by one, weights below 2^-24 of that sum would be lost however many there are.
 // ============================================================================
 #include "reader.hpp"
 
@@ -689,13 +690,15 @@ __device__ void few_part(const AttendArgs& a, const Part& it, FewLds<D>& lds) {
             // the weights as a 16-bit value and a 16-bit rest: the second product costs little where the cache's bytes bound the
             // kernel, and the output's error is that of its own rounding alone (with one product 1.4 times that, as in k_attend_many)
             V p, rest;
+            float sum = 0.0f;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const float w = __builtin_amdgcn_exp2f(x[j] - mref);
-                l += w;
+                sum += w;
                 p[j] = T(w);
                 rest[j] = T(w - float(p[j]));
             }
+            l += sum;
             // infinities and NaN: see add_not_finite (in every step: a rest may be 0 or negative). Slots past the request's keys
             // hold anything.
             uint32_t odd = 0;
@@ -1233,14 +1236,16 @@ __device__ void many_rows(const AttendArgs& a, int block, ManyShared<D>& lds) {
                 }
             }
             V p[4];
+            float sum = 0.0f;
 #pragma unroll
             for (int b = 0; b < 2; ++b)
 #pragma unroll
                 for (int j = 0; j < 16; ++j) {
                     const float w = __builtin_amdgcn_exp2f(fmaf(x[b][j], c, -mref));
-                    l += w;
+                    sum += w;
                     p[2 * b + (j >> 3)][j & 7] = T(w);
                 }
+            l += sum;
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
                 if (t < 3) read_v(t + 1);

@@ -750,3 +750,49 @@ def test_read_memories_example():
         assert np.all(np.abs(t["out"].astype(np.float64) - want) <= tol)
     first, last = s.steps[0], s.steps[-1]
     assert (last["lens"] == np.array(first["new_lens"]) + [5 + i for i in range(3)] + 4).all()
+
+
+# ---- attend: what the weights' range holds --------------------------------------------
+def dense(s, v, es, dtype):
+    """Scores s (rows, keys; -inf: not seen) over v (keys, D) in 64 bits, and the bounds of out and lse: the roundings of output
+    and weights, scores off by es (rows,), and for float16 the spacing of its subnormals, 2^-25 a weight against a largest of 2^7 or more."""
+    top = s.max(1, keepdims=True)
+    w = np.exp(s - top)
+    total = w.sum(1, keepdims=True)
+    o, size, u = w @ v / total, w @ np.abs(v) / total, ref.U[dtype]
+    tiny = 2.0 ** -32 * np.sum(np.isfinite(s), 1, keepdims=True) * np.abs(v).max() / total if dtype == "float16" else 0.0
+    lse = (top + np.log(total))[:, 0]
+    return o, lse, u * np.abs(o) + u * size + 2.2 * es[:, None] * size + tiny + 2.0 ** -24, es + 2.0 ** -20 * (1 + np.abs(lse))
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16"])
+@pytest.mark.parametrize("kind", ["few", "many"])
+def test_attend_long_tails(kind, dtype):
+    """One key far above tens of thousands of others that weigh something together, e^-17.4 each: none of that is lost, neither in
+    requests of single tokens nor in tiles of many rows, each over all keys in one piece."""
+    rng = np.random.default_rng(20)
+    L, D, page = 32_768, 64, 256
+    requests, n, hq, hkv = (256, 1, 4, 4) if kind == "few" else (1, 768, 64, 1)
+    one, k, v = make_cache(rng, [L], hkv, D, dtype, page)
+    k = np.zeros_like(k)
+    k[one[0][0], :, 5, 0] = ref.to_bits(17.4, dtype)
+    v = np.full(v.shape, 0, v.dtype)
+    j = np.arange(L)
+    tail = ref.to_bits(rng.uniform(0.5, 1.5, (L, D)), dtype)
+    tail[5] = ref.to_bits(np.where(np.arange(D) < D // 2, 0.0, 1.0), dtype)
+    for g in range(hkv):
+        v[one[0][j // page], g, :, j % page] = tail
+    q = np.zeros((requests * n, hq, D))
+    q[..., 0] = 8.0                                      # times D^-0.5: the score is k's element 0
+    cache = PagedCache(dev(k, dtype), dev(v, dtype))
+    out, lse = dev(ref.to_bits(np.zeros(q.shape), dtype), dtype), dev(np.zeros(q.shape[:2], np.float32))
+    Reader(hq, hkv, D, dtype, page).attend(cache, dev(ref.to_bits(q, dtype), dtype), out, dev((np.arange(requests + 1) * n).astype(np.int32)),
+                                           dev(np.full(requests, L, np.int32)), dev(np.repeat(one, requests, 0)), lse=lse, max_new=n,
+                                           prefix_lens=dev(np.full(requests, L, np.int32)))
+    s = np.zeros((1, L))
+    s[0, 5] = ref.rounded(17.4, dtype)
+    want, wlse, tol, ltol = dense(s, ref.from_bits(tail, dtype), np.array([(D + 8) * 2.0 ** -24 * s.max() + 2.0 ** -20]), dtype)
+    assert 8e-4 < want[0, 0] < 1e-3
+    err = np.abs(ref.from_bits(out.numpy(), dtype) - want[0]) - tol[0]
+    assert np.all(err <= 0), float(err.max())
+    assert np.all(np.abs(lse.numpy() - wlse[0]) <= ltol[0])
