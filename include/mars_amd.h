@@ -811,7 +811,8 @@ int mars_kv_store(const mars_reader* r, const mars_kv_cache* cache, const mars_k
  * none is 0 with lse -inf. Keys not seen have no effect, whatever the cache holds there (NaN too);
  * an infinity or NaN that a row sees makes that element of the row one of them.
  * The sums are fp32. For the product with v the weights of requests of many rows are rounded to the
- * cache's type; those of few rows keep a second value of that type for what the first leaves.
+ * cache's type; those of few rows keep a second value of that type for what the first leaves. In float16
+ * either is off by up to 2^-32 of the row's largest weight besides, a key (bfloat16 has fp32's range).
  * max_new: an upper bound of the requests' new tokens if the caller knows one (0: unknown); it picks
  * the kernel, and a wrong one costs speed alone. num_tokens rows of q; rows no request owns are left. */
 typedef struct mars_kv_attend_args {

@@ -12,9 +12,11 @@
 //  all read the same keys and values.
 //
 //  Softmax in base 2 (log2 e is folded into the scale), one pass: each row has a reference
-//  m and sums exp2(s - m), fp32. m moves only when a score exceeds it by more than 8 (in a
-//  wave of rows together): exp2 stays below 2^8, exact in 16-bit range, and the usual step
-//  needs no lane exchange and no rescaling of O. The weights are rounded to 16 bits for the
+//  m and sums exp2(s - m), fp32. m moves only when a score exceeds the one it was taken from by
+//  more than 8 (in a wave of rows together), so the usual step needs no lane exchange and no
+//  rescaling of O. For fp16 m lies 7 below that score: weights reach 2^15 of the type's 2^16, and
+//  those as low as 2^-32 of the largest still count (2^-25 without; it takes no instruction more).
+//  bf16 has fp32's range. The weights are rounded to 16 bits for the
 //  second product (the matrix cores take no more at that rate); their sum is that of the
 //  unrounded ones, fp32 as every other sum. A lane adds a step's weights up before it adds them to
 //  the row's sum: one by one, weights below 2^-24 of that sum would be lost however many there are.
@@ -42,7 +44,7 @@ constexpr float kLn2 = 0.69314718055994530942f;
 constexpr int kWaitVm0 = (7 << 4) | (15 << 8);
 constexpr int kWaitVm0Lgkm0 = 7 << 4;
 constexpr int kWaitLgkm0 = 15 | (3 << 14) | (7 << 4);
-constexpr float kSlack = 8.0f;       // how far a score may exceed the row's reference
+constexpr float kSlack = 8.0f;       // how far a score may exceed the one that the row's reference comes from
 
 // Every load of this wave is done, those into LDS and the reads of LDS too (a product that takes one may come later: the
 // buffer it was read from is refilled after this), and every other wave got here.
@@ -84,6 +86,7 @@ template <> struct Vec<_Float16> {
     using v8 = f16x8;
     using v4 = f16x4;
     static constexpr uint32_t exp_mask = 0x7C00u;
+    static constexpr float lift = 7.0f;                      // of the weights: 2^7 where the score is the reference's own
     __device__ static f32x4 mma(v8 a, v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
     __device__ static f32x16 mma32(v8 a, v8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 };
@@ -91,6 +94,7 @@ template <> struct Vec<__bf16> {
     using v8 = bf16x8;
     using v4 = bf16x4;
     static constexpr uint32_t exp_mask = 0x7F80u;
+    static constexpr float lift = 0.0f;
     __device__ static f32x4 mma(v8 a, v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
     __device__ static f32x16 mma32(v8 a, v8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 };
@@ -611,7 +615,7 @@ __device__ void few_part(const AttendArgs& a, const Part& it, FewLds<D>& lds) {
     f32x4 o[VB];
 #pragma unroll
     for (int d = 0; d < VB; ++d) o[d] = f32x4{0, 0, 0, 0};
-    float mref = 0.0f, mtop = -kInf, l = 0.0f;              // mtop: -inf until the row has seen a key, then mref + kSlack
+    float mref = 0.0f, mtop = -kInf, l = 0.0f;              // mtop: -inf until the row has seen a key, then mref + lift + kSlack
     bool dirty = false;                                     // a value that is not finite was left out
 
     auto keep_pages = [&] {
@@ -677,18 +681,19 @@ __device__ void few_part(const AttendArgs& a, const Part& it, FewLds<D>& lds) {
                 top = fmaxf(top, __shfl_xor(top, 16));
                 top = fmaxf(top, __shfl_xor(top, 32));
                 const bool none = mtop == -kInf;
-                const float mnew = none ? top : fmaxf(mref, top);
+                const float mnew = none ? top - Vec<T>::lift : fmaxf(mref, top - Vec<T>::lift);
                 if (mnew > -kInf) {                          // not NaN either: the row's sum is then NaN
                     const float f = none ? 0.0f : __builtin_amdgcn_exp2f(mref - mnew);
                     mref = mnew;
-                    mtop = mnew + kSlack;
+                    mtop = mnew + (Vec<T>::lift + kSlack);
                     l *= f;
 #pragma unroll
                     for (int d = 0; d < VB; ++d) o[d] *= f;
                 }
             }
             // the weights as a 16-bit value and a 16-bit rest: the second product costs little where the cache's bytes bound the
-            // kernel, and the output's error is that of its own rounding alone (with one product 1.4 times that, as in k_attend_many)
+            // kernel, and the output's error is that of its own rounding (with one product 1.4 times that, as in k_attend_many).
+            // fp16's rests end at 2^-25 as its values do: a weight is off by up to 2^-32 of the row's largest
             V p, rest;
             float sum = 0.0f;
 #pragma unroll
@@ -1095,7 +1100,7 @@ __device__ void many_rows(const AttendArgs& a, int block, ManyShared<D>& lds) {
     for (int d = 0; d < DB; ++d)
 #pragma unroll
         for (int j = 0; j < 16; ++j) o[d][j] = 0.0f;
-    float mref = 0.0f, mtop = -kInf, l = 0.0f;               // mtop: -inf until the row has seen a key, then mref + kSlack
+    float mref = 0.0f, mtop = -kInf, l = 0.0f;               // mtop: -inf until the row has seen a key, then mref + lift + kSlack
     bool dirty = false;                                      // a value that is not finite was left out
 
     // K's row of lane `col` in a block of 32 keys: reg j of S then holds key 16 (j / 8) + 8 h + j % 8 of the block
@@ -1225,11 +1230,11 @@ __device__ void many_rows(const AttendArgs& a, int block, ManyShared<D>& lds) {
             if (__any(top > mtop)) {
                 top = fmaxf(top, __shfl_xor(top, 32));
                 const bool none = mtop == -kInf;
-                const float mnew = none ? top : fmaxf(mref, top);
+                const float mnew = none ? top - Vec<T>::lift : fmaxf(mref, top - Vec<T>::lift);
                 if (mnew > -kInf) {                          // not NaN either: the row's sum is then NaN
                     const float f = none ? 0.0f : __builtin_amdgcn_exp2f(mref - mnew);
                     mref = mnew;
-                    mtop = mnew + kSlack;
+                    mtop = mnew + (Vec<T>::lift + kSlack);
                     l *= f;
 #pragma unroll
                     for (int d = 0; d < DB; ++d) o[d] *= f;

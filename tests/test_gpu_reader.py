@@ -765,7 +765,7 @@ def dense(s, v, es, dtype):
     return o, lse, u * np.abs(o) + u * size + 2.2 * es[:, None] * size + tiny + 2.0 ** -24, es + 2.0 ** -20 * (1 + np.abs(lse))
 
 
-@pytest.mark.parametrize("dtype", ["bfloat16"])
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
 @pytest.mark.parametrize("kind", ["few", "many"])
 def test_attend_long_tails(kind, dtype):
     """One key far above tens of thousands of others that weigh something together, e^-17.4 each: none of that is lost, neither in
