@@ -796,3 +796,31 @@ def test_attend_long_tails(kind, dtype):
     err = np.abs(ref.from_bits(out.numpy(), dtype) - want[0]) - tol[0]
     assert np.all(err <= 0), float(err.max())
     assert np.all(np.abs(lse.numpy() - wlse[0]) <= ltol[0])
+
+
+@pytest.mark.parametrize("n,length", [(1, 2_000), (1, 20_001), (13, 5_000), (70, 6_007), (200, 3_333)])
+@pytest.mark.parametrize("hq,hkv,D,dtype,page", [(8, 2, 128, "bfloat16", 64), (6, 6, 64, "float16", 16), (2, 1, 256, "float16", 32)])
+def test_attend_scores_that_rise_and_fall(n, length, hq, hkv, D, dtype, page):
+    """Scores that rise, fall, or rise and fall along the keys by more than the weights' range with every tile: the running reference
+    moves in each, rows in the middle of a wave at other keys than their neighbours, and pieces that are joined differ by hundreds."""
+    rng = np.random.default_rng(n + D)
+    table, k, v = make_cache(rng, [length], hkv, D, dtype, page)
+    j = np.arange(length)
+    kf = ref.from_bits(k, dtype)
+    q = rng.standard_normal((n, hq, D)) * 0.5
+    q[..., 0] = D ** 0.5 * np.where(rng.random((n, hq)) < 0.5, 1.0, -0.5)    # times D^-0.5: that part of the score is +-k's element 0
+    for shape in (j, length - j, length / 2 - np.abs(j - length // 2)):
+        kf[table[0][j // page], :, j % page, 0] = (shape * (400.0 / length) + shape % 7 * 0.1)[:, None] if length > 4000 else (shape * 0.1)[:, None]
+        check_attend(Reader(hq, hkv, D, dtype, page), dtype, ref.to_bits(q, dtype), ref.to_bits(kf, dtype), v, [0, n], [length], table, max_new=(0, n))
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+def test_attend_scores_of_any_size_in_tiles(dtype):
+    """Scores far from zero in requests of many rows, in one piece and in many."""
+    rng = np.random.default_rng(16)
+    n, D, page = 40, 64, 16
+    for L in (200, 3_000):
+        table, k, v = make_cache(rng, [L, L], 1, D, dtype, page)
+        q = ref.to_bits(rng.standard_normal((2 * n, 2, D)), dtype)
+        for scale in (-40.0, 1e-6, 30.0):
+            check_attend(Reader(2, 1, D, dtype, page), dtype, q, k, v, [0, n, 2 * n], [L, L], table, max_new=(0, n), scale=scale)
