@@ -824,3 +824,37 @@ def test_attend_scores_of_any_size_in_tiles(dtype):
         q = ref.to_bits(rng.standard_normal((2 * n, 2, D)), dtype)
         for scale in (-40.0, 1e-6, 30.0):
             check_attend(Reader(2, 1, D, dtype, page), dtype, q, k, v, [0, n, 2 * n], [L, L], table, max_new=(0, n), scale=scale)
+
+
+@pytest.mark.parametrize("n,dtype", [(1, "float16"), (1, "bfloat16"), (40, "float16"), (40, "bfloat16")])
+def test_attend_caps_of_any_size(n, dtype):
+    """s = cap tanh(s / cap) for caps from below the scores to far above them, where it is s itself. Scores off by 2^-20 cap for
+    caps up to 64, and by 2^-19 |s| (tanh to 2^-20 of its value, and its argument's roundings) above."""
+    rng = np.random.default_rng(n)
+    D, page, L = 64, 16, 300 + n
+    table, k, v = make_cache(rng, [L], 1, D, dtype, page)
+    q = ref.to_bits(6.0 * rng.standard_normal((n, 2, D)), dtype)
+    cache, j = PagedCache(dev(k, dtype), dev(v, dtype)), np.arange(L)
+    kf, vf = (ref.from_bits(x, dtype) for x in (k, v))
+    kf, vf = kf[table[0][j // page], 0, j % page], vf[table[0][j // page], 0, :, j % page]
+    r, start, lens, d_table, dq = Reader(2, 1, D, dtype, page), dev(np.array([0, n], np.int32)), dev(np.array([L], np.int32)), dev(table), dev(q, dtype)
+
+    def call(cap):
+        out, lse = dev(ref.to_bits(np.zeros(q.shape), dtype), dtype), dev(np.zeros((n, 2), np.float32))
+        r.attend(cache, dq, out, start, lens, d_table, lse=lse, cap=cap, max_new=n)
+        return ref.from_bits(out.numpy(), dtype), lse.numpy()
+
+    seen = j[None] <= (L - n + np.arange(n))[:, None]
+    none = call(0.0)
+    for cap in (1e-3, 20.0, 64.0, 65.0, 130.0, 300.0, 1e4, 1e6, 1e8, 1e30, 3.4e38):
+        got, glse = call(cap)
+        for h in range(2):
+            s = ref.from_bits(q, dtype)[:, h] @ kf.T * D ** -0.5
+            most = np.max(np.where(seen, np.abs(s), 0), 1)
+            es = (D + 8) * 2.0 ** -24 * np.max(np.where(seen, np.abs(ref.from_bits(q, dtype)[:, h]) @ np.abs(kf.T) * D ** -0.5, 0), 1)
+            es = es + (2.0 ** -20 * cap if cap <= 64 else 2.0 ** -19 * most) + 2.0 ** -20
+            want, wlse, tol, ltol = dense(np.where(seen, cap * np.tanh(s / cap), -np.inf), vf, es, dtype)
+            assert np.all(np.abs(got[:, h] - want) <= tol), (cap, h, float((np.abs(got[:, h] - want) - tol).max()))
+            assert np.all(np.abs(glse[:, h] - wlse) <= ltol), (cap, h, float((np.abs(glse[:, h] - wlse) - ltol).max()))
+            if cap >= 1e8:                               # no cap at all, to the last bits of the scores
+                assert np.all(np.abs(got - none[0])[:, h] <= 2 * tol) and np.all(np.abs(glse - none[1])[:, h] <= 2 * ltol)
