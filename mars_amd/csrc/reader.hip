@@ -601,7 +601,8 @@ int mars_kv_attend(const mars_reader* r, const mars_kv_cache* c, const mars_kv_a
     a.q_flip = scale < 0.0 ? 0x80008000u : 0u;
     const double cap = double(s->cap);
     const bool far = s->cap > kCapNear;
-    a.scale_log2 = float(std::fabs(cap > 0.0 && !far ? 2.0 * kLog2e * scale / cap : kLog2e * scale));
+    // finite: a score of 0 times an infinity would be NaN
+    a.scale_log2 = float(std::min(std::fabs(cap > 0.0 && !far ? 2.0 * kLog2e * scale / cap : kLog2e * scale), double(FLT_MAX)));
     a.cap_log2 = float(std::min(kLog2e * cap, double(FLT_MAX)));
     a.cap_rcp = far ? float(std::max(1.0 / (kLog2e * cap), double(FLT_MIN))) : 0.0f;
     a.requests = s->num_requests; a.max_pages = s->max_pages; a.tokens = s->num_tokens; a.num_pages = c->num_pages;

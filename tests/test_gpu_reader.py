@@ -858,3 +858,21 @@ def test_attend_caps_of_any_size(n, dtype):
             assert np.all(np.abs(glse[:, h] - wlse) <= ltol), (cap, h, float((np.abs(glse[:, h] - wlse) - ltol).max()))
             if cap >= 1e8:                               # no cap at all, to the last bits of the scores
                 assert np.all(np.abs(got - none[0])[:, h] <= 2 * tol) and np.all(np.abs(glse - none[1])[:, h] <= 2 * ltol)
+
+
+@pytest.mark.parametrize("n", [1, 40])
+def test_attend_scores_of_zero_at_the_largest_scales(n):
+    """Scores of exactly 0 stay 0 where the scale, or the scale over the cap, is as large as its type holds: every key weighs the same."""
+    rng = np.random.default_rng(n)
+    D, page, L, dtype = 64, 16, 200 + n, "float16"
+    table, k, v = make_cache(rng, [L], 1, D, dtype, page)
+    q = np.zeros((n, 2, D), np.float16)
+    j = np.arange(L)
+    vf = v.astype(np.float64)[table[0][j // page], 0, :, j % page]
+    s = np.where(j[None] <= (L - n + np.arange(n))[:, None], 0.0, -np.inf)
+    want, _, tol, _ = dense(s, vf, np.full(n, 2.0 ** -20), dtype)
+    for opt in (dict(scale=3.4e38), dict(scale=-3.4e38), dict(cap=1e-40), dict(scale=3e38, cap=30.0), dict(scale=3e38, cap=1e5)):
+        out = dev(np.ones(q.shape, np.float16))
+        Reader(2, 1, D, dtype, page).attend(PagedCache(dev(k), dev(v)), dev(q), out, dev(np.array([0, n], np.int32)), dev(np.array([L], np.int32)),
+                                            dev(table), max_new=n, **opt)
+        assert np.all(np.abs(out.numpy().astype(np.float64) - want[:, None]) <= tol[:, None]), opt
