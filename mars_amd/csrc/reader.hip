@@ -124,8 +124,9 @@ __global__ __launch_bounds__(kPlanThreads) void k_kv_plan(mars_kv_plan_args a, i
             a.block_table[int64_t(r) * a.max_pages + j] = a.free_pages[free - 1 - (fresh[r] + j - have)];
     }
     // slots and positions of this workgroup's rows
-    const int t0 = int(blockIdx.x) * kPlanTokens, t1 = min(t0 + kPlanTokens, a.num_tokens);
-    for (int t = t0 + tid; t < t1; t += kPlanThreads) {
+    const int t0 = int(blockIdx.x) * kPlanTokens, rows = min(kPlanTokens, a.num_tokens - t0);    // t0 + kPlanTokens may pass 2^31
+    for (int i = tid; i < rows; i += kPlanThreads) {
+        const int t = t0 + i;
         int64_t slot = -1;
         int32_t pos = 0;
         if (t < start[R]) {

@@ -876,3 +876,24 @@ def test_attend_scores_of_zero_at_the_largest_scales(n):
         Reader(2, 1, D, dtype, page).attend(PagedCache(dev(k), dev(v)), dev(q), out, dev(np.array([0, n], np.int32)), dev(np.array([L], np.int32)),
                                             dev(table), max_new=n, **opt)
         assert np.all(np.abs(out.numpy().astype(np.float64) - want[:, None]) <= tol[:, None]), opt
+
+
+def test_plan_of_the_most_tokens():
+    """num_tokens of 2^31 - 1, all but a few of them padding: the last rows are written as the first ones are."""
+    T, page, width = 2 ** 31 - 1, 16, 4
+    slots, pos = DeviceArray((T,), "int64"), DeviceArray((T,), "int32")
+    ends = (0, T - 3_000)                                # the first rows and the last
+    for a, dt in ((slots, np.int64), (pos, np.int32)):
+        mark = np.full(3_000, -7, dt)
+        for at in ends:
+            _lib.check(_lib.lib.mars_copy_to_device(C.c_void_p(a.data_ptr() + at * mark.itemsize), C.c_void_p(mark.ctypes.data), mark.nbytes), "copy")
+    free = np.arange(9, dtype=np.int32)
+    q_start, kv, out, table = DeviceArray((3,), "int32"), DeviceArray((2,), "int32"), DeviceArray((1,), "int32"), dev(np.zeros((2, width), np.int32))
+    Reader(page_size=page).plan(dev(np.array([20, 3], np.int32)), dev(np.array([0, 5], np.int32)), table, dev(free), dev(np.array([9], np.int32)),
+                                q_start=q_start, kv_lens=kv, slots=slots, positions=pos, free_count_out=out)
+    want = ref.plan(np.array([20, 3]), np.array([0, 5]), np.zeros((2, width), np.int32), free, 9, 3_000, page)
+    for a, w, pad in ((slots, want[3], -1), (pos, want[4], 0)):
+        for at in ends:
+            got = np.empty(3_000, w.dtype)
+            _lib.check(_lib.lib.mars_copy_to_host(C.c_void_p(got.ctypes.data), C.c_void_p(a.data_ptr() + at * got.itemsize), got.nbytes), "copy")
+            np.testing.assert_array_equal(got, w if at == 0 else np.full(3_000, pad, w.dtype))
