@@ -897,3 +897,80 @@ def test_plan_of_the_most_tokens():
             got = np.empty(3_000, w.dtype)
             _lib.check(_lib.lib.mars_copy_to_host(C.c_void_p(got.ctypes.data), C.c_void_p(a.data_ptr() + at * got.itemsize), got.nbytes), "copy")
             np.testing.assert_array_equal(got, w if at == 0 else np.full(3_000, pad, w.dtype))
+
+
+# ---- store: more tokens than k_kv_store takes -------------------------------------------
+@pytest.mark.parametrize("D,rope,sections,adjacent", [(64, 64, (32,), False), (64, 64, (32,), True), (64, 48, (4, 20, 0), True), (64, 16, (0, 3, 5), False),
+                                                      (64, 0, (), False), (128, 64, (32,), False), (128, 128, (16, 24, 24), True),
+                                                      (128, 32, (16,), True), (256, 256, (128,), False), (256, 256, (40, 40, 48), True),
+                                                      (256, 112, (56,), False), (256, 0, (), False)])
+@pytest.mark.parametrize("tokens", [1025, 1089])
+def test_store_many_rotations(D, rope, sections, adjacent, tokens):
+    run_store(tokens, 6, 3, D, "float16", 32, rope, sections, adjacent, packed=tokens == 1025, seed=rope + D)
+    run_store(tokens, 2, 1, D, "bfloat16", 64, rope, sections, adjacent, inverse=True, seed=rope + D + 1)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("tokens", [1025, 1100])
+def test_store_many_layouts(tokens, D):
+    run_store(tokens, 4, 2, D, "bfloat16", 64, D, (D // 2,), interleaved=True, seed=1)
+    run_store(tokens, 4, 2, D, "float16", 16, D, (D // 4, D // 8, D // 8), in_place=True, seed=2)
+    run_store(tokens, 4, 2, D, "float16", 128, D // 2, (D // 4,), True, in_place=True, seed=2)
+    run_store(tokens, 4, 2, D, "float16", 16, D, (D // 2,), inverse=True, packed=False, in_place=True, seed=3)
+    # slots in no order, one page for each token, chunks that go on at slots that are not multiples of 8, forwards and backwards
+    rng = np.random.default_rng(5)
+    run_store(tokens, 2, 1, D, "float16", 16, D, (D // 2,), slots=rng.permutation(tokens * 3)[:tokens].astype(np.int64), pages=-(-tokens * 3 // 16))
+    run_store(tokens, 2, 1, D, "bfloat16", 16, D, (D // 2,), slots=np.arange(tokens, dtype=np.int64)[::-1].copy() + 3, pages=-(-tokens // 16) + 1)
+    run_store(tokens, 2, 2, D, "bfloat16", 32, D, (D // 2,), slots=np.arange(tokens, dtype=np.int64) + 5, pages=-(-tokens // 32) + 1)
+    run_store(tokens, 2, 2, D, "float16", 256, D, (D // 2,), slots=np.arange(tokens, dtype=np.int64) + 8, pages=-(-tokens // 256) + 1)
+
+
+@pytest.mark.parametrize("tokens", [40, 1100])
+def test_store_in_parts(tokens):
+    """q alone and k, v alone: the bits of the call that takes all; times and episodes left as they are where none are given."""
+    rng = np.random.default_rng(tokens)
+    hq, hkv, D, page, dtype = 6, 2, 64, 32, "float16"
+    r = Reader(hq, hkv, D, dtype, page, rope_dim=D, rope_sections=(16, 8, 8))
+    q, k, v = (dev(ref.to_bits(rng.standard_normal((tokens, h, D)), dtype)) for h in (hq, hkv, hkv))
+    pages = -(-tokens // page) + 2
+    pos, slots = dev(rng.integers(0, 5_000, (3, tokens)).astype(np.int32)), dev((rng.permutation(tokens) + 11).astype(np.int64))
+
+    def cache():
+        return PagedCache(dev(np.zeros((pages, hkv, page, D), np.float16)), dev(np.zeros((pages, hkv, D, page), np.float16)),
+                          dev(np.full(pages * page, -3, np.float32)), dev(np.full(pages * page, -3, np.int32)))
+
+    both, alone = cache(), cache()
+    q_both, q_alone = (dev(np.zeros((tokens, hq, D), np.float16)) for _ in range(2))
+    r.store(both, q, k, v, pos, slots, q_out=q_both, times=dev(np.ones(tokens, np.float32)), episodes=dev(np.ones(tokens, np.int32)))
+    r.store(None, q, None, None, pos, None, q_out=q_alone)
+    r.store(alone, None, k, v, pos, slots)
+    np.testing.assert_array_equal(q_alone.numpy().view(np.uint16), q_both.numpy().view(np.uint16))
+    np.testing.assert_array_equal(alone.k_pages.numpy().view(np.uint16), both.k_pages.numpy().view(np.uint16))
+    np.testing.assert_array_equal(alone.v_pages.numpy().view(np.uint16), both.v_pages.numpy().view(np.uint16))
+    assert np.all(alone.times.numpy() == -3) and np.all(alone.episodes.numpy() == -3)
+    hit = np.isin(np.arange(pages * page), slots.numpy())
+    np.testing.assert_array_equal(both.times.numpy(), np.where(hit, 1, -3))
+    np.testing.assert_array_equal(both.episodes.numpy(), np.where(hit, 1, -3))
+    assert alone.k_pages.numpy().any() and q_alone.numpy().any()
+
+
+def test_store_many_past_32_bits():
+    """More tokens than k_kv_store takes, to pages whose elements lie past 2^31: the slots read back by their own addresses."""
+    hkv, D, page, dtype, tokens = 2, 128, 256, "float16", 1_100
+    n = hkv * page * D
+    pages = 2 ** 31 // n + 40
+    kb, vb = (DeviceArray((pages, hkv, page, D), dtype) for _ in range(2))
+    rng = np.random.default_rng(13)
+    ids = np.array([pages - 1, 3, pages - 9, pages - 30, 2 ** 31 // n + 1])
+    j = np.arange(tokens)
+    slots = ids[j // page].astype(np.int64) * page + j % page
+    assert slots.max() * hkv * D > 2 ** 31
+    x = [ref.to_bits(rng.standard_normal((tokens, hkv, D)), dtype) for _ in range(2)]
+    Reader(hkv, hkv, D, dtype, page).store(PagedCache(kb, _As(vb, (pages, hkv, D, page))), None, dev(x[0]), dev(x[1]), None, dev(slots))
+    for base, want, order in ((kb, x[0], (0, 2, 1, 3)), (vb, x[1], (0, 3, 1, 2))):
+        for p, i in enumerate(ids):
+            got = np.empty(n, np.float16)
+            _lib.check(_lib.lib.mars_copy_to_host(C.c_void_p(got.ctypes.data), C.c_void_p(base.data_ptr() + 2 * n * int(i)), got.nbytes), "copy")
+            got = got.reshape((1, hkv, page, D) if base is kb else (1, hkv, D, page)).transpose(order)[0]
+            rows = want[p * page:(p + 1) * page]
+            np.testing.assert_array_equal(got[:len(rows)].view(np.uint16), rows.view(np.uint16))
