@@ -580,6 +580,7 @@ int mars_device_free(void* ptr);
 int mars_copy_to_device(void* dst, const void* src, size_t bytes);
 int mars_copy_to_host(void* dst, const void* src, size_t bytes);
 int mars_copy_device(void* dst, const void* src, size_t bytes);   /* device to device */
+int mars_device_current(int32_t* device);                          /* hipGetDevice of the calling thread */
 int mars_device_memory(size_t* free_bytes, size_t* total_bytes);  /* hipMemGetInfo of the device */
 int mars_device_synchronize(void);   /* hipDeviceSynchronize: all streams of the device drained */
 

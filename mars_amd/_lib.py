@@ -303,6 +303,7 @@ SIGNATURES = {
     "mars_copy_to_device": (C.c_int, [VP, VP, C.c_size_t]),
     "mars_copy_to_host": (C.c_int, [VP, VP, C.c_size_t]),
     "mars_copy_device": (C.c_int, [VP, VP, C.c_size_t]),
+    "mars_device_current": (C.c_int, [C.POINTER(I32)]),
     "mars_device_synchronize": (C.c_int, []),
     "mars_bench_queries": (C.c_int, [VP, VP, VP, I64, I32, C.c_float, C.POINTER(RetrievalConfigC), I32, VP, VP,
                                      VP, VP]),

@@ -1265,6 +1265,14 @@ int mars_device_memory(size_t* free_bytes, size_t* total_bytes) {
     return MARS_OK;
 }
 
+int mars_device_current(int32_t* device) {
+    MARS_CHECK(device, MARS_ERR_INVALID, "null argument");
+    int d = 0;
+    MARS_HIP(hipGetDevice(&d));
+    *device = d;
+    return MARS_OK;
+}
+
 int mars_device_synchronize(void) {
     MARS_TRY(ensure_device(nullptr));
     MARS_HIP(hipDeviceSynchronize());

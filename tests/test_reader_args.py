@@ -123,6 +123,86 @@ def test_plan_shapes(change):
                         positions=a["positions"], free_count_out=a["left"])
 
 
+class On(Fake):
+    """The same that also says where it lies: a GPU's number, or -1 for host memory."""
+
+    def __init__(self, x, device, pinned=False):
+        super().__init__(*x.shape, dtype=x.dtype, strides=x._s)
+        self._device, self._pinned = device, pinned
+
+    def get_device(self):
+        return self._device
+
+    def is_pinned(self):
+        return self._pinned
+
+
+def f32(*shape):
+    return Fake(*shape, dtype="float32")
+
+
+def calls():
+    """Every call with all its arrays by name."""
+    k, v, times, eps = Fake(9, 2, 16, 64), Fake(9, 2, 64, 16), f32(9 * 16), i32(9 * 16)
+    cache = dict(k_pages=k, v_pages=v, c_times=times, c_episodes=eps)
+
+    def paged(a):
+        return PagedCache(a["k_pages"], a["v_pages"], a["c_times"], a["c_episodes"])
+
+    def plan(r, a):
+        r.plan(a["new"], a["cached"], a["table"], a["free"], a["count"], q_start=a["q_start"], kv_lens=a["kv_lens"], slots=a["slots"],
+               positions=a["positions"], free_count_out=a["left"], next_lens=a["next_lens"])
+
+    def store(r, a):
+        r.store(paged(a), a["q"], a["k"], a["v"], a["positions"], a["slots"], q_out=a["q_out"], times=a["times"], episodes=a["episodes"])
+
+    def attend(r, a):
+        r.attend(paged(a), a["q"], a["out"], a["q_start"], a["kv_lens"], a["table"], lse=a["lse"], decay=a["decay"], q_times=a["q_times"],
+                 q_episodes=a["q_eps"], prefix_lens=a["prefix"])
+
+    def release(r, a):
+        r.release(a["done"], a["kv_lens"], a["table"], a["free"], a["count"])
+
+    slots = Fake(7, dtype="int64")
+    return [(plan, dict(new=i32(3), cached=i32(3), table=i32(3, 5), free=i32(20), count=i32(1), q_start=i32(4), kv_lens=i32(3), slots=slots,
+                        positions=i32(7), left=i32(1), next_lens=i32(3))),
+            (store, dict(cache, q=Fake(7, 4, 64), k=Fake(7, 2, 64), v=Fake(7, 2, 64), positions=i32(7), slots=slots, q_out=Fake(7, 4, 64),
+                         times=f32(7), episodes=i32(7))),
+            (attend, dict(cache, q=Fake(7, 4, 64), out=Fake(7, 4, 64), q_start=i32(4), kv_lens=i32(3), table=i32(3, 5), lse=f32(7, 4),
+                          decay=f32(4), q_times=f32(7), q_eps=i32(7), prefix=i32(3))),
+            (release, dict(done=i32(3), kv_lens=i32(3), table=i32(3, 5), free=i32(20), count=i32(1)))]
+
+
+@pytest.mark.parametrize("call,arrays", calls(), ids=["plan", "store", "attend", "release"])
+def test_arrays_on_the_host_or_another_gpu(call, arrays):
+    """An address in host memory, or in another GPU's, never reaches a kernel; pinned memory, which kernels read, may."""
+    here = {n: On(x, 1) for n, x in arrays.items()}
+
+    def reaches_c(a, r):
+        with pytest.raises(MarsError) as e:              # no handle: refused there, before any device work
+            call(r, a)
+        assert e.value.code == INVALID
+
+    reaches_c(arrays, a_reader())                        # arrays that do not say where they are
+    reaches_c(arrays, a_reader(device=1))
+    reaches_c(here, a_reader(device=1))
+    for n, x in arrays.items():
+        for at in (-1, 0, 2):
+            with pytest.raises(ValueError):
+                call(a_reader(device=1), dict(here, **{n: On(x, at)}))
+        reaches_c(dict(here, **{n: On(x, -1, pinned=True)}), a_reader(device=1))
+    with pytest.raises(ValueError):
+        call(a_reader(device=0), here)
+
+
+def test_release_shapes():
+    for kw in (dict(kv_lens=i32(2)), dict(table=i32(3)), dict(table=i32(2, 5)), dict(count=i32(2)), dict(free=f32(20))):
+        a = dict(kv_lens=i32(3), table=i32(3, 5), free=i32(20), count=i32(1))
+        a.update(kw)
+        with pytest.raises(ValueError):
+            a_reader().release(i32(3), a["kv_lens"], a["table"], a["free"], a["count"])
+
+
 def test_null_arguments():
     """The C entries report a missing handle or argument block, and touch nothing."""
     for name, args in (("mars_kv_plan", (None, None, None)), ("mars_kv_store", (None, None, None, None)),
