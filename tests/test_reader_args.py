@@ -213,6 +213,51 @@ def test_null_arguments():
 
 
 @pytest.mark.gpu
+def test_refusals_of_live_arrays():
+    """The refusals of the tests below on arrays that are there, zeros of a size that any of these calls stays in: where a check
+    is lost, this test fails, and nothing is touched that is not its own."""
+    import mars_amd
+    from mars_amd.reader import DeviceArray
+    mars_amd.init(0)
+    r = Reader(4, 2, 64, "float16", 16, rope_dim=64)
+    names = ("q", "k", "v", "out", "q_out", "k_pages", "v_pages", "times", "episodes", "q_start", "kv_lens", "block_table", "slots", "positions",
+             "new_lens", "cached_lens", "free_pages", "free_count", "free_count_out", "other")
+    zeros = {n: DeviceArray.from_numpy(np.zeros(1 << 16, np.int64)) for n in names}
+    p = {n: x.data_ptr() for n, x in zeros.items()}
+
+    def cache(**kw):
+        return _lib.KvCacheC(**{**dict(k_pages=p["k_pages"], v_pages=p["v_pages"], num_pages=9), **kw})
+
+    def some(keys, **kw):
+        return {**{n: p[n] for n in keys.split()}, **kw}
+
+    attend = some("q out q_start kv_lens block_table", q_stride=256, out_stride=256, num_requests=3, max_pages=5, num_tokens=7)
+    for kw, code in ((dict(q=None), INVALID), (dict(num_requests=0), INVALID), (dict(num_requests=4097), CAPACITY), (dict(max_pages=0), INVALID),
+                     (dict(max_pages=2 ** 28), CAPACITY), (dict(num_tokens=-1), INVALID), (dict(num_tokens=2 ** 30), CAPACITY),
+                     (dict(q_stride=248), INVALID), (dict(q_stride=260), INVALID), (dict(q=p["q"] + 2), INVALID), (dict(out_stride=12), INVALID),
+                     (dict(cap=-1.0), INVALID), (dict(cap=float("nan")), INVALID), (dict(scale=float("inf")), INVALID), (dict(decay=p["other"]), INVALID),
+                     (dict(q_episodes=p["other"]), INVALID), (dict(max_new=-1), INVALID)):
+        assert lib.mars_kv_attend(r.handle, C.byref(cache()), C.byref(_lib.KvAttendArgsC(**{**attend, **kw})), None) == code, kw
+    for kw in (dict(k_pages=None), dict(num_pages=0), dict(k_page_stride=8), dict(v_page_stride=4097), dict(k_pages=p["k_pages"] + 8),
+               dict(times=p["times"] + 4)):
+        assert lib.mars_kv_attend(r.handle, C.byref(cache(**kw)), C.byref(_lib.KvAttendArgsC(**attend)), None) == INVALID, kw
+    store = some("q k v q_out positions slots", q_stride=256, k_stride=128, v_stride=128, q_out_stride=256, num_tokens=7)
+    for kw in (dict(q=None, k=None, v=None), dict(v=None), dict(q_out=None), dict(slots=None), dict(positions=None), dict(k_stride=120),
+               dict(v_stride=130), dict(q_out=p["q"], q_out_stride=512), dict(times=p["other"]), dict(episodes=p["other"]), dict(num_tokens=-1),
+               dict(k=p["k"] + 2)):
+        assert lib.mars_kv_store(r.handle, C.byref(cache()), C.byref(_lib.KvStoreArgsC(**{**store, **kw})), None) == INVALID, kw
+    plan = some("new_lens cached_lens block_table free_pages free_count q_start kv_lens slots positions free_count_out", num_requests=3, max_pages=5,
+                num_tokens=7, free_capacity=9)
+    for kw, code in ((dict(new_lens=None), INVALID), (dict(slots=None), INVALID), (dict(free_count_out=p["free_count"]), INVALID),
+                     (dict(num_requests=0), INVALID), (dict(num_requests=4097), CAPACITY), (dict(max_pages=0), INVALID), (dict(free_capacity=-1), INVALID),
+                     (dict(num_tokens=-1), INVALID), (dict(kv_lens=p["cached_lens"]), INVALID), (dict(kv_lens=p["new_lens"]), INVALID),
+                     (dict(q_start=p["cached_lens"]), INVALID), (dict(q_start=p["new_lens"]), INVALID)):
+        assert lib.mars_kv_plan(r.handle, C.byref(_lib.KvPlanArgsC(**{**plan, **kw})), None) == code, kw
+    for name, x in zeros.items():
+        assert not x.numpy().any(), name
+
+
+@pytest.mark.gpu
 def test_c_refusals():
     """Arguments that only the C entries can check, on a live reader; nothing is launched."""
     import mars_amd
