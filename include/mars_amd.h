@@ -697,7 +697,8 @@ int mars_bench_serve(mars_graph* g, mars_ctx* ctx_global, mars_ctx* ctx_episode,
  * layer mars_kv_store and mars_kv_attend; mars_kv_release when requests end.
  * The calls run on `stream` (a hipStream_t; NULL = the null stream), allocate nothing and
  * return without waiting, so they can be captured into a HIP graph. One reader serves one
- * stream at a time (calls that overlap share its scratch and race). Lengths, tables and
+ * stream at a time (calls that overlap share its scratch and race); the scratch is 41, 77 or 144 MB
+ * for heads of 64, 128 or 256, whatever the batch. Lengths, tables and
  * slots are read on the device: their values are not checked on the host, and kernels keep
  * every access inside the arrays described to them whatever they hold. */
 #define MARS_DTYPE_F16  0
@@ -759,7 +760,9 @@ int mars_kv_plan(const mars_reader* r, const mars_kv_plan_args* args, void* stre
 /* Gives back the pages of the requests with done[r] != 0: the ceil(kv_lens[r] / page_size) pages
  * of their table rows are pushed onto free_pages in request order, free_count[0] grows, and
  * kv_lens[r] becomes 0. kv_lens: the tokens in the cache (mars_kv_plan's next_lens). Pages beyond
- * free_capacity are dropped. */
+ * free_capacity are dropped. Nothing counts a page's holders: one that several rows name (attention reads
+ * such rows like any other) may be given back with one of them alone, the last; the caller takes it out
+ * of the others' lengths or hands their pages back itself, or the page would be free twice. */
 int mars_kv_release(const mars_reader* r, const int32_t* done, int32_t* kv_lens, const int32_t* block_table,
                     int32_t num_requests, int32_t max_pages, int32_t* free_pages, int32_t* free_count,
                     int32_t free_capacity, void* stream);

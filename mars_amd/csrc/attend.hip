@@ -964,8 +964,8 @@ __device__ inline bool own_pieces(const AttendArgs& a, Part* it, int piece) {
 // 4 waves of 32 rows each share tiles of 64 keys: K (keys, elements) and V (elements, keys) come straight into two LDS
 // buffers, one tile ahead. 16-byte pieces of a row are XORed with the row number so that the 16 lanes of a fragment read hit
 // the 16 bank groups (no conflicts counted). The other workgroup of the CU fills the matrix cores while this one's waves are
-// in the softmax. 2 x 4,096 tokens over 8,196 keys, bf16, 32/8 heads of 128: 802 to 827 us on two boxes, about 1,000 TFLOP/s (a product of
-// 8,192 cubed reaches 1,168). With cap and decay a score takes three transcendental instructions instead of one: 2 x 4,001
+// in the softmax. 2 x 4,096 tokens over 8,196 keys, bf16, 32/8 heads of 128: 782 to 838 us by the box, 985 to 1,055 TFLOP/s (a product
+// of 8,192 cubed reaches 1,168). With cap and decay a score takes three transcendental instructions instead of one: 2 x 4,001
 // tokens of 12 heads of 64 within their episodes, vector units busy 69%, matrix cores 11%.
 constexpr int kManyKeys = 64;
 

@@ -149,6 +149,8 @@ __global__ __launch_bounds__(kPlanThreads) void k_kv_plan(mars_kv_plan_args a, i
 }
 
 // ---- release ------------------------------------------------------------------------
+// One workgroup, since the free list is one line: bound by its own reads and writes where many pages come back at once
+// (768 requests of 125 pages 42 us), by latency else (8 of 125 pages 2.6 us).
 __global__ __launch_bounds__(kPlanThreads) void k_kv_release(const int32_t* __restrict__ done, int32_t* __restrict__ kv_lens,
                                                              const int32_t* __restrict__ table, int R, int max_pages,
                                                              int32_t* __restrict__ free_pages, int32_t* __restrict__ free_count,
@@ -241,9 +243,13 @@ __global__ __launch_bounds__(256) void k_kv_store(StoreArgs a) {
 // tokens are computed once a workgroup (LDS), q and k move in pieces of 16 bytes, and v, whose pages hold the tokens of an
 // element side by side, goes through LDS: where 8 consecutive tokens fill 8 consecutive slots from a multiple of 8 on
 // they are written as 16 bytes, and the lanes of a wave fill whole rows of a page; other tokens value by value.
-// Bound by the bytes in and out: 4,099 tokens of 32/8 heads of 128, 101 MB, 27 us with all of it in the caches, 37 us from
-// and to memory. Up to kStoreFew tokens (of 32/8 heads of 128) k_kv_store has the shorter call: 1,024 tokens 15.4 us there,
-// 18.5 us here; 2,048 tokens 22.0 us there, 19.7 us here. (12/12 heads of 64: 12 us on both sides, 4,099 tokens 19.8 and 14.4.)
+// Bound by the bytes in and out: 4,099 tokens of 32/8 heads of 128, 101 MB, 27 us with all of it in the caches, 36 us from
+// and to memory. (A group of 8 has to lie in one workgroup's 64 tokens: where the step's tokens do not begin at a multiple of 8
+// slots, 8 of every 64 are written value by value.) Up to kStoreFew tokens k_kv_store has the shorter call, there and here:
+//   tokens            512           1,024         1,536         2,048         4,099
+//   32/8 of 128       13.3  15.5    15.2  17.2    18.5  18.1    21.7  19.1    65.8  36.3 us
+//   8/2 of 256        12.7  15.4    12.7  16.5    12.9  17.0    13.7  17.4    21.6  19.8
+//   12/12 of 64       12.7  12.5    12.8  12.3    12.9  12.2    13.0  12.5    20.2  15.2
 template <int D>
 constexpr int store_tile() { return D == 256 ? 32 : 64; }
 
