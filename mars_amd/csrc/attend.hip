@@ -63,13 +63,19 @@ __device__ inline void lds_barrier() {
     asm volatile("" ::: "memory");
 }
 
-// A score x (base 2) under a cap above kCapNear, x tanh(y) / y with y = x rcp: the odd series up to |y| = 1/4 (its next term is
-// 1e-8 there), beyond it cap (1 - 2 / (1 + e^2y)), whose error of 2^-22 cap or so would swallow small scores under large caps.
-__device__ inline float cap_far(float x, float cap, float rcp) {
+// Scores x (base 2) under a cap: cap tanh(y) = x tanh(y) / y, y = x rcp. Up to |y| = 1/2 an odd polynomial (tanh(y) / y fitted
+// in y^2 to 1.5e-8 of its value there, 1 at 0), exact to fp32's last bits however small the score beside the cap; beyond it
+// cap (1 - 2 / (1 + e^2y)), whose error of 2^-22 cap is no more than 2^-20 of the score there (for scores of a few units it would
+// be 6e-6 under a cap of 50, 0.09 under 1e6). k_attend_many looks first whether a wave's tile has a score above half the cap:
+// 2 x 4,001 packed tokens 83.5 us where none has, 100 to 107 us where some have, 85.3 us with the second form alone.
+__device__ inline float cap_near(float x, float rcp) {
     const float y = x * rcp, z = y * y;
-    const float near = x * fmaf(z, fmaf(z, fmaf(z, fmaf(z, 62.0f / 2835.0f, -17.0f / 315.0f), 2.0f / 15.0f), -1.0f / 3.0f), 1.0f);
+    return x * fmaf(z, fmaf(z, fmaf(z, fmaf(z, 0.017241491f, -0.053045493f), 0.13325879f), -0.33333144f), 1.0f);
+}
+__device__ inline float cap_any(float x, float cap, float rcp) {
+    const float y = x * rcp;
     const float far = cap * (1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(2.88539008177792681472f * y)));
-    return fabsf(y) < 0.25f ? near : far;
+    return fabsf(y) < 0.5f ? cap_near(x, rcp) : far;
 }
 
 // A pointer the wave holds in SGPRs (the same in every lane), for loads of the form scalar base plus 32-bit offset: the
@@ -544,7 +550,7 @@ struct FewLds {
 };
 constexpr int kFewStep = 32;
 
-template <typename T, int D, bool EXTRA, bool FAR>
+template <typename T, int D, bool EXTRA, bool CAP>
 __device__ void few_part(const AttendArgs& a, const Part& it, FewLds<D>& lds) {
     using V = typename Vec<T>::v8;
     constexpr int KC = D / 32, VB = D / 16;
@@ -662,13 +668,9 @@ __device__ void few_part(const AttendArgs& a, const Part& it, FewLds<D>& lds) {
             float x[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) x[j] = acc[j >> 2][j & 3] * a.scale_log2;
-            if (FAR) {
+            if (CAP) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) x[j] = cap_far(x[j], a.cap_log2, a.cap_rcp);
-            } else if (EXTRA && a.cap_log2 != 0.0f) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    x[j] = a.cap_log2 * (1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x[j])));
+                for (int j = 0; j < 8; ++j) x[j] = cap_any(x[j], a.cap_log2, a.cap_rcp);
             }
             if (EXTRA && a.k_times) {
 #pragma unroll
@@ -870,7 +872,7 @@ struct FewShared {
     FewLds<D> part;
     SpanLds span;
 };
-template <typename T, int D, bool EXTRA, bool FAR>
+template <typename T, int D, bool EXTRA, bool CAP>
 __device__ void few_rows(const AttendArgs& a, int block, int blocks, FewShared<D>& shared) {
     FewLds<D>& lds = shared.part;
     SpanLds& sp = shared.span;
@@ -939,7 +941,7 @@ __device__ void few_rows(const AttendArgs& a, int block, int blocks, FewShared<D
         }
         if (!first) __syncthreads();                        // the LDS of the piece before is done with
         first = false;
-        few_part<T, D, EXTRA, FAR>(a, uniform_part(it), lds);
+        few_part<T, D, EXTRA, CAP>(a, uniform_part(it), lds);
         if (left <= steps) return;
         s0 = 0;
         ++unit;
@@ -965,8 +967,8 @@ __device__ inline bool own_pieces(const AttendArgs& a, Part* it, int piece) {
 // buffers, one tile ahead. 16-byte pieces of a row are XORed with the row number so that the 16 lanes of a fragment read hit
 // the 16 bank groups (no conflicts counted). The other workgroup of the CU fills the matrix cores while this one's waves are
 // in the softmax. 2 x 4,096 tokens over 8,196 keys, bf16, 32/8 heads of 128: 782 to 838 us by the box, 985 to 1,055 TFLOP/s (a product
-// of 8,192 cubed reaches 1,168). With cap and decay a score takes three transcendental instructions instead of one: 2 x 4,001
-// tokens of 12 heads of 64 within their episodes, vector units busy 69%, matrix cores 11%.
+// of 8,192 cubed reaches 1,168). With cap and decay a score takes twice the vector instructions: 2 x 4,001 tokens of 12 heads of
+// 64 within their episodes, vector units busy 72%, matrix cores 11%.
 constexpr int kManyKeys = 64;
 
 // Heads of 256 have one wave a SIMD, which nothing covers while it waits for LDS: LDS reads and products stay in the order
@@ -991,7 +993,7 @@ struct ManyShared {
     union { ManyLds<D> tiles; SchedLds sched; int any_dirty; };
     StepLds list;
 };
-template <typename T, int D, bool EXTRA, bool FAR>
+template <typename T, int D, bool EXTRA, bool CAP>
 __device__ void many_rows(const AttendArgs& a, int block, ManyShared<D>& lds) {
     using V = typename Vec<T>::v8;
     constexpr int KS = D / 16, DB = D / 32, RC = D / 8;      // k-steps of S, blocks of O, 16-byte pieces of a key's row
@@ -1193,17 +1195,23 @@ __device__ void many_rows(const AttendArgs& a, int block, ManyShared<D>& lds) {
                 for (int b = 0; b < 2; ++b)
 #pragma unroll
                     for (int j = 0; j < 16; ++j) x[b][j] *= a.scale_log2;
-                if constexpr (FAR) {
+                if constexpr (CAP) {
+                    float most = 0.0f;
 #pragma unroll
                     for (int b = 0; b < 2; ++b)
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) x[b][j] = cap_far(x[b][j], a.cap_log2, a.cap_rcp);
-                } else if (a.cap_log2 != 0.0f) {
+                        for (int j = 0; j < 16; ++j) most = fmaxf(most, fabsf(x[b][j]));
+                    if (__builtin_expect(__any(most * a.cap_rcp >= 0.5f), 0)) {
 #pragma unroll
-                    for (int b = 0; b < 2; ++b)
+                        for (int b = 0; b < 2; ++b)
 #pragma unroll
-                        for (int j = 0; j < 16; ++j)
-                            x[b][j] = a.cap_log2 * (1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x[b][j])));
+                            for (int j = 0; j < 16; ++j) x[b][j] = cap_any(x[b][j], a.cap_log2, a.cap_rcp);
+                    } else {
+#pragma unroll
+                        for (int b = 0; b < 2; ++b)
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) x[b][j] = cap_near(x[b][j], a.cap_rcp);
+                    }
                 }
                 if (a.k_times) {
 #pragma unroll
@@ -1370,19 +1378,19 @@ __global__ __launch_bounds__(256) void k_attend_join(AttendArgs a) {
 }
 
 // ---- the kernels ------------------------------------------------------------------------
-template <typename T, int D, bool EXTRA, bool FAR>
+template <typename T, int D, bool EXTRA, bool CAP>
 __global__ __launch_bounds__(256, D > 128 ? 1 : D == 128 ? 2 : 3) void k_attend_few(AttendArgs a) {
     __shared__ __attribute__((aligned(16))) FewShared<D> lds;
-    few_rows<T, D, EXTRA, FAR>(a, int(blockIdx.x), int(gridDim.x), lds);
+    few_rows<T, D, EXTRA, CAP>(a, int(blockIdx.x), int(gridDim.x), lds);
 }
 
-template <typename T, int D, bool EXTRA, bool FAR>
-__global__ __launch_bounds__(256, D > 128 ? 1 : D == 64 && FAR ? 3 : 2) void k_attend_many(AttendArgs a) {
+template <typename T, int D, bool EXTRA, bool CAP>
+__global__ __launch_bounds__(256, D > 128 ? 1 : 2) void k_attend_many(AttendArgs a) {
     __shared__ __attribute__((aligned(16))) ManyShared<D> lds;
-    many_rows<T, D, EXTRA, FAR>(a, int(blockIdx.x), lds);
+    many_rows<T, D, EXTRA, CAP>(a, int(blockIdx.x), lds);
 }
 
-template <typename T, int D, bool EXTRA, bool FAR>
+template <typename T, int D, bool EXTRA, bool CAP>
 int launch_dim(AttendArgs a, int32_t max_new, hipStream_t s) {
     // Requests of at most kFewMost rows (new tokens x query heads per kv head) are k_attend_few's, the others
     // k_attend_many's: 64 requests over 3,000 keys of 16 rows 149 us by the one and 152 by the other, of 20 rows (which few
@@ -1395,13 +1403,13 @@ int launch_dim(AttendArgs a, int32_t max_new, hipStream_t s) {
     // few: one workgroup for each that the CUs hold at a time, fewer where there are not so many steps
     const int64_t few_tiles = few_only ? rows / kFewRows + std::min(a.requests, a.tokens) : std::min(a.requests, a.tokens);
     const int64_t few = std::min<int64_t>(few_tiles * a.kv_heads * ((keys + kFewStep - 1) / kFewStep), few_groups(D));
-    if (!many_only) MARS_LAUNCH((k_attend_few<T, D, EXTRA, FAR>), dim3(unsigned(few)), dim3(256), 0, s, a);
+    if (!many_only) MARS_LAUNCH((k_attend_few<T, D, EXTRA, CAP>), dim3(unsigned(few)), dim3(256), 0, s, a);
     if (few_only) return MARS_OK;
     // many: no more than chunks of kMinChunk or more of the tiles' keys, or 2^kManyItemsLog2 chunks and one for each tile
     const int64_t tiles = rows / kManyRows + std::min<int64_t>(a.requests, rows / (kFewMost + 1));
     const int64_t many = std::min(tiles * a.kv_heads * ((keys + kMinChunk - 1) / kMinChunk), (int64_t(1) << kManyItemsLog2) + tiles * a.kv_heads);
     MARS_CHECK(many <= INT32_MAX, MARS_ERR_CAPACITY, "%lld tiles of rows", (long long)tiles);
-    MARS_LAUNCH((k_attend_many<T, D, EXTRA, FAR>), dim3(unsigned(many)), dim3(256), 0, s, a);
+    MARS_LAUNCH((k_attend_many<T, D, EXTRA, CAP>), dim3(unsigned(many)), dim3(256), 0, s, a);
     // no tile is in pieces where a row of the table is one chunk
     if (keys > kMinChunk) {
         const int64_t blocks = std::min<int64_t>(tiles * a.kv_heads * (kManyRows / kJoinRows), 1024);
@@ -1410,12 +1418,12 @@ int launch_dim(AttendArgs a, int32_t max_new, hipStream_t s) {
     return MARS_OK;
 }
 
-// Kernels without extra terms, with them, and with a far cap: that one's code in the second kind cost every call with terms
-// (48 single tokens within episodes 36.2 us for 35.3, 2 x 4,001 packed tokens 85.9 for 85.1).
+// Kernels without extra terms, with times or episodes, and with a cap: its code costs calls without one (two chunks of 511
+// tokens among 22 single ones, decayed, 121.7 us without it and 123.9 with it).
 template <typename T, int D>
 int launch_terms(const AttendArgs& a, int32_t max_new, hipStream_t s) {
     if (a.cap_rcp != 0.0f) return launch_dim<T, D, true, true>(a, max_new, s);
-    return a.cap_log2 != 0.0f || a.k_times || a.k_eps ? launch_dim<T, D, true, false>(a, max_new, s) : launch_dim<T, D, false, false>(a, max_new, s);
+    return a.k_times || a.k_eps ? launch_dim<T, D, true, false>(a, max_new, s) : launch_dim<T, D, false, false>(a, max_new, s);
 }
 
 template <typename T>

@@ -606,12 +606,10 @@ int mars_kv_attend(const mars_reader* r, const mars_kv_cache* c, const mars_kv_a
     a.k_stride = c->k_page_stride ? c->k_page_stride : dense;
     a.v_stride = c->v_page_stride ? c->v_page_stride : dense;
     a.q_flip = scale < 0.0 ? 0x80008000u : 0u;
-    const double cap = double(s->cap);
-    const bool far = s->cap > kCapNear;
     // finite: a score of 0 times an infinity would be NaN
-    a.scale_log2 = float(std::min(std::fabs(cap > 0.0 && !far ? 2.0 * kLog2e * scale / cap : kLog2e * scale), double(FLT_MAX)));
-    a.cap_log2 = float(std::min(kLog2e * cap, double(FLT_MAX)));
-    a.cap_rcp = far ? float(std::max(1.0 / (kLog2e * cap), double(FLT_MIN))) : 0.0f;
+    a.scale_log2 = float(std::min(std::fabs(kLog2e * scale), double(FLT_MAX)));
+    a.cap_log2 = float(std::min(kLog2e * double(s->cap), double(FLT_MAX)));
+    a.cap_rcp = s->cap > 0.0f ? float(std::clamp(1.0 / (kLog2e * double(s->cap)), double(FLT_MIN), double(FLT_MAX))) : 0.0f;
     a.requests = s->num_requests; a.max_pages = s->max_pages; a.tokens = s->num_tokens; a.num_pages = c->num_pages;
     a.q_heads = d.q_heads; a.kv_heads = d.kv_heads; a.group = d.q_heads / d.kv_heads;
     a.page_shift = r->page_shift;

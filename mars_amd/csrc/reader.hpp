@@ -40,11 +40,6 @@ constexpr int32_t kJoinRows = 16;            // of a tile's rows, joined by a wo
 constexpr int32_t kMinChunk = 256;
 constexpr int32_t kMaxSplits = 256;          // pieces of a tile, as many as a join keeps references of in LDS
 
-// Caps up to here bend scores by cap (1 - 2 / (1 + e^(2s / cap))), off by at most 2^-20 cap = 6e-5 (8e-6 measured); above it by
-// cap_far, which is as close for any cap and slower where the scores bound the call: 2 x 4,001 packed tokens of 12 heads of 64
-// 86.0 us with a cap of 64, 101.2 with one of 65; single tokens alike on both sides.
-constexpr float kCapNear = 64.0f;
-
 struct AttendArgs {
     const void* q;
     void* out;
@@ -67,13 +62,13 @@ struct AttendArgs {
     uint32_t* arrived;
     int64_t q_stride, out_stride, k_stride, v_stride;
     uint32_t q_flip;       // sign bits of a pair of q's elements if the scale is negative
-    float scale_log2;      // |scale| * log2(e); with a cap of up to kCapNear: 2 * log2(e) * |scale| / cap
+    float scale_log2;      // |scale| * log2(e)
     float cap_log2;        // cap * log2(e); 0: no cap
     int32_t requests, max_pages, tokens, num_pages;
     int32_t q_heads, kv_heads, group;
     int32_t page_shift;
     int32_t few_rows;           // requests of up to so many rows are k_attend_few's
-    float cap_rcp;         // 1 / (cap * log2(e)) with a cap above kCapNear, else 0
+    float cap_rcp;         // 1 / (cap * log2(e)); 0: no cap
 };
 
 int launch_attend(const mars_reader& r, const AttendArgs& a, int32_t max_new, hipStream_t s);

@@ -974,3 +974,28 @@ def test_store_many_past_32_bits():
             got = got.reshape((1, hkv, page, D) if base is kb else (1, hkv, D, page)).transpose(order)[0]
             rows = want[p * page:(p + 1) * page]
             np.testing.assert_array_equal(got[:len(rows)].view(np.uint16), rows.view(np.uint16))
+
+
+@pytest.mark.parametrize("kind", ["few", "many"])
+def test_attend_capped_scores_one_by_one(kind):
+    """Every row sees one key, so its lse is that key's capped score: within 2^-19 of its value and 2^-21 (the reference lies up to 7
+    away), however small it is beside the cap, for scores from far below the cap to far above it."""
+    D, page, n = 64, 16, 200
+    s = np.concatenate([np.geomspace(1e-4, 100.0, n // 2), -np.geomspace(1e-4, 100.0, n // 2)])
+    k = np.zeros((-(-n // page) if kind == "many" else n, 1, page, D))
+    k[(np.arange(n) // page, 0, np.arange(n) % page, 0) if kind == "many" else (np.arange(n), 0, 0, 0)] = s
+    q = np.zeros((n, 1, D))
+    q[..., 0] = 8.0                                      # times D^-0.5: the score is k's element 0
+    s = ref.rounded(s, "float16")
+    cache = PagedCache(dev(k.astype(np.float16)), dev(np.ones((len(k), 1, D, page), np.float16)), None, dev(np.arange(len(k) * page, dtype=np.int32)))
+    few = kind == "few"
+    start, lens = (np.arange(n + 1), np.ones(n)) if few else (np.array([0, n]), np.array([n]))
+    table = np.arange(len(k), dtype=np.int32).reshape((n, 1) if few else (1, -1))
+    for cap in (1.0, 20.0, 30.0, 50.0, 64.0, 65.0, 1e3, 1e5):
+        out, lse = dev(np.zeros((n, 1, D), np.float16)), dev(np.zeros((n, 1), np.float32))
+        Reader(1, 1, D, "float16", page).attend(cache, dev(q.astype(np.float16)), out, dev(start.astype(np.int32)), dev(lens.astype(np.int32)), dev(table),
+                                                lse=lse, cap=cap, max_new=1 if few else n, q_episodes=dev(np.full(n, -1, np.int32)) if few else dev(np.arange(n, dtype=np.int32)))
+        want = cap * np.tanh(s / cap)
+        err = np.abs(lse.numpy()[:, 0] - want)
+        assert np.all(err <= 2.0 ** -19 * np.abs(want) + 2.0 ** -21), (cap, float((err - 2.0 ** -19 * np.abs(want)).max()))
+        assert np.all(out.numpy() == 1)
