@@ -727,8 +727,8 @@ int mars_reader_destroy(mars_reader* r);
  * Request r's row of block_table holds the ceil(cached / page_size) pages it owns; the pages it
  * needs more are taken from the top of free_pages (free_count[0] of them) and written behind
  * those. Requests are served in order; one that needs pages is served if it and all before it
- * fit what is free. One whose tokens exceed its table row (max_pages) or the num_tokens rows
- * of the step takes none and is not served. Outputs (all device):
+ * fit what is free. One whose tokens exceed its table row (max_pages), the num_tokens rows
+ * of the step or 2^31 - 1 takes none and is not served. Outputs (all device):
  *   q_start[R + 1]      first row of each request; q_start[R] = total of new_lens
  *   kv_lens[R]          tokens with this step's (cached + new), 0 if not served: what mars_kv_attend reads
  *   next_lens[R]        tokens in the cache after the step: cached + new, or cached if not served (its pages

@@ -78,7 +78,7 @@ __global__ __launch_bounds__(kPlanThreads) void k_kv_plan(mars_kv_plan_args a, i
         at += n_new[i];
         const int64_t len = int64_t(n_old[i]) + n_new[i];
         const int64_t pages = (len + page - 1) >> page_shift, have = (int64_t(n_old[i]) + page - 1) >> page_shift;
-        fits[i] = pages <= a.max_pages && at <= a.num_tokens;
+        fits[i] = pages <= a.max_pages && at <= a.num_tokens && len <= INT32_MAX;
         need[i] = fits[i] ? int32_t(pages - have) : 0;
         sum += need[i];
     }

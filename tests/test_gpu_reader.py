@@ -999,3 +999,19 @@ def test_attend_capped_scores_one_by_one(kind):
         err = np.abs(lse.numpy()[:, 0] - want)
         assert np.all(err <= 2.0 ** -19 * np.abs(want) + 2.0 ** -21), (cap, float((err - 2.0 ** -19 * np.abs(want)).max()))
         assert np.all(out.numpy() == 1)
+
+
+def test_plan_of_more_tokens_than_lengths_hold():
+    """A request that would pass 2^31 - 1 tokens is not served; one that reaches them is."""
+    page, width = 256, 2 ** 23 + 1
+    table, free = dev(np.full((2, width), 5, np.int32)), dev(np.array([70, 71, 72], np.int32))
+    q_start, kv, slots, pos, out, after = (DeviceArray((n,), d) for n, d in ((3, "int32"), (2, "int32"), (31, "int64"), (31, "int32"), (1, "int32"),
+                                                                            (2, "int32")))
+    have = np.array([2 ** 31 - 10, 2 ** 31 - 12], np.int32)
+    Reader(page_size=page).plan(dev(np.array([20, 11], np.int32)), dev(have), table, free, dev(np.array([3], np.int32)), q_start=q_start, kv_lens=kv,
+                                slots=slots, positions=pos, free_count_out=out, next_lens=after)
+    np.testing.assert_array_equal(kv.numpy(), [0, 2 ** 31 - 1])
+    np.testing.assert_array_equal(after.numpy(), [2 ** 31 - 10, 2 ** 31 - 1])
+    np.testing.assert_array_equal(slots.numpy(), [-1] * 20 + [5 * page + 244 + i for i in range(11)])
+    np.testing.assert_array_equal(pos.numpy()[20:], have[1] + np.arange(11))
+    assert out.numpy()[0] == 3 and np.all(table.numpy() == 5)
