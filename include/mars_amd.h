@@ -697,7 +697,7 @@ int mars_bench_serve(mars_graph* g, mars_ctx* ctx_global, mars_ctx* ctx_episode,
  * layer mars_kv_store and mars_kv_attend; mars_kv_release when requests end.
  * The calls run on `stream` (a hipStream_t; NULL = the null stream), allocate nothing and
  * return without waiting, so they can be captured into a HIP graph. One reader serves one
- * stream at a time (calls that overlap share its scratch and race); the scratch is 41, 77 or 144 MB
+ * stream at a time (calls that overlap share its scratch and race); the scratch is 50, 94 or 178 MB
  * for heads of 64, 128 or 256, whatever the batch. Lengths, tables and
  * slots are read on the device: their values are not checked on the host, and kernels keep
  * every access inside the arrays described to them whatever they hold. */
@@ -839,6 +839,69 @@ typedef struct mars_kv_attend_args {
     int32_t        max_new;
 } mars_kv_attend_args;
 int mars_kv_attend(const mars_reader* r, const mars_kv_cache* cache, const mars_kv_attend_args* args, void* stream);
+
+/* Tokens' k, v, time and episode read back from their slots, in any order (a slot may be named more than once): row t, kv head h of k
+ * at k + t * k_stride + h * head_dim (elements; strides a multiple of 8), v alike. k and v come together or not at all, as do
+ * times and episodes each for themselves; rows of tokens whose slot lies outside the cache are left as they are. Keys
+ * come as they are held, turned by their positions: mars_kv_store of them with positions that are the
+ * difference (or inverse) turns them on, since rotations add up. */
+typedef struct mars_kv_load_args {
+    const int64_t* slots;           /* num_tokens */
+    void*          k;
+    void*          v;
+    float*         times;           /* NULL: not wanted (else cache times are needed)       */
+    int32_t*       episodes;        /* NULL: not wanted (else cache episodes are needed)    */
+    int64_t        k_stride, v_stride;
+    int32_t        num_tokens;
+    int32_t        pad0;
+} mars_kv_load_args;
+int mars_kv_load(const mars_reader* r, const mars_kv_cache* cache, const mars_kv_load_args* args, void* stream);
+
+/* A cache of 8 bits, half the memory and half the bytes that attention reads: pages as in mars_kv_cache, of e4m3 values
+ * (1 sign, 4 exponent, 3 fraction bits, largest 448, NaN but no infinities), and for each token and kv head a byte e for k and one
+ * for v: an element is its e4m3 value times 2^(e - 127). Exponents are dense, (page, kv_head, token). Page strides (in bytes, a
+ * multiple of 16, 0 = dense) let layers interleave. Stored values: e is the least with which the head's largest finite
+ * element stays within 448, but at least 112 (float16) or 10 (bfloat16), so that every value is one of the reader's type;
+ * each element is rounded once, to nearest even (k from its turned fp32 value), and is off by at most 2^-4 of itself
+ * or 2^-10 times 2^(e - 127). Infinities and NaN become NaN, and leave the head's other elements alone. A cache is read by readers of
+ * the type that wrote it. Bytes e of 0 stand for 0, of 255 for 254. */
+typedef struct mars_kv_cache8 {
+    void*    k_pages;
+    void*    v_pages;
+    uint8_t* k_scales;
+    uint8_t* v_scales;
+    float*   times;
+    int32_t* episodes;
+    int64_t  k_page_stride;
+    int64_t  v_page_stride;
+    int32_t  num_pages;
+    int32_t  pad0;
+} mars_kv_cache8;
+int mars_kv_store8(const mars_reader* r, const mars_kv_cache8* cache, const mars_kv_store_args* args, void* stream);
+int mars_kv_load8(const mars_reader* r, const mars_kv_cache8* cache, const mars_kv_load_args* args, void* stream);
+
+/* Requests that have their first tokens in common, as answers to several questions about the same memories have: group g
+ * is requests group_start[g] .. group_start[g + 1] - 1 (rising, from 0; requests in no group share nothing), whose first shared_lens[g]
+ * tokens, rounded down to whole pages, lie in the same pages. Attention reads such a prefix once for all rows of a group, by the
+ * row of the table of its first request, and gives what it gives without groups, but for the order of the sums. A request whose cached tokens
+ * (kv_lens less its new ones) are fewer than the prefix reads everything for itself. Calls of more than 2^15 rows times query heads
+ * read every request's tokens for themselves too (their products cost more than the reads). */
+typedef struct mars_kv_shared {
+    const int32_t* group_start;     /* num_groups + 1 */
+    const int32_t* shared_lens;     /* num_groups     */
+    int32_t        num_groups;
+    int32_t        pad0;
+} mars_kv_shared;
+int mars_kv_attend_shared(const mars_reader* r, const mars_kv_cache* cache, const mars_kv_attend_args* args, const mars_kv_shared* shared,
+                          void* stream);
+/* mars_kv_attend over a cache of 8 bits, as over the values that mars_kv_load8 gives. shared: NULL: none. */
+int mars_kv_attend8(const mars_reader* r, const mars_kv_cache8* cache, const mars_kv_attend_args* args, const mars_kv_shared* shared,
+                    void* stream);
+/* mars_kv_release of the pages behind the shared prefixes alone: the prefix's pages stay the caller's, who gives them
+ * back once, with the request (or table row) that it keeps for the prefix itself. */
+int mars_kv_release_shared(const mars_reader* r, const int32_t* done, int32_t* kv_lens, const int32_t* block_table,
+                           int32_t num_requests, int32_t max_pages, const mars_kv_shared* shared, int32_t* free_pages,
+                           int32_t* free_count, int32_t free_capacity, void* stream);
 
 #ifdef __cplusplus
 }

@@ -210,6 +210,21 @@ class KvCacheC(C.Structure):
                 ("k_page_stride", C.c_int64), ("v_page_stride", C.c_int64), ("num_pages", C.c_int32), ("pad0", C.c_int32)]
 
 
+class KvCache8C(C.Structure):
+    _fields_ = [("k_pages", C.c_void_p), ("v_pages", C.c_void_p), ("k_scales", C.c_void_p), ("v_scales", C.c_void_p),
+                ("times", C.c_void_p), ("episodes", C.c_void_p), ("k_page_stride", C.c_int64), ("v_page_stride", C.c_int64),
+                ("num_pages", C.c_int32), ("pad0", C.c_int32)]
+
+
+class KvLoadArgsC(C.Structure):
+    _fields_ = [("slots", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("times", C.c_void_p), ("episodes", C.c_void_p),
+                ("k_stride", C.c_int64), ("v_stride", C.c_int64), ("num_tokens", C.c_int32), ("pad0", C.c_int32)]
+
+
+class KvSharedC(C.Structure):
+    _fields_ = [("group_start", C.c_void_p), ("shared_lens", C.c_void_p), ("num_groups", C.c_int32), ("pad0", C.c_int32)]
+
+
 class KvStoreArgsC(C.Structure):
     _fields_ = [("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("q_out", C.c_void_p), ("positions", C.c_void_p),
                 ("slots", C.c_void_p), ("times", C.c_void_p), ("episodes", C.c_void_p), ("q_stride", C.c_int64),
@@ -323,6 +338,12 @@ SIGNATURES = {
     "mars_kv_release": (C.c_int, [VP, VP, VP, VP, I32, I32, VP, VP, I32, VP]),
     "mars_kv_store": (C.c_int, [VP, C.POINTER(KvCacheC), C.POINTER(KvStoreArgsC), VP]),
     "mars_kv_attend": (C.c_int, [VP, C.POINTER(KvCacheC), C.POINTER(KvAttendArgsC), VP]),
+    "mars_kv_attend_shared": (C.c_int, [VP, C.POINTER(KvCacheC), C.POINTER(KvAttendArgsC), C.POINTER(KvSharedC), VP]),
+    "mars_kv_load": (C.c_int, [VP, C.POINTER(KvCacheC), C.POINTER(KvLoadArgsC), VP]),
+    "mars_kv_store8": (C.c_int, [VP, C.POINTER(KvCache8C), C.POINTER(KvStoreArgsC), VP]),
+    "mars_kv_load8": (C.c_int, [VP, C.POINTER(KvCache8C), C.POINTER(KvLoadArgsC), VP]),
+    "mars_kv_attend8": (C.c_int, [VP, C.POINTER(KvCache8C), C.POINTER(KvAttendArgsC), C.POINTER(KvSharedC), VP]),
+    "mars_kv_release_shared": (C.c_int, [VP, VP, VP, VP, I32, I32, C.POINTER(KvSharedC), VP, VP, I32, VP]),
     # mars_corpus.h
     "mars_corpus_default": (None, [C.POINTER(CorpusParamsC), I64, I32, C.c_uint64]),
     "mars_corpus_generate": (C.c_int, [C.POINTER(CorpusParamsC), VP, VP, VP, VP, I32]),

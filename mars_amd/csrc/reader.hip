@@ -151,11 +151,13 @@ __global__ __launch_bounds__(kPlanThreads) void k_kv_plan(mars_kv_plan_args a, i
 // ---- release ------------------------------------------------------------------------
 // One workgroup, since the free list is one line: bound by its own reads and writes where many pages come back at once
 // (768 requests of 125 pages 42 us), by latency else (8 of 125 pages 2.6 us).
+// SHARED: a request's first pages, its group's prefix, stay.
+template <bool SHARED>
 __global__ __launch_bounds__(kPlanThreads) void k_kv_release(const int32_t* __restrict__ done, int32_t* __restrict__ kv_lens,
-                                                             const int32_t* __restrict__ table, int R, int max_pages,
+                                                             const int32_t* __restrict__ table, int R, int max_pages, mars_kv_shared g,
                                                              int32_t* __restrict__ free_pages, int32_t* __restrict__ free_count,
                                                              int free_capacity, int page_shift) {
-    __shared__ int32_t rank[kMaxRequests], count[kMaxRequests];
+    __shared__ int32_t rank[kMaxRequests], count[kMaxRequests], from[SHARED ? kMaxRequests : 1];
     __shared__ int64_t wsum[kPlanThreads / 64];
     const int tid = int(threadIdx.x), per = (R + kPlanThreads - 1) / kPlanThreads;
     const int first = min(tid * per, R), last = min(first + per, R);
@@ -164,6 +166,16 @@ __global__ __launch_bounds__(kPlanThreads) void k_kv_release(const int32_t* __re
     for (int r = first; r < last; ++r) {
         const int64_t pages = (int64_t(max(kv_lens[r], 0)) + (1 << page_shift) - 1) >> page_shift;
         count[r] = done[r] ? int32_t(min(pages, int64_t(max_pages))) : 0;
+        if constexpr (SHARED) {
+            int lo = 0, hi = g.num_groups;                  // the last group that begins at or before r
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (g.group_start[mid] <= r) lo = mid; else hi = mid;
+            }
+            const bool in = g.group_start[lo] <= r && r < g.group_start[lo + 1];
+            from[r] = in ? min(max(g.shared_lens[lo], 0) >> page_shift, count[r]) : 0;
+            count[r] -= from[r];
+        }
         sum += count[r];
     }
     int64_t total, at = block_scan(sum, wsum, &total);
@@ -175,31 +187,11 @@ __global__ __launch_bounds__(kPlanThreads) void k_kv_release(const int32_t* __re
     __syncthreads();
     for (int r = tid >> 6; r < R; r += kPlanThreads / 64)
         for (int j = tid & 63; j < count[r]; j += 64)
-            if (int64_t(rank[r]) + j < free_capacity) free_pages[rank[r] + j] = table[int64_t(r) * max_pages + j];
+            if (int64_t(rank[r]) + j < free_capacity) free_pages[rank[r] + j] = table[int64_t(r) * max_pages + (SHARED ? from[r] : 0) + j];
     if (tid == 0) free_count[0] = int32_t(min(held + total, int64_t(free_capacity)));
 }
 
 // ---- store --------------------------------------------------------------------------
-struct StoreArgs {
-    mars_kv_store_args s;
-    void* k_pages;
-    void* v_pages;
-    float* times;
-    int32_t* eps;
-    const uint64_t* freq;
-    const int32_t* axis;
-    int64_t k_stride, v_stride, slots;                   // page strides (elements); slots the cache has
-    int32_t q_heads, kv_heads, head_dim, rope_dim, adjacent, page_shift;
-};
-
-// sin and cos of 2 pi * pos * f, f in units of 2^-64 turns per position: whole turns drop out of the 64-bit product
-// by themselves, so the phase is exact to pos * 2^-65 turns for every int32 position, and the angle to the rounding of
-// its upper 32 bits to fp32. (A product in fp32 is off by 2^-24 of the whole angle: 0.004 rad at position 70,000.)
-__device__ inline void turn(int32_t pos, uint64_t f, float* sn, float* cs) {
-    const uint64_t phase = uint64_t(int64_t(pos)) * f;
-    sincospif(float(int32_t(uint32_t(phase >> 32))) * 0x1p-31f, sn, cs);
-}
-
 // Few tokens: a workgroup to each, a pair of values a thread and turn. Latency bound (32 tokens 5.0 us).
 constexpr int32_t kStoreFew = 1024;       // see k_kv_store_tile
 template <typename T>
@@ -407,17 +399,48 @@ int launch_store(const StoreArgs& a, hipStream_t s) {
     return a.head_dim == 64 ? launch_store_tile<T, 64>(a, s) : a.head_dim == 128 ? launch_store_tile<T, 128>(a, s) : launch_store_tile<T, 256>(a, s);
 }
 
-int check_cache(const mars_reader& r, const mars_kv_cache& c) {
+// A cache of either kind, checked, its strides filled in.
+struct Cache {
+    void* k_pages;
+    void* v_pages;
+    uint8_t* k_scales;
+    uint8_t* v_scales;
+    float* times;
+    int32_t* episodes;
+    int64_t k_stride, v_stride;
+    int32_t num_pages;
+};
+
+template <typename C>
+int check_pages(const mars_reader& r, const C& c, int64_t unit, Cache* out) {
     MARS_CHECK(c.k_pages && c.v_pages, MARS_ERR_INVALID, "cache without pages");
     MARS_CHECK(c.num_pages > 0, MARS_ERR_INVALID, "cache of %d pages", c.num_pages);
     const int64_t dense = int64_t(r.d.kv_heads) * r.d.page_size * r.d.head_dim;
     for (const int64_t s : {c.k_page_stride, c.v_page_stride})
-        MARS_CHECK(s == 0 || (s >= dense && s % 8 == 0), MARS_ERR_INVALID,
-                   "page stride %lld: 0, or a multiple of 8 of at least %lld elements", (long long)s, (long long)dense);
+        MARS_CHECK(s == 0 || (s >= dense && s % unit == 0), MARS_ERR_INVALID,
+                   "page stride %lld: 0, or a multiple of %lld of at least %lld elements", (long long)s, (long long)unit, (long long)dense);
     MARS_CHECK((reinterpret_cast<uintptr_t>(c.k_pages) | reinterpret_cast<uintptr_t>(c.v_pages)) % 16 == 0, MARS_ERR_INVALID,
                "cache pages are not aligned to 16 bytes");
     MARS_CHECK((reinterpret_cast<uintptr_t>(c.times) | reinterpret_cast<uintptr_t>(c.episodes)) % 16 == 0, MARS_ERR_INVALID,
                "cache times or episodes are not aligned to 16 bytes");
+    *out = Cache{c.k_pages, c.v_pages, nullptr, nullptr, c.times, c.episodes, c.k_page_stride ? c.k_page_stride : dense,
+                 c.v_page_stride ? c.v_page_stride : dense, c.num_pages};
+    return MARS_OK;
+}
+int check_cache(const mars_reader& r, const mars_kv_cache& c, Cache* out) { return check_pages(r, c, 8, out); }
+int check_cache(const mars_reader& r, const mars_kv_cache8& c, Cache* out) {
+    MARS_TRY(check_pages(r, c, 16, out));
+    MARS_CHECK(c.k_scales && c.v_scales, MARS_ERR_INVALID, "cache without exponents");
+    MARS_CHECK((reinterpret_cast<uintptr_t>(c.k_scales) | reinterpret_cast<uintptr_t>(c.v_scales)) % 16 == 0, MARS_ERR_INVALID,
+               "cache exponents are not aligned to 16 bytes");
+    out->k_scales = c.k_scales;
+    out->v_scales = c.v_scales;
+    return MARS_OK;
+}
+
+int check_shared(const mars_kv_shared& g) {
+    MARS_CHECK(g.group_start && g.shared_lens, MARS_ERR_INVALID, "groups without starts or lengths");
+    MARS_CHECK(g.num_groups >= 1 && g.num_groups <= kMaxRequests, MARS_ERR_INVALID, "%d groups (1 to %d)", g.num_groups, kMaxRequests);
     return MARS_OK;
 }
 
@@ -426,6 +449,140 @@ int check_rows(const char* what, const void* p, int64_t stride, int64_t width) {
                what, (long long)stride, (long long)width);
     MARS_CHECK(reinterpret_cast<uintptr_t>(p) % 16 == 0, MARS_ERR_INVALID, "%s is not aligned to 16 bytes", what);
     return MARS_OK;
+}
+
+int release(const mars_reader* r, const int32_t* done, int32_t* kv_lens, const int32_t* block_table, int32_t num_requests,
+            int32_t max_pages, const mars_kv_shared* shared, int32_t* free_pages, int32_t* free_count, int32_t free_capacity, void* stream) {
+    MARS_CHECK(r && done && kv_lens && block_table && free_pages && free_count, MARS_ERR_INVALID, "null argument");
+    MARS_CHECK(num_requests >= 1 && max_pages >= 1 && free_capacity >= 0, MARS_ERR_INVALID,
+               "%d requests, %d pages a row, %d free entries", num_requests, max_pages, free_capacity);
+    MARS_CHECK(num_requests <= kMaxRequests, MARS_ERR_CAPACITY, "%d requests (at most %d)", num_requests, kMaxRequests);
+    if (shared) MARS_TRY(check_shared(*shared));
+    MARS_TRY(use_device(r->device));
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    if (shared)
+        MARS_LAUNCH(k_kv_release<true>, dim3(1), dim3(kPlanThreads), 0, st, done, kv_lens, block_table, num_requests, max_pages, *shared, free_pages,
+                    free_count, free_capacity, r->page_shift);
+    else
+        MARS_LAUNCH(k_kv_release<false>, dim3(1), dim3(kPlanThreads), 0, st, done, kv_lens, block_table, num_requests, max_pages, mars_kv_shared{},
+                    free_pages, free_count, free_capacity, r->page_shift);
+    return MARS_OK;
+}
+
+template <typename C>
+int store(const mars_reader* r, const C* c, const mars_kv_store_args* s, void* stream) {
+    MARS_CHECK(r && s, MARS_ERR_INVALID, "null argument");
+    MARS_CHECK(s->num_tokens >= 0, MARS_ERR_INVALID, "%d tokens", s->num_tokens);
+    MARS_CHECK(s->q || s->k, MARS_ERR_INVALID, "neither q nor k");
+    MARS_CHECK(!s->k == !s->v, MARS_ERR_INVALID, "k and v come together");
+    const mars_reader_desc& d = r->d;
+    StoreArgs a{};
+    a.s = *s;
+    if (s->q) {
+        MARS_CHECK(s->q_out, MARS_ERR_INVALID, "q without q_out");
+        MARS_TRY(check_rows("q", s->q, s->q_stride, int64_t(d.q_heads) * d.head_dim));
+        MARS_TRY(check_rows("q_out", s->q_out, s->q_out_stride, int64_t(d.q_heads) * d.head_dim));
+        MARS_CHECK(s->q != s->q_out || s->q_stride == s->q_out_stride, MARS_ERR_INVALID, "q_out is q with another stride");
+    }
+    if (s->k) {
+        MARS_CHECK(c && s->slots, MARS_ERR_INVALID, "k and v need a cache and slots");
+        Cache k{};
+        MARS_TRY(check_cache(*r, *c, &k));
+        MARS_TRY(check_rows("k", s->k, s->k_stride, int64_t(d.kv_heads) * d.head_dim));
+        MARS_TRY(check_rows("v", s->v, s->v_stride, int64_t(d.kv_heads) * d.head_dim));
+        MARS_CHECK(!s->times || c->times, MARS_ERR_INVALID, "times for a cache without them");
+        MARS_CHECK(!s->episodes || c->episodes, MARS_ERR_INVALID, "episodes for a cache without them");
+        a.k_pages = k.k_pages; a.v_pages = k.v_pages; a.times = k.times; a.eps = k.episodes;
+        a.k_scales = k.k_scales; a.v_scales = k.v_scales;
+        a.k_stride = k.k_stride; a.v_stride = k.v_stride;
+        a.slots = int64_t(c->num_pages) << r->page_shift;
+    }
+    MARS_CHECK(d.rope_dim == 0 || s->positions, MARS_ERR_INVALID, "rotary heads need positions");
+    if (s->num_tokens == 0) return MARS_OK;
+    a.freq = r->freq; a.axis = r->axis;
+    a.q_heads = d.q_heads; a.kv_heads = d.kv_heads; a.head_dim = d.head_dim; a.rope_dim = d.rope_dim; a.adjacent = d.rope_adjacent;
+    a.page_shift = r->page_shift;
+    MARS_TRY(use_device(r->device));
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    if (a.k_scales) return launch_store8(*r, a, st);
+    return d.dtype == MARS_DTYPE_F16 ? launch_store<_Float16>(a, st) : launch_store<__bf16>(a, st);
+}
+
+template <typename C>
+int load(const mars_reader* r, const C* c, const mars_kv_load_args* s, void* stream) {
+    MARS_CHECK(r && c && s, MARS_ERR_INVALID, "null argument");
+    MARS_CHECK(s->num_tokens >= 0, MARS_ERR_INVALID, "%d tokens", s->num_tokens);
+    MARS_CHECK(s->num_tokens == 0 || s->slots, MARS_ERR_INVALID, "null argument");
+    MARS_CHECK(s->k || s->times || s->episodes, MARS_ERR_INVALID, "nothing to read");
+    MARS_CHECK(!s->k == !s->v, MARS_ERR_INVALID, "k and v come together");
+    Cache k{};
+    MARS_TRY(check_cache(*r, *c, &k));
+    const mars_reader_desc& d = r->d;
+    if (s->k) {
+        MARS_TRY(check_rows("k", s->k, s->k_stride, int64_t(d.kv_heads) * d.head_dim));
+        MARS_TRY(check_rows("v", s->v, s->v_stride, int64_t(d.kv_heads) * d.head_dim));
+    }
+    MARS_CHECK(!s->times || k.times, MARS_ERR_INVALID, "times of a cache without them");
+    MARS_CHECK(!s->episodes || k.episodes, MARS_ERR_INVALID, "episodes of a cache without them");
+    if (s->num_tokens == 0) return MARS_OK;
+    LoadArgs a{};
+    a.s = *s;
+    a.k_pages = k.k_pages; a.v_pages = k.v_pages; a.k_scales = k.k_scales; a.v_scales = k.v_scales; a.times = k.times; a.eps = k.episodes;
+    a.k_stride = k.k_stride; a.v_stride = k.v_stride; a.slots = int64_t(k.num_pages) << r->page_shift;
+    a.kv_heads = d.kv_heads; a.page_shift = r->page_shift;
+    MARS_TRY(use_device(r->device));
+    return launch_load(*r, a, static_cast<hipStream_t>(stream));
+}
+
+template <typename C>
+int attend(const mars_reader* r, const C* c, const mars_kv_attend_args* s, const mars_kv_shared* shared, void* stream) {
+    MARS_CHECK(r && c && s && s->q && s->out && s->q_start && s->kv_lens && s->block_table, MARS_ERR_INVALID, "null argument");
+    MARS_CHECK(s->num_requests >= 1 && s->max_pages >= 1 && s->num_tokens >= 0 && s->max_new >= 0, MARS_ERR_INVALID,
+               "%d requests, %d pages a row, %d tokens, max_new %d", s->num_requests, s->max_pages, s->num_tokens, s->max_new);
+    MARS_CHECK(s->num_requests <= kMaxRequests, MARS_ERR_CAPACITY, "%d requests (at most %d)", s->num_requests, kMaxRequests);
+    Cache k{};
+    MARS_TRY(check_cache(*r, *c, &k));
+    if (shared) MARS_TRY(check_shared(*shared));
+    const mars_reader_desc& d = r->d;
+    MARS_CHECK(int64_t(s->max_pages) * d.page_size <= (1 << 30), MARS_ERR_CAPACITY, "%d pages of %d tokens a row", s->max_pages, d.page_size);
+    MARS_CHECK(int64_t(s->num_tokens) * d.q_heads <= INT32_MAX, MARS_ERR_CAPACITY, "%d tokens of %d heads", s->num_tokens, d.q_heads);
+    MARS_TRY(check_rows("q", s->q, s->q_stride, int64_t(d.q_heads) * d.head_dim));
+    MARS_TRY(check_rows("out", s->out, s->out_stride, int64_t(d.q_heads) * d.head_dim));
+    MARS_CHECK(!s->decay || (s->q_times && c->times), MARS_ERR_INVALID, "decay needs q_times and the cache's times");
+    MARS_CHECK(!s->q_episodes || c->episodes, MARS_ERR_INVALID, "q_episodes needs the cache's episodes");
+    MARS_CHECK(std::isfinite(s->cap) && s->cap >= 0.0f, MARS_ERR_INVALID, "cap %g", double(s->cap));
+    MARS_CHECK(std::isfinite(s->scale), MARS_ERR_INVALID, "scale %g", double(s->scale));
+    if (s->num_tokens == 0) return MARS_OK;
+    constexpr double kLog2e = 1.4426950408889634074;
+    const double scale = s->scale == 0.0f ? 1.0 / std::sqrt(double(d.head_dim)) : double(s->scale);
+    AttendArgs a{};
+    a.q = s->q; a.out = s->out; a.lse = s->lse;
+    a.k_pages = k.k_pages; a.v_pages = k.v_pages; a.k_scales = k.k_scales; a.v_scales = k.v_scales;
+    a.k_times = s->decay ? c->times : nullptr;
+    a.k_eps = s->q_episodes ? c->episodes : nullptr;
+    a.q_start = s->q_start; a.kv_lens = s->kv_lens; a.table = s->block_table;
+    a.decay = s->decay; a.q_times = s->q_times; a.q_eps = s->q_episodes; a.prefix = s->prefix_lens;
+    a.part_o = r->part_o; a.part_ml = r->part_ml; a.arrived = r->arrived;
+    a.many_o = r->part_o + r->few_slots * kFewRows * size_t(d.head_dim);
+    a.many_ml = r->part_ml + r->few_slots * kFewRows;
+    a.q_stride = s->q_stride; a.out_stride = s->out_stride;
+    a.k_stride = k.k_stride; a.v_stride = k.v_stride;
+    a.q_flip = scale < 0.0 ? 0x80008000u : 0u;
+    // finite: a score of 0 times an infinity would be NaN
+    a.scale_log2 = float(std::min(std::fabs(kLog2e * scale), double(FLT_MAX)));
+    a.cap_log2 = float(std::min(kLog2e * double(s->cap), double(FLT_MAX)));
+    a.cap_rcp = s->cap > 0.0f ? float(std::clamp(1.0 / (kLog2e * double(s->cap)), double(FLT_MIN), double(FLT_MAX))) : 0.0f;
+    a.requests = s->num_requests; a.max_pages = s->max_pages; a.tokens = s->num_tokens; a.num_pages = c->num_pages;
+    a.q_heads = d.q_heads; a.kv_heads = d.kv_heads; a.group = d.q_heads / d.kv_heads;
+    a.page_shift = r->page_shift;
+    MARS_TRY(use_device(r->device));
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    if (shared && int64_t(s->num_tokens) * d.q_heads <= kStateRows) {
+        a.group_start = shared->group_start; a.shared_lens = shared->shared_lens; a.groups = shared->num_groups;
+        a.skips = r->skips; a.state_o = r->state_o; a.state_ml = r->state_ml;
+    }
+    if (a.k_scales) return launch_attend8(*r, a, s->max_new, st);
+    return a.group_start ? launch_attend_shared(*r, a, s->max_new, st) : launch_attend(*r, a, s->max_new, st);
 }
 
 }  // namespace
@@ -484,6 +641,9 @@ int mars_reader_create(const mars_reader_desc* d, mars_reader** out) try {
         MARS_TRY(dmalloc(&r->part_ml, rows));
         MARS_TRY(dmalloc(&r->arrived, r->few_slots));
         MARS_HIP(hipMemset(r->arrived, 0, r->few_slots * sizeof(uint32_t)));
+        MARS_TRY(dmalloc(&r->state_o, size_t(kStateRows) * size_t(d->head_dim)));
+        MARS_TRY(dmalloc(&r->state_ml, size_t(kStateRows)));
+        MARS_TRY(dmalloc(&r->skips, size_t(kMaxRequests)));
         MARS_HIP(hipDeviceSynchronize());
         return MARS_OK;
     }();
@@ -501,6 +661,7 @@ int mars_reader_destroy(mars_reader* r) {
     if (!r) return MARS_OK;
     (void)use_device(r->device);
     dfree(r->freq); dfree(r->axis); dfree(r->part_o); dfree(r->part_ml); dfree(r->arrived);
+    dfree(r->state_o); dfree(r->state_ml); dfree(r->skips);
     delete r;
     return MARS_OK;
 }
@@ -526,95 +687,29 @@ int mars_kv_plan(const mars_reader* r, const mars_kv_plan_args* a, void* stream)
 
 int mars_kv_release(const mars_reader* r, const int32_t* done, int32_t* kv_lens, const int32_t* block_table, int32_t num_requests,
                     int32_t max_pages, int32_t* free_pages, int32_t* free_count, int32_t free_capacity, void* stream) {
-    MARS_CHECK(r && done && kv_lens && block_table && free_pages && free_count, MARS_ERR_INVALID, "null argument");
-    MARS_CHECK(num_requests >= 1 && max_pages >= 1 && free_capacity >= 0, MARS_ERR_INVALID,
-               "%d requests, %d pages a row, %d free entries", num_requests, max_pages, free_capacity);
-    MARS_CHECK(num_requests <= kMaxRequests, MARS_ERR_CAPACITY, "%d requests (at most %d)", num_requests, kMaxRequests);
-    MARS_TRY(use_device(r->device));
-    MARS_LAUNCH(k_kv_release, dim3(1), dim3(kPlanThreads), 0, static_cast<hipStream_t>(stream), done, kv_lens, block_table, num_requests,
-                max_pages, free_pages, free_count, free_capacity, r->page_shift);
-    return MARS_OK;
+    return release(r, done, kv_lens, block_table, num_requests, max_pages, nullptr, free_pages, free_count, free_capacity, stream);
 }
 
-int mars_kv_store(const mars_reader* r, const mars_kv_cache* c, const mars_kv_store_args* s, void* stream) {
-    MARS_CHECK(r && s, MARS_ERR_INVALID, "null argument");
-    MARS_CHECK(s->num_tokens >= 0, MARS_ERR_INVALID, "%d tokens", s->num_tokens);
-    MARS_CHECK(s->q || s->k, MARS_ERR_INVALID, "neither q nor k");
-    MARS_CHECK(!s->k == !s->v, MARS_ERR_INVALID, "k and v come together");
-    const mars_reader_desc& d = r->d;
-    StoreArgs a{};
-    a.s = *s;
-    if (s->q) {
-        MARS_CHECK(s->q_out, MARS_ERR_INVALID, "q without q_out");
-        MARS_TRY(check_rows("q", s->q, s->q_stride, int64_t(d.q_heads) * d.head_dim));
-        MARS_TRY(check_rows("q_out", s->q_out, s->q_out_stride, int64_t(d.q_heads) * d.head_dim));
-        MARS_CHECK(s->q != s->q_out || s->q_stride == s->q_out_stride, MARS_ERR_INVALID, "q_out is q with another stride");
-    }
-    if (s->k) {
-        MARS_CHECK(c && s->slots, MARS_ERR_INVALID, "k and v need a cache and slots");
-        MARS_TRY(check_cache(*r, *c));
-        MARS_TRY(check_rows("k", s->k, s->k_stride, int64_t(d.kv_heads) * d.head_dim));
-        MARS_TRY(check_rows("v", s->v, s->v_stride, int64_t(d.kv_heads) * d.head_dim));
-        MARS_CHECK(!s->times || c->times, MARS_ERR_INVALID, "times for a cache without them");
-        MARS_CHECK(!s->episodes || c->episodes, MARS_ERR_INVALID, "episodes for a cache without them");
-        const int64_t dense = int64_t(d.kv_heads) * d.page_size * d.head_dim;
-        a.k_pages = c->k_pages; a.v_pages = c->v_pages; a.times = c->times; a.eps = c->episodes;
-        a.k_stride = c->k_page_stride ? c->k_page_stride : dense;
-        a.v_stride = c->v_page_stride ? c->v_page_stride : dense;
-        a.slots = int64_t(c->num_pages) << r->page_shift;
-    }
-    MARS_CHECK(d.rope_dim == 0 || s->positions, MARS_ERR_INVALID, "rotary heads need positions");
-    if (s->num_tokens == 0) return MARS_OK;
-    a.freq = r->freq; a.axis = r->axis;
-    a.q_heads = d.q_heads; a.kv_heads = d.kv_heads; a.head_dim = d.head_dim; a.rope_dim = d.rope_dim; a.adjacent = d.rope_adjacent;
-    a.page_shift = r->page_shift;
-    MARS_TRY(use_device(r->device));
-    const hipStream_t st = static_cast<hipStream_t>(stream);
-    return d.dtype == MARS_DTYPE_F16 ? launch_store<_Float16>(a, st) : launch_store<__bf16>(a, st);
+int mars_kv_release_shared(const mars_reader* r, const int32_t* done, int32_t* kv_lens, const int32_t* block_table, int32_t num_requests,
+                           int32_t max_pages, const mars_kv_shared* shared, int32_t* free_pages, int32_t* free_count,
+                           int32_t free_capacity, void* stream) {
+    MARS_CHECK(shared, MARS_ERR_INVALID, "null argument");
+    return release(r, done, kv_lens, block_table, num_requests, max_pages, shared, free_pages, free_count, free_capacity, stream);
 }
 
-int mars_kv_attend(const mars_reader* r, const mars_kv_cache* c, const mars_kv_attend_args* s, void* stream) {
-    MARS_CHECK(r && c && s && s->q && s->out && s->q_start && s->kv_lens && s->block_table, MARS_ERR_INVALID, "null argument");
-    MARS_CHECK(s->num_requests >= 1 && s->max_pages >= 1 && s->num_tokens >= 0 && s->max_new >= 0, MARS_ERR_INVALID,
-               "%d requests, %d pages a row, %d tokens, max_new %d", s->num_requests, s->max_pages, s->num_tokens, s->max_new);
-    MARS_CHECK(s->num_requests <= kMaxRequests, MARS_ERR_CAPACITY, "%d requests (at most %d)", s->num_requests, kMaxRequests);
-    MARS_TRY(check_cache(*r, *c));
-    const mars_reader_desc& d = r->d;
-    MARS_CHECK(int64_t(s->max_pages) * d.page_size <= (1 << 30), MARS_ERR_CAPACITY, "%d pages of %d tokens a row", s->max_pages, d.page_size);
-    MARS_CHECK(int64_t(s->num_tokens) * d.q_heads <= INT32_MAX, MARS_ERR_CAPACITY, "%d tokens of %d heads", s->num_tokens, d.q_heads);
-    MARS_TRY(check_rows("q", s->q, s->q_stride, int64_t(d.q_heads) * d.head_dim));
-    MARS_TRY(check_rows("out", s->out, s->out_stride, int64_t(d.q_heads) * d.head_dim));
-    MARS_CHECK(!s->decay || (s->q_times && c->times), MARS_ERR_INVALID, "decay needs q_times and the cache's times");
-    MARS_CHECK(!s->q_episodes || c->episodes, MARS_ERR_INVALID, "q_episodes needs the cache's episodes");
-    MARS_CHECK(std::isfinite(s->cap) && s->cap >= 0.0f, MARS_ERR_INVALID, "cap %g", double(s->cap));
-    MARS_CHECK(std::isfinite(s->scale), MARS_ERR_INVALID, "scale %g", double(s->scale));
-    if (s->num_tokens == 0) return MARS_OK;
-    constexpr double kLog2e = 1.4426950408889634074;
-    const double scale = s->scale == 0.0f ? 1.0 / std::sqrt(double(d.head_dim)) : double(s->scale);
-    const int64_t dense = int64_t(d.kv_heads) * d.page_size * d.head_dim;
-    AttendArgs a{};
-    a.q = s->q; a.out = s->out; a.lse = s->lse;
-    a.k_pages = c->k_pages; a.v_pages = c->v_pages;
-    a.k_times = s->decay ? c->times : nullptr;
-    a.k_eps = s->q_episodes ? c->episodes : nullptr;
-    a.q_start = s->q_start; a.kv_lens = s->kv_lens; a.table = s->block_table;
-    a.decay = s->decay; a.q_times = s->q_times; a.q_eps = s->q_episodes; a.prefix = s->prefix_lens;
-    a.part_o = r->part_o; a.part_ml = r->part_ml; a.arrived = r->arrived;
-    a.many_o = r->part_o + r->few_slots * kFewRows * size_t(d.head_dim);
-    a.many_ml = r->part_ml + r->few_slots * kFewRows;
-    a.q_stride = s->q_stride; a.out_stride = s->out_stride;
-    a.k_stride = c->k_page_stride ? c->k_page_stride : dense;
-    a.v_stride = c->v_page_stride ? c->v_page_stride : dense;
-    a.q_flip = scale < 0.0 ? 0x80008000u : 0u;
-    // finite: a score of 0 times an infinity would be NaN
-    a.scale_log2 = float(std::min(std::fabs(kLog2e * scale), double(FLT_MAX)));
-    a.cap_log2 = float(std::min(kLog2e * double(s->cap), double(FLT_MAX)));
-    a.cap_rcp = s->cap > 0.0f ? float(std::clamp(1.0 / (kLog2e * double(s->cap)), double(FLT_MIN), double(FLT_MAX))) : 0.0f;
-    a.requests = s->num_requests; a.max_pages = s->max_pages; a.tokens = s->num_tokens; a.num_pages = c->num_pages;
-    a.q_heads = d.q_heads; a.kv_heads = d.kv_heads; a.group = d.q_heads / d.kv_heads;
-    a.page_shift = r->page_shift;
-    MARS_TRY(use_device(r->device));
-    return launch_attend(*r, a, s->max_new, static_cast<hipStream_t>(stream));
+int mars_kv_store(const mars_reader* r, const mars_kv_cache* c, const mars_kv_store_args* s, void* stream) { return store(r, c, s, stream); }
+int mars_kv_store8(const mars_reader* r, const mars_kv_cache8* c, const mars_kv_store_args* s, void* stream) { return store(r, c, s, stream); }
+
+int mars_kv_load(const mars_reader* r, const mars_kv_cache* c, const mars_kv_load_args* s, void* stream) { return load(r, c, s, stream); }
+int mars_kv_load8(const mars_reader* r, const mars_kv_cache8* c, const mars_kv_load_args* s, void* stream) { return load(r, c, s, stream); }
+
+int mars_kv_attend(const mars_reader* r, const mars_kv_cache* c, const mars_kv_attend_args* s, void* stream) { return attend(r, c, s, nullptr, stream); }
+int mars_kv_attend_shared(const mars_reader* r, const mars_kv_cache* c, const mars_kv_attend_args* s, const mars_kv_shared* shared, void* stream) {
+    MARS_CHECK(shared, MARS_ERR_INVALID, "null argument");
+    return attend(r, c, s, shared, stream);
+}
+int mars_kv_attend8(const mars_reader* r, const mars_kv_cache8* c, const mars_kv_attend_args* s, const mars_kv_shared* shared, void* stream) {
+    return attend(r, c, s, shared, stream);
 }
 
 }  // extern "C"

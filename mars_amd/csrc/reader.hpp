@@ -1,6 +1,6 @@
 // ============================================================================
 //  reader.hpp — shared internals of the reading path (reader.hip: handle, plan,
-//  store, release; attend.hip: attention).
+//  store, release; store8.hip: store into 8 bits, load; attend.hpp: attention).
 // ============================================================================
 #pragma once
 
@@ -19,6 +19,10 @@ struct mars_reader {
     float* part_o = nullptr;
     float2* part_ml = nullptr;
     uint32_t* arrived = nullptr;
+    // Attention with shared prefixes: the sums of the first phase (kStateRows rows and query heads) and every request's skip.
+    float* state_o = nullptr;
+    float2* state_ml = nullptr;
+    int32_t* skips = nullptr;
 };
 
 namespace mars {
@@ -39,6 +43,10 @@ constexpr int32_t kJoinRows = 16;            // of a tile's rows, joined by a wo
 // At least 128, in multiples of 128: two chunks of 511 tokens among 22 single ones (32/8 of 128) 147 us (122).
 constexpr int32_t kMinChunk = 256;
 constexpr int32_t kMaxSplits = 256;          // pieces of a tile, as many as a join keeps references of in LDS
+
+// Rows times query heads whose sums the first phase of attention with shared prefixes can keep; calls with more read each
+// request's own prefix.
+constexpr int64_t kStateRows = 1 << 15;
 
 struct AttendArgs {
     const void* q;
@@ -69,8 +77,57 @@ struct AttendArgs {
     int32_t page_shift;
     int32_t few_rows;           // requests of up to so many rows are k_attend_few's
     float cap_rcp;         // 1 / (cap * log2(e)); 0: no cap
+    const uint8_t* k_scales;    // a cache of 8 bits: the exponents of its slots
+    const uint8_t* v_scales;
+    // Shared prefixes (NULL: none): group g is requests group_start[g] .. group_start[g + 1] - 1 of `members`. phase 0: no
+    // prefixes; 1: `requests` are the groups; 2: the requests, each behind the skips[r] keys that phase 1 read for it.
+    const int32_t* group_start;
+    const int32_t* shared_lens;
+    int32_t* skips;
+    float* state_o;             // sums of phase 1, a row and query head each, and their (reference, sum of weights)
+    float2* state_ml;
+    int32_t groups, members, phase;
 };
 
+struct StoreArgs {
+    mars_kv_store_args s;
+    void* k_pages;
+    void* v_pages;
+    float* times;
+    int32_t* eps;
+    const uint64_t* freq;
+    const int32_t* axis;
+    int64_t k_stride, v_stride, slots;                   // page strides (elements); slots the cache has
+    int32_t q_heads, kv_heads, head_dim, rope_dim, adjacent, page_shift;
+    uint8_t* k_scales;                                   // a cache of 8 bits: the exponents of its slots
+    uint8_t* v_scales;
+};
+
+// sin and cos of 2 pi * pos * f, f in units of 2^-64 turns per position: whole turns drop out of the 64-bit product
+// by themselves, so the phase is exact to pos * 2^-65 turns for every int32 position, and the angle to the rounding of
+// its upper 32 bits to fp32. (A product in fp32 is off by 2^-24 of the whole angle: 0.004 rad at position 70,000.)
+__device__ inline void turn(int32_t pos, uint64_t f, float* sn, float* cs) {
+    const uint64_t phase = uint64_t(int64_t(pos)) * f;
+    sincospif(float(int32_t(uint32_t(phase >> 32))) * 0x1p-31f, sn, cs);
+}
+
+int launch_store8(const mars_reader& r, const StoreArgs& a, hipStream_t s);
+
+struct LoadArgs {
+    mars_kv_load_args s;
+    const void* k_pages;
+    const void* v_pages;
+    const float* times;
+    const int32_t* eps;
+    const uint8_t* k_scales;    // NULL: a cache of 16 bits
+    const uint8_t* v_scales;
+    int64_t k_stride, v_stride, slots;                   // page strides (elements); slots the cache has
+    int32_t kv_heads, page_shift;
+};
+int launch_load(const mars_reader& r, const LoadArgs& a, hipStream_t s);
+
 int launch_attend(const mars_reader& r, const AttendArgs& a, int32_t max_new, hipStream_t s);
+int launch_attend8(const mars_reader& r, const AttendArgs& a, int32_t max_new, hipStream_t s);
+int launch_attend_shared(const mars_reader& r, const AttendArgs& a, int32_t max_new, hipStream_t s);
 
 }  // namespace mars

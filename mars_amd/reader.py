@@ -7,6 +7,10 @@
     r.store(cache, q, k, v, positions, slots, q_out=q, times=..., episodes=...)            # once a layer
     r.attend(cache, q, out, q_start, kv_lens, block_table, decay=..., q_times=..., ...)
     r.release(done, next_lens, block_table, free_pages, free_count)                        # ended requests
+    r.load(cache, slots, k, v)                                                             # tokens read back, to be moved or kept
+
+A cache is of the reader's 16-bit type, or of 8 bits (e4m3 pages with an exponent a token and kv head): store quantises, attend and load
+read what was held. Where requests have their first tokens in common, attend(..., group_start=, shared_lens=) reads those once.
 
 The calls mirror mars_kv_* of include/mars_amd.h, which defines their results. They run on
 `stream` (the integer of a hipStream_t; 0 is the null stream) and return without waiting.
@@ -28,7 +32,8 @@ from ._lib import check, lib
 __all__ = ["Reader", "PagedCache", "DeviceArray"]
 
 _DTYPES = {"float16": 0, "bfloat16": 1}
-_ITEM = {"float16": 2, "bfloat16": 2, "float32": 4, "int32": 4, "int64": 8}
+_ITEM = {"float16": 2, "bfloat16": 2, "float32": 4, "int32": 4, "int64": 8, "uint8": 1, "float8_e4m3fn": 1}
+_EIGHT = ("uint8", "float8_e4m3fn")           # what pages of 8 bits may be declared as
 _NAMES: dict = {}
 
 
@@ -64,14 +69,14 @@ class DeviceArray:
 
     @classmethod
     def from_numpy(cls, a: np.ndarray, dtype: Optional[str] = None) -> "DeviceArray":
-        """dtype "bfloat16": `a` holds the bits as uint16."""
+        """dtype "bfloat16": `a` holds the bits as uint16; "float8_e4m3fn": as uint8."""
         a = np.ascontiguousarray(a)
         return cls(a.shape, dtype or str(a.dtype), DeviceBuffer.from_array(a) if a.size else None)
 
     def numpy(self) -> np.ndarray:
-        """The contents once all work is done; bfloat16 as uint16 bits."""
+        """The contents once all work is done; bfloat16 as uint16 bits, float8_e4m3fn as uint8."""
         check(lib.mars_device_synchronize(), "mars_device_synchronize")
-        dt = np.uint16 if self.dtype == "bfloat16" else np.dtype(self.dtype)
+        dt = np.uint16 if self.dtype == "bfloat16" else np.dtype(np.uint8 if self.dtype in _EIGHT else self.dtype)
         return self.buffer.to_array(dt, self.size).reshape(self.shape)
 
     def data_ptr(self) -> int:
@@ -161,25 +166,30 @@ def _rows(x, name: str, dtype: str, device: Optional[int], tokens: Optional[int]
 
 class PagedCache:
     """The pages of one layer (mars_kv_cache): k_pages (pages, kv_heads, page_size, head_dim), v_pages (pages,
-    kv_heads, head_dim, page_size), each page dense; times (float32) and episodes (int32) one per slot."""
+    kv_heads, head_dim, page_size), each page dense; times (float32) and episodes (int32) one per slot. With k_scales and v_scales
+    (pages, kv_heads, page_size; uint8) the pages are of 8 bits, uint8 or float8_e4m3fn (mars_kv_cache8)."""
 
-    def __init__(self, k_pages, v_pages, times=None, episodes=None):
+    def __init__(self, k_pages, v_pages, times=None, episodes=None, k_scales=None, v_scales=None):
         if len(k_pages.shape) != 4 or len(v_pages.shape) != 4:
             raise ValueError("k_pages, v_pages: 4 axes expected")
         n, h, p, d = (int(s) for s in k_pages.shape)
         if tuple(v_pages.shape) != (n, h, d, p):
             raise ValueError(f"v_pages: shape {tuple(v_pages.shape)}, expected {(n, h, d, p)}")
-        if _dtype(k_pages) != _dtype(v_pages) or _dtype(k_pages) not in _DTYPES:
-            raise ValueError(f"k_pages {_dtype(k_pages)}, v_pages {_dtype(v_pages)}")
+        if (k_scales is None) != (v_scales is None):
+            raise ValueError("k_scales and v_scales come together")
+        self.held8 = k_scales is not None
+        if _dtype(k_pages) != _dtype(v_pages) or _dtype(k_pages) not in (_EIGHT if self.held8 else _DTYPES):
+            raise ValueError(f"k_pages {_dtype(k_pages)}, v_pages {_dtype(v_pages)}{' with exponents' if self.held8 else ''}")
         for name, x, inner in (("k_pages", k_pages, (p * d, d, 1)), ("v_pages", v_pages, (p * d, p, 1))):
             if any(x.shape[i + 1] != 1 and x.stride(i + 1) != inner[i] for i in range(3)):
                 raise ValueError(f"{name}: a page is not dense")
         self.k_pages, self.v_pages, self.times, self.episodes = k_pages, v_pages, times, episodes
+        self.k_scales, self.v_scales = k_scales, v_scales
         self.num_pages, self.kv_heads, self.page_size, self.head_dim = n, h, p, d
         self.dtype = _dtype(k_pages)
         self.geometry = (h, p, d, self.dtype)
         # the GPU of the arrays that are on one (pinned host memory is on none)
-        self.device = next((at for at in map(_device, (k_pages, v_pages, times, episodes)) if at is not None and at >= 0), None)
+        self.device = next((at for at in map(_device, (k_pages, v_pages, k_scales, v_scales, times, episodes)) if at is not None and at >= 0), None)
         for name, x in (("k_pages", k_pages), ("v_pages", v_pages)):
             _place(x, name, _device(x), self.device)
         strides = [x.stride(0) if n > 1 else 0 for x in (k_pages, v_pages)]
@@ -187,8 +197,12 @@ class PagedCache:
             if x is not None and int(np.prod(tuple(x.shape), dtype=np.int64)) != n * p:
                 raise ValueError(f"{name}: shape {tuple(x.shape)}, expected one per slot, {n * p}")
             _arg(x, name, want, None, self.device)
-        self.c = _lib.KvCacheC(k_pages.data_ptr(), v_pages.data_ptr(), times.data_ptr() if times is not None else None,
-                               episodes.data_ptr() if episodes is not None else None, strides[0], strides[1], n, 0)
+        at = [x.data_ptr() if x is not None else None for x in (times, episodes)]
+        if self.held8:
+            scales = [_arg(x, name, "uint8", (n, h, p), self.device) for name, x in (("k_scales", k_scales), ("v_scales", v_scales))]
+            self.c = _lib.KvCache8C(k_pages.data_ptr(), v_pages.data_ptr(), *scales, *at, strides[0], strides[1], n, 0)
+        else:
+            self.c = _lib.KvCacheC(k_pages.data_ptr(), v_pages.data_ptr(), *at, strides[0], strides[1], n, 0)
         self.ref = C.byref(self.c)
 
 
@@ -228,7 +242,7 @@ class Reader:
             pass
 
     def _cache(self, cache: PagedCache):
-        if cache.geometry != self.geometry:
+        if cache.geometry != self.geometry and not (cache.held8 and cache.geometry[:3] == self.geometry[:3]):
             raise ValueError(f"cache of {cache.kv_heads} heads of {cache.head_dim}, pages of {cache.page_size}, {cache.dtype}; the reader has "
                              f"{self.kv_heads}, {self.head_dim}, {self.page_size}, {self.dtype}")
         if cache.device != self.device:
@@ -253,8 +267,17 @@ class Reader:
         if rc:
             check(rc, "mars_kv_plan")
 
-    def release(self, done, kv_lens, block_table, free_pages, free_count, stream: int = 0) -> None:
-        """The pages of requests with done != 0 pushed onto free_pages; their kv_lens (plan's next_lens) become 0 (mars_kv_release)."""
+    def _shared(self, group_start, shared_lens):
+        """What mars_kv_shared takes of the groups' arrays."""
+        if group_start is None or shared_lens is None:
+            raise ValueError("group_start and shared_lens come together")
+        groups = int(shared_lens.shape[0])
+        return _lib.KvSharedC(*_args(self.device, (group_start, "group_start", "int32", (groups + 1,)), (shared_lens, "shared_lens", "int32", (groups,))),
+                              groups, 0)
+
+    def release(self, done, kv_lens, block_table, free_pages, free_count, group_start=None, shared_lens=None, stream: int = 0) -> None:
+        """The pages of requests with done != 0 pushed onto free_pages; their kv_lens (plan's next_lens) become 0 (mars_kv_release).
+        group_start, shared_lens: as for attend; the pages of the shared prefixes stay (mars_kv_release_shared)."""
         r = int(done.shape[0])
         if len(block_table.shape) != 2:
             raise ValueError(f"block_table: shape {tuple(block_table.shape)}, expected (requests, pages)")
@@ -262,11 +285,15 @@ class Reader:
         done, kv_lens, table, pages, count = _args(
             self.device, (done, "done", "int32", (r,)), (kv_lens, "kv_lens", "int32", (r,)), (block_table, "block_table", "int32", (r, width)),
             (free_pages, "free_pages", "int32", None), (free_count, "free_count", "int32", (1,)))
+        if group_start is not None or shared_lens is not None:
+            check(lib.mars_kv_release_shared(self.handle, done, kv_lens, table, r, width, self._shared(group_start, shared_lens), pages, count,
+                                             int(free_pages.shape[0]), stream), "mars_kv_release_shared")
+            return
         check(lib.mars_kv_release(self.handle, done, kv_lens, table, r, width, pages, count, int(free_pages.shape[0]), stream), "mars_kv_release")
 
     def store(self, cache: Optional[PagedCache], q, k, v, positions, slots, *, q_out=None, times=None, episodes=None,
               inverse: bool = False, stream: int = 0) -> None:
-        """q and k turned by their positions (axes, tokens), k, v, times, episodes written to `slots` (mars_kv_store).
+        """q and k turned by their positions (axes, tokens), k, v, times, episodes written to `slots` (mars_kv_store, mars_kv_store8).
         q_out: where the turned q goes (default q itself). k and v None: only q is turned; q None: only stores."""
         first = q if q is not None else k
         if first is None:
@@ -290,14 +317,34 @@ class Reader:
                 raise ValueError("positions are needed")
             want = (t,) if self.rope_axes == 1 and len(positions.shape) == 1 else (self.rope_axes, t)
             a.positions, = _args(g, (positions, "positions", "int32", want))
-        rc = lib.mars_kv_store(self.handle, ref, a, stream)
+        name = "mars_kv_store8" if ref is not None and cache.held8 else "mars_kv_store"
+        rc = getattr(lib, name)(self.handle, ref, a, stream)
         if rc:
-            check(rc, "mars_kv_store")
+            check(rc, name)
+
+    def load(self, cache: PagedCache, slots, k=None, v=None, *, times=None, episodes=None, stream: int = 0) -> None:
+        """k and v (tokens, kv_heads, head_dim), times, episodes of `slots` read back (mars_kv_load, mars_kv_load8). Rows of tokens
+        whose slot is outside the cache are left as they are."""
+        t, g = int(slots.shape[0]), self.device
+        ref = self._cache(cache)
+        a = _lib.KvLoadArgsC(num_tokens=t)
+        if k is not None or v is not None:
+            if k is None or v is None:
+                raise ValueError("k and v come together")
+            a.k, a.k_stride = _rows(k, "k", self.dtype, g, t, self.kv_heads, self.head_dim)
+            a.v, a.v_stride = _rows(v, "v", self.dtype, g, t, self.kv_heads, self.head_dim)
+        a.slots, a.times, a.episodes = _args(g, (slots, "slots", "int64", (t,)), (times, "times", "float32", (t,)), (episodes, "episodes", "int32", (t,)))
+        name = "mars_kv_load8" if cache.held8 else "mars_kv_load"
+        rc = getattr(lib, name)(self.handle, ref, a, stream)
+        if rc:
+            check(rc, name)
 
     def attend(self, cache: PagedCache, q, out, q_start, kv_lens, block_table, *, lse=None, scale: float = 0.0,
-               cap: float = 0.0, decay=None, q_times=None, q_episodes=None, prefix_lens=None, max_new: int = 0,
-               stream: int = 0) -> None:
-        """Attention of each request's rows of q over its cached tokens, into out (mars_kv_attend)."""
+               cap: float = 0.0, decay=None, q_times=None, q_episodes=None, prefix_lens=None, group_start=None, shared_lens=None,
+               max_new: int = 0, stream: int = 0) -> None:
+        """Attention of each request's rows of q over its cached tokens, into out (mars_kv_attend, mars_kv_attend8). group_start
+        (groups + 1), shared_lens (groups): requests group_start[g] .. group_start[g + 1] - 1 have their first shared_lens[g] tokens, in
+        whole pages, in common; these are read once for the group (mars_kv_attend_shared)."""
         t, r, g = q.shape[0], kv_lens.shape[0], self.device
         ref = self._cache(cache)
         qp, qs = _rows(q, "q", self.dtype, g, None, self.q_heads, self.head_dim)
@@ -311,6 +358,12 @@ class Reader:
                            (decay, "decay", "float32", (self.q_heads,)), (q_times, "q_times", "float32", (t,)),
                            (q_episodes, "q_episodes", "int32", (t,)), (prefix_lens, "prefix_lens", "int32", (r,))),
             qs, os_, scale, cap, r, width, t, max_new)
-        rc = lib.mars_kv_attend(self.handle, ref, a, stream)
+        shared = None if group_start is None and shared_lens is None else self._shared(group_start, shared_lens)
+        if cache.held8:
+            name, rc = "mars_kv_attend8", lib.mars_kv_attend8(self.handle, ref, a, shared, stream)
+        elif shared is not None:
+            name, rc = "mars_kv_attend_shared", lib.mars_kv_attend_shared(self.handle, ref, a, shared, stream)
+        else:
+            name, rc = "mars_kv_attend", lib.mars_kv_attend(self.handle, ref, a, stream)
         if rc:
-            check(rc, "mars_kv_attend")
+            check(rc, name)
