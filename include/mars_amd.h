@@ -863,8 +863,9 @@ int mars_kv_load(const mars_reader* r, const mars_kv_cache* cache, const mars_kv
  * multiple of 16, 0 = dense) let layers interleave. Stored values: e is the least with which the head's largest finite
  * element stays within 448, but at least 112 (float16) or 10 (bfloat16), so that every value is one of the reader's type;
  * each element is rounded once, to nearest even (k from its turned fp32 value), and is off by at most 2^-4 of itself
- * or 2^-10 times 2^(e - 127). Infinities and NaN become NaN, and leave the head's other elements alone. A cache is read by readers of
- * the type that wrote it. Bytes e of 0 stand for 0, of 255 for 254. */
+ * or 2^-10 times 2^(e - 127); finite ones beyond 61440 (float16) or 240 * 2^120 become that. Infinities and NaN become NaN, and leave the
+ * head's other elements alone. Read, a value is rounded to the reader's type, which changes none that a reader of that type wrote; e
+ * of 255 (never written) is NaN. */
 typedef struct mars_kv_cache8 {
     void*    k_pages;
     void*    v_pages;
@@ -884,8 +885,8 @@ int mars_kv_load8(const mars_reader* r, const mars_kv_cache8* cache, const mars_
  * is requests group_start[g] .. group_start[g + 1] - 1 (rising, from 0; requests in no group share nothing), whose first shared_lens[g]
  * tokens, rounded down to whole pages, lie in the same pages. Attention reads such a prefix once for all rows of a group, by the
  * row of the table of its first request, and gives what it gives without groups, but for the order of the sums. A request whose cached tokens
- * (kv_lens less its new ones) are fewer than the prefix reads everything for itself. Calls of more than 2^15 rows times query heads
- * read every request's tokens for themselves too (their products cost more than the reads). */
+ * (kv_lens less its new ones) are fewer than the prefix reads everything for itself. So do all in calls of more than 2^15 rows times
+ * query heads (their products cost more than the reads), and where the rows of the table name less than 128 MiB (one pass is shorter). */
 typedef struct mars_kv_shared {
     const int32_t* group_start;     /* num_groups + 1 */
     const int32_t* shared_lens;     /* num_groups     */

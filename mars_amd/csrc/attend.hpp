@@ -28,14 +28,16 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 namespace mars {
 namespace {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -103,6 +105,7 @@ template <typename T> struct Vec;
 template <> struct Vec<_Float16> {
     using v8 = f16x8;
     using v4 = f16x4;
+    using v2 = f16x2;
     static constexpr uint32_t exp_mask = 0x7C00u;
     static constexpr float lift = 7.0f;                      // of the weights: 2^7 where the score is the reference's own
     __device__ static f32x4 mma(v8 a, v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
@@ -111,6 +114,7 @@ template <> struct Vec<_Float16> {
 template <> struct Vec<__bf16> {
     using v8 = bf16x8;
     using v4 = bf16x4;
+    using v2 = bf16x2;
     static constexpr uint32_t exp_mask = 0x7F80u;
     static constexpr float lift = 0.0f;
     __device__ static f32x4 mma(v8 a, v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
@@ -145,10 +149,19 @@ __device__ inline u32x4 finite_part(u32x4 b) {
 }
 
 // ---- e4m3 values times powers of two. The conversions are exact: store picks exponents that keep the values within T.
-// The power of two of an exponent byte (255 counts as 254: a slot that holds no token may hold anything, and 0 times it is 0).
-__device__ inline float power_of(uint32_t e) { return __uint_as_float(min(e, 254u) << 23); }
-// Byte j of a word.
-__device__ inline uint32_t byte_of(uint32_t w, int j) { return (w >> (8 * j)) & 0xFFu; }
+// (gfx950's conversions take the scale's exponent and nothing else of it, 0 for 2^-127 and 255 for NaN; their results are rounded to T.)
+// Byte j of a word where a scale's exponent lies.
+template <int J>
+__device__ inline float scale_at(uint32_t w) { return __uint_as_float(J == 3 ? w >> 1 : w << (23 - 8 * J)); }
+__device__ inline void scales16(u32x4 w, float (&s)[16]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        s[4 * j] = scale_at<0>(w[j]);
+        s[4 * j + 1] = scale_at<1>(w[j]);
+        s[4 * j + 2] = scale_at<2>(w[j]);
+        s[4 * j + 3] = scale_at<3>(w[j]);
+    }
+}
 // Two e4m3 values of a word (its upper half if HI) as T, times `scale`.
 template <typename T, bool HI>
 __device__ inline uint32_t from_e4m3(uint32_t w, float scale) {
@@ -167,9 +180,14 @@ __device__ inline u32x4 element_e4m3(uint32_t w0, uint32_t w1, const float* s) {
     return u32x4{join(from_e4m3<T, false>(w0, s[0]), from_e4m3<T, false>(w0, s[1])), join(from_e4m3<T, true>(w0, s[2]), from_e4m3<T, true>(w0, s[3])),
                  join(from_e4m3<T, false>(w1, s[4]), from_e4m3<T, false>(w1, s[5])), join(from_e4m3<T, true>(w1, s[6]), from_e4m3<T, true>(w1, s[7]))};
 }
-// Of 16 values: nonzero if one of them is NaN (e4m3 has no infinities); the values with those replaced by 0.
+// Of 4 values: nonzero if one of them is NaN (e4m3 has no infinities). Of 4 exponents: nonzero if one of them is 128 or more above
+// zero's, that is above the `most` with which every e4m3 value is a finite one of T: 134 or 246.
 __device__ inline uint32_t nan_e4m3(uint32_t w) { return ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u; }
-__device__ inline uint32_t finite_e4m3(uint32_t w) { return w & ~((nan_e4m3(w) >> 7) * 0xFFu); }
+template <typename T>
+__device__ inline uint32_t wide_exponents(uint32_t w) {
+    constexpr uint32_t room = 127u - ((__is_same(T, _Float16) ? 134u : 246u) & 127u);       // 0x80 and these 7 bits above `most`
+    return (((w & 0x7F7F7F7Fu) + room * 0x01010101u) & w) & 0x80808080u;
+}
 // The first `n` bytes of 16 kept (n may be negative or above 16), the others 0.
 __device__ inline u32x4 first_bytes(u32x4 w, int n) {
 #pragma unroll
@@ -197,6 +215,12 @@ __device__ inline TablePtr table_row(const AttendArgs& a, int request) {
 __device__ inline int page_of(const AttendArgs& a, TablePtr table, int key, int last) {
     const int id = table[min(key >> a.page_shift, last)];
     return uint32_t(id) < uint32_t(a.num_pages) ? id : 0;
+}
+
+// The u-th of four values. (Of an array's elements the compiler makes a read from scratch memory at u.)
+__device__ inline int pick4(int u, int p0, int p1, int p2, int p3) {
+    const int even = u & 2 ? p2 : p0, odd = u & 2 ? p3 : p1;
+    return u & 1 ? odd : even;
 }
 
 // A piece of a launch's work: a tile of rows of a request under one kv head, over the keys [k0, k1). Where several pieces
@@ -250,15 +274,17 @@ __device__ inline int shared_of(const AttendArgs& a, int g) {
     return int(min(int64_t(max(a.shared_lens[g], 0)), int64_t(a.max_pages) << a.page_shift)) >> a.page_shift << a.page_shift;
 }
 // The second phase's skips, by one workgroup of the first: 0 for a request in no group, or that has not the whole prefix cached
-// (one that was not served has no keys at all): it reads everything itself.
-__device__ inline void find_skips(const AttendArgs& a) {
+// (one that was not served has no keys at all): it reads everything itself. lds: room for the groups' starts.
+__device__ inline void find_skips(const AttendArgs& a, int32_t* lds) {
+    for (int g = int(threadIdx.x); g <= a.requests; g += 256) lds[g] = a.group_start[g];
+    __syncthreads();
     for (int r = int(threadIdx.x); r < a.members; r += 256) {
         int lo = 0, hi = a.requests;                        // the last group that begins at or before r
         while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
-            if (a.group_start[mid] <= r) lo = mid; else hi = mid;
+            if (lds[mid] <= r) lo = mid; else hi = mid;
         }
-        const int s = group_at(a, lo) <= r && r < group_at(a, lo + 1) ? shared_of(a, lo) : 0;
+        const int s = lds[lo] <= r && r < lds[lo + 1] ? shared_of(a, lo) : 0;
         const int row0 = max(a.q_start[r], 0), n = max(0, min(a.q_start[r + 1], a.tokens) - row0);
         const int64_t keys = min(int64_t(a.kv_lens[r]), int64_t(a.max_pages) << a.page_shift);
         a.skips[r] = s <= keys - n ? s : 0;
@@ -292,6 +318,10 @@ __device__ inline Request request_of(const AttendArgs& a, int r) {
     if (F::share && a.phase == 2) q.skip = min(a.skips[r], q.keys);
     return q;
 }
+// Where the pieces of a phase 1 row's sums lie, if phase 2 joins them (AttendArgs::defer): rows of part_o and part_ml.
+__device__ inline int64_t state_row(const AttendArgs& a, int64_t row, int hq) { return row * a.q_heads + hq; }
+__device__ inline i32x4 one_piece(const AttendArgs& a, int64_t at) { return i32x4{int32_t(a.state_row0 + at), 0, 0, 1}; }
+
 // Keys [0, limit) that row i of a request's n may see.
 template <typename F>
 __device__ inline int limit_of(const AttendArgs& a, int keys, int n, int i, int prefix) {
@@ -312,6 +342,10 @@ __device__ inline int prefix_of(const AttendArgs& a, int request, int keys) {
 // A tile has at most 2 L / C chunks where it has two, and C is at least sum(L) / 2^9 by either rule: 2^10 partial slots.
 // The launch has enough workgroups for every item (fewer than 2^31); the last ones may find none. JOIN: the items are
 // the blocks of kJoinRows rows of the tiles in several pieces instead, the block's number in Part::slot.
+// Rows of a tile that a workgroup of k_attend_join takes: with caches of 8 bits and shared prefixes, where there are few tiles (which
+// are in many pieces then), as many as it has threads for (see launch_dim).
+template <typename F>
+__device__ __host__ inline int join_rows_of(const AttendArgs& a) { return F::share ? a.join_rows : kJoinRows; }
 template <bool JOIN, typename F>
 struct ManySched {
     const AttendArgs& a;
@@ -361,7 +395,7 @@ struct ManySched {
         chunk = max(chunk0, (len + kMaxSplits * 256 - 1) / (kMaxSplits * 256) * 256);
         splits = max(1u, (len + chunk - 1) / chunk);
         const uint32_t heads = uint32_t(q.tiles) * uint32_t(a.kv_heads), parts = splits > 1 ? heads * splits : 0;
-        each = JOIN ? (splits > 1 ? kManyRows / kJoinRows : 0) : splits;
+        each = JOIN ? (splits > 1 ? kManyRows / join_rows_of<F>(a) : 0) : splits;
         items = heads * each;
         uint32_t xi = items, xp = parts;
 #pragma unroll
@@ -459,6 +493,10 @@ struct JoinLds {
     float scale[kFewRows], lse[kFewRows];
     float2 w[kMaxSplits][kFewRows];                         // (max, sum) of a piece, then its weight
     __attribute__((aligned(16))) float part[4][128 * 4];
+    // join_state: a row's pieces, reference and sum; the joined rows, D + 4 floats each, in place of the weights
+    i32x4 where[kFewRows];
+    float2 ml[kFewRows];
+    __device__ float* sum() { return reinterpret_cast<float*>(&w[0][0]); }
 };
 template <typename T, int D, typename F>
 __device__ void join_rows(const AttendArgs& a, const Part& it, JoinLds& lds) {
@@ -529,6 +567,82 @@ __device__ void join_rows(const AttendArgs& a, const Part& it, JoinLds& lds) {
         *reinterpret_cast<typename Vec<T>::v4*>(static_cast<T*>(a.out) + (int64_t(it.row0) + ii) * a.out_stride + int64_t(hh) * D + d4 * 4) = o;
         if (a.lse && d4 == 0) a.lse[(int64_t(it.row0) + ii) * a.q_heads + hh] = lds.lse[rr];
     }
+}
+
+// Joins the pieces of the first phase's sums of a tile's rows, as join_rows does: into lds.sum(), the lane's row's (reference, sum of
+// weights) returned. All threads call it; the LDS is free again after the next barrier.
+template <int D, int U>
+__device__ float2 join_state(const AttendArgs& a, const Part& it, JoinLds& lds) {
+    const int tid = int(threadIdx.x), rows = min(kFewRows, it.n * a.group - it.tile * kFewRows), units = rows * (D / 4);
+    auto row_of = [](i32x4 where, int s) { return int64_t(s == 0 ? where[0] : where[1] + (s - 1) * where[2]); };
+    {
+        const int rr = tid >> 4, s0 = tid & 15, m = it.tile * kFewRows + rr;
+        i32x4 where = {0, 0, 0, 0};
+        if (rr < rows) {
+            const int64_t at = state_row(a, int64_t(it.row0) + m / a.group, it.head * a.group + m % a.group);
+            where = a.defer ? a.state_at[at] : one_piece(a, at);
+        }
+        float top = -kInf, sum = 0.0f;
+        for (int s1 = s0; s1 < where[3]; s1 += 64) {         // four on the way together
+            float2 p[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) p[u] = s1 + 16 * u < where[3] ? a.part_ml[row_of(where, s1 + 16 * u)] : make_float2(-kInf, 0.0f);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                if (s1 + 16 * u < where[3]) lds.w[s1 + 16 * u][rr] = p[u];
+                top = fmaxf(top, p[u].x);
+            }
+        }
+#pragma unroll
+        for (int o = 1; o < 16; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
+        for (int s = s0; s < where[3]; s += 16) {
+            const float2 p = lds.w[s][rr];
+            const float f = p.x == -kInf ? 0.0f : __builtin_amdgcn_exp2f(p.x - top);
+            sum += p.x == -kInf ? 0.0f : f * p.y;
+            lds.w[s][rr].x = f;
+        }
+#pragma unroll
+        for (int o = 1; o < 16; o <<= 1) sum += __shfl_xor(sum, o);
+        if (s0 == 0) {
+            lds.where[rr] = where;
+            lds.ml[rr] = make_float2(top, sum);
+        }
+    }
+    __syncthreads();
+    int ways = 1;                                            // threads per unit of 4 elements
+    while (ways < 4 && units * ways * 2 <= 256) ways *= 2;
+    const int per = 256 / ways, w = tid / per;
+    constexpr int N = (kFewRows * (D / 4) + 255) / 256;     // U: pieces on the way together
+    f32x4 sum[N];
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        const int e = n * per + tid % per, rr = e / (D / 4), d4 = e % (D / 4);
+        sum[n] = f32x4{0, 0, 0, 0};
+        if (e >= units) continue;
+        const i32x4 where = lds.where[rr];
+        for (int s = w; s < where[3]; s += U * ways) {
+            f32x4 o[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (s + u * ways < where[3]) o[u] = *reinterpret_cast<const f32x4*>(a.part_o + row_of(where, s + u * ways) * D + d4 * 4);
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (s + u * ways < where[3]) sum[n] += lds.w[s + u * ways][rr].x * o[u];
+        }
+    }
+    if (ways > 1) {                                          // then every thread has one unit or none
+        *reinterpret_cast<f32x4*>(&lds.part[w][(tid % per) * 4]) = sum[0];
+        __syncthreads();
+        for (int v = 1; v < ways && w == 0; ++v) sum[0] += *reinterpret_cast<const f32x4*>(&lds.part[v][tid * 4]);
+    }
+    __syncthreads();                                         // the weights are read
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        const int e = n * per + tid % per;
+        if (e < units && w == 0) *reinterpret_cast<f32x4*>(&lds.sum()[e / (D / 4) * (D + 4) + e % (D / 4) * 4]) = sum[n];
+    }
+    __syncthreads();
+    return lds.ml[tid & 15];
 }
 
 // Called by every thread of a workgroup that wrote one piece's partial: the tile's last workgroup to arrive joins them.
@@ -621,7 +735,9 @@ __device__ void add_not_finite(const AttendArgs& a, const Part& it, int prefix) 
             }
             const int64_t at = page * a.v_stride + ((int64_t(it.head) * D + d) << a.page_shift) + off;
             if constexpr (F::c8) {
-                if ((static_cast<const uint8_t*>(a.v_pages)[at] & 0x7F) == 0x7F) sum = __builtin_nanf("");
+                const float e = scale_at<0>(a.v_scales[((page * a.kv_heads + it.head) << a.page_shift) + off]);
+                const float v = float(__builtin_bit_cast(typename Vec<T>::v2, from_e4m3<T, false>(static_cast<const uint8_t*>(a.v_pages)[at], e))[0]);
+                if (!(fabsf(v) < kInf)) sum += v;
             } else {
                 const float v = float(static_cast<const T*>(a.v_pages)[at]);
                 if (!(fabsf(v) < kInf)) sum += v;
@@ -651,7 +767,7 @@ __device__ void add_not_finite(const AttendArgs& a, const Part& it, int prefix) 
 // a CU have 128 KB in flight for heads of 128. The waves' sums are joined at the end. bf16, 32/8 heads of 128:
 // 64 single tokens over 780 to 7,800 keys (1.15 GB) 215 us, 5.4 TB/s; one over 131,072 (0.54 GB) 110 us.
 // Steps of 64 keys spill: 228 and 119 us (first case with cap and decay: 288 and 225 us).
-template <int D>
+template <int D, typename F>
 struct FewLds {
     union {
         struct { float ml[4][16][2]; __attribute__((aligned(16))) float ob[2][16][D + 4]; } wave;
@@ -659,25 +775,35 @@ struct FewLds {
         StepLds steps;
     };
     int any_dirty;
+    u32x4 q[F::share && D == (F::c8 ? 128 : 64) ? D / 32 * 64 : 1];            // see kLean
+    u32x4 row[F::share ? kFewRows : 1];                     // of a row: decay and time of the query (fp32), limit, episode
 };
+// Waves a SIMD of the kernels of few rows, as their registers allow.
+template <int D, typename F>
+constexpr int few_waves() { return D > 128 ? 1 : D == 128 ? 2 : F::c8 ? 2 : 3; }
 template <typename F>
 constexpr int few_step() { return F::c8 ? 64 : 32; }
 
 template <typename T, int D, bool EXTRA, bool CAP, typename F>
-__device__ void few_part(const AttendArgs& a, const Part& it, FewLds<D>& lds) {
+__device__ void few_part(const AttendArgs& a, const Part& it, FewLds<D, F>& lds) {
     using V = typename Vec<T>::v8;
     // a step's keys; its groups of 16; keys of a lane, in NB blocks of the first product and NT fragments of the second
     constexpr int kStep = few_step<F>(), NG = kStep / 16, NK = kStep / 4, NB = NK / 4, NT = NK / 8, KC = D / 32, VB = D / 16;
+    // With times on the way the registers do not suffice for 64 keys a step of heads of 128, nor for heads of 64 three waves a SIMD,
+    // and a kernel that keeps one value in scratch memory takes 13 us more a launch: there q, which the four waves have in
+    // common, and the terms of the rows are read from LDS in every step, and a lane's places in K and V are found anew
+    constexpr bool kLean = F::share && EXTRA && D == (F::c8 ? 128 : 64);
     int tid = int(threadIdx.x);
     asm volatile("" : "+v"(tid));                          // nothing of a piece is kept in registers for the next
-    const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int col = lane & 15, h = lane >> 4;
+    int lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    int col = lane & 15, h = lane >> 4;
     const int r = it.request, head = it.head, row0 = it.row0, n = it.n, keys = it.keys, P1 = (1 << a.page_shift) - 1;
     if (tid == 0) lds.any_dirty = 0;                        // read after barriers
-    const int m = it.tile * kFewRows + col;                 // this lane's row: token i, head of the group
-    const bool row_ok = m < n * a.group;
-    const int i = row_ok ? m / a.group : 0, hq = head * a.group + (row_ok ? m - i * a.group : 0);
-    const int64_t row = int64_t(row0) + i;
+    int m = it.tile * kFewRows + col;                       // this lane's row: token i, head of the group
+    bool row_ok = m < n * a.group;
+    int i = row_ok ? m / a.group : 0, hq = head * a.group + (row_ok ? m - i * a.group : 0);
+    int64_t row = int64_t(row0) + i;
     const int prefix = prefix_of<F>(a, r, keys);
     const int limit = row_ok ? limit_of<F>(a, keys, n, i, prefix) : 0;         // keys [0, limit) may be seen
     const float dec = EXTRA && a.decay ? a.decay[hq] * 1.4426950408889634f : 0.0f;
@@ -701,6 +827,10 @@ __device__ void few_part(const AttendArgs& a, const Part& it, FewLds<D>& lds) {
             eq_max = max(eq_max, __shfl_xor(eq_max, o));
         }
     }
+    if constexpr (F::share) {                               // the same in every lane
+        eq_min = __builtin_amdgcn_readfirstlane(eq_min);
+        eq_max = __builtin_amdgcn_readfirstlane(eq_max);
+    }
     const int k0 = it.k0, k1 = min(it.k1, hi);
     const int steps = k1 > k0 ? (k1 - k0 + kStep - 1) / kStep : 0;
 
@@ -721,7 +851,8 @@ __device__ void few_part(const AttendArgs& a, const Part& it, FewLds<D>& lds) {
     auto load_k = [&](int s) {
         const int kt = k0 + s * kStep;
         if constexpr (F::c8) {
-            const int pg = kg & 2 ? (kg & 1 ? pages[3] : pages[2]) : (kg & 1 ? pages[1] : pages[0]), off = (kt + kg * 16) & P1;
+            const int ln = kLean ? int(here(uint32_t(lane))) : lane, col = ln & 15, h = ln >> 4, kg = col >> 2, kin = col & 3;
+            const int pg = pick4(kg, pages[0], pages[1], pages[2], pages[3]), off = (kt + kg * 16) & P1;
             const uint8_t* const p = static_cast<const uint8_t*>(a.k_pages) + pg * a.k_stride + ((int64_t(head) << a.page_shift) + off + kin) * D + h * 16;
 #pragma unroll
             for (int b = 0; b < NB; ++b)
@@ -742,7 +873,8 @@ __device__ void few_part(const AttendArgs& a, const Part& it, FewLds<D>& lds) {
         const int kt = k0 + s * kStep;
         int64_t slot;
         if constexpr (F::c8) {
-            const int pg = h & 2 ? (h & 1 ? v_pages[3] : v_pages[2]) : (h & 1 ? v_pages[1] : v_pages[0]), off = (kt + h * 16) & P1;
+            const int ln = kLean ? int(here(uint32_t(lane))) : lane, col = ln & 15, h = ln >> 4;
+            const int pg = pick4(h, v_pages[0], v_pages[1], v_pages[2], v_pages[3]), off = (kt + h * 16) & P1;
             const uint8_t* const p = static_cast<const uint8_t*>(a.v_pages) + pg * a.v_stride + ((int64_t(head) * D + col) << a.page_shift) + off;
 #pragma unroll
             for (int d = 0; d < VL; ++d) vf[d] = *reinterpret_cast<const u32x4*>(p + (int64_t(d) * 16 << a.page_shift));
@@ -760,10 +892,17 @@ __device__ void few_part(const AttendArgs& a, const Part& it, FewLds<D>& lds) {
 #pragma unroll
             for (int b = 0; b < NB; ++b) tk[b] = *reinterpret_cast<const f32x4*>(a.k_times + slot + 4 * b);
         }
-        if (EXTRA && a.k_eps) {
+        if (EXTRA && !F::share && a.k_eps) {
 #pragma unroll
             for (int b = 0; b < NB; ++b) ek[b] = *reinterpret_cast<const i32x4*>(a.k_eps + slot + 4 * b);
         }
+    };
+    // the episodes of a step whose rows and keys have to be compared one by one: seldom, and not worth registers for one on the way
+    auto load_eps = [&](int ks) {
+        const int key = ks + NK * h, id = a.table[int64_t(r) * a.max_pages + min(key >> a.page_shift, last_page)];
+        const int64_t slot = (int64_t(uint32_t(id) < uint32_t(a.num_pages) ? id : 0) << a.page_shift) + (key & P1);
+#pragma unroll
+        for (int b = 0; b < NB; ++b) ek[b] = *reinterpret_cast<const i32x4*>(a.k_eps + slot + 4 * b);
     };
 
     // q in the order of K's elements: a piece of 16 bytes holds those of two products where the cache is e4m3
@@ -771,27 +910,34 @@ __device__ void few_part(const AttendArgs& a, const Part& it, FewLds<D>& lds) {
     const T* const qp = static_cast<const T*>(a.q) + row * a.q_stride + int64_t(hq) * D + h * (F::c8 ? 16 : 8);
 #pragma unroll
     for (int c = 0; c < KC; ++c) q[c] = load_q<V>(qp + (F::c8 ? c / 2 * 64 + c % 2 * 8 : c * 32), a.q_flip);
+    if constexpr (kLean) {
+        if (wave == 0) {
+#pragma unroll
+            for (int c = 0; c < KC; ++c) lds.q[c * 64 + lane] = __builtin_bit_cast(u32x4, q[c]);
+        }
+        if (wave == 0 && h == 0) lds.row[col] = u32x4{__float_as_uint(dec), __float_as_uint(tq), uint32_t(limit), uint32_t(eq)};
+        __syncthreads();
+    }
     f32x4 o[VB];
 #pragma unroll
     for (int d = 0; d < VB; ++d) o[d] = f32x4{0, 0, 0, 0};
     float mref = 0.0f, mtop = -kInf, l = 0.0f;              // mtop: -inf until the row has seen a key, then mref + lift + kSlack
-    if (F::share && it.skip > 0 && k0 == it.skip && wave == 0 && row_ok) {     // the prefix's sums
-        const int64_t at = row * a.q_heads + hq;
-        const float2 ml = a.state_ml[at];
-        if (ml.x != -kInf) {
-            mref = ml.x;
-            mtop = mref + (Vec<T>::lift + kSlack);
-            l = h == 0 ? ml.y : 0.0f;
-#pragma unroll
-            for (int d = 0; d < VB; ++d) o[d] = *reinterpret_cast<const f32x4*>(a.state_o + at * D + d * 16 + h * 4);
-        }
-    }
-    bool dirty = false;                                     // a value that is not finite was left out
-
     auto keep_pages = [&] {
 #pragma unroll
         for (int u = 0; u < NG; ++u) v_pages[u] = pages[u];
     };
+    if (F::share && it.skip > 0 && k0 == it.skip) {         // the prefix's sums
+        const float2 ml = join_state<D, 8>(a, it, lds.join);
+        if (wave == 0 && row_ok && ml.x != -kInf) {
+            mref = ml.x;
+            mtop = mref + (Vec<T>::lift + kSlack);
+            l = h == 0 ? ml.y : 0.0f;
+#pragma unroll
+            for (int d = 0; d < VB; ++d) o[d] = *reinterpret_cast<const f32x4*>(&lds.join.sum()[col * (D + 4) + d * 16 + h * 4]);
+        }
+    }
+    bool dirty = false;                                     // a value that is not finite was left out
+
     for (int w0 = 0; w0 < steps; w0 += kWindow) {
         const int count = listed ? list_steps<kStep>(a, r, last_page, k0, k1, w0, steps, eq_min, eq_max, lds.steps) : steps;
         auto step_at = [&](int x) { return listed ? w0 + (__builtin_amdgcn_readfirstlane(int(lds.steps.list[x])) & (kWindow - 1)) : x; };
@@ -806,11 +952,16 @@ __device__ void few_part(const AttendArgs& a, const Part& it, FewLds<D>& lds) {
             const int ks = k0 + step_at(x0) * kStep;
             const bool mixed = listed && (__builtin_amdgcn_readfirstlane(int(lds.steps.list[x0])) & kMixed);
             f32x4 acc[NB];
+            if constexpr (kLean) {
+                const uint32_t at = here(uint32_t(lane));   // not ahead of the loop
+#pragma unroll
+                for (int c = 0; c < KC; ++c) q[c] = load16<V>(&lds.q[c * 64 + at]);
+            }
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
                 acc[b] = f32x4{0, 0, 0, 0};
                 float ks8 = 0.0f;
-                if constexpr (F::c8) ks8 = power_of((kx[b] >> (8 * (col & 3))) & 0xFFu);
+                if constexpr (F::c8) ks8 = scale_at<0>(kx[b] >> (8 * (col & 3)));
 #pragma unroll
                 for (int c = 0; c < KC; ++c) {
                     u32x4 w;
@@ -834,18 +985,28 @@ __device__ void few_part(const AttendArgs& a, const Part& it, FewLds<D>& lds) {
 #pragma unroll
                 for (int j = 0; j < NK; ++j) x[j] = cap_any(x[j], a.cap_log2, a.cap_rcp);
             }
+            float dec_now = dec, tq_now = tq;
+            int limit_now = limit, eq_now = eq;
+            if constexpr (kLean) {
+                const u32x4 w = lds.row[here(uint32_t(lane)) & 15];
+                dec_now = __uint_as_float(w[0]);
+                tq_now = __uint_as_float(w[1]);
+                limit_now = int(w[2]);
+                eq_now = int(w[3]);
+            }
             if (EXTRA && a.k_times) {
 #pragma unroll
-                for (int j = 0; j < NK; ++j) x[j] -= dec * fmaxf(0.0f, tq - tk[j >> 2][j & 3]);
+                for (int j = 0; j < NK; ++j) x[j] -= dec_now * fmaxf(0.0f, tq_now - tk[j >> 2][j & 3]);
             }
             const bool whole = ks + kStep <= lo && !mixed;
             if (!whole) {
+                if (EXTRA && F::share && mixed) load_eps(ks);
 #pragma unroll
                 for (int j = 0; j < NK; ++j) {
-                    bool in = ks + NK * h + j < limit;
+                    bool in = ks + NK * h + j < limit_now;
                     if (mixed) {
                         const int e = ek[j >> 2][j & 3];
-                        in = in && (e < 0 || eq < 0 || e == eq);
+                        in = in && (e < 0 || eq_now < 0 || e == eq_now);
                     }
                     x[j] = in ? x[j] : -kInf;
                 }
@@ -872,43 +1033,60 @@ __device__ void few_part(const AttendArgs& a, const Part& it, FewLds<D>& lds) {
             // fp16's rests end at 2^-25 as its values do: a weight is off by up to 2^-32 of the row's largest
             V p[NT], rest[NT];
             float sum = 0.0f;
+            auto weigh = [&](int t) {
 #pragma unroll
-            for (int j = 0; j < NK; ++j) {
-                const float w = __builtin_amdgcn_exp2f(x[j] - mref);
-                sum += w;
-                p[j >> 3][j & 7] = T(w);
-                rest[j >> 3][j & 7] = T(w - float(p[j >> 3][j & 7]));
-            }
-            l += sum;
+                for (int j = 0; j < 8; ++j) {
+                    const float w = __builtin_amdgcn_exp2f(x[8 * t + j] - mref);
+                    sum += w;
+                    p[t][j] = T(w);
+                    rest[t][j] = T(w - float(p[t][j]));
+                }
+            };
             // infinities and NaN: see add_not_finite (in every step: a rest may be 0 or negative). Slots past the request's keys
             // hold anything.
             uint32_t odd = 0;
             const int kb = ks + NK * h;
             if constexpr (F::c8) {
-                float vs[NK];
+                if (!whole && kb + NK > keys) {
+                    vx = first_bytes(vx, keys - kb);
 #pragma unroll
-                for (int j = 0; j < NK; ++j) vs[j] = power_of(byte_of(vx[j >> 2], j & 3));
-#pragma unroll
-                for (int d = 0; d < VB; ++d) {
-                    u32x4 b = vf[d];
-                    if (!whole && kb + NK > keys) b = first_bytes(b, keys - kb);
-                    const uint32_t full = nan_e4m3(b[0]) | nan_e4m3(b[1]) | nan_e4m3(b[2]) | nan_e4m3(b[3]);
-                    odd |= full;
-                    if (__any(full != 0)) {
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) b[j] = finite_e4m3(b[j]);
-                    }
-                    vf[d] = b;
+                    for (int d = 0; d < VB; ++d) vf[d] = first_bytes(vf[d], keys - kb);
                 }
-                if (__any(odd != 0)) dirty = true;
 #pragma unroll
-                for (int d = 0; d < VB; ++d)
+                for (int j = 0; j < 4; ++j) odd |= wide_exponents<T>(vx[j]);
+#pragma unroll
+                for (int d = 0; d < VB; ++d) odd |= nan_e4m3(vf[d][0]) | nan_e4m3(vf[d][1]) | nan_e4m3(vf[d][2]) | nan_e4m3(vf[d][3]);
+                const bool look = __any(odd != 0);           // perhaps: then at the values themselves
+                auto add = [&](int d, int t) {
+                    const float vs[8] = {scale_at<0>(vx[2 * t]), scale_at<1>(vx[2 * t]), scale_at<2>(vx[2 * t]), scale_at<3>(vx[2 * t]),
+                                         scale_at<0>(vx[2 * t + 1]), scale_at<1>(vx[2 * t + 1]), scale_at<2>(vx[2 * t + 1]), scale_at<3>(vx[2 * t + 1])};
+                    u32x4 b = element_e4m3<T>(vf[d][2 * t], vf[d][2 * t + 1], vs);
+                    if (look) {
+                        if (__any(exponents_full<T>(b) != 0)) dirty = true;
+                        b = finite_part<T>(b);
+                    }
+                    const V w = __builtin_bit_cast(V, b);
+                    o[d] = Vec<T>::mma(w, rest[t], Vec<T>::mma(w, p[t], o[d]));
+                };
+                // element by element, so that the registers of V are free for the next step's one after the other (one token over
+                // 4,001 keys of 64 requests 93 us, key by key 106); kLean has no registers for all weights at once
+                if constexpr (kLean) {
 #pragma unroll
                     for (int t = 0; t < NT; ++t) {
-                        const V w = __builtin_bit_cast(V, element_e4m3<T>(vf[d][2 * t], vf[d][2 * t + 1], vs + 8 * t));
-                        o[d] = Vec<T>::mma(w, rest[t], Vec<T>::mma(w, p[t], o[d]));
+                        weigh(t);
+#pragma unroll
+                        for (int d = 0; d < VB; ++d) add(d, t);
                     }
+                } else {
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) weigh(t);
+#pragma unroll
+                    for (int d = 0; d < VB; ++d)
+#pragma unroll
+                        for (int t = 0; t < NT; ++t) add(d, t);
+                }
             } else {
+                weigh(0);
 #pragma unroll
                 for (int d = 0; d < VB; ++d) {
                     u32x4 b = vf[d];
@@ -928,11 +1106,24 @@ __device__ void few_part(const AttendArgs& a, const Part& it, FewLds<D>& lds) {
                     o[d] = Vec<T>::mma(w, rest[0], Vec<T>::mma(w, p[0], o[d]));
                 }
             }
+            l += sum;
             if (more) load_v(next);
         }
         if (!listed) break;
     }
 
+    if constexpr (F::share) {                               // found again, rather than kept in registers that the loop needs
+        tid = int(threadIdx.x);
+        asm volatile("" : "+v"(tid));
+        lane = tid & 63;
+        col = lane & 15;
+        h = lane >> 4;
+        m = it.tile * kFewRows + col;
+        row_ok = m < n * a.group;
+        i = row_ok ? m / a.group : 0;
+        hq = head * a.group + (row_ok ? m - i * a.group : 0);
+        row = int64_t(row0) + i;
+    }
     // join the waves: references first, then sums and O, in wave order
     auto& ml = lds.wave.ml;
     auto& ob = lds.wave.ob;
@@ -972,10 +1163,11 @@ __device__ void few_part(const AttendArgs& a, const Part& it, FewLds<D>& lds) {
 #pragma unroll
         for (int d = 0; d < VB; ++d) o[d] += *reinterpret_cast<const f32x4*>(&ob[0][col][d * 16 + h * 4]);
         if (F::share && a.phase == 1 && row_ok && !joined) {
-            const int64_t at = row * a.q_heads + hq;
+            const int64_t at = state_row(a, row, hq);
 #pragma unroll
             for (int d = 0; d < VB; ++d) *reinterpret_cast<f32x4*>(a.state_o + at * D + d * 16 + h * 4) = o[d];
             if (h == 0) a.state_ml[at] = make_float2(mall, lall);
+            if (h == 0) a.state_at[at] = one_piece(a, at);
         } else if (row_ok && !joined) {
             const float inv = mall == -kInf ? 0.0f : 1.0f / lall;
             T* const op = static_cast<T*>(a.out) + row * a.out_stride + int64_t(hq) * D + h * 4;
@@ -992,6 +1184,9 @@ __device__ void few_part(const AttendArgs& a, const Part& it, FewLds<D>& lds) {
 #pragma unroll
             for (int d = 0; d < VB; ++d) *reinterpret_cast<f32x4*>(&ob[0][col][d * 16 + h * 4]) = o[d];
             if (row_ok && h == 0) put_part(a.part_ml + int64_t(it.slot) * kFewRows + col, make_float2(mall, lall));
+            if (F::share && a.phase == 1 && a.defer && row_ok && h == 0 && it.slot == it.slot0)
+                a.state_at[state_row(a, row, hq)] = i32x4{int32_t(a.many_row0) + it.slot0 * kFewRows + col, int32_t(a.many_row0) + it.slot1 * kFewRows + col,
+                                                          it.slot_step * kFewRows, it.splits};
         }
     }
     if (joined) {
@@ -1006,7 +1201,7 @@ __device__ void few_part(const AttendArgs& a, const Part& it, FewLds<D>& lds) {
         __syncthreads();
         add_not_finite<T, D, kFewRows, F>(a, it, prefix);
     }
-    if (!joined) return;
+    if (!joined || (F::share && a.phase == 1 && a.defer)) return;
     __syncthreads();
     join_last<T, D, F>(a, it, lds.join);
 }
@@ -1018,11 +1213,18 @@ __device__ void few_part(const AttendArgs& a, const Part& it, FewLds<D>& lds) {
 // Cuts 2, 4, 8 steps from an end: 24 x 5 tokens over up to 3,000 keys 23.3, 22.3, 20.4 us, 4 x 4 over 3,000 29.7, 24.7,
 // 25.1 us (with 12 steps of twice the length it was slower again).
 constexpr int kFewCut = 8;
+// Where there are no more tiles than workgroups, and none of more steps than this, each workgroup takes whole tiles: equal lengths of the
+// line would give some of them the ends of two. 64 single tokens over 500 to 1,000 keys (32/8 heads of 128, 8 bits) 27.2 us, 38.4
+// without; one over 4,160 (65 steps) 20 and, whole, 44.6. (mars_kv_attend over 16 bits keeps to equal lengths, and its bits.)
+constexpr int kFewWhole = 36;
+// Steps of a piece of a prefix at least: 2 prefixes of 4,160 tokens for 4 requests each 33.0 us (1: 35.4, 16: 37.0).
+constexpr int kFirstSpan = 4;
 template <typename F>
 struct SpanLds {
     int64_t start[257];        // of 256 requests: steps of the launch before each
     int32_t row0[256], n[256], keys[256];
     int32_t skip[F::share ? 256 : 1], row[F::share ? 256 : 1];     // Request's skip and at
+    int64_t total, span;       // F::share: read again after every piece, rather than kept in registers
     int64_t wsum[4];
     int32_t wmost[4];
     int32_t at, most;          // most: steps of the longest tile so far
@@ -1032,12 +1234,13 @@ __device__ inline int steps_of(int keys) { return max(1, (keys + few_step<F>() -
 __device__ inline int units_of(const AttendArgs& a, int n) { return (n * a.group + kFewRows - 1) / kFewRows * a.kv_heads; }
 
 // Requests r0 .. r0 + 255 into the LDS; returns the launch's steps up to their end (base: before them).
-template <typename F>
+// TILES: tiles instead of steps.
+template <typename F, bool TILES = false>
 __device__ int64_t load_span(const AttendArgs& a, int r0, int64_t base, SpanLds<F>& lds) {
     const int tid = int(threadIdx.x), lane = tid & 63, wave = tid >> 6;
     const Request q = request_of<true, F>(a, r0 + tid);
     const int own = steps_of<F>(F::share ? q.keys - q.skip : q.keys);
-    const int64_t work = int64_t(q.tiles) * a.kv_heads * own;
+    const int64_t work = int64_t(q.tiles) * a.kv_heads * (TILES ? 1 : own);
     int64_t x = work;
     int most = own;
 #pragma unroll
@@ -1071,33 +1274,46 @@ __device__ int64_t load_span(const AttendArgs& a, int r0, int64_t base, SpanLds<
 
 template <int D, typename F>
 struct FewShared {
-    FewLds<D> part;
+    FewLds<D, F> part;
     SpanLds<F> span;
 };
 template <typename T, int D, bool EXTRA, bool CAP, typename F>
 __device__ void few_rows(const AttendArgs& a, int block, int blocks, FewShared<D, F>& shared) {
-    FewLds<D>& lds = shared.part;
+    FewLds<D, F>& lds = shared.part;
     SpanLds<F>& sp = shared.span;
     const int tid = int(threadIdx.x);
     const int64_t w = block;
     int r0 = 0;
-    int64_t end = load_span(a, 0, 0, sp), total = end;
-    for (int r = 256; r < a.requests; r += 256) total = load_span(a, r, total, sp);
-    const int most = __builtin_amdgcn_readfirstlane(sp.most);
-    if (a.requests > 256) end = load_span(a, 0, 0, sp);            // back to the first
-    // no tile in more than kMaxSplits pieces
-    const int64_t span = max((total + blocks - 1) / blocks, int64_t((most + kMaxSplits - 2) / (kMaxSplits - 1))), x0 = w * span, x1 = min(x0 + span, total);
-    if (x0 >= total) return;                                // no steps at all, or none for this workgroup
-    while (x0 >= end) {
-        r0 += 256;
-        end = load_span(a, r0, end, sp);
+    bool whole = false;
+    int next = block;                                       // whole: the tile to take next
+    if (F::share && a.whole) {
+        int64_t tiles = load_span<F, true>(a, 0, 0, sp);
+        for (int r = 256; r < a.requests; r += 256) tiles = load_span<F, true>(a, r, tiles, sp);
+        if (tid == 0) sp.total = tiles;
+        whole = __builtin_amdgcn_readfirstlane(sp.most) <= kFewWhole;
+        __syncthreads();
     }
-    if (x0 >= sp.start[tid] && x0 < sp.start[tid + 1]) sp.at = tid;
-    __syncthreads();
-    int k = __builtin_amdgcn_readfirstlane(sp.at), steps = steps_of<F>(__builtin_amdgcn_readfirstlane(F::share ? sp.keys[k] - sp.skip[k] : sp.keys[k]));
-    // the first tile and step: ends near a tile's own move to it
-    int unit, s0;
-    {
+    auto span_of = [&](int r, int64_t base) { return F::share && whole ? load_span<F, true>(a, r, base, sp) : load_span<F>(a, r, base, sp); };
+    int64_t end = F::share && whole && a.requests <= 256 ? 0 : span_of(0, 0), total = end;
+    if (!(F::share && whole))
+        for (int r = 256; r < a.requests; r += 256) total = span_of(r, total);
+    const int most = __builtin_amdgcn_readfirstlane(sp.most);
+    if (!(F::share && whole) && a.requests > 256) end = span_of(0, 0);   // back to the first
+    // no tile in more than kMaxSplits pieces
+    const int64_t span = max(max((total + blocks - 1) / blocks, int64_t(F::share && a.phase == 1 ? kFirstSpan : 1)), int64_t((most + kMaxSplits - 2) / (kMaxSplits - 1))), x0 = w * span, x1 = min(x0 + span, total);
+    if (F::share && !whole && tid == 0) { sp.total = total; sp.span = span; }
+    int k = 0, steps = 1, unit = 0, s0 = 0;
+    if (!(F::share && whole)) {
+        if (x0 >= total) return;                            // no steps at all, or none for this workgroup
+        while (x0 >= end) {
+            r0 += 256;
+            end = span_of(r0, end);
+        }
+        if (x0 >= sp.start[tid] && x0 < sp.start[tid + 1]) sp.at = tid;
+        __syncthreads();
+        k = __builtin_amdgcn_readfirstlane(sp.at);
+        steps = steps_of<F>(__builtin_amdgcn_readfirstlane(F::share ? sp.keys[k] - sp.skip[k] : sp.keys[k]));
+        // the first tile and step: ends near a tile's own move to it
         const int64_t local = x0 - uniform(sp.start[k]);
         unit = __builtin_amdgcn_readfirstlane(int(local / steps));
         s0 = __builtin_amdgcn_readfirstlane(int(local - int64_t(unit) * steps));
@@ -1106,12 +1322,25 @@ __device__ void few_rows(const AttendArgs& a, int block, int blocks, FewShared<D
     }
     bool first = true;
     for (;;) {
-        while (unit >= units_of(a, __builtin_amdgcn_readfirstlane(sp.n[k]))) {      // on to the next request that has rows
+        if (F::share && whole) {
+            if (next >= uniform(sp.total)) return;
+            for (int64_t e = uniform(sp.start[256]); next >= e;) {
+                r0 += 256;
+                e = span_of(r0, e);
+            }
+            __syncthreads();                                // the tile before is done with
+            if (next >= sp.start[tid] && next < sp.start[tid + 1]) sp.at = tid;
+            __syncthreads();
+            k = __builtin_amdgcn_readfirstlane(sp.at);
+            unit = __builtin_amdgcn_readfirstlane(int(next - uniform(sp.start[k])));
+            next += blocks;
+        }
+        while (!(F::share && whole) && unit >= units_of(a, __builtin_amdgcn_readfirstlane(sp.n[k]))) {      // on to the next request that has rows
             unit = 0;
             if (r0 + ++k >= a.requests) return;
             if (k < 256) continue;
             r0 += 256;
-            end = load_span(a, r0, end, sp);
+            end = span_of(r0, F::share ? uniform(sp.start[256]) : end);
             k = 0;
         }
         Part it;
@@ -1121,7 +1350,9 @@ __device__ void few_rows(const AttendArgs& a, int block, int blocks, FewShared<D
         it.n = __builtin_amdgcn_readfirstlane(sp.n[k]);
         it.keys = __builtin_amdgcn_readfirstlane(sp.keys[k]);
         steps = steps_of<F>(it.keys - it.skip);
-        const int64_t u0 = uniform(sp.start[k]) + int64_t(unit) * steps, left = x1 - u0;       // the tile's first step; ours of it
+        // the tile's first step; ours of it
+        const int64_t u0 = uniform(sp.start[k]) + int64_t(unit) * steps;
+        const int64_t left = !F::share ? x1 - u0 : whole ? int64_t(steps) : min((w + 1) * uniform(sp.span), uniform(sp.total)) - u0;
         const int low = min(kFewCut, (steps + 1) / 2);
         if (left < low) return;
         const int s1 = left >= steps || steps - left < kFewCut ? steps : int(left);
@@ -1135,7 +1366,8 @@ __device__ void few_rows(const AttendArgs& a, int block, int blocks, FewShared<D
         if (s0 > 0 || s1 < steps) {
             // the cuts of this tile: ends c span with low <= c span - u0 <= steps - kFewCut. The piece before the first is
             // the last of workgroup c - 1, the one after cut c the first of workgroup c.
-            const int64_t c0 = (u0 + low + span - 1) / span, c1 = (u0 + steps - kFewCut) / span;
+            const int64_t length = F::share ? uniform(sp.span) : span;
+            const int64_t c0 = (u0 + low + length - 1) / length, c1 = (u0 + steps - kFewCut) / length;
             it.splits = int(c1 - c0) + 2;
             it.slot0 = int(2 * (c0 - 1) + 1);
             it.slot1 = int(2 * c0);
@@ -1145,7 +1377,8 @@ __device__ void few_rows(const AttendArgs& a, int block, int blocks, FewShared<D
         if (!first) __syncthreads();                        // the LDS of the piece before is done with
         first = false;
         few_part<T, D, EXTRA, CAP, F>(a, uniform_part(it), lds);
-        if (left <= steps) return;
+        if (F::share && whole) continue;
+        if (!F::share && left <= steps) return;             // else the next tile's bounds say so
         s0 = 0;
         ++unit;
     }
@@ -1320,23 +1553,46 @@ __device__ void many_rows(const AttendArgs& a, int block, ManyShared<D>& lds) {
     uint32_t kx[RL];
     float time_raw = 0.0f;
     int32_t eps_raw = 0;
-    const int krow8 = tid / KP, kpiece8 = tid % KP, vrow8 = tid >> 2, vgroup8 = tid & 3;
+    // a thread's place in the tile, found anew for every tile where the registers are short
+    auto thread = [&] { return D == 256 || (EXTRA && D == 128) ? int(here(uint32_t(tid))) : tid; };
+    auto page4 = [&](int u) { return pick4(u, pages[0], pages[1], pages[2], pages[3]); };
     auto fetch = [&](int s) {
-        const int kt = k0 + s * kManyKeys;
-        const uint8_t* const kb = static_cast<const uint8_t*>(a.k_pages);
-        const uint8_t* const vb = static_cast<const uint8_t*>(a.v_pages);
-        auto page4 = [&](int u) { return u & 2 ? (u & 1 ? pages[3] : pages[2]) : (u & 1 ? pages[1] : pages[0]); };
+        const int kt = k0 + s * kManyKeys, th = thread();
+        // where the tile lies in one page the place is the same for every load: a base and a constant offset
+        const int krow8 = th / KP, kpiece8 = th % KP, vrow8 = th >> 2, vgroup8 = th & 3;
+        const uint32_t k_at8 = uint32_t(krow8 * D + kpiece8 * 16), kx_at8 = uint32_t(krow8);
+        const uint32_t v_at8 = uint32_t((vrow8 << a.page_shift) + vgroup8 * 16), vx_at8 = uint32_t(vgroup8 * 16);
+        const char* const kb = static_cast<const char*>(a.k_pages) + (int64_t(head) << a.page_shift) * D;
+        const char* const vb = static_cast<const char*>(a.v_pages) + (int64_t(head) << a.page_shift) * D;
+        const char* const kxb = reinterpret_cast<const char*>(a.k_scales);
+        const char* const vxb = reinterpret_cast<const char*>(a.v_scales);
+        if (a.page_shift >= 6) {                             // the tile lies in one page
+            const int pg = pages[0], off = kt & P1;
+            const int64_t at = ((int64_t(pg) * a.kv_heads + head) << a.page_shift) + off;
+            const char* const kt0 = kb + pg * a.k_stride + int64_t(off) * D;
+            const char* const vt0 = vb + pg * a.v_stride + off;
 #pragma unroll
-        for (int j = 0; j < RL; ++j) {
-            const int w = krow8 + j * (256 / KP), pg = page4(w >> 4), off = (kt + w) & P1;
-            kr[j] = *reinterpret_cast<const u32x4*>(kb + pg * a.k_stride + ((int64_t(head) << a.page_shift) + off) * D + kpiece8 * 16);
-            kx[j] = a.k_scales[((int64_t(pg) * a.kv_heads + head) << a.page_shift) + off];
+            for (int j = 0; j < RL; ++j) {
+                kr[j] = *reinterpret_cast<const u32x4*>(kt0 + (k_at8 + j * (256 * 16)));
+                kx[j] = *reinterpret_cast<const uint8_t*>(kxb + at + (kx_at8 + j * (256 / KP)));
+            }
+#pragma unroll
+            for (int j = 0; j < RL; ++j) {
+                vr[j] = *reinterpret_cast<const u32x4*>(vt0 + (int64_t(j) * 64 << a.page_shift) + v_at8);
+            }
+            vx = *reinterpret_cast<const u32x4*>(vxb + at + vx_at8);
+        } else {
+#pragma unroll
+            for (int j = 0; j < RL; ++j) {
+                const int w = krow8 + j * (256 / KP), pg = page4(w >> 4), off = (kt + w) & P1;
+                kr[j] = *reinterpret_cast<const u32x4*>(kb + pg * a.k_stride + int64_t(off) * D + kpiece8 * 16);
+                kx[j] = *reinterpret_cast<const uint8_t*>(kxb + ((int64_t(pg) * a.kv_heads + head) << a.page_shift) + off);
+            }
+            const int pg = page4(vgroup8), off = (kt + vgroup8 * 16) & P1;
+#pragma unroll
+            for (int j = 0; j < RL; ++j) vr[j] = *reinterpret_cast<const u32x4*>(vb + pg * a.v_stride + (int64_t(vrow8 + j * 64) << a.page_shift) + off);
+            vx = *reinterpret_cast<const u32x4*>(vxb + ((int64_t(pg) * a.kv_heads + head) << a.page_shift) + off);
         }
-        const int pg = page4(vgroup8), off = (kt + vgroup8 * 16) & P1;
-#pragma unroll
-        for (int j = 0; j < RL; ++j)
-            vr[j] = *reinterpret_cast<const u32x4*>(vb + pg * a.v_stride + ((int64_t(head) * D + vrow8 + j * 64) << a.page_shift) + off);
-        vx = *reinterpret_cast<const u32x4*>(a.v_scales + ((int64_t(pg) * a.kv_heads + head) << a.page_shift) + off);
         if constexpr (EXTRA) {
             if (wave == 0) {
                 const int64_t slot = (int64_t(page4(lane >> 4)) << a.page_shift) + ((kt + lane) & P1);
@@ -1348,36 +1604,34 @@ __device__ void many_rows(const AttendArgs& a, int block, ManyShared<D>& lds) {
     bool dirty = false;                                      // a value that is not finite was left out
     // The tile of step s, fetched before, into buffer buf. Where some row of the workgroup does not see some key: see add_not_finite;
     // slots past the request's keys hold anything and become 0.
-    auto put = [&](int s, bool mixed, int buf) {
-        const int kt = k0 + s * kManyKeys;
-        if (kt + kManyKeys > first_limit || mixed) {
-            const int left = keys - (kt + vgroup8 * 16);
+    auto put_as = [&](auto look, int kt, int buf) {
+        const int th = thread(), krow8 = th / KP, kpiece8 = th % KP, vrow8 = th >> 2, vgroup8 = th & 3, left = keys - (kt + vgroup8 * 16);
+        if (look && left < 16) {
+            vx = first_bytes(vx, left);
 #pragma unroll
-            for (int j = 0; j < RL; ++j) {
-                if (left < 16) vr[j] = first_bytes(vr[j], left);
-                const bool full = (nan_e4m3(vr[j][0]) | nan_e4m3(vr[j][1]) | nan_e4m3(vr[j][2]) | nan_e4m3(vr[j][3])) != 0;
-                dirty |= full;
-                if (full) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) vr[j][e] = finite_e4m3(vr[j][e]);
-                }
-            }
+            for (int j = 0; j < RL; ++j) vr[j] = first_bytes(vr[j], left);
         }
 #pragma unroll
         for (int j = 0; j < RL; ++j) {
             const int w = krow8 + j * (256 / KP);
-            const float ks = power_of(kx[j]);
+            const float ks = scale_at<0>(kx[j]);
 #pragma unroll
             for (int u = 0; u < 2; ++u) sh.k[buf][w * RC + ((2 * kpiece8 + u) ^ kswz(w))] = token_e4m3<T>(kr[j][2 * u], kr[j][2 * u + 1], ks);
         }
         float vs[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) vs[e] = power_of(byte_of(vx[e >> 2], e & 3));
+        scales16(vx, vs);
 #pragma unroll
         for (int j = 0; j < RL; ++j) {
             const int w = vrow8 + j * 64;
 #pragma unroll
-            for (int u = 0; u < 2; ++u) sh.v[buf][w * 8 + ((2 * vgroup8 + u) ^ vswz(w))] = element_e4m3<T>(vr[j][2 * u], vr[j][2 * u + 1], vs + 8 * u);
+            for (int u = 0; u < 2; ++u) {
+                u32x4 b = element_e4m3<T>(vr[j][2 * u], vr[j][2 * u + 1], vs + 8 * u);
+                if constexpr (look) {
+                    dirty |= exponents_full<T>(b) != 0;
+                    b = finite_part<T>(b);
+                }
+                sh.v[buf][w * 8 + ((2 * vgroup8 + u) ^ vswz(w))] = b;
+            }
         }
         if constexpr (EXTRA) {
             if (wave == 0) {
@@ -1385,6 +1639,11 @@ __device__ void many_rows(const AttendArgs& a, int block, ManyShared<D>& lds) {
                 sh.eps[buf][lane] = eps_raw;
             }
         }
+    };
+    auto put = [&](int s, bool mixed, int buf) {
+        const int kt = k0 + s * kManyKeys;
+        if (kt + kManyKeys > first_limit || mixed) put_as(std::true_type{}, kt, buf);
+        else put_as(std::false_type{}, kt, buf);
     };
 
     f32x16 o[DB];
@@ -1609,6 +1868,7 @@ __device__ void many_rows(const AttendArgs& a, int block, ManyShared<D>& lds) {
                 for (int g = 0; g < 4; ++g)
                     *reinterpret_cast<f32x4*>(a.state_o + at * D + d * 32 + g * 8 + h * 4) = f32x4{o[d][g * 4], o[d][g * 4 + 1], o[d][g * 4 + 2], o[d][g * 4 + 3]};
             if (h == 0) a.state_ml[at] = make_float2(empty ? -kInf : mref, l);
+            if (h == 0) a.state_at[at] = one_piece(a, at);
         }
     } else if (it.splits == 1 && row_ok) {
         const float inv = empty ? 0.0f : 1.0f / l;
@@ -1633,6 +1893,10 @@ __device__ void many_rows(const AttendArgs& a, int block, ManyShared<D>& lds) {
             for (int g = 0; g < 4; ++g)
                 *reinterpret_cast<f32x4*>(po + d * 32 + g * 8) = f32x4{o[d][g * 4], o[d][g * 4 + 1], o[d][g * 4 + 2], o[d][g * 4 + 3]};
         if (h == 0) a.many_ml[at] = make_float2(empty ? -kInf : mref, l);
+        if (F::share && a.phase == 1 && a.defer && h == 0 && it.slot == it.slot0) {
+            const int32_t from = int32_t(a.many_row0 + at);
+            a.state_at[state_row(a, row, hq)] = i32x4{from, from + kManyRows, kManyRows, it.splits};
+        }
     }
     __syncthreads();                                         // the LDS of the tiles is free, the rows are written
     if (tid == 0) lds.any_dirty = 0;
@@ -1654,7 +1918,8 @@ __global__ __launch_bounds__(256) void k_attend_join(AttendArgs a) {
     if (!sched.start()) return;
     Part it;
     for (uint32_t block = blockIdx.x; sched.find(block, &it); block += gridDim.x) {
-        const int r0 = it.slot * kJoinRows, rows = min(kJoinRows, it.n * a.group - it.tile * kManyRows - r0);
+        const int jr = join_rows_of<F>(a);
+        const int r0 = it.slot * jr, rows = min(jr, it.n * a.group - it.tile * kManyRows - r0);
         if (!own_pieces<F>(a, &it, 0) || it.splits == 1) continue;
         const float2* const ml = a.many_ml + int64_t(it.slot0) * kManyRows + r0;
         const float* const po = a.many_o + (int64_t(it.slot0) * kManyRows + r0) * D;
@@ -1703,16 +1968,13 @@ __global__ __launch_bounds__(256) void k_attend_join(AttendArgs a) {
 }
 
 // ---- the kernels ------------------------------------------------------------------------
-// Waves a SIMD of the kernels of few rows, as their registers allow.
-template <int D, typename F>
-constexpr int few_waves() { return D > 128 ? 1 : D == 128 ? 2 : F::c8 ? 2 : 3; }
-
 template <typename T, int D, bool EXTRA, bool CAP, typename F>
 __global__ __launch_bounds__(256, (few_waves<D, F>())) void k_attend_few(AttendArgs a) {
     __shared__ __attribute__((aligned(16))) FewShared<D, F> lds;
     int blocks = int(gridDim.x);
     if (F::share && a.phase == 1 && int(blockIdx.x) == --blocks) {
-        find_skips(a);
+        static_assert(sizeof(lds) >= (kMaxRequests + 1) * sizeof(int32_t), "room for the starts");
+        find_skips(a, reinterpret_cast<int32_t*>(&lds));
         return;
     }
     few_rows<T, D, EXTRA, CAP, F>(a, int(blockIdx.x), blocks, lds);
@@ -1722,7 +1984,8 @@ template <typename T, int D, bool EXTRA, bool CAP, typename F>
 __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void k_attend_many(AttendArgs a) {
     __shared__ __attribute__((aligned(16))) ManyShared<D> lds;
     if (F::share && a.phase == 1 && blockIdx.x + 1 == gridDim.x) {
-        find_skips(a);
+        static_assert(sizeof(lds) >= (kMaxRequests + 1) * sizeof(int32_t), "room for the starts");
+        find_skips(a, reinterpret_cast<int32_t*>(&lds));
         return;
     }
     many_rows<T, D, EXTRA, CAP, F>(a, int(blockIdx.x), lds);
@@ -1737,34 +2000,49 @@ int launch_dim(AttendArgs a, int32_t max_new, hipStream_t s) {
     const int64_t rows = int64_t(a.tokens) * a.group, keys = int64_t(a.max_pages) << a.page_shift;
     const int64_t most = std::min<int64_t>(max_new > 0 ? max_new : a.tokens, a.tokens) * a.group;
     const bool first = F::share && a.phase == 1;
-    const bool few_only = first ? rows <= int64_t(kFewMost) * a.requests : most <= kFewMost;
+    const bool few_only = first ? rows <= int64_t(kFewMost) * a.requests : F::share && a.phase == 2 ? a.defer != 0 : most <= kFewMost;
     const bool many_only = !few_only && (first || a.requests == 1);
     a.few_rows = few_only ? INT32_MAX : many_only ? -1 : kFewMost;
     // few: one workgroup for each that the CUs hold at a time, fewer where there are not so many steps
     const int64_t few_tiles = few_only ? rows / kFewRows + std::min(a.requests, a.tokens) : std::min(a.requests, a.tokens);
     const int64_t few = std::min<int64_t>(few_tiles * a.kv_heads * ((keys + few_step<F>() - 1) / few_step<F>()), 256 * few_waves<D, F>());
+    // no more tiles than workgroups: by the bound on the new tokens, since the rows of each request are not known here
+    const int64_t each = (std::min<int64_t>(max_new > 0 ? max_new : a.tokens, a.tokens) * a.group + kFewRows - 1) / kFewRows;
+    a.whole = !first && few_only && std::min<int64_t>(few_tiles, each * std::min(a.requests, a.tokens)) * a.kv_heads <= 256 * few_waves<D, F>();
     if (!many_only) MARS_LAUNCH((k_attend_few<T, D, EXTRA, CAP, F>), dim3(unsigned(few + first)), dim3(256), 0, s, a);
     if (few_only) return MARS_OK;
     // many: no more than chunks of kMinChunk or more of the tiles' keys, or 2^kManyItemsLog2 chunks and one for each tile
     const int64_t tiles = rows / kManyRows + std::min<int64_t>(a.requests, first ? a.tokens : rows / (kFewMost + 1));
     const int64_t many = std::min(tiles * a.kv_heads * ((keys + kMinChunk - 1) / kMinChunk), (int64_t(1) << kManyItemsLog2) + tiles * a.kv_heads);
     MARS_CHECK(many < INT32_MAX, MARS_ERR_CAPACITY, "%lld tiles of rows", (long long)tiles);
+    a.join_rows = tiles * a.kv_heads * (kManyRows / kJoinRows) < 1024 ? 1024 / D : kJoinRows;
     MARS_LAUNCH((k_attend_many<T, D, EXTRA, CAP, F>), dim3(unsigned(many + first)), dim3(256), 0, s, a);
-    // no tile is in pieces where a row of the table is one chunk
-    if (keys > kMinChunk) {
-        const int64_t blocks = std::min<int64_t>(tiles * a.kv_heads * (kManyRows / kJoinRows), 1024);
+    // no tile is in pieces where a row of the table is one chunk. Rows a workgroup of the join, 16 or 1024 / D: 256 rows under 8 heads over
+    // 32,768 keys 17.0 and 12.3 us, two chunks of 511 tokens among 22 single ones 13.4 and 17.8.
+    if (keys > kMinChunk && !(first && a.defer)) {
+        const int64_t blocks = std::min<int64_t>(tiles * a.kv_heads * (kManyRows / join_rows_of<F>(a)), a.join_rows < kJoinRows ? 2048 : 1024);
         MARS_LAUNCH((k_attend_join<T, D, F>), dim3(unsigned(blocks)), dim3(256), 0, s, a);
     }
     return MARS_OK;
 }
 
-// With a.group_start: the groups over their prefixes, then every request from behind them on.
+// With a.group_start: the groups over their prefixes, then every request from behind them on. Requests of up to shared_few_most() rows
+// are then k_attend_few's, which reads their own keys once for every 16 rows, and which joins the pieces of the prefix's sums itself
+// as it begins; with more rows three launches take what is one here. 32 requests of 20, 40 and 64 rows behind 6,016 shared keys (32/8
+// heads of 128): over some 45 of their own 59, 76, 102 us (67, 88, 109 with three launches), over 675 86, 112, 143 (89, 111, 133), over
+// 3,000 187, 267, 329 (184, 214, 235); in 8 bits 74, 92, 123 (92, 115, 140), 88, 118, 152 (110, 135, 158), 148, 192, 242 (190, 219, 239).
+template <typename F>
+constexpr int shared_few_most() { return F::c8 ? 64 : 48; }
 template <typename T, int D, bool EXTRA, bool CAP, typename F>
 int launch_phases(AttendArgs a, int32_t max_new, hipStream_t s) {
     if constexpr (F::share) {
         if (a.group_start) {
+            const int64_t most = std::min<int64_t>(max_new > 0 ? max_new : a.tokens, a.tokens) * a.group;
+            a.defer = most <= shared_few_most<F>();
             AttendArgs first = a;
             first.phase = 1;
+            first.part_o = a.many_o;                         // k_attend_few's pieces of the one phase are read while it writes those of the other
+            first.part_ml = a.many_ml;
             first.members = a.requests;
             first.requests = a.groups;
             MARS_TRY((launch_dim<T, D, EXTRA, CAP, F>(first, 0, s)));

@@ -577,9 +577,14 @@ int attend(const mars_reader* r, const C* c, const mars_kv_attend_args* s, const
     a.page_shift = r->page_shift;
     MARS_TRY(use_device(r->device));
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    if (shared && int64_t(s->num_tokens) * d.q_heads <= kStateRows) {
+    const int64_t all = int64_t(s->num_requests) * s->max_pages * d.page_size * d.kv_heads * d.head_dim * (k.k_scales ? 2 : 4);
+    if (shared && int64_t(s->num_tokens) * d.q_heads <= kStateRows && all >= kSharedBytes) {
         a.group_start = shared->group_start; a.shared_lens = shared->shared_lens; a.groups = shared->num_groups;
-        a.skips = r->skips; a.state_o = r->state_o; a.state_ml = r->state_ml;
+        a.skips = r->skips; a.state_at = r->state_at;
+        a.many_row0 = int64_t(r->few_slots) * kFewRows;
+        a.state_row0 = a.many_row0 + (int64_t(2) << kManyItemsLog2) * kManyRows;
+        a.state_o = r->part_o + a.state_row0 * d.head_dim;
+        a.state_ml = r->part_ml + a.state_row0;
     }
     if (a.k_scales) return launch_attend8(*r, a, s->max_new, st);
     return a.group_start ? launch_attend_shared(*r, a, s->max_new, st) : launch_attend(*r, a, s->max_new, st);
@@ -636,14 +641,14 @@ int mars_reader_create(const mars_reader_desc* d, mars_reader** out) try {
             MARS_HIP(hipMemcpy(r->axis, axis.data(), size_t(half) * sizeof(int32_t), hipMemcpyHostToDevice));
         }
         r->few_slots = size_t(2) * few_groups(d->head_dim);
-        const size_t rows = r->few_slots * kFewRows + (size_t(2) << kManyItemsLog2) * kManyRows;
+        const size_t rows = r->few_slots * kFewRows + (size_t(2) << kManyItemsLog2) * kManyRows + size_t(kStateRows);
         MARS_TRY(dmalloc(&r->part_o, rows * size_t(d->head_dim)));
         MARS_TRY(dmalloc(&r->part_ml, rows));
         MARS_TRY(dmalloc(&r->arrived, r->few_slots));
         MARS_HIP(hipMemset(r->arrived, 0, r->few_slots * sizeof(uint32_t)));
-        MARS_TRY(dmalloc(&r->state_o, size_t(kStateRows) * size_t(d->head_dim)));
-        MARS_TRY(dmalloc(&r->state_ml, size_t(kStateRows)));
+        MARS_TRY(dmalloc(&r->state_at, size_t(kStateRows)));
         MARS_TRY(dmalloc(&r->skips, size_t(kMaxRequests)));
+        MARS_HIP(hipMemset(r->state_at, 0, size_t(kStateRows) * sizeof(i32x4)));     // no pieces
         MARS_HIP(hipDeviceSynchronize());
         return MARS_OK;
     }();
@@ -661,7 +666,7 @@ int mars_reader_destroy(mars_reader* r) {
     if (!r) return MARS_OK;
     (void)use_device(r->device);
     dfree(r->freq); dfree(r->axis); dfree(r->part_o); dfree(r->part_ml); dfree(r->arrived);
-    dfree(r->state_o); dfree(r->state_ml); dfree(r->skips);
+    dfree(r->state_at); dfree(r->skips);
     delete r;
     return MARS_OK;
 }

@@ -6,6 +6,10 @@
 
 #include "internal.hpp"
 
+namespace mars {
+typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
+}
+
 struct mars_reader {
     mars_reader_desc d{};
     int32_t device = 0;
@@ -19,9 +23,9 @@ struct mars_reader {
     float* part_o = nullptr;
     float2* part_ml = nullptr;
     uint32_t* arrived = nullptr;
-    // Attention with shared prefixes: the sums of the first phase (kStateRows rows and query heads) and every request's skip.
-    float* state_o = nullptr;
-    float2* state_ml = nullptr;
+    // Attention with shared prefixes: behind those the sums of the first phase (kStateRows rows and query heads), where their
+    // pieces lie, and every request's skip.
+    mars::i32x4* state_at = nullptr;
     int32_t* skips = nullptr;
 };
 
@@ -47,6 +51,12 @@ constexpr int32_t kMaxSplits = 256;          // pieces of a tile, as many as a j
 // Rows times query heads whose sums the first phase of attention with shared prefixes can keep; calls with more read each
 // request's own prefix.
 constexpr int64_t kStateRows = 1 << 15;
+// Nor does a shared prefix pay where all that the tables' rows can name is not more than this: two phases cost some 13 us more than
+// one, and pages that several requests read come from the caches at about 9 TB/s. us with groups and without, 32/8 heads of 128 in
+// 16 bits (8 bits), one token each: 4 requests over 4,160 shared tokens, 70 MB, 33 and 24 (30 and 26); 16 over 1,000, 74 MB, 28 and 25;
+// 8 over 4,160, 140 MB, 35 and 28; 64 over 1,000, 297 MB, 32 and 48 (149 MB: 32 and 29); 16 over 4,160, 280 MB, 31 and 50 (141 MB: 29 and
+// 38); 4 over 20,000, 330 MB, 43 and 55 (166 MB: 38 and 40); 64 over 32,768 107 and 937 (91 and 496).
+constexpr int64_t kSharedBytes = 128 << 20;
 
 struct AttendArgs {
     const void* q;
@@ -84,9 +94,13 @@ struct AttendArgs {
     const int32_t* group_start;
     const int32_t* shared_lens;
     int32_t* skips;
-    float* state_o;             // sums of phase 1, a row and query head each, and their (reference, sum of weights)
+    float* state_o;             // sums of phase 1, a row and query head each, and their (reference, sum of weights): behind many_o, many_ml
     float2* state_ml;
-    int32_t groups, members, phase;
+    i32x4* state_at;            // with defer, where phase 2 finds a row's pieces: row of part_o of the first, the second, rows between the next, how many
+    int64_t many_row0, state_row0;   // rows of part_o before many_o and state_o
+    int32_t groups, members, phase, defer;
+    int32_t join_rows;          // of a tile, by a workgroup of k_attend_join
+    int32_t whole;              // there are no more tiles than workgroups of k_attend_few
 };
 
 struct StoreArgs {

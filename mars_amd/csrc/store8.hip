@@ -4,9 +4,10 @@
 //
 //  A head of a token is D elements x. Its exponent k is the least integer with max |x| <= 448 2^k over the finite x (448 is
 //  e4m3's largest value), but at least that of the reader's type: -15 (float16), -117 (bfloat16), so that 2^(k - 9), the least
-//  value that can be held, is one of that type's. Held: e4m3(x 2^-k), rounded once to nearest even, and the byte k + 127. The scaling is exact,
-//  powers of two lose nothing, and one scale a token and head keeps each token's precision whatever its neighbours are:
-//  the values keep e4m3's own relative precision of 2^-4 down to 2^-15 of the head's largest.
+//  value that can be held, is one of that type's. Held: e4m3(x 2^-k), rounded once to nearest even, and the byte k + 127.
+//  Finite elements beyond 61440 (or 240 2^120), the largest held values that the type has too, become that. The scaling is
+//  exact, powers of two lose nothing, and one scale a token and head keeps each token's precision whatever its
+//  neighbours are: the values keep e4m3's own relative precision of 2^-4 down to 2^-15 of the head's largest.
 // ============================================================================
 #include "reader.hpp"
 
@@ -21,6 +22,12 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 template <typename T>
 constexpr int least_exponent() { return __is_same(T, _Float16) ? -15 : -117; }
 
+// x, or where it is finite and larger than what can be held as a finite T, that.
+template <typename T>
+__device__ inline float holdable(float x) {
+    constexpr float most = __is_same(T, _Float16) ? 61440.0f : 240.0f * 0x1p120f;
+    return fabsf(x) < __builtin_inff() ? fminf(fmaxf(x, -most), most) : x;
+}
 __device__ inline float finite_size(float x) {
     const float m = fabsf(x);
     return m < __builtin_inff() ? m : 0.0f;
@@ -43,10 +50,20 @@ __device__ inline uint32_t to_e4m3(uint32_t word, float x, float y, float inv) {
     return uint32_t(__builtin_amdgcn_cvt_pk_fp8_f32(x, y, int(word), HI));
 }
 
+// The largest of N neighbouring lanes (from a multiple of N on), in each of them. Up to 16 within a row of lanes: the neighbour, the other
+// pair of four, then mirrored halves, whose lanes agree by then.
+template <int CTRL>
+__device__ inline float max_dpp(float x) {
+    return fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xF, 0xF, true)));
+}
 template <int N>
 __device__ inline float max_over(float x) {
-#pragma unroll
-    for (int o = 1; o < N; o <<= 1) x = fmaxf(x, __shfl_xor(x, o));
+    if constexpr (N > 1) x = max_dpp<0xB1>(x);
+    if constexpr (N > 2) x = max_dpp<0x4E>(x);
+    if constexpr (N > 4) x = max_dpp<0x141>(x);
+    if constexpr (N > 8) x = max_dpp<0x140>(x);
+    if constexpr (N > 16) x = fmaxf(x, __shfl_xor(x, 16));
+    if constexpr (N > 32) x = fmaxf(x, __shfl_xor(x, 32));
     return x;
 }
 
@@ -83,7 +100,7 @@ __global__ __launch_bounds__(256) void k_kv_store8(StoreArgs a) {
         const T* const v = static_cast<const T*>(a.s.v) + t * a.s.v_stride + h * D;
         float w[N];
 #pragma unroll
-        for (int u = 0; u < N; ++u) w[u] = float(v[lane + 64 * u]);
+        for (int u = 0; u < N; ++u) w[u] = holdable<T>(float(v[lane + 64 * u]));
         constexpr int NP = (N + 1) / 2;
         float lo[NP], hi[NP], top = 0.0f;
         int i0[NP], i1[NP];
@@ -94,8 +111,8 @@ __global__ __launch_bounds__(256) void k_kv_store8(StoreArgs a) {
             i0[u] = turns && !a.adjacent ? j : 2 * j;
             i1[u] = turns && !a.adjacent ? j + half : 2 * j + 1;
             const float y = float(k[i0[u]]), z = float(k[i1[u]]);
-            lo[u] = turns ? y * cs[j] - z * sn[j] : y;
-            hi[u] = turns ? y * sn[j] + z * cs[j] : z;
+            lo[u] = holdable<T>(turns ? y * cs[j] - z * sn[j] : y);
+            hi[u] = holdable<T>(turns ? y * sn[j] + z * cs[j] : z);
             top = fmaxf(top, fmaxf(finite_size(lo[u]), finite_size(hi[u])));
         }
         const uint32_t ek = exponent_for<T>(max_over<64>(top));
@@ -128,7 +145,7 @@ __global__ __launch_bounds__(256) void k_kv_store8(StoreArgs a) {
 // (k, pieces of 16) or D / 8 (v) neighbouring lanes, which find its largest between them; v goes through LDS as bytes, and a
 // thread that has 4 elements of 8 tokens turns them with byte permutations into 8 bytes a row of the page.
 template <int D>
-constexpr int store8_tile() { return D == 256 ? 32 : 64; }
+constexpr int store8_tile() { return D == 256 ? 16 : D == 128 ? 32 : 64; }
 
 // 4 x 4 bytes: word j of `in` holds 4 elements of token j; word e of the result element e of 4 tokens.
 __device__ inline u32x4 turned4(u32x4 in) {
@@ -159,34 +176,40 @@ __global__ __launch_bounds__(256) void k_kv_store8_tile(StoreArgs a) {
         const int64_t s = k && tid < nt ? a.s.slots[t0 + tid] : -1;
         slot_of[tid] = s >= 0 && s < a.slots ? s : -1;
     }
-    // everything the workgroup reads is on the way before the angles are computed: its v, and of q and k the first pieces
-    constexpr int VU = kTile * (D / 8) / 256;
-    v8 vr[VU];
-    if (v) {
+    // everything the workgroup reads is on the way before the angles are computed: its v and k, and of q the first pieces.
+    // q and k: two pieces of 8 elements of a head a thread, the partners of each other where they turn (both are read
+    // before either is written: q_out may be q)
+    constexpr int VU = kTile * (D / 8) / 256, KU = kTile * (D / 16) / 256, U = 4;
+    const int turning = half / 8, pairs = nt * group * (D / 16);
+    auto first_of = [&](int c) { return c < turning && !a.adjacent ? c * 8 : c * 16; };
+    auto second_of = [&](int c) { return c < turning && !a.adjacent ? half + c * 8 : c * 16 + 8; };
+    v8 vr[VU], ky[KU], kz[KU], y[U], z[U];
+    if (k) {
+#pragma unroll
+        for (int u = 0; u < KU; ++u) {
+            const int e = tid + u * 256, i = e / (D / 16), c = e % (D / 16);
+            if (i >= nt) break;
+            const T* const x = k + (t0 + i) * a.s.k_stride + head * D;
+            ky[u] = *reinterpret_cast<const v8*>(x + first_of(c));
+            kz[u] = *reinterpret_cast<const v8*>(x + second_of(c));
+        }
 #pragma unroll
         for (int u = 0; u < VU; ++u) {
             const int e = tid + u * 256, i = e / (D / 8), c = e % (D / 8);
             if (i < nt) vr[u] = *reinterpret_cast<const v8*>(v + (t0 + i) * a.s.v_stride + head * D + c * 8);
         }
     }
-    // q and k: two pieces of 8 elements of a head a thread, the partners of each other where they turn (both are read
-    // before either is written: q_out may be q), and four such pairs on the way together
-    constexpr int U = 4;
-    const int heads = group + (k ? 1 : 0), turning = half / 8, pairs = nt * heads * (D / 16);
-    v8 y[U], z[U];
-    auto first_of = [&](int c) { return c < turning && !a.adjacent ? c * 8 : c * 16; };
-    auto second_of = [&](int c) { return c < turning && !a.adjacent ? half + c * 8 : c * 16 + 8; };
     auto read_pairs = [&](int e0) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int e = e0 + u * 256, c = e % (D / 16), ih = e / (D / 16), i = ih / heads, hh = ih % heads;
+            const int e = e0 + u * 256, c = e % (D / 16), ih = e / (D / 16), i = ih / group, hh = ih % group;
             if (e >= pairs) break;
-            const T* const x = hh < group ? q + (t0 + i) * a.s.q_stride + (head * group + hh) * D : k + (t0 + i) * a.s.k_stride + head * D;
+            const T* const x = q + (t0 + i) * a.s.q_stride + (head * group + hh) * D;
             y[u] = *reinterpret_cast<const v8*>(x + first_of(c));
             z[u] = *reinterpret_cast<const v8*>(x + second_of(c));
         }
     };
-    read_pairs(tid);
+    if (q) read_pairs(tid);
     for (int e = tid; e < nt * half; e += 256) {
         const int i = e / half, f = e % half;
         float sn, cs;
@@ -194,30 +217,77 @@ __global__ __launch_bounds__(256) void k_kv_store8_tile(StoreArgs a) {
         turns[i][f] = make_float2(cs, a.s.inverse ? -sn : sn);
     }
     __syncthreads();
-    if (v) {
+    // both pieces of a pair turned, in fp32
+    auto turned = [&](int i, int c, v8 yy, v8 zz, float (&u)[8], float (&w)[8]) {
 #pragma unroll
-        for (int u = 0; u < VU; ++u) {
-            const int e = tid + u * 256, i = e / (D / 8), c = e % (D / 8);
+        for (int j = 0; j < 8; ++j) { u[j] = float(yy[j]); w[j] = float(zz[j]); }
+        if (c < turning && !a.adjacent) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float2 f = turns[i][c * 8 + j];
+                const float p = u[j], r = w[j];
+                u[j] = p * f.x - r * f.y;
+                w[j] = p * f.y + r * f.x;
+            }
+        } else if (c < turning) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float2 f = turns[i][c * 8 + j], g = turns[i][c * 8 + 4 + j];          // pairs j and 4 + j of the 16 elements
+                const float ya = u[2 * j], yb = u[2 * j + 1], za = w[2 * j], zb = w[2 * j + 1];
+                u[2 * j] = ya * f.x - yb * f.y;
+                u[2 * j + 1] = ya * f.y + yb * f.x;
+                w[2 * j] = za * g.x - zb * g.y;
+                w[2 * j + 1] = za * g.y + zb * g.x;
+            }
+        }
+    };
+    if (k) {
+        auto eight = [](const float (&x)[8], float inv) {
+            return u32x2{to_e4m3<true>(to_e4m3<false>(0, x[0], x[1], inv), x[2], x[3], inv), to_e4m3<true>(to_e4m3<false>(0, x[4], x[5], inv), x[6], x[7], inv)};
+        };
+#pragma unroll
+        for (int n = 0; n < VU; ++n) {
+            const int e = tid + n * 256, i = e / (D / 8), c = e % (D / 8);
             if (i >= nt) break;                              // a token's lanes go together
             float x[8], top = 0.0f;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                x[j] = float(vr[u][j]);
+                x[j] = holdable<T>(float(vr[n][j]));
                 top = fmaxf(top, finite_size(x[j]));
             }
             const uint32_t ev = exponent_for<T>(max_over<D / 8>(top));
-            const float inv = inverse_power(ev);
-            vt[i][c * 2] = to_e4m3<true>(to_e4m3<false>(0, x[0], x[1], inv), x[2], x[3], inv);
-            vt[i][c * 2 + 1] = to_e4m3<true>(to_e4m3<false>(0, x[4], x[5], inv), x[6], x[7], inv);
+            const u32x2 b = eight(x, inverse_power(ev));
+            vt[i][c * 2] = b[0];
+            vt[i][c * 2 + 1] = b[1];
             const int64_t s = slot_of[i];
             if (c == 0 && s >= 0) a.v_scales[((s >> a.page_shift) * a.kv_heads + head) * P + (s & (P - 1))] = uint8_t(ev);
         }
-    }
-    if (k && tid < kTile) {
-        const int64_t s = slot_of[tid];
-        bool first = s >= 0 && s % 8 == 0 && tid + 8 <= nt;
-        for (int j = 1; j < 8 && first; ++j) first = slot_of[tid + j] == s + j;
-        lead[tid] = first;
+#pragma unroll
+        for (int n = 0; n < KU; ++n) {
+            const int e = tid + n * 256, i = e / (D / 16), c = e % (D / 16);
+            if (i >= nt) break;                              // as above
+            float u[8], w[8], top = 0.0f;
+            turned(i, c, ky[n], kz[n], u, w);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                u[j] = holdable<T>(u[j]);
+                w[j] = holdable<T>(w[j]);
+                top = fmaxf(top, fmaxf(finite_size(u[j]), finite_size(w[j])));
+            }
+            const uint32_t ek = exponent_for<T>(max_over<D / 16>(top));
+            if (slot_of[i] < 0) continue;
+            const int64_t page = slot_of[i] >> a.page_shift, off = slot_of[i] & (P - 1);
+            uint8_t* const to = static_cast<uint8_t*>(a.k_pages) + page * a.k_stride + (int64_t(head) * P + off) * D;
+            *reinterpret_cast<u32x2*>(to + first_of(c)) = eight(u, inverse_power(ek));
+            *reinterpret_cast<u32x2*>(to + second_of(c)) = eight(w, inverse_power(ek));
+            if (c == 0) a.k_scales[(page * a.kv_heads + head) * P + off] = uint8_t(ek);
+        }
+        if (tid < kTile) {
+            const int64_t s = slot_of[tid];
+            bool first = s >= 0 && s % 8 == 0 && tid + 8 <= nt;
+            for (int j = 1; j < 8 && first; ++j) first = slot_of[tid + j] == s + j;
+            lead[tid] = first;
+        }
     }
     __syncthreads();
     if (k && tid < 64) {                                     // one wave: the groups, and the tokens of none
@@ -238,53 +308,18 @@ __global__ __launch_bounds__(256) void k_kv_store8_tile(StoreArgs a) {
         if (e0 != tid) read_pairs(e0);
 #pragma unroll
         for (int n = 0; n < U; ++n) {
-            const int e = e0 + n * 256, c = e % (D / 16), ih = e / (D / 16), i = ih / heads, hh = ih % heads;
-            if (e >= pairs) break;                           // a head's lanes go together
-            float u[8], w[8];
+            const int e = e0 + n * 256, c = e % (D / 16), ih = e / (D / 16), i = ih / group, hh = ih % group;
+            if (e >= pairs) break;
+            T* const to = static_cast<T*>(a.s.q_out) + (t0 + i) * a.s.q_out_stride + (head * group + hh) * D;
+            v8 lo = y[n], hi = z[n];
+            if (c < turning) {
+                float u[8], w[8];
+                turned(i, c, lo, hi, u, w);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) { u[j] = float(y[n][j]); w[j] = float(z[n][j]); }
-            if (c < turning && !a.adjacent) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float2 f = turns[i][c * 8 + j];
-                    const float yy = u[j], zz = w[j];
-                    u[j] = yy * f.x - zz * f.y;
-                    w[j] = yy * f.y + zz * f.x;
-                }
-            } else if (c < turning) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float2 f = turns[i][c * 8 + j], g = turns[i][c * 8 + 4 + j];      // pairs j and 4 + j of the 16 elements
-                    const float ya = u[2 * j], yb = u[2 * j + 1], za = w[2 * j], zb = w[2 * j + 1];
-                    u[2 * j] = ya * f.x - yb * f.y;
-                    u[2 * j + 1] = ya * f.y + yb * f.x;
-                    w[2 * j] = za * g.x - zb * g.y;
-                    w[2 * j + 1] = za * g.y + zb * g.x;
-                }
+                for (int j = 0; j < 8; ++j) { lo[j] = T(u[j]); hi[j] = T(w[j]); }
             }
-            float top = 0.0f;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) top = fmaxf(top, fmaxf(finite_size(u[j]), finite_size(w[j])));
-            const uint32_t ek = exponent_for<T>(max_over<D / 16>(top));
-            if (hh < group) {
-                T* const to = static_cast<T*>(a.s.q_out) + (t0 + i) * a.s.q_out_stride + (head * group + hh) * D;
-                v8 lo = y[n], hi = z[n];
-                if (c < turning) {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) { lo[j] = T(u[j]); hi[j] = T(w[j]); }
-                }
-                *reinterpret_cast<v8*>(to + first_of(c)) = lo;
-                *reinterpret_cast<v8*>(to + second_of(c)) = hi;
-            } else if (slot_of[i] >= 0) {
-                const int64_t page = slot_of[i] >> a.page_shift, off = slot_of[i] & (P - 1);
-                uint8_t* const to = static_cast<uint8_t*>(a.k_pages) + page * a.k_stride + (int64_t(head) * P + off) * D;
-                const float inv = inverse_power(ek);
-                *reinterpret_cast<u32x2*>(to + first_of(c)) = u32x2{to_e4m3<true>(to_e4m3<false>(0, u[0], u[1], inv), u[2], u[3], inv),
-                                                                    to_e4m3<true>(to_e4m3<false>(0, u[4], u[5], inv), u[6], u[7], inv)};
-                *reinterpret_cast<u32x2*>(to + second_of(c)) = u32x2{to_e4m3<true>(to_e4m3<false>(0, w[0], w[1], inv), w[2], w[3], inv),
-                                                                     to_e4m3<true>(to_e4m3<false>(0, w[4], w[5], inv), w[6], w[7], inv)};
-                if (c == 0) a.k_scales[(page * a.kv_heads + head) * P + off] = uint8_t(ek);
-            }
+            *reinterpret_cast<v8*>(to + first_of(c)) = lo;
+            *reinterpret_cast<v8*>(to + second_of(c)) = hi;
         }
     }
     if (!v) return;
@@ -340,7 +375,7 @@ __global__ __launch_bounds__(256) void k_kv_load(LoadArgs a) {
     }
     __syncthreads();
     if (!a.s.k) return;
-    auto power_of = [](uint32_t e) { return __uint_as_float(min(e, 254u) << 23); };
+    auto power_of = [](uint32_t e) { return __uint_as_float(e << 23); };         // the conversions read the exponent alone
     auto two = [](uint32_t w, float s, auto hi) {
         if constexpr (__is_same(T, _Float16)) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, s, decltype(hi)::value));
         else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, s, decltype(hi)::value));
@@ -399,15 +434,21 @@ __global__ __launch_bounds__(256) void k_kv_load(LoadArgs a) {
     }
 }
 
-constexpr int32_t kStore8Few = 1024;      // tokens up to which a workgroup takes one
+// Tokens up to which a workgroup takes one of them; twice as many where tiles would not give most CUs a workgroup. us by token and by tile
+// (more heads of less: tiles sooner):
+//   tokens            1,024         1,100         2,048         4,099
+//   32/8 of 128       14.4          -     14.5    -     17.1    -     26.5
+//   8/2 of 256        8.8           -     12.9    -     14.2    -     19.4
+//   12/12 of 64       8.6           -     10.0    -     11.8    -     18.0
+constexpr int32_t kStore8Few = 1024;
 
 template <typename T, int D>
 int launch_store_dim(const StoreArgs& a, hipStream_t s) {
-    if (a.s.num_tokens <= kStore8Few) {
+    const int64_t tiles = (int64_t(a.s.num_tokens) + store8_tile<D>() - 1) / store8_tile<D>();
+    if (a.s.num_tokens <= kStore8Few || (a.s.num_tokens <= 2 * kStore8Few && tiles * a.kv_heads < 192)) {
         MARS_LAUNCH((k_kv_store8<T, D>), dim3(unsigned(a.s.num_tokens)), dim3(256), 0, s, a);
     } else {
-        const unsigned tiles = unsigned((int64_t(a.s.num_tokens) + store8_tile<D>() - 1) / store8_tile<D>());
-        MARS_LAUNCH((k_kv_store8_tile<T, D>), dim3(tiles, unsigned(a.kv_heads)), dim3(256), 0, s, a);
+        MARS_LAUNCH((k_kv_store8_tile<T, D>), dim3(unsigned(tiles), unsigned(a.kv_heads)), dim3(256), 0, s, a);
     }
     return MARS_OK;
 }

@@ -45,16 +45,23 @@ def exponent(x, dtype):
     return (np.where(pos, np.maximum(k, g), k) + 127).astype(np.uint8)
 
 
+MOST = {"float16": 61440.0, "bfloat16": 240.0 * 2.0 ** 120}       # the largest that is held: a finite value of the type
+
+
+def limited(x, dtype):
+    return np.where(np.isfinite(x), np.clip(x, -MOST[dtype], MOST[dtype]), x)
+
+
 def hold(x, dtype):
     """x (..., D) -> e4m3 bytes, exponent bytes."""
+    x = limited(x, dtype)
     e = exponent(x, dtype)
     return to_e4m3(x * 2.0 ** (127.0 - e.astype(np.float64))[..., None]), e
 
 
 def held(b, e):
     """What bytes b under exponent bytes e (broadcast) stand for."""
-    e = np.minimum(e, 254).astype(np.float64)
-    return VALUES[b] * np.where(e == 0, 0.0, 2.0 ** (e - 127))
+    return VALUES[b] * np.where(e == 255, np.nan, 2.0 ** (e.astype(np.float64) - 127))
 
 
 def pages_held(k, v, ks, vs):

@@ -82,6 +82,8 @@ def run_store(tokens, hq, hkv, D, dtype, page, rope, sections, adjacent=False, i
     with np.errstate(invalid="ignore"):
         want, size = ref.rotate(xx[:, :hq + hkv], pos, theta, rope, sections, adjacent, inverse)
     err = 2.0 ** -19 * size
+    turned = want[:, hq:].copy()
+    want = np.concatenate([want[:, :hq], ref8.limited(turned, dtype)], 1)
     got_q = ref.from_bits((d if in_place else q_out).numpy(), dtype)[:, :hq]
     fine = np.isfinite(want[:, :hq])
     off = np.where(size == 0, 0, ref.U[dtype] * np.abs(want) + err + 2.0 ** -25)[:, :hq]
@@ -131,7 +133,7 @@ STORES = [(12, 12, 64, "float16", 16), (8, 2, 128, "bfloat16", 64), (3, 1, 256, 
           (4, 2, 256, "bfloat16", 16)]
 
 
-@pytest.mark.parametrize("tokens", [1, 2, 17, 64, 130, 1029])
+@pytest.mark.parametrize("tokens", [1, 2, 17, 64, 130, 1029, 2101])
 @pytest.mark.parametrize("hq,hkv,D,dtype,page", STORES)
 def test_store(tokens, hq, hkv, D, dtype, page):
     run_store(tokens, hq, hkv, D, dtype, page, D, (D // 8, D // 4, D // 8), seed=tokens)
@@ -139,12 +141,12 @@ def test_store(tokens, hq, hkv, D, dtype, page):
 
 @pytest.mark.parametrize("D,rope,sections,adjacent", [(64, 64, (32,), False), (64, 64, (32,), True), (64, 48, (4, 20, 0), True), (64, 16, (0, 3, 5), False),
                                                       (128, 64, (32,), True), (128, 128, (64,), False), (256, 32, (16,), False), (64, 0, (), False)])
-@pytest.mark.parametrize("tokens", [5, 200, 1089])
+@pytest.mark.parametrize("tokens", [5, 200, 2089])
 def test_store_rotations(tokens, D, rope, sections, adjacent):
     run_store(tokens, 4, 2, D, "bfloat16", 32, rope, sections, adjacent, seed=rope)
 
 
-@pytest.mark.parametrize("tokens", [3, 150, 1100])
+@pytest.mark.parametrize("tokens", [3, 150, 2100])
 @pytest.mark.parametrize("D", [64, 128, 256])
 def test_store_layouts(tokens, D):
     run_store(tokens, 6, 2, D, "float16", 16, 64, (32,), interleaved=True, seed=1)
@@ -154,7 +156,7 @@ def test_store_layouts(tokens, D):
 
 
 @pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
-@pytest.mark.parametrize("tokens", [40, 1060])
+@pytest.mark.parametrize("tokens", [40, 2060])
 def test_store_values_of_any_size(tokens, dtype):
     """Heads of zeros, of the types' largest and least values, at the borders of an exponent, with infinities and NaN."""
     rng = np.random.default_rng(5)
@@ -182,14 +184,14 @@ def test_store_past_32_bits():
     ks, vs = (DeviceArray((pages, hkv, page), "uint8") for _ in range(2))
     cache = PagedCache(kb, _As(vb, (pages, hkv, D, page)), k_scales=ks, v_scales=vs)
     rng = np.random.default_rng(12)
-    L = 1500
-    table = np.array([[pages - 1, 2, pages - 17, pages - 3, 5, pages - 30]], np.int32)
+    L = 2500
+    table = np.array([[pages - 1, 2, pages - 17, pages - 3, 5, pages - 30, 7, pages - 12, pages - 13, 9]], np.int32)
     j = np.arange(L)
     slots = table[0][j // page].astype(np.int64) * page + j % page
     x = ref.to_bits(rng.standard_normal((L, hq + 2 * hkv, D)), dtype)
     r = Reader(hq, hkv, D, dtype, page)
     k, v = (dev(np.ascontiguousarray(x[:, hq + i * hkv:hq + (i + 1) * hkv]), dtype) for i in range(2))
-    for a, b in ((0, 40), (40, L)):                      # both forms
+    for a, b in ((0, 400), (400, L)):                      # both forms
         part = [View(y, (b - a, hkv, D), (hkv * D, D, 1), a * hkv * D) for y in (k, v)]
         r.store(cache, None, *part, None, dev(slots[a:b]))
     back = [DeviceArray((L, hkv, D), dtype) for _ in range(2)]
@@ -199,10 +201,10 @@ def test_store_past_32_bits():
         b, e = ref8.hold(ref.from_bits(x[:, hq + i * hkv:hq + (i + 1) * hkv], dtype), dtype)
         small.append(ref8.held(b, e[..., None]))
         np.testing.assert_array_equal(back[i].numpy().astype(np.float64), small[i])
-    pad = np.zeros((2, 6 * page, hkv, D))
+    pad = np.zeros((2, 10 * page, hkv, D))
     pad[0, :L], pad[1, :L] = small
-    want, _, tol, _ = ref.attend(ref.from_bits(x[-40:, :hq], dtype), pad[0].reshape(6, page, hkv, D).transpose(0, 2, 1, 3),
-                                 pad[1].reshape(6, page, hkv, D).transpose(0, 2, 3, 1), [0, 40], [L], np.arange(6)[None], dtype)
+    want, _, tol, _ = ref.attend(ref.from_bits(x[-40:, :hq], dtype), pad[0].reshape(10, page, hkv, D).transpose(0, 2, 1, 3),
+                                 pad[1].reshape(10, page, hkv, D).transpose(0, 2, 3, 1), [0, 40], [L], np.arange(10)[None], dtype)
     q = dev(np.ascontiguousarray(x[-40:, :hq]), dtype)
     for m in (0, 1):
         out = DeviceArray((40, hq, D), dtype)
@@ -332,7 +334,13 @@ def poison8(table, lens, c, page):
         ks[pg, :, off] = vs[pg, :, off] = (255, 254, 0)[(pg + off) % 3]
 
 
-def check(r, dtype, q, cache, pages, q_start, lens, table, max_new=(0,), groups=None, stream=0, **opt):
+def widened(table, page, hkv, D):
+    """The table with room for 128 MiB of 8-bit slots, as a server's rows have: only then prefixes are read apart. Garbage in what no row uses."""
+    width = max(table.shape[1], -(-(128 << 20) // (len(table) * page * hkv * D * 2)))
+    return np.concatenate([table, np.full((len(table), width - table.shape[1]), 10 ** 6, np.int32)], 1)
+
+
+def check(r, dtype, q, cache, pages, q_start, lens, table, max_new=(0,), groups=None, stream=0, wide=True, **opt):
     """One call, twice for each max_new (the same bits), held to the restatement over 64-bit pages."""
     T, hq, D = q.shape
     kt, ke = opt.pop("k_times", None), opt.pop("k_eps", None)
@@ -346,6 +354,8 @@ def check(r, dtype, q, cache, pages, q_start, lens, table, max_new=(0,), groups=
         d.update(group_start=dev(np.asarray(groups[0], np.int32)), shared_lens=dev(np.asarray(groups[1], np.int32)))
     want, wlse, tol, ltol = ref.attend(ref.from_bits(q, dtype), *pages, q_start, lens, table, dtype, k_times=kt, k_eps=ke, **opt)
     owned = np.isin(np.arange(T), np.concatenate([np.arange(a, b) for a, b in zip(q_start[:-1], q_start[1:])] or [[]]))
+    if groups and wide:
+        table = widened(table, r.page_size, r.kv_heads, D)
     for m in max_new:
         bits = None
         for _ in range(2):
@@ -546,9 +556,9 @@ GROUPS = {"one": [(515, [(0, 1), (33, 1), (1, 1), (700, 1), (64, 1)])],
 
 @pytest.mark.parametrize("held8", [False, True])
 @pytest.mark.parametrize("which", ["", "decay", "cap decay episode prefix"])
-@pytest.mark.parametrize("kind", sorted(GROUPS))
+@pytest.mark.parametrize("kind,wide", [(k, True) for k in sorted(GROUPS)] + [("several", False)])
 @pytest.mark.parametrize("hq,hkv,D,dtype,page", [(12, 12, 64, "float16", 16), (8, 2, 128, "bfloat16", 64), (7, 1, 128, "float16", 32), (4, 2, 256, "bfloat16", 16)])
-def test_shared(hq, hkv, D, dtype, page, kind, which, held8):
+def test_shared(hq, hkv, D, dtype, page, kind, wide, which, held8):
     rng = np.random.default_rng(hq + len(kind))
     table, k, v, q_start, lens, starts, shared = make_shared(rng, GROUPS[kind], hkv, D, dtype, page)
     T = int(q_start[-1]) + 2
@@ -560,7 +570,7 @@ def test_shared(hq, hkv, D, dtype, page, kind, which, held8):
         poison(table, lens, k, v, page, dtype)
         c = (k, v)
     q = ref.to_bits(rng.standard_normal((T, hq, D)), dtype)
-    check(Reader(hq, hkv, D, dtype, page), dtype, q, c, pages, q_start, lens, table, max_new=(0, max(1, int(np.diff(q_start).max()))), groups=(starts, shared),
+    check(Reader(hq, hkv, D, dtype, page), dtype, q, c, pages, q_start, lens, table, max_new=(0, max(1, int(np.diff(q_start).max()))), groups=(starts, shared), wide=wide,
           **options(rng, which, T, hq, k.shape[0] * page, len(lens)))
 
 
@@ -589,6 +599,7 @@ def test_shared_values_that_tables_should_not_hold():
     want, _, tol, _ = ref.attend(ref.from_bits(q, dtype), ref.from_bits(k, dtype), ref.from_bits(v, dtype), q_start, lens, table, dtype)
     r = Reader(hq, hkv, D, dtype, page)
     cache = PagedCache(dev(k, dtype), dev(v, dtype))
+    table = widened(table, page, hkv, D)
     for starts, shared, bad in (([1, 0, 2], [64, 64], None), ([-7, 2], [64], None), ([2 ** 31 - 1, -2 ** 31, 2], [64, 64], None), ([0, 2], [64], [10 ** 9, -4, 3, 2 ** 31 - 1])):
         t = table.copy()
         if bad:
@@ -673,7 +684,7 @@ def test_answers_from_one_memory(held8):
     stream = C.c_void_p()
     assert hip.hipStreamCreateWithFlags(C.byref(stream), 1) == 0
     rng = np.random.default_rng(31)
-    hq, hkv, D, page, dtype, R, width, pages = 8, 2, 64, 16, "float16", 5, 30, 120
+    hq, hkv, D, page, dtype, R, width, pages = 8, 2, 64, 16, "float16", 5, 6_600, 120
     S, T = 200, 12                                       # the memory's tokens: 12 whole pages are shared
     r = Reader(hq, hkv, D, dtype, page, rope_dim=D)
     if held8:
