@@ -1217,6 +1217,10 @@ constexpr int kFewCut = 8;
 // line would give some of them the ends of two. 64 single tokens over 500 to 1,000 keys (32/8 heads of 128, 8 bits) 27.2 us, 38.4
 // without; one over 4,160 (65 steps) 20 and, whole, 44.6. (mars_kv_attend over 16 bits keeps to equal lengths, and its bits.)
 constexpr int kFewWhole = 36;
+// The same where steps outside the rows' episodes are skipped: equal lengths leave most pieces without any. 48 single tokens that ask within
+// 900 of up to 6,001 keys (94 steps) 38 us, 57 cut (16/2 heads 31 and 37). Rows that ask within no episode read all of it: twice the bound's
+// steps would then take a workgroup 50 us.
+constexpr int kFewWholeListed = 108;
 // Steps of a piece of a prefix at least: 2 prefixes of 4,160 tokens for 4 requests each 33.0 us (1: 35.4, 16: 37.0).
 constexpr int kFirstSpan = 4;
 template <typename F>
@@ -1290,7 +1294,7 @@ __device__ void few_rows(const AttendArgs& a, int block, int blocks, FewShared<D
         int64_t tiles = load_span<F, true>(a, 0, 0, sp);
         for (int r = 256; r < a.requests; r += 256) tiles = load_span<F, true>(a, r, tiles, sp);
         if (tid == 0) sp.total = tiles;
-        whole = __builtin_amdgcn_readfirstlane(sp.most) <= kFewWhole;
+        whole = __builtin_amdgcn_readfirstlane(sp.most) <= (EXTRA && a.k_eps ? kFewWholeListed : kFewWhole);
         __syncthreads();
     }
     auto span_of = [&](int r, int64_t base) { return F::share && whole ? load_span<F, true>(a, r, base, sp) : load_span<F>(a, r, base, sp); };
@@ -2008,7 +2012,8 @@ int launch_dim(AttendArgs a, int32_t max_new, hipStream_t s) {
     const int64_t few = std::min<int64_t>(few_tiles * a.kv_heads * ((keys + few_step<F>() - 1) / few_step<F>()), 256 * few_waves<D, F>());
     // no more tiles than workgroups: by the bound on the new tokens, since the rows of each request are not known here
     const int64_t each = (std::min<int64_t>(max_new > 0 ? max_new : a.tokens, a.tokens) * a.group + kFewRows - 1) / kFewRows;
-    a.whole = !first && few_only && std::min<int64_t>(few_tiles, each * std::min(a.requests, a.tokens)) * a.kv_heads <= 256 * few_waves<D, F>();
+    const int64_t most_tiles = few_only ? std::min<int64_t>(few_tiles, each * std::min(a.requests, a.tokens)) : few_tiles;
+    a.whole = !first && most_tiles * a.kv_heads <= 256 * few_waves<D, F>();
     if (!many_only) MARS_LAUNCH((k_attend_few<T, D, EXTRA, CAP, F>), dim3(unsigned(few + first)), dim3(256), 0, s, a);
     if (few_only) return MARS_OK;
     // many: no more than chunks of kMinChunk or more of the tiles' keys, or 2^kManyItemsLog2 chunks and one for each tile
