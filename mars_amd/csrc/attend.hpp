@@ -162,6 +162,8 @@ __device__ inline void scales16(u32x4 w, float (&s)[16]) {
         s[4 * j + 3] = scale_at<3>(w[j]);
     }
 }
+// The power of two of exponent byte j of a word, in fp32 (of 0 it is 0, of 255 an infinity).
+__device__ inline float power(uint32_t w, int j) { return __uint_as_float((j == 3 ? w >> 1 : w << (23 - 8 * j)) & 0x7F800000u); }
 // Two e4m3 values of a word (its upper half if HI) as T, times `scale`.
 template <typename T, bool HI>
 __device__ inline uint32_t from_e4m3(uint32_t w, float scale) {
@@ -180,14 +182,8 @@ __device__ inline u32x4 element_e4m3(uint32_t w0, uint32_t w1, const float* s) {
     return u32x4{join(from_e4m3<T, false>(w0, s[0]), from_e4m3<T, false>(w0, s[1])), join(from_e4m3<T, true>(w0, s[2]), from_e4m3<T, true>(w0, s[3])),
                  join(from_e4m3<T, false>(w1, s[4]), from_e4m3<T, false>(w1, s[5])), join(from_e4m3<T, true>(w1, s[6]), from_e4m3<T, true>(w1, s[7]))};
 }
-// Of 4 values: nonzero if one of them is NaN (e4m3 has no infinities). Of 4 exponents: nonzero if one of them is 128 or more above
-// zero's, that is above the `most` with which every e4m3 value is a finite one of T: 134 or 246.
+// Of 4 values: nonzero if one of them is NaN (e4m3 has no infinities).
 __device__ inline uint32_t nan_e4m3(uint32_t w) { return ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u; }
-template <typename T>
-__device__ inline uint32_t wide_exponents(uint32_t w) {
-    constexpr uint32_t room = 127u - ((__is_same(T, _Float16) ? 134u : 246u) & 127u);       // 0x80 and these 7 bits above `most`
-    return (((w & 0x7F7F7F7Fu) + room * 0x01010101u) & w) & 0x80808080u;
-}
 // The first `n` bytes of 16 kept (n may be negative or above 16), the others 0.
 __device__ inline u32x4 first_bytes(u32x4 w, int n) {
 #pragma unroll
@@ -775,11 +771,11 @@ struct FewLds {
         StepLds steps;
     };
     int any_dirty;
-    u32x4 q[F::share && D == (F::c8 ? 128 : 64) ? D / 32 * 64 : 1];            // see kLean
-    u32x4 row[F::share ? kFewRows : 1];                     // of a row: decay and time of the query (fp32), limit, episode
+    u32x4 q[F::c8 && D == 128 ? D / 32 * 64 : 1];           // see kLean
+    u32x4 row[F::c8 && D == 128 ? kFewRows : 1];                     // of a row: decay and time of the query (fp32), limit, episode
 };
 // Waves a SIMD of the kernels of few rows, as their registers allow.
-template <int D, typename F>
+template <int D, typename F, bool EXTRA>
 constexpr int few_waves() { return D > 128 ? 1 : D == 128 ? 2 : F::c8 ? 2 : 3; }
 template <typename F>
 constexpr int few_step() { return F::c8 ? 64 : 32; }
@@ -787,12 +783,17 @@ constexpr int few_step() { return F::c8 ? 64 : 32; }
 template <typename T, int D, bool EXTRA, bool CAP, typename F>
 __device__ void few_part(const AttendArgs& a, const Part& it, FewLds<D, F>& lds) {
     using V = typename Vec<T>::v8;
+    // The second product's type. Of 8 bits it is bfloat16 whatever T is: e4m3 values are exact in it, and a key's power of two goes to its
+    // weight, which needs fp32's range. (Converted into T instead, a pair of one element's values takes three instructions for one.)
+    using W = std::conditional_t<F::c8, __bf16, T>;
+    using VW = typename Vec<W>::v8;
+    constexpr float lift = Vec<W>::lift;
     // a step's keys; its groups of 16; keys of a lane, in NB blocks of the first product and NT fragments of the second
     constexpr int kStep = few_step<F>(), NG = kStep / 16, NK = kStep / 4, NB = NK / 4, NT = NK / 8, KC = D / 32, VB = D / 16;
-    // With times on the way the registers do not suffice for 64 keys a step of heads of 128, nor for heads of 64 three waves a SIMD,
-    // and a kernel that keeps one value in scratch memory takes 13 us more a launch: there q, which the four waves have in
-    // common, and the terms of the rows are read from LDS in every step, and a lane's places in K and V are found anew
-    constexpr bool kLean = F::share && EXTRA && D == (F::c8 ? 128 : 64);
+    // With times on the way the registers do not suffice for 64 keys a step of heads of 128: there q, which the four waves have in
+    // common, and the terms of the rows are read from LDS in every step, and a lane's places in K and V are found anew (64
+    // single tokens over 2,000 to 4,000 keys, decayed, 95 us; 108 with 22 values a lane in scratch memory)
+    constexpr bool kLean = F::c8 && EXTRA && D == 128;
     int tid = int(threadIdx.x);
     asm volatile("" : "+v"(tid));                          // nothing of a piece is kept in registers for the next
     int lane = tid & 63;
@@ -930,7 +931,7 @@ __device__ void few_part(const AttendArgs& a, const Part& it, FewLds<D, F>& lds)
         const float2 ml = join_state<D, 8>(a, it, lds.join);
         if (wave == 0 && row_ok && ml.x != -kInf) {
             mref = ml.x;
-            mtop = mref + (Vec<T>::lift + kSlack);
+            mtop = mref + (lift + kSlack);
             l = h == 0 ? ml.y : 0.0f;
 #pragma unroll
             for (int d = 0; d < VB; ++d) o[d] = *reinterpret_cast<const f32x4*>(&lds.join.sum()[col * (D + 4) + d * 16 + h * 4]);
@@ -1018,11 +1019,11 @@ __device__ void few_part(const AttendArgs& a, const Part& it, FewLds<D, F>& lds)
                 top = fmaxf(top, __shfl_xor(top, 16));
                 top = fmaxf(top, __shfl_xor(top, 32));
                 const bool none = mtop == -kInf;
-                const float mnew = none ? top - Vec<T>::lift : fmaxf(mref, top - Vec<T>::lift);
+                const float mnew = none ? top - lift : fmaxf(mref, top - lift);
                 if (mnew > -kInf) {                          // not NaN either: the row's sum is then NaN
                     const float f = none ? 0.0f : __builtin_amdgcn_exp2f(mref - mnew);
                     mref = mnew;
-                    mtop = mnew + (Vec<T>::lift + kSlack);
+                    mtop = mnew + (lift + kSlack);
                     l *= f;
 #pragma unroll
                     for (int d = 0; d < VB; ++d) o[d] *= f;
@@ -1031,15 +1032,16 @@ __device__ void few_part(const AttendArgs& a, const Part& it, FewLds<D, F>& lds)
             // the weights as a 16-bit value and a 16-bit rest: the second product costs little where the cache's bytes bound the
             // kernel, and the output's error is that of its own rounding (with one product 1.4 times that, as in k_attend_many).
             // fp16's rests end at 2^-25 as its values do: a weight is off by up to 2^-32 of the row's largest
-            V p[NT], rest[NT];
+            VW p[NT], rest[NT];
             float sum = 0.0f;
             auto weigh = [&](int t) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    const float w = __builtin_amdgcn_exp2f(x[8 * t + j] - mref);
+                    float w = __builtin_amdgcn_exp2f(x[8 * t + j] - mref);
                     sum += w;
-                    p[t][j] = T(w);
-                    rest[t][j] = T(w - float(p[t][j]));
+                    if constexpr (F::c8) w *= power(vx[2 * t + j / 4], j % 4);
+                    p[t][j] = W(w);
+                    rest[t][j] = W(w - float(p[t][j]));
                 }
             };
             // infinities and NaN: see add_not_finite (in every step: a rest may be 0 or negative). Slots past the request's keys
@@ -1052,21 +1054,23 @@ __device__ void few_part(const AttendArgs& a, const Part& it, FewLds<D, F>& lds)
 #pragma unroll
                     for (int d = 0; d < VB; ++d) vf[d] = first_bytes(vf[d], keys - kb);
                 }
+                // exponents of 255 stand for NaN
 #pragma unroll
-                for (int j = 0; j < 4; ++j) odd |= wide_exponents<T>(vx[j]);
+                for (int j = 0; j < 4; ++j) odd |= nan_e4m3(vx[j]) & vx[j];
 #pragma unroll
                 for (int d = 0; d < VB; ++d) odd |= nan_e4m3(vf[d][0]) | nan_e4m3(vf[d][1]) | nan_e4m3(vf[d][2]) | nan_e4m3(vf[d][3]);
-                const bool look = __any(odd != 0);           // perhaps: then at the values themselves
+                if (__any(odd != 0)) {
+                    dirty = true;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) vx[j] &= ~(((nan_e4m3(vx[j]) & vx[j]) >> 7) * 0xFFu);
+#pragma unroll
+                    for (int d = 0; d < VB; ++d)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) vf[d][j] &= ~((nan_e4m3(vf[d][j]) >> 7) * 0xFFu);
+                }
                 auto add = [&](int d, int t) {
-                    const float vs[8] = {scale_at<0>(vx[2 * t]), scale_at<1>(vx[2 * t]), scale_at<2>(vx[2 * t]), scale_at<3>(vx[2 * t]),
-                                         scale_at<0>(vx[2 * t + 1]), scale_at<1>(vx[2 * t + 1]), scale_at<2>(vx[2 * t + 1]), scale_at<3>(vx[2 * t + 1])};
-                    u32x4 b = element_e4m3<T>(vf[d][2 * t], vf[d][2 * t + 1], vs);
-                    if (look) {
-                        if (__any(exponents_full<T>(b) != 0)) dirty = true;
-                        b = finite_part<T>(b);
-                    }
-                    const V w = __builtin_bit_cast(V, b);
-                    o[d] = Vec<T>::mma(w, rest[t], Vec<T>::mma(w, p[t], o[d]));
+                    const VW w = __builtin_bit_cast(VW, token_e4m3<W>(vf[d][2 * t], vf[d][2 * t + 1], 1.0f));
+                    o[d] = Vec<W>::mma(w, rest[t], Vec<W>::mma(w, p[t], o[d]));
                 };
                 // element by element, so that the registers of V are free for the next step's one after the other (one token over
                 // 4,001 keys of 64 requests 93 us, key by key 106); kLean has no registers for all weights at once
@@ -1076,6 +1080,7 @@ __device__ void few_part(const AttendArgs& a, const Part& it, FewLds<D, F>& lds)
                         weigh(t);
 #pragma unroll
                         for (int d = 0; d < VB; ++d) add(d, t);
+                        __builtin_amdgcn_sched_barrier(0);
                     }
                 } else {
 #pragma unroll
@@ -1102,8 +1107,8 @@ __device__ void few_part(const AttendArgs& a, const Part& it, FewLds<D, F>& lds)
                 if (__any(odd != 0)) dirty = true;
 #pragma unroll
                 for (int d = 0; d < VB; ++d) {
-                    const V w = __builtin_bit_cast(V, vf[d]);
-                    o[d] = Vec<T>::mma(w, rest[0], Vec<T>::mma(w, p[0], o[d]));
+                    const VW w = __builtin_bit_cast(VW, vf[d]);
+                    o[d] = Vec<W>::mma(w, rest[0], Vec<W>::mma(w, p[0], o[d]));
                 }
             }
             l += sum;
@@ -1557,8 +1562,8 @@ __device__ void many_rows(const AttendArgs& a, int block, ManyShared<D>& lds) {
     uint32_t kx[RL];
     float time_raw = 0.0f;
     int32_t eps_raw = 0;
-    // a thread's place in the tile, found anew for every tile where the registers are short
-    auto thread = [&] { return D == 256 || (EXTRA && D == 128) ? int(here(uint32_t(tid))) : tid; };
+    // a thread's place in the tile, found anew for every tile where the registers are short (heads of 256 with cap and age 743 us, 794)
+    auto thread = [&] { return D == 256 ? int(here(uint32_t(tid))) : tid; };
     auto page4 = [&](int u) { return pick4(u, pages[0], pages[1], pages[2], pages[3]); };
     auto fetch = [&](int s) {
         const int kt = k0 + s * kManyKeys, th = thread();
@@ -1973,7 +1978,7 @@ __global__ __launch_bounds__(256) void k_attend_join(AttendArgs a) {
 
 // ---- the kernels ------------------------------------------------------------------------
 template <typename T, int D, bool EXTRA, bool CAP, typename F>
-__global__ __launch_bounds__(256, (few_waves<D, F>())) void k_attend_few(AttendArgs a) {
+__global__ __launch_bounds__(256, (few_waves<D, F, EXTRA>())) void k_attend_few(AttendArgs a) {
     __shared__ __attribute__((aligned(16))) FewShared<D, F> lds;
     int blocks = int(gridDim.x);
     if (F::share && a.phase == 1 && int(blockIdx.x) == --blocks) {
@@ -2009,11 +2014,11 @@ int launch_dim(AttendArgs a, int32_t max_new, hipStream_t s) {
     a.few_rows = few_only ? INT32_MAX : many_only ? -1 : kFewMost;
     // few: one workgroup for each that the CUs hold at a time, fewer where there are not so many steps
     const int64_t few_tiles = few_only ? rows / kFewRows + std::min(a.requests, a.tokens) : std::min(a.requests, a.tokens);
-    const int64_t few = std::min<int64_t>(few_tiles * a.kv_heads * ((keys + few_step<F>() - 1) / few_step<F>()), 256 * few_waves<D, F>());
+    const int64_t few = std::min<int64_t>(few_tiles * a.kv_heads * ((keys + few_step<F>() - 1) / few_step<F>()), 256 * few_waves<D, F, EXTRA>());
     // no more tiles than workgroups: by the bound on the new tokens, since the rows of each request are not known here
     const int64_t each = (std::min<int64_t>(max_new > 0 ? max_new : a.tokens, a.tokens) * a.group + kFewRows - 1) / kFewRows;
     const int64_t most_tiles = few_only ? std::min<int64_t>(few_tiles, each * std::min(a.requests, a.tokens)) : few_tiles;
-    a.whole = !first && most_tiles * a.kv_heads <= 256 * few_waves<D, F>();
+    a.whole = !first && most_tiles * a.kv_heads <= 256 * few_waves<D, F, EXTRA>();
     if (!many_only) MARS_LAUNCH((k_attend_few<T, D, EXTRA, CAP, F>), dim3(unsigned(few + first)), dim3(256), 0, s, a);
     if (few_only) return MARS_OK;
     // many: no more than chunks of kMinChunk or more of the tiles' keys, or 2^kManyItemsLog2 chunks and one for each tile
