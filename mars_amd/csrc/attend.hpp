@@ -21,6 +21,11 @@
 //  second product (the matrix cores take no more at that rate); their sum is that of the
 //  unrounded ones, fp32 as every other sum. A lane adds a step's weights up before it adds them to
 //  the row's sum: one by one, weights below 2^-24 of that sum would be lost however many there are.
+//
+//  A cache of 8 bits (mars_kv_cache8) holds e4m3 values times a power of two a token and head. K's values become T's on the
+//  way to the first product, exactly; V's too in the tiles of many rows, while few rows take them as bf16 and put the key's power of
+//  two on its weight. Prefixes that several requests share (mars_kv_shared) are read in a launch of their own, whose
+//  sums (O, m and the sum of weights, fp32) the requests' own launch goes on from.
 // ============================================================================
 #pragma once
 
@@ -763,6 +768,8 @@ __device__ void add_not_finite(const AttendArgs& a, const Part& it, int prefix) 
 // a CU have 128 KB in flight for heads of 128. The waves' sums are joined at the end. bf16, 32/8 heads of 128:
 // 64 single tokens over 780 to 7,800 keys (1.15 GB) 215 us, 5.4 TB/s; one over 131,072 (0.54 GB) 110 us.
 // Steps of 64 keys spill: 228 and 119 us (first case with cap and decay: 288 and 225 us).
+// Of 8 bits a step is 64 keys, the same bytes: the first case (0.58 GB) 122 us, 4.8 TB/s, the other (0.27 GB) 66 us; twice the scores
+// and weights a byte: vector units busy 36% of the cycles, and waves wait 41% of their time for data, 35% for an instruction's turn.
 template <int D, typename F>
 struct FewLds {
     union {
@@ -1415,6 +1422,11 @@ __device__ inline bool own_pieces(const AttendArgs& a, Part* it, int piece) {
 // in the softmax. 2 x 4,096 tokens over 8,196 keys, bf16, 32/8 heads of 128: 782 to 838 us by the box, 985 to 1,055 TFLOP/s (a product
 // of 8,192 cubed reaches 1,168). With cap and decay a score takes twice the vector instructions: 2 x 4,001 tokens of 12 heads of
 // 64 within their episodes, vector units busy 72%, matrix cores 11%.
+// Of 8 bits the tiles go through registers, where they become T: half as many vector instructions again (bytes to 16 bits 64, their
+// addresses and the writes to LDS some 35, beside 207 a wave and tile). 2 x 2,048 tokens over 6,148 keys, heads of 128: 393 to 411
+// us by the box (875 to 835 TFLOP/s), 362 to 372 of 16 bits; matrix cores busy 41% and 51%, vector units 53% and 47%. Pieces of 8 bytes,
+// whose writes to LDS have no bank conflicts (10% of the cycles here), take more loads: 496 us for 485 (under a profiler), heads of 256
+// 631 for 569.
 constexpr int kManyKeys = 64;
 
 // Heads of 256 have one wave a SIMD, which nothing covers while it waits for LDS: LDS reads and products stay in the order

@@ -1,7 +1,7 @@
 // ============================================================================
 //  reader.hip — the reading path's handle, plan, store and release (mars_reader,
 //  mars_kv_*): how the tokens of retrieved memories are laid out in a paged cache.
-//  attend.hip holds the attention over it.
+//  store8.hip holds the store into 8 bits and the way back, attend.hpp the attention.
 // ============================================================================
 #include "reader.hpp"
 

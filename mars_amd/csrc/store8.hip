@@ -67,7 +67,8 @@ __device__ inline float max_over(float x) {
     return x;
 }
 
-// Few tokens: a workgroup to each. q as in k_kv_store, a pair a thread and turn; a wave to a head of k or v. Latency bound.
+// Few tokens: a workgroup to each. q as in k_kv_store, a pair a thread and turn; a wave to a head of k or v. Latency bound (32
+// tokens 5.8 us).
 template <typename T, int D>
 __global__ __launch_bounds__(256) void k_kv_store8(StoreArgs a) {
     const int t = int(blockIdx.x), half = a.rope_dim / 2, tid = int(threadIdx.x), lane = tid & 63, wave = tid >> 6;
@@ -143,7 +144,8 @@ __global__ __launch_bounds__(256) void k_kv_store8(StoreArgs a) {
 
 // Many tokens: a workgroup takes kTile of them under one kv head, as k_kv_store_tile does. A head's elements lie with D / 16
 // (k, pieces of 16) or D / 8 (v) neighbouring lanes, which find its largest between them; v goes through LDS as bytes, and a
-// thread that has 4 elements of 8 tokens turns them with byte permutations into 8 bytes a row of the page.
+// thread that has 4 elements of 8 tokens turns them with byte permutations into 8 bytes a row of the page. 4,099 tokens, 3 axes:
+// 32/8 heads of 128 27 to 29 us (tiles of 64 tokens 30), 8/2 heads of 256 19 us (tiles of 32 24).
 template <int D>
 constexpr int store8_tile() { return D == 256 ? 16 : D == 128 ? 32 : 64; }
 
@@ -343,7 +345,8 @@ __global__ __launch_bounds__(256) void k_kv_store8_tile(StoreArgs a) {
 // ---- load ---------------------------------------------------------------------------
 // A workgroup takes 64 tokens under one kv head. k's rows lie as the outputs do. Of v, whose pages hold the tokens of an element side by
 // side, a run of tokens that lies within 8 slots from a multiple of 8 on is read as one piece an element (8 bytes of e4m3, 16 of
-// T: always inside the page, whichever of the 8 are wanted), and goes through LDS to rows.
+// T: always inside the page, whichever of the 8 are wanted), and goes through LDS to rows. Bound by the bytes: 20,011 tokens of 8 heads
+// of 128 in runs of 700, 124 MB, 28 us (4.4 TB/s); 137 tokens of 12 heads of 64 4.7 us.
 constexpr int kLoadTile = 64;
 
 template <typename T, int D, bool C8>
