@@ -652,6 +652,34 @@ def test_shared_scores_of_any_size(n, dtype):
               groups=(starts, shared))
 
 
+@pytest.mark.parametrize("held8", [False, True])
+@pytest.mark.parametrize("n,own", [(1, 30), (3, 700), (40, 30), (40, 700)])
+def test_shared_not_finite(n, own, held8):
+    """NaN in a shared prefix's keys and values, and in a request's own, the prefix ending inside a tile, in pieces and not: they reach the rows
+    that see them and no other."""
+    rng = np.random.default_rng(25 + n)
+    hq, hkv, D, page, dtype = 4, 2, 64, 16, "float16"
+    for S in (144, 3_024):                               # 16 tokens more than steps of 32, 64
+        table, k, v, q_start, lens, starts, shared = make_shared(rng, [(S, [(own, n), (0, n), (5, 1)]), (48, [(9, n)])], hkv, D, dtype, page)
+        T = int(q_start[-1])
+        nan = 0x7E00
+        v[table[0, 2], 0, 7, 5] = nan                    # of the first group, head 0: all its rows' element 7 of query heads 0 and 1
+        v[table[0, S // page - 1], 1, 20, page - 1] = nan
+        v[table[1, S // page], 1, 33, 0] = nan           # the second request's own first key
+        other = table[0, 3] * page + np.arange(page)     # another episode's keys, all NaN
+        k[table[0, 3]] = nan
+        v[table[0, 3]] = nan
+        k_eps, q_eps = np.full(k.shape[0] * page, 1, np.int32), np.ones(T, np.int32)
+        k_eps[other] = 2
+        q = ref.to_bits(rng.standard_normal((T, hq, D)), dtype)
+        c, pages = quantise(k, v, dtype) if held8 else ((k, v), (ref.from_bits(k, dtype), ref.from_bits(v, dtype)))
+        check(Reader(hq, hkv, D, dtype, page), dtype, q, c, pages, q_start, lens, table, max_new=(0, n), groups=(starts, shared), q_eps=q_eps, k_eps=k_eps)
+        k[table[0, 3]] = v[table[0, 3]] = 0              # without episodes, and one score of NaN
+        k[table[0, 1], 1, 3, 9] = nan
+        c, pages = quantise(k, v, dtype) if held8 else ((k, v), (ref.from_bits(k, dtype), ref.from_bits(v, dtype)))
+        check(Reader(hq, hkv, D, dtype, page), dtype, q, c, pages, q_start, lens, table, max_new=(0, n), groups=(starts, shared))
+
+
 @pytest.mark.parametrize("page", [16, 64])
 def test_release_shared(page):
     """The pages behind the prefixes come back, in request order; those of the prefixes stay."""
