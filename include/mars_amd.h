@@ -884,9 +884,10 @@ int mars_kv_load8(const mars_reader* r, const mars_kv_cache8* cache, const mars_
 /* Requests that have their first tokens in common, as answers to several questions about the same memories have: group g
  * is requests group_start[g] .. group_start[g + 1] - 1 (rising, from 0; requests in no group share nothing), whose first shared_lens[g]
  * tokens, rounded down to whole pages, lie in the same pages. Attention reads such a prefix once for all rows of a group, by the
- * row of the table of its first request, and gives what it gives without groups, but for the order of the sums. A request whose cached tokens
- * (kv_lens less its new ones) are fewer than the prefix reads everything for itself. So do all in calls of more than 2^15 rows times
- * query heads (their products cost more than the reads), and where the rows of the table name less than 128 MiB (one pass is shorter). */
+ * row of the table of its first request that has the whole prefix cached, and gives what it gives without groups, but for the order of the sums. A
+ * request whose cached tokens (kv_lens less its new ones) are fewer than the prefix reads everything for itself, by its own row. So do all in calls
+ * of more than 2^15 rows times query heads (their products cost more than the reads), and where the rows of the table name less than 128 MiB
+ * (one pass is shorter). */
 typedef struct mars_kv_shared {
     const int32_t* group_start;     /* num_groups + 1 */
     const int32_t* shared_lens;     /* num_groups     */

@@ -267,15 +267,35 @@ __device__ inline int64_t wave_sum(int64_t v) {
 struct Request { int row0, n, tiles, keys, skip, at; };       // at: its row of the table
 
 // Shared prefixes are read in two phases. The first takes each group for a request: all rows of its members over the
-// prefix, which all of them see, with the pages of the first member; sums and references go to the state, a row and query
-// head each. The second takes the requests again, from behind the prefix on and from that state.
+// prefix, which all of them see that have it cached, with the pages of the first of those; sums and references go to the state, a row
+// and query head each. The second takes the requests again, from behind the prefix on and from that state.
 __device__ inline int group_at(const AttendArgs& a, int g) { return min(max(a.group_start[g], 0), a.members); }
 // Tokens of group g's prefix: whole pages, no more than a row of the table names.
 __device__ inline int shared_of(const AttendArgs& a, int g) {
     return int(min(int64_t(max(a.shared_lens[g], 0)), int64_t(a.max_pages) << a.page_shift)) >> a.page_shift << a.page_shift;
 }
-// The second phase's skips, by one workgroup of the first: 0 for a request in no group, or that has not the whole prefix cached
-// (one that was not served has no keys at all): it reads everything itself. lds: room for the groups' starts.
+// Whether request r has `s` tokens cached, its new ones apart (one that was not served has no keys at all).
+__device__ inline bool has_cached(const AttendArgs& a, int r, int s) {
+    const int row0 = max(a.q_start[r], 0), n = max(0, min(a.q_start[r + 1], a.tokens) - row0);
+    const int64_t keys = min(int64_t(a.kv_lens[r]), int64_t(a.max_pages) << a.page_shift);
+    return s <= keys - n;
+}
+// The first of requests [first, end) that has `s` tokens cached: its row of the table names the prefix, that of one before it need
+// not. `end`: none. Four are looked at together, and mostly the first is it.
+__device__ inline int holder_of(const AttendArgs& a, int first, int end, int s) {
+    constexpr int U = 4;
+    for (int m = first; m < end; m += U) {
+        bool has[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) has[u] = has_cached(a, min(m + u, end - 1), s);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (has[u]) return min(m + u, end - 1);
+    }
+    return end;
+}
+// The second phase's skips, by one workgroup of the first: 0 for a request in no group, or that has not the whole prefix cached:
+// it reads everything itself. lds: room for the groups' starts.
 __device__ inline void find_skips(const AttendArgs& a, int32_t* lds) {
     for (int g = int(threadIdx.x); g <= a.requests; g += 256) lds[g] = a.group_start[g];
     __syncthreads();
@@ -286,9 +306,7 @@ __device__ inline void find_skips(const AttendArgs& a, int32_t* lds) {
             if (lds[mid] <= r) lo = mid; else hi = mid;
         }
         const int s = lds[lo] <= r && r < lds[lo + 1] ? shared_of(a, lo) : 0;
-        const int row0 = max(a.q_start[r], 0), n = max(0, min(a.q_start[r + 1], a.tokens) - row0);
-        const int64_t keys = min(int64_t(a.kv_lens[r]), int64_t(a.max_pages) << a.page_shift);
-        a.skips[r] = s <= keys - n ? s : 0;
+        a.skips[r] = has_cached(a, r, s) ? s : 0;
     }
 }
 
@@ -299,12 +317,15 @@ __device__ inline Request request_of(const AttendArgs& a, int r) {
     if (r >= a.requests) return q;
     int start, end, len;
     if (F::share && a.phase == 1) {
-        q.at = group_at(a, r);
-        start = a.q_start[q.at];
-        end = a.q_start[max(group_at(a, r + 1), q.at)];
+        const int first = group_at(a, r), behind = max(group_at(a, r + 1), first);
+        start = a.q_start[first];
+        end = a.q_start[behind];
         len = shared_of(a, r);
-        q.at = min(q.at, a.members - 1);
+        q.at = min(first, a.members - 1);
         if (len == 0) return q;
+        const int holder = holder_of(a, first, behind, len);
+        if (holder == behind) return q;                      // every member reads everything itself
+        q.at = holder;
     } else {
         start = a.q_start[r];
         end = a.q_start[r + 1];
