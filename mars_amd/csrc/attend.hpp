@@ -1695,19 +1695,23 @@ __device__ void many_rows(const AttendArgs& a, int block, ManyShared<D>& lds) {
         for (int j = 0; j < 16; ++j) o[d][j] = 0.0f;
     float mref = 0.0f, mtop = -kInf, l = 0.0f;               // mtop: -inf until the row has seen a key, then mref + lift + kSlack
     if (F::share && it.skip > 0 && k0 == it.skip && row_ok) {        // the prefix's sums
+        // Over 8 bits their reference may be the largest score itself (k_attend_few weighs in bfloat16 there): taken `lift` lower, so that
+        // fp16's weights reach as far down as they do without a prefix.
+        constexpr float lower = F::c8 ? Vec<T>::lift : 0.0f, times = lower > 0.0f ? 128.0f : 1.0f;
+        static_assert(lower == 0.0f || lower == 7.0f, "2^lower");
         const int64_t at = row * a.q_heads + hq;
         const float2 ml = a.state_ml[at];
         if (ml.x != -kInf) {
-            mref = ml.x;
+            mref = ml.x - lower;
             mtop = mref + (Vec<T>::lift + kSlack);
-            l = h == 0 ? ml.y : 0.0f;
+            l = h == 0 ? ml.y * times : 0.0f;
 #pragma unroll
             for (int d = 0; d < DB; ++d)
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
                     const f32x4 w = *reinterpret_cast<const f32x4*>(a.state_o + at * D + d * 32 + g * 8 + h * 4);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) o[d][g * 4 + j] = w[j];
+                    for (int j = 0; j < 4; ++j) o[d][g * 4 + j] = w[j] * times;
                 }
         }
     }
