@@ -817,6 +817,7 @@ int mars_kv_store(const mars_reader* r, const mars_kv_cache* cache, const mars_k
  * The sums are fp32. For the product with v the weights of requests of many rows are rounded to the
  * cache's type; those of few rows keep a second value of that type for what the first leaves. In float16
  * either is off by up to 2^-32 of the row's largest weight besides, a key (bfloat16 has fp32's range).
+ * Weights reach 2^8 in the sums (2^15 in float16): elements with values from 2^119 on, which bfloat16 has, may leave fp32's range.
  * max_new: an upper bound of the requests' new tokens if the caller knows one (0: unknown); it picks
  * the kernel, and a wrong one costs speed alone. num_tokens rows of q; rows no request owns are left. */
 typedef struct mars_kv_attend_args {
@@ -865,7 +866,7 @@ int mars_kv_load(const mars_reader* r, const mars_kv_cache* cache, const mars_kv
  * each element is rounded once, to nearest even (k from its turned fp32 value), and is off by at most 2^-4 of itself
  * or 2^-10 times 2^(e - 127); finite ones beyond 61440 (float16) or 240 * 2^120 become that. Infinities and NaN become NaN, and leave the
  * head's other elements alone. Read, a value is rounded to the reader's type, which changes none that a reader of that type wrote; e
- * of 255 (never written) is NaN. */
+ * is 247 at most as it is written, larger ones may leave the range of the attention's sums, and 255 is NaN. */
 typedef struct mars_kv_cache8 {
     void*    k_pages;
     void*    v_pages;

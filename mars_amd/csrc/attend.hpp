@@ -805,6 +805,7 @@ struct FewLds {
 // Waves a SIMD of the kernels of few rows, as their registers allow.
 template <int D, typename F, bool EXTRA>
 constexpr int few_waves() { return D > 128 ? 1 : D == 128 ? 2 : F::c8 ? 2 : 3; }
+constexpr float kLift8 = -1.0f;     // Vec::lift of k_attend_few over 8 bits
 template <typename F>
 constexpr int few_step() { return F::c8 ? 64 : 32; }
 
@@ -815,7 +816,8 @@ __device__ void few_part(const AttendArgs& a, const Part& it, FewLds<D, F>& lds)
     // weight, which needs fp32's range. (Converted into T instead, a pair of one element's values takes three instructions for one.)
     using W = std::conditional_t<F::c8, __bf16, T>;
     using VW = typename Vec<W>::v8;
-    constexpr float lift = Vec<W>::lift;
+    // A weight takes its key's power of two, up to 2^120: kept to 2^7, so that the product stays in fp32's range (infinity times 0 is NaN).
+    constexpr float lift = F::c8 ? kLift8 : Vec<W>::lift;
     // a step's keys; its groups of 16; keys of a lane, in NB blocks of the first product and NT fragments of the second
     constexpr int kStep = few_step<F>(), NG = kStep / 16, NK = kStep / 4, NB = NK / 4, NT = NK / 8, KC = D / 32, VB = D / 16;
     // With times on the way the registers do not suffice for 64 keys a step of heads of 128: there q, which the four waves have in
@@ -1695,10 +1697,10 @@ __device__ void many_rows(const AttendArgs& a, int block, ManyShared<D>& lds) {
         for (int j = 0; j < 16; ++j) o[d][j] = 0.0f;
     float mref = 0.0f, mtop = -kInf, l = 0.0f;               // mtop: -inf until the row has seen a key, then mref + lift + kSlack
     if (F::share && it.skip > 0 && k0 == it.skip && row_ok) {        // the prefix's sums
-        // Over 8 bits their reference may be the largest score itself (k_attend_few weighs in bfloat16 there): taken `lift` lower, so that
-        // fp16's weights reach as far down as they do without a prefix.
-        constexpr float lower = F::c8 ? Vec<T>::lift : 0.0f, times = lower > 0.0f ? 128.0f : 1.0f;
-        static_assert(lower == 0.0f || lower == 7.0f, "2^lower");
+        // Over 8 bits their reference may be k_attend_few's, which weighs in bfloat16 there: taken lower in fp16, so that its weights reach
+        // as far down as they do without a prefix.
+        constexpr float lower = F::c8 && Vec<T>::lift > 0.0f ? Vec<T>::lift - kLift8 : 0.0f, times = lower > 0.0f ? 256.0f : 1.0f;
+        static_assert(lower == 0.0f || lower == 8.0f, "2^lower");
         const int64_t at = row * a.q_heads + hq;
         const float2 ml = a.state_ml[at];
         if (ml.x != -kInf) {

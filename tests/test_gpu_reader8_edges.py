@@ -1,12 +1,14 @@
-"""Shared prefixes whose first request does not hold them, or beside whose weights a request's own are small."""
+"""Shared prefixes whose first request does not hold them, and 8-bit values and weights at the ends of their ranges."""
 from __future__ import annotations
 
 import numpy as np
 import pytest
 
 import mars_amd
+import reader8_ref as ref8
 import reader_ref as ref
-from mars_amd.reader import Reader
+from mars_amd.reader import PagedCache, Reader
+from test_gpu_reader import dev, make_cache
 from test_gpu_reader8 import check, make_shared, quantise
 
 pytestmark = pytest.mark.gpu
@@ -67,3 +69,63 @@ def test_own_keys_far_below_a_shared_prefix(D):
     # the output's rounding and its weights' to 2^-32 of the largest; scores of fp32 as in reader_ref
     tol = 2.0 ** -11 * want + keys * 2.0 ** -32 * 40960.0 / total + 2.2 * ((D + 8) * 2.0 ** -24 * 20 + 2.0 ** -20) * want + 2.0 ** -24
     assert np.all(np.abs(got - want) <= tol), (float(got[0, 0, 0]), float(want[0, 0, 0]))
+
+
+# ---- values at the ends of bfloat16 ------------------------------------------------------
+@pytest.mark.parametrize("decay", [False, True])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("held8", [True, False])
+def test_attend_largest_values(held8, D, decay):
+    """A key whose values are near the type's largest and whose weight is nearly 2^8 times the reference's, some of its values 0: those elements get
+    what the other keys give. The large ones are beyond the sums' range (2^7 times 3.19e38 is 2^134.9, fp32 ends at 2^128): infinities, or their average."""
+    hq, hkv, page, dtype, L = 2, 1, 64, "bfloat16", 900
+    rng = np.random.default_rng(D)
+    table, k, v = make_cache(rng, [L], hkv, D, dtype, page)
+    at = 256                                             # the fifth step of 64 keys: the wave of the first one
+    pg, off = table[0][at // page], at % page
+    x = ref.from_bits(v, dtype)
+    large = np.arange(D) % 3 == 0
+    x[pg, 0, :, off] = np.where(large, 240 * 2.0 ** 120, 0.0)
+    k = np.zeros(k.shape)
+    k[pg, 0, off] = 1.0
+    k, v = ref.to_bits(k, dtype), ref.to_bits(x, dtype)
+    c, held = quantise(k, v, dtype) if held8 else ((k, v), (ref.from_bits(k, dtype), ref.from_bits(v, dtype)))
+    assert not held8 or c[3][pg, 0, off] == 247          # the largest that is stored
+    q = ref.to_bits(np.ones((1, hq, D)), dtype)
+    opt = dict(decay=np.zeros(hq, np.float32), q_times=np.zeros(1, np.float32), k_times=np.zeros(k.shape[0] * page, np.float32)) if decay else {}
+    want, _, tol, _ = ref.attend(ref.from_bits(q, dtype), *held, [0, 1], [L], table, dtype, scale=5.5445 / D, **opt)
+    t = {n: dev(opt[n]) for n in ("decay", "q_times") if n in opt}
+    cache = PagedCache(dev(c[0], None if held8 else dtype), dev(c[1], None if held8 else dtype), dev(opt["k_times"]) if opt else None, None,
+                       *(dev(y) for y in c[2:]))
+    for m in (0, 1):
+        out = dev(np.zeros(q.shape, np.uint16), dtype)
+        Reader(hq, hkv, D, dtype, page).attend(cache, dev(q, dtype), out, dev(np.array([0, 1], np.int32)), dev(np.array([L], np.int32)), dev(table), scale=5.5445 / D,
+                                               max_new=m, **t)
+        got = ref.from_bits(out.numpy(), dtype)
+        with np.errstate(invalid="ignore"):
+            fine = np.abs(got - want) <= tol
+        assert np.all(fine[:, :, ~large]) and np.all((fine | (got == np.inf))[:, :, large]), (m, got[0, 0, :6], want[0, 0, :6])
+
+
+@pytest.mark.parametrize("decay", [False, True])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_attend_smallest_values(D, decay):
+    """Heads whose values all take the least exponent, weights times 2^-117 still count."""
+    hq, hkv, page, dtype, L = 2, 1, 64, "bfloat16", 700
+    rng = np.random.default_rng(D)
+    table, k, v = make_cache(rng, [L], hkv, D, dtype, page)
+    c, _ = quantise(k, v, dtype)
+    c[3][...] = 10
+    c[1][...] = np.where(c[1] & 0x40, c[1], c[1] | 0x40)                 # sizes of 2 to 448 times 2^-117
+    c[1][(c[1] & 0x7F) == 0x7F] ^= 1
+    held = ref8.pages_held(*c)
+    q = ref.to_bits(rng.standard_normal((1, hq, D)), dtype)
+    opt = dict(decay=np.zeros(hq, np.float32), q_times=np.zeros(1, np.float32), k_times=np.zeros(k.shape[0] * page, np.float32)) if decay else {}
+    out = np.asarray(check(Reader(hq, hkv, D, dtype, page), dtype, q, c, held, [0, 1], [L], table, max_new=(1,), **opt))
+    want, _, tol, _ = ref.attend(ref.from_bits(q, dtype), held[0], held[1] * 2.0 ** 117, [0, 1], [L], table, dtype)
+    # scaled to sizes of 1. reader_ref's bound, and for a weight's two parts in bfloat16, whose least step is 2^-133: half of that a key, at 2^-117
+    # and values of up to 448; weights are at least half of exp(s - top)
+    j = np.arange(L)
+    s = np.einsum("hd,jd->hj", ref.from_bits(q, dtype)[0], held[0][table[0][j // page], 0, j % page]) * D ** -0.5
+    least = 2.0 ** -17 * 448 * L / (0.5 * np.exp(s - s.max(1, keepdims=True)).sum(1))
+    assert np.all(np.abs(out * 2.0 ** 117 - want) <= tol + least[None, :, None]), float(np.max(np.abs(out * 2.0 ** 117 - want) - tol))
