@@ -897,7 +897,9 @@ typedef struct mars_kv_shared {
 } mars_kv_shared;
 int mars_kv_attend_shared(const mars_reader* r, const mars_kv_cache* cache, const mars_kv_attend_args* args, const mars_kv_shared* shared,
                           void* stream);
-/* mars_kv_attend over a cache of 8 bits, as over the values that mars_kv_load8 gives. shared: NULL: none. */
+/* mars_kv_attend over a cache of 8 bits, as over the values that mars_kv_load8 gives. Where the cache holds values that the reader's type
+ * does not have (a reader of the other type wrote it), those of v are taken as they are held for requests of few rows, of e 0 as 0.
+ * shared: NULL: none. */
 int mars_kv_attend8(const mars_reader* r, const mars_kv_cache8* cache, const mars_kv_attend_args* args, const mars_kv_shared* shared,
                     void* stream);
 /* mars_kv_release of the pages behind the shared prefixes alone: the prefix's pages stay the caller's, who gives them

@@ -757,9 +757,10 @@ __device__ void add_not_finite(const AttendArgs& a, const Part& it, int prefix) 
             }
             const int64_t at = page * a.v_stride + ((int64_t(it.head) * D + d) << a.page_shift) + off;
             if constexpr (F::c8) {
-                const float e = scale_at<0>(a.v_scales[((page * a.kv_heads + it.head) << a.page_shift) + off]);
-                const float v = float(__builtin_bit_cast(typename Vec<T>::v2, from_e4m3<T, false>(static_cast<const uint8_t*>(a.v_pages)[at], e))[0]);
-                if (!(fabsf(v) < kInf)) sum += v;
+                // what the products left out: k_attend_few, which takes values as they are held, NaN; k_attend_many what is not finite as T
+                const uint32_t b = static_cast<const uint8_t*>(a.v_pages)[at], e = a.v_scales[((page * a.kv_heads + it.head) << a.page_shift) + off];
+                const float v = float(__builtin_bit_cast(typename Vec<T>::v2, from_e4m3<T, false>(b, scale_at<0>(e)))[0]);
+                if (BM == kFewRows ? (b & 0x7Fu) == 0x7Fu || e == 255u : !(fabsf(v) < kInf)) sum += v;
             } else {
                 const float v = float(static_cast<const T*>(a.v_pages)[at]);
                 if (!(fabsf(v) < kInf)) sum += v;

@@ -129,3 +129,26 @@ def test_attend_smallest_values(D, decay):
     s = np.einsum("hd,jd->hj", ref.from_bits(q, dtype)[0], held[0][table[0][j // page], 0, j % page]) * D ** -0.5
     least = 2.0 ** -17 * 448 * L / (0.5 * np.exp(s - s.max(1, keepdims=True)).sum(1))
     assert np.all(np.abs(out * 2.0 ** 117 - want) <= tol + least[None, :, None]), float(np.max(np.abs(out * 2.0 ** 117 - want) - tol))
+
+
+# ---- values that the reader's type does not have -----------------------------------------
+@pytest.mark.parametrize("n,length", [(1, 200), (1, 5_000), (3, 200)])
+def test_attend_values_of_the_other_type(n, length):
+    """A cache with values beyond float16's largest, read by a float16 reader's few rows: taken as they are held, also where a NaN elsewhere has rows
+    looked over again."""
+    hq, hkv, D, page, dtype = 4, 2, 64, 16, "float16"
+    rng = np.random.default_rng(length)
+    table, k, v = make_cache(rng, [length], hkv, D, dtype, page)
+    k = ref.to_bits(ref.from_bits(k, dtype) / 4, dtype)
+    c, _ = quantise(k, v, dtype)
+    for j in (5, 70, 150):
+        pg, off = table[0][j // page], j % page
+        c[1][pg, :, :, off] = 0x70                       # 128 times 2^13: over the keys some 2^20 / length
+        c[3][pg, :, off] = 140
+    for nan in (False, True):
+        if nan:
+            c[1][table[0][40 // page], 1, 7, 40 % page] = 0x7F
+        held = ref8.pages_held(*c)
+        q = ref.to_bits(rng.standard_normal((n, hq, D)), dtype)
+        out = check(Reader(hq, hkv, D, dtype, page), dtype, q, c, held, [0, n], [length], table, max_new=(n,))
+        assert np.isfinite(out).sum() == out.size - (2 * n if nan else 0)
