@@ -275,9 +275,20 @@ class Reader:
         return _lib.KvSharedC(*_args(self.device, (group_start, "group_start", "int32", (groups + 1,)), (shared_lens, "shared_lens", "int32", (groups,))),
                               groups, 0)
 
-    def release(self, done, kv_lens, block_table, free_pages, free_count, group_start=None, shared_lens=None, stream: int = 0) -> None:
+    def release(self, done, kv_lens, block_table, free_pages, free_count, *more, group_start=None, shared_lens=None, stream=None) -> None:
         """The pages of requests with done != 0 pushed onto free_pages; their kv_lens (plan's next_lens) become 0 (mars_kv_release).
-        group_start, shared_lens: as for attend; the pages of the shared prefixes stay (mars_kv_release_shared)."""
+        group_start, shared_lens: as for attend; the pages of the shared prefixes stay (mars_kv_release_shared). By position the
+        stream is the sixth argument, or the eighth behind group_start and shared_lens."""
+        grouped = more and (more[0] is None or len(getattr(more[0], "shape", ())) > 0)
+        names = ("group_start", "shared_lens", "stream") if grouped else ("stream",)
+        if len(more) > len(names):
+            raise TypeError(f"release takes no more than {5 + len(names)} arguments by position here")
+        given = dict(group_start=group_start, shared_lens=shared_lens, stream=stream)
+        for name, x in zip(names, more):
+            if given[name] is not None:
+                raise TypeError(f"{name} given twice")
+            given[name] = x
+        group_start, shared_lens, stream = given["group_start"], given["shared_lens"], given["stream"] or 0
         r = int(done.shape[0])
         if len(block_table.shape) != 2:
             raise ValueError(f"block_table: shape {tuple(block_table.shape)}, expected (requests, pages)")

@@ -138,6 +138,36 @@ def test_null_arguments():
         assert e.value.code == INVALID
 
 
+def test_release_stream_and_groups(monkeypatch):
+    """The stream stands sixth, as it does without groups, or behind the groups, or by name."""
+    from mars_amd import reader
+    seen = []
+
+    class Calls:
+        def mars_kv_release(self, handle, done, lens, table, r, width, free, count, capacity, stream):
+            seen.append((r, width, capacity, None, stream))
+            return 0
+
+        def mars_kv_release_shared(self, handle, done, lens, table, r, width, shared, free, count, capacity, stream):
+            seen.append((r, width, capacity, shared.num_groups, stream))
+            return 0
+
+    monkeypatch.setattr(reader, "lib", Calls())
+    r, a = a_reader(), (i32(3), i32(3), i32(3, 5), i32(20), i32(1))
+    g = i32(3), i32(2)
+    named = dict(group_start=g[0], shared_lens=g[1])
+    for args, kw, want in (((), {}, (None, 0)), ((77,), {}, (None, 77)), ((0,), {}, (None, 0)), ((), dict(stream=77), (None, 77)), (g, {}, (2, 0)), ((*g, 77), {}, (2, 77)),
+                           (g, dict(stream=77), (2, 77)), ((g[0],), dict(shared_lens=g[1], stream=77), (2, 77)), ((), dict(named, stream=77), (2, 77)), ((77,), named, (2, 77)),
+                           ((None, None, 77), {}, (None, 77))):
+        r.release(*a, *args, **kw)
+        assert seen.pop() == (3, 5, 20, *want), (args, kw)
+    for args, kw, error in (((g[0],), {}, ValueError), ((77,), dict(group_start=g[0]), ValueError), ((77, 78), {}, TypeError), ((77,), dict(stream=78), TypeError),
+                            (g, named, TypeError), ((*g, 77, 78), {}, TypeError)):
+        with pytest.raises(error):
+            r.release(*a, *args, **kw)
+    assert not seen
+
+
 @pytest.mark.gpu
 def test_c_refusals():
     """Arguments that only the C entries can check, on arrays that are there; nothing is launched, nothing written."""
