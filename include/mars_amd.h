@@ -903,7 +903,9 @@ int mars_kv_attend_shared(const mars_reader* r, const mars_kv_cache* cache, cons
 int mars_kv_attend8(const mars_reader* r, const mars_kv_cache8* cache, const mars_kv_attend_args* args, const mars_kv_shared* shared,
                     void* stream);
 /* mars_kv_release of the pages behind the shared prefixes alone: the prefix's pages stay the caller's, who gives them
- * back once, with the request (or table row) that it keeps for the prefix itself. */
+ * back once, with the request (or table row) that it keeps for the prefix itself. The first pages of every request of a group
+ * count as the prefix's, also of one that has fewer tokens; a request that has those tokens in pages of its own (attention
+ * lets it read for itself while they are fewer) is left out of the groups here, or these pages are given back by nobody. */
 int mars_kv_release_shared(const mars_reader* r, const int32_t* done, int32_t* kv_lens, const int32_t* block_table,
                            int32_t num_requests, int32_t max_pages, const mars_kv_shared* shared, int32_t* free_pages,
                            int32_t* free_count, int32_t free_capacity, void* stream);
