@@ -815,8 +815,9 @@ int mars_kv_store(const mars_reader* r, const mars_kv_cache* cache, const mars_k
  * none is 0 with lse -inf. Keys not seen have no effect, whatever the cache holds there (NaN too);
  * an infinity or NaN that a row sees makes that element of the row one of them.
  * The sums are fp32. For the product with v the weights of requests of many rows are rounded to the
- * cache's type; those of few rows keep a second value of that type for what the first leaves. In float16
- * either is off by up to 2^-32 of the row's largest weight besides, a key (bfloat16 has fp32's range).
+ * cache's type (over 8 bits the reader's); those of few rows keep a second value of that type for what the first leaves (over 8 bits both
+ * are bfloat16, 16 bits of a weight). In float16 either is off by up to 2^-32 of the row's largest weight besides, a key (bfloat16
+ * has fp32's range).
  * Weights reach 2^8 in the sums (2^15 in float16): elements with values from 2^119 on, which bfloat16 has, may leave fp32's range.
  * max_new: an upper bound of the requests' new tokens if the caller knows one (0: unknown); it picks
  * the kernel, and a wrong one costs speed alone. num_tokens rows of q; rows no request owns are left. */
@@ -885,8 +886,9 @@ int mars_kv_load8(const mars_reader* r, const mars_kv_cache8* cache, const mars_
 /* Requests that have their first tokens in common, as answers to several questions about the same memories have: group g
  * is requests group_start[g] .. group_start[g + 1] - 1 (rising, from 0; requests in no group share nothing), whose first shared_lens[g]
  * tokens, rounded down to whole pages, lie in the same pages. Attention reads such a prefix once for all rows of a group, by the
- * row of the table of its first request that has the whole prefix cached, and gives what it gives without groups, but for the order of the sums. A
- * request whose cached tokens (kv_lens less its new ones) are fewer than the prefix reads everything for itself, by its own row. So do all in calls
+ * row of the table of its first request that has the whole prefix cached, and gives what it gives without groups, but for the order of the sums
+ * and for the weights over the prefix, which are rounded as those of many rows where the step has more than 16 rows (tokens times query heads
+ * a kv head) a group. A request whose cached tokens (kv_lens less its new ones) are fewer than the prefix reads everything for itself, by its own row. So do all in calls
  * of more than 2^15 rows times query heads (their products cost more than the reads), and where the rows of the table name less than 128 MiB
  * (one pass is shorter). */
 typedef struct mars_kv_shared {

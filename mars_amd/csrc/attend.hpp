@@ -1251,11 +1251,13 @@ __device__ void few_part(const AttendArgs& a, const Part& it, FewLds<D, F>& lds)
 constexpr int kFewCut = 8;
 // Where there are no more tiles than workgroups, and none of more steps than this, each workgroup takes whole tiles: equal lengths of the
 // line would give some of them the ends of two. 64 single tokens over 500 to 1,000 keys (32/8 heads of 128, 8 bits) 27.2 us, 38.4
-// without; one over 4,160 (65 steps) 20 and, whole, 44.6. (mars_kv_attend over 16 bits keeps to equal lengths, and its bits.)
+// without; one over 4,160 (65 steps) 20 and, whole, 44.6. (mars_kv_attend over 16 bits keeps to equal lengths, and its bits.) The bound does not
+// look at how many tiles there are, and few long ones leave CUs idle: 1, 4, 16 and 48 requests over 2,304 keys (36 steps) 25.5, 26.0, 28.6
+// and 46.1 us; cut, over 16 bits, 16.2, 21.6, 32.0 and 93.5.
 constexpr int kFewWhole = 36;
 // The same where steps outside the rows' episodes are skipped: equal lengths leave most pieces without any. 48 single tokens that ask within
-// 900 of up to 6,001 keys (94 steps) 38 us, 57 cut (16/2 heads 31 and 37). Rows that ask within no episode read all of it: twice the bound's
-// steps would then take a workgroup 50 us.
+// 900 of up to 6,001 keys (94 steps) 38 us, 57 cut (16/2 heads 31 and 37). Rows that ask within no episode read all of it, some 0.65 us
+// a step: 1, 4, 16 and 48 such requests over 6,912 keys (108 steps) 75, 85, 86 and 158 us; cut, over 16 bits, 24, 32, 91 and 263.
 constexpr int kFewWholeListed = 108;
 // Steps of a piece of a prefix at least: 2 prefixes of 4,160 tokens for 4 requests each 33.0 us (1: 35.4, 16: 37.0).
 constexpr int kFirstSpan = 4;

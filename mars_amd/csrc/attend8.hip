@@ -1,4 +1,4 @@
-// attend8.hip — attention over a cache of 8 bits, with or without shared prefixes (mars_kv_attend8, mars_kv_attend8_shared).
+// attend8.hip — attention over a cache of 8 bits, with or without shared prefixes (mars_kv_attend8).
 #include "attend.hpp"
 
 namespace mars {

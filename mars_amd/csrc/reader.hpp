@@ -56,6 +56,8 @@ constexpr int64_t kStateRows = 1 << 15;
 // 16 bits (8 bits), one token each: 4 requests over 4,160 shared tokens, 70 MB, 33 and 24 (30 and 26); 16 over 1,000, 74 MB, 28 and 25;
 // 8 over 4,160, 140 MB, 35 and 28; 64 over 1,000, 297 MB, 32 and 48 (149 MB: 32 and 29); 16 over 4,160, 280 MB, 31 and 50 (141 MB: 29 and
 // 38); 4 over 20,000, 330 MB, 43 and 55 (166 MB: 38 and 40); 64 over 32,768 107 and 937 (91 and 496).
+// The host knows the tables' width alone, not what is shared, so the bound errs both ways near it, and a short prefix under wide rows
+// pays the two phases: 16 requests that share 64 of some 560 tokens, rows of 2,000 pages, 28 and 23 (22 and 14).
 constexpr int64_t kSharedBytes = 128 << 20;
 
 struct AttendArgs {

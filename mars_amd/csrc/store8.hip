@@ -7,7 +7,8 @@
 //  value that can be held, is one of that type's. Held: e4m3(x 2^-k), rounded once to nearest even, and the byte k + 127.
 //  Finite elements beyond 61440 (or 240 2^120), the largest held values that the type has too, become that. The scaling is
 //  exact, powers of two lose nothing, and one scale a token and head keeps each token's precision whatever its
-//  neighbours are: the values keep e4m3's own relative precision of 2^-4 down to 2^-15 of the head's largest.
+//  neighbours are: the values keep e4m3's own relative precision of 2^-4 down to 2^-6 units of 2^k, the head's largest being 224 to 448 of
+//  them: to 2^-13.8 to 2^-14.8 of it.
 // ============================================================================
 #include "reader.hpp"
 
@@ -39,7 +40,7 @@ __device__ inline uint32_t exponent_for(float top) {
     const int k = int(b >> 23) - 127 - 8 + ((b & 0x7FFFFFu) > 0x600000u ? 1 : 0);
     return uint32_t(max(k, least_exponent<T>()) + 127);
 }
-// 2^-k of an exponent byte (k + 127 in 10 .. 248).
+// 2^-k of an exponent byte (k + 127 in 10 .. 247).
 __device__ inline float inverse_power(uint32_t e) { return __uint_as_float((254u - e) << 23); }
 // Two values into half of a word; infinities become NaN. Sizes are at most 448: nothing saturates.
 template <bool HI>
